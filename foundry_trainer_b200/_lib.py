@@ -44,12 +44,17 @@ class fa_rope_t(C.Structure):
                 ("theta", C.c_float)]
 
 
+class fa_matrix_t(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("stride_batch", C.c_int64), ("stride_row", C.c_int64)]
+
+
 class fa_peer_handle_t(C.Structure):
     _fields_ = [("bytes", C.c_ubyte * 64)]
 
 
 _T = C.POINTER(fa_tensor_t)
 _R = C.POINTER(fa_rope_t)
+_M = C.POINTER(fa_matrix_t)
 _F = C.c_void_p  # float* (device)
 
 # name -> (restype, argtypes)
@@ -105,6 +110,22 @@ SIGNATURES = {
                                      C.c_int64, _T, _T, C.c_float, _R, C.c_void_p]),
     "fa_merge_f32": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _F, _F, _F, _F, _T, _F,
                                C.c_void_p]),
+    "fa_layer_norm_fwd": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, _T, C.c_void_p, C.c_void_p,
+                                    C.c_int, C.c_int64, C.c_int, C.c_float, _T, _F, C.c_void_p]),
+    "fa_layer_norm_bwd": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, _T, C.c_void_p, C.c_int,
+                                    C.c_int64, C.c_int, _T, _F, _T, _F, _F, C.c_void_p, C.c_size_t,
+                                    C.c_void_p]),
+    "fa_layer_norm_bwd_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
+    "fa_lora_linear_fwd": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _M, _M, _M, _M,
+                                     C.c_float, C.c_void_p, _M, C.c_void_p, C.c_void_p]),
+    "fa_lora_linear_bwd": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _M, _M, _M, _M,
+                                     C.c_float, C.c_void_p, _M, _M, C.c_void_p, C.c_void_p,
+                                     C.c_void_p, C.c_size_t, C.c_void_p]),
+    "fa_lora_linear_bwd_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "fa_lora_linear_many": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _M, _M,
+                                      _M, _M, C.c_void_p, _F, C.c_void_p, _M, C.c_void_p,
+                                      C.c_size_t, C.c_void_p]),
+    "fa_lora_linear_many_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
     "fa_timing_enable": (C.c_int, [C.c_int]),
     "fa_timing_read": (C.c_int, [C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_int)]),
     "fa_status_string": (C.c_char_p, [C.c_int]),

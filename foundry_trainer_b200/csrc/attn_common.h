@@ -30,7 +30,9 @@ enum KernelId {
   kKernelBwdBf16 = 1,
   kKernelF32Fwd = 2,
   kKernelF32Bwd = 3,
-  kKernelCount = 8
+  kKernelWide = 4,     // + 0..11: the wide product by operand layout, epilogue and tile
+  kKernelSkinny = 16,  // + 0..7
+  kKernelCount = 24
 };
 
 // FA_OK when the last CUDA runtime call / launch on this thread succeeded;
@@ -44,6 +46,9 @@ void record_error_text(const char* msg);
 // Shape rules every attention entry point shares: dtype F32 or BF16, positive
 // sizes, head_dim 128, B and H within a grid dimension, B*S*H*D < 2^40.
 int check_attn_shape(int dtype, int B, int S, int H, int D);
+
+// FA_OK when the current device is an sm_100 one, else FA_ERR_NO_DEVICE.
+int check_sm100();
 
 // Raises the dynamic shared-memory limit of `fn` once per (device, kernel).
 int ensure_smem_attr(const void* fn, int bytes, int kernel_id);
@@ -155,6 +160,18 @@ int launch_qk_norm_rope_bwd(int B, int T, int I, int H, const fa_tensor_t* x_txt
                             float eps, const fa_rope_t* rope, const fa_tensor_t* dy,
                             const fa_tensor_t* dx_txt, const fa_tensor_t* dx_img, float* dw_txt,
                             float* dw_img, cudaStream_t stream);
+
+// Layer norm (layer_norm.cu): x, y, dy, dx are (groups, rows, 1, dim); weight
+// and bias (dim) or (groups, dim), par_stride apart per group (0: shared)
+int launch_layer_norm_fwd(int dtype, int groups, int rows, int dim, const fa_tensor_t* x,
+                          const void* w, const void* b, int par_dtype, int64_t par_stride,
+                          int unit_offset, float eps, const fa_tensor_t* y, float* stats,
+                          cudaStream_t st);
+size_t layer_norm_bwd_workspace(int groups, int rows, int dim);
+int launch_layer_norm_bwd(int dtype, int groups, int rows, int dim, const fa_tensor_t* x,
+                          const void* w, int par_dtype, int64_t par_stride, int unit_offset,
+                          const fa_tensor_t* dy, const float* stats, const fa_tensor_t* dx,
+                          float* dw, float* db, int shared, void* ws, cudaStream_t st);
 
 // Sequence-parallel exchange (peer.cu): bounded barrier over the ranks' flag
 // blocks, the owner's sum of received dK/dV contributions (dK un-rotated and

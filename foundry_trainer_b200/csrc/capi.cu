@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "attn_common.h"
+#include "gemm.h"
 #include "rope.cuh"
 #include "sm100_ptx.cuh"
 
@@ -72,6 +73,29 @@ int make_tmap_bshd_f32(CUtensorMap* map, const fa_tensor_t* t, int B, int S,
                      CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, 32);
 }
 
+int make_tmap_3d(CUtensorMap* map, const Mat3& m, int box_inner, int box_rows) {
+  auto enc = encode_fn();
+  if (!enc) return FA_ERR_LAUNCH;
+  // size-1 modes may carry any stride; give them a legal one
+  int64_t sr = m.stride_row, sb = m.stride_batch;
+  if (m.rows == 1) sr = (m.cols + 7) / 8 * 8;
+  if (m.batch == 1) sb = m.rows * sr;
+  cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)m.batch};
+  cuuint64_t strides[2] = {(cuuint64_t)(sr * 2), (cuuint64_t)(sb * 2)};
+  if (sr < 0 || sb < 0) return FA_ERR_ALIGNMENT;
+  for (int i = 0; i < 2; ++i)
+    if (strides[i] % 16 != 0 || strides[i] >= (1ull << 40)) return FA_ERR_ALIGNMENT;
+  if (reinterpret_cast<uintptr_t>(m.p) % 16 != 0) return FA_ERR_ALIGNMENT;
+  cuuint32_t box[3] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, m.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                   3, const_cast<void*>(m.p), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? FA_OK : FA_ERR_ALIGNMENT;
+}
+
 // ------------------------------------------------------ CUDA error text
 static thread_local char g_last_error[256] = "";
 
@@ -121,7 +145,7 @@ RopeArgs make_rope_args(const fa_rope_t* rope, int round_bf16, int pos_offset) {
 }
 
 // --------------------------------------------------------------- validation
-static int check_sm100() {
+int check_sm100() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return FA_ERR_NO_DEVICE;
   int major = 0;
@@ -254,7 +278,8 @@ int fa_device_status(void) {
   // every translation unit's word is read (and cleared); the first code wins
   int first = 0;
   for (int v : {fwd_device_status(), bwd_device_status(), f32_device_status(),
-                misc_device_status(), qkp_device_status(), peer_device_status()}) {
+                misc_device_status(), qkp_device_status(), peer_device_status(),
+                wide_device_status(), skinny_device_status()}) {
     if (v < 0) return FA_ERR_LAUNCH;
     if (first == 0) first = v;
   }

@@ -1,0 +1,106 @@
+// gemm.h — host interface of the matrix-product kernels (gemm_wide_sm100.cu,
+// gemm_skinny_sm100.cu) that the adapter linears and the orthogonalisation use.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "attn_common.h"
+
+namespace fa {
+
+// A 16-bit (batch, rows, cols) matrix, cols contiguous; strides in elements.
+struct Mat3 {
+  const void* p = nullptr;
+  int64_t batch = 1, rows = 0, cols = 0;
+  int64_t stride_batch = 0, stride_row = 0;
+  int bf16 = 1;  // else fp16
+};
+
+// 3-D TMA descriptor over `m`, box (inner, rows, 1), SWIZZLE_128B, zero fill.
+int make_tmap_3d(CUtensorMap* map, const Mat3& m, int box_inner, int box_rows);
+
+enum WideEpi {
+  kEpiLinear = 0,  // bf16 D (+ bias)
+  kEpiGram = 1,    // fp16 D = alpha acc, mirrored (symmetric)
+  kEpiPoly = 2,    // fp16 D = c0 in + c1 acc, mirrored (symmetric)
+  kEpiUpdate = 3,  // D = c0 (hi + lo) + c1 acc as fp16 hi and lo
+  kEpiLast = 4     // the same, as bf16 alpha D, straight or transposed
+};
+
+struct WideOperands {
+  Mat3 a, b, e, d, d2;
+  bool b_mn = false;
+};
+
+struct WideParams {
+  int M = 0, N = 0, K = 0, batch = 1;
+  int fmt = 1;  // 0 fp16, 1 bf16 operands
+  int tiles_m = 0, tiles_n = 0, tiles_per_batch = 0, symmetric = 0;
+  // adapters: low (M, low_ld) bf16, low_ld = the rank rounded up to 16;
+  // per 256-row block the adapters in use and their count, per row its slot
+  // (no lists: adapter 0 for every row)
+  const __nv_bfloat16* low = nullptr;
+  int low_ld = 0, rank = 0;
+  const int* list_cnt = nullptr;
+  const int* list_ids = nullptr;
+  const int* slot = nullptr;
+  const __nv_bfloat16* bias = nullptr;
+  // orthogonalisation
+  float alpha = 1.f;
+  const float* coef = nullptr;
+  const __half* in_hi = nullptr;
+  const __half* in_lo = nullptr;
+  int64_t in_batch = 0;
+  int in_ld = 0;
+  void* sym_out = nullptr;
+  int64_t sym_batch = 0;
+  int sym_ld = 0;
+  uint16_t* out_t = nullptr;
+  int64_t out_t_batch = 0, out_t_ld = 0;
+};
+
+// out[i, j] = sum_k Big[i, k] Small[j, k], j < n <= 256
+enum SkinnyOut {
+  kSkinnyCols = 0,  // out[j, i] bf16 + bias[i] + the adapters' term of row j
+  kSkinnyLow = 1,   // out[i, j] bf16, scaled: a row's own adapter's columns
+  kSkinnyGrad = 2   // out[j out_j + i out_ld] bf16
+};
+
+struct SkinnyParams {
+  int rows = 0;  // i
+  int cols = 0;  // j that are stored
+  int n = 0;     // cols rounded up to 16
+  int K = 0;
+  __nv_bfloat16* out = nullptr;
+  int64_t out_ld = 0, out_j = 0;
+  const __nv_bfloat16* bias = nullptr;
+  // adapters: as WideParams; `fac` (E, i, k) with element strides
+  const __nv_bfloat16* low = nullptr;
+  int low_ld = 0, rank = 0, E = 1;
+  const int* ids = nullptr;
+  const __nv_bfloat16* fac = nullptr;
+  int64_t fac_e = 0, fac_i = 0, fac_k = 0;
+  float scale = 1.f;
+  const float* scales = nullptr;
+  const int* list_cnt = nullptr;
+  const int* list_ids = nullptr;
+  const int* slot = nullptr;
+  int slots_per_pass = 1;
+};
+
+// early: the launch may start before its predecessor ends (programmatic
+// dependent launch); only `low` may then come from that predecessor.
+int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool small_mn,
+                       SkinnyParams p, int out, bool early, cudaStream_t st);
+int launch_low_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int64_t a_e,
+                    int64_t a_r, const int* ids, int E, const float* scales, float scale, int rows,
+                    int K, int rank, int low_ld, __nv_bfloat16* low, cudaStream_t st);
+int launch_adapter_plan(const int* ids, int rows, int E, int* cnt, int* list, int* slot,
+                        cudaStream_t st);
+int skinny_device_status();
+
+int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t st);
+int wide_device_status();
+
+}  // namespace fa

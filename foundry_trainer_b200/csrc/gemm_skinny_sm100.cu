@@ -1,0 +1,417 @@
+// gemm_skinny_sm100.cu — products with one short side, on the tensor cores:
+//
+//   out[i, j] = sum_k Big[i, k] Small[j, k],   j < 256
+//
+// Uses: a linear for few tokens (Big = the weight, Small = the tokens), the
+// adapters' inner products low = s x A^T and s dy B (Big = the tokens), and
+// the factors' gradients (Big = x or dy with the tokens as contraction).
+//
+// Bound by reading Big once from memory. A cluster of C CTAs shares a 128-row
+// tile of Big and splits the contraction, so that even few tiles occupy all
+// SMs; each CTA streams its K blocks through a TMA ring (two CTAs an SM while
+// the short side is at most 128, about 96 KB in flight each) into tcgen05.mma
+// with Big as the 128-row operand and the short side as its columns. The partial
+// sums stay on chip: every CTA sends the columns it does not own to their
+// owner through distributed shared memory, and the owner adds them in CTA
+// order (fp32, the same bits every time), then applies the epilogue.
+#include <algorithm>
+
+#include "attn_common.h"
+#include "gemm.h"
+#include "gemm_ptx.cuh"
+
+namespace fa {
+namespace skinny {
+
+constexpr int kThreads = 192;
+constexpr int kBig = 16384;  // 128 x 64 elements
+constexpr int kMaxStages = 8;
+constexpr int kBarBytes = 256;
+
+struct Layout {
+  int stage, stages, smem, cols;  // stage bytes, ring depth, launch bytes, TMEM columns
+};
+
+// n: columns of the product (multiple of 16), small_mn: Small stored with its
+// short side contiguous (64-wide blocks)
+static Layout layout_of(int n, bool small_mn) {
+  Layout l{};
+  const int small = small_mn ? (n + 63) / 64 * 8192 : (n * 128 + 1023) / 1024 * 1024;
+  l.stage = kBig + small;
+  const int budget = n <= 128 ? 100 * 1024 : 200 * 1024;
+  l.stages = std::min(kMaxStages, budget / l.stage);
+  const int exchange = (n + 8) * 512;  // the columns' owner's partial sums
+  l.smem = std::max(l.stage * l.stages, exchange) + kBarBytes + 1024;
+  l.cols = 32;
+  while (l.cols < n) l.cols *= 2;
+  return l;
+}
+
+template <bool BIG_MN, bool SMALL_MN, int OUT>
+__global__ void __launch_bounds__(kThreads, 2)
+skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ CUtensorMap tsmall,
+              const __grid_constant__ SkinnyParams p, int split, int stage_bytes, int stages,
+              int bar_off, int tmem_cols) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + bar_off);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + kMaxStages;
+  uint64_t* done = bars + 2 * kMaxStages;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
+  const int warp = warp_id(), lane = lane_id();
+  const int tile = blockIdx.x / split, part = blockIdx.x - tile * split;
+  const int i0 = tile * 128;
+
+  // columns of this pass: adapters [s0, s0 + ns) of the tile's list, or all
+  int n = p.n, s0 = 0, ns = 1;
+  if constexpr (OUT == kSkinnyLow) {
+    if (p.list_cnt != nullptr) {
+      s0 = blockIdx.y * p.slots_per_pass;
+      ns = min(p.slots_per_pass, p.list_cnt[i0 >> 8] - s0);
+      if (ns <= 0) return;  // the same for the whole cluster
+      n = ns * p.low_ld;
+    }
+  }
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tbig);
+    tma_prefetch_desc(&tsmall);
+  }
+  if (warp == 5) {
+    tmem_alloc(slot, tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+  const int kbs = (p.K + 63) >> 6;
+  const int kb0 = (int)((int64_t)kbs * part / split), kb1 = (int)((int64_t)kbs * (part + 1) / split);
+  bool ok = true;
+
+  if (warp == 4) {
+    if (lane == 0) {
+      if constexpr (OUT != kSkinnyCols) pdl_wait_previous();
+      const int small_blocks = (n + 63) >> 6;
+      const uint32_t bytes = kBig + (SMALL_MN ? small_blocks * 8192
+                                              : (OUT == kSkinnyCols ? p.n * 128 : n * 128));
+      int s = 0;
+      uint32_t ph = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!(ok = mbar_wait(&empty[s], ph ^ 1))) break;
+        uint8_t* sa = smem + s * stage_bytes;
+        uint8_t* sb = sa + kBig;
+        mbar_arrive_expect_tx(&full[s], bytes);
+        if constexpr (BIG_MN) {
+          tma_load_3d(sa, &tbig, &full[s], i0, kb * 64, 0);
+          tma_load_3d(sa + 8192, &tbig, &full[s], i0 + 64, kb * 64, 0);
+        } else {
+          tma_load_3d(sa, &tbig, &full[s], kb * 64, i0, 0);
+        }
+        if constexpr (SMALL_MN) {
+          for (int j = 0; j < small_blocks; ++j)
+            tma_load_3d(sb + j * 8192, &tsmall, &full[s], j * 64, kb * 64, 0);
+        } else if constexpr (OUT == kSkinnyLow) {
+          for (int q = 0; q < ns; ++q) {
+            const int e = p.list_ids != nullptr ? p.list_ids[(int64_t)(i0 >> 8) * 256 + s0 + q] : 0;
+            tma_load_3d(sb + q * p.low_ld * 128, &tsmall, &full[s], kb * 64, 0, e);
+          }
+        } else {
+          tma_load_3d(sb, &tsmall, &full[s], kb * 64, 0, 0);
+        }
+        if (++s == stages) { s = 0; ph ^= 1; }
+      }
+      if (!ok) *abort_flag = 1;
+    }
+  } else if (warp == 5) {
+    const uint32_t idesc = idesc_f16(1, 128, n, BIG_MN, SMALL_MN);
+    int s = 0;
+    uint32_t ph = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!(ok = mbar_wait_w(&full[s], ph))) break;
+      tc_fence_after();
+      const uint32_t a = smem_u32(smem + s * stage_bytes), b = a + kBig;
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          umma_ss(tmem, BIG_MN ? mnmajor_desc(a, kk, 8192) : kmajor_desc(a, kk, 0),
+                  SMALL_MN ? mnmajor_desc(b, kk, 8192) : kmajor_desc(b, kk, 0), idesc,
+                  kb > kb0 || kk > 0);
+        umma_commit(&empty[s]);
+        if (kb == kb1 - 1) umma_commit(done);
+      }
+      __syncwarp();
+      if (++s == stages) { s = 0; ph ^= 1; }
+    }
+    if (!ok) *abort_flag = 1;
+  } else {
+    ok = mbar_wait_w(done, 0);
+    if (!ok) *abort_flag = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) drain_delay();
+  if (split > 1) cluster_sync();  // every ring of the cluster is idle: its memory takes the sums
+  tc_fence_after();
+
+  // columns of owner q: [q * own, (q + 1) * own)
+  const int own = (n + split - 1) / split;
+  const int j0 = part * own, j1 = min(n, j0 + own);
+  const int r = threadIdx.x;
+  float* recv = reinterpret_cast<float*>(smem);  // (split, own, 128)
+  const bool good = *abort_flag == 0;
+  if (warp < 4 && good) {
+    const uint32_t taddr = tmem + ((uint32_t)(warp * 32) << 16);
+    const uint32_t mine = smem_u32(recv) + (uint32_t)(part * own * 128 + r) * 4u;
+    int q = 0, at = 0;  // owner of the column, its place there
+    uint32_t dst = split > 1 ? mapa(mine, 0) : mine;
+    for (int c = 0; c < n; c += 16) {
+      uint32_t v[16];
+      tmem_ld16(taddr + c, v);
+      tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if (split > 1) st_cluster_f32(dst + (uint32_t)at * 512u, __uint_as_float(v[i]));
+        else recv[(c + i) * 128 + r] = __uint_as_float(v[i]);
+        if (++at == own && q + 1 < split) {
+          at = 0;
+          dst = mapa(mine, ++q);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  if (split > 1) cluster_sync();
+  else __syncthreads();
+  tc_fence_after();
+  if (warp == 5) {
+    __syncwarp();
+    tmem_dealloc(tmem, tmem_cols);
+  }
+  const int i = i0 + r;
+  if (warp < 4 && good && i < p.rows) {
+    if constexpr (OUT == kSkinnyCols) {
+      // out[j, i] (+ bias[i] + the row's low-rank term), a column a token
+      if (p.low != nullptr) pdl_wait_previous();
+      const float bias = p.bias != nullptr ? __bfloat162float(p.bias[i]) : 0.f;
+      for (int j = j0; j < j1; ++j) {
+        float acc = bias;
+        for (int q = 0; q < split; ++q) acc += recv[(q * own + j - j0) * 128 + r];
+        if (j >= p.cols) break;
+        if (p.low != nullptr) {
+          const int e = p.ids != nullptr ? p.ids[j] : 0;
+          if (e >= 0 && e < p.E) {
+            const __nv_bfloat16* lw = p.low + (int64_t)j * p.low_ld;
+            const __nv_bfloat16* f = p.fac + (int64_t)e * p.fac_e + (int64_t)i * p.fac_i;
+            if (p.fac_i != 1) {  // the adapter's row i, its rank contiguous (16-byte rows)
+              for (int k = 0; k < p.rank; k += 8) {
+                const uint4 b4 = __ldg(reinterpret_cast<const uint4*>(f + k));
+                const uint4 l4 = __ldcg(reinterpret_cast<const uint4*>(lw + k));
+                const uint32_t bw[4] = {b4.x, b4.y, b4.z, b4.w}, xw[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                  acc = fmaf(bf16_lo(bw[u]), bf16_lo(xw[u]), acc);
+                  acc = fmaf(bf16_hi(bw[u]), bf16_hi(xw[u]), acc);
+                }
+              }
+            } else {  // its column i, consecutive over the threads
+              for (int k = 0; k < p.rank; ++k)
+                acc = fmaf(__bfloat162float(f[(int64_t)k * p.fac_k]), __bfloat162float(lw[k]), acc);
+            }
+          }
+        }
+        p.out[(int64_t)j * p.out_ld + i] = __float2bfloat16_rn(acc);
+      }
+    } else if constexpr (OUT == kSkinnyLow) {
+      // out[i, j]: the columns of the row's own adapter, scaled, in bf16 (the
+      // operand type of the product that follows; one rounding of a term that
+      // is added to the fp32 sum)
+      const int sl = p.slot != nullptr ? p.slot[i] - s0 : 0;
+      float sc = p.scale;
+      if (p.scales != nullptr && sl >= 0 && sl < ns)
+        sc = p.scales[p.list_ids[(int64_t)(i0 >> 8) * 256 + s0 + sl]];
+      const int lo = max(j0, sl * p.low_ld), hi = min(j1, (sl + 1) * p.low_ld);
+      if (sl >= 0 && sl < ns) {
+        for (int j = lo; j < hi; ++j) {
+          float acc = 0.f;
+          for (int q = 0; q < split; ++q) acc += recv[(q * own + j - j0) * 128 + r];
+          p.out[(int64_t)i * p.out_ld + j - sl * p.low_ld] = __float2bfloat16_rn(acc * sc);
+        }
+      }
+    } else {
+      for (int j = j0; j < min(j1, p.cols); ++j) {
+        float acc = 0.f;
+        for (int q = 0; q < split; ++q) acc += recv[(q * own + j - j0) * 128 + r];
+        p.out[(int64_t)j * p.out_j + (int64_t)i * p.out_ld] = __float2bfloat16_rn(acc);
+      }
+    }
+  }
+}
+
+// Inner products of few rows with their own adapters: low[n, j] = s x[n] A_e[j],
+// a warp each; columns [rank, low_ld) are zero.
+__global__ void __launch_bounds__(256)
+low_rows_kernel(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int64_t a_e,
+                int64_t a_r, const int* ids, int E, const float* scales, float scale, int K,
+                int rank, int low_ld, __nv_bfloat16* low) {
+  pdl_launch_next();
+  const int groups = low_ld / 8;
+  const int row = blockIdx.x / groups, j = (blockIdx.x - row * groups) * 8 + warp_id();
+  const int e = ids != nullptr ? ids[row] : 0;
+  const bool has = e >= 0 && e < E;
+  float acc = 0.f;
+  if (has && j < rank) {
+    const uint4* xr = reinterpret_cast<const uint4*>(x + (int64_t)row * ldx);
+    const uint4* ar = reinterpret_cast<const uint4*>(a + (int64_t)e * a_e + (int64_t)j * a_r);
+    const int nv = K >> 3;
+#pragma unroll 8
+    for (int i = lane_id(); i < nv; i += 32) {
+      const uint4 u = __ldg(xr + i), v = __ldg(ar + i);
+      const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        acc = fmaf(bf16_lo(uw[k]), bf16_lo(vw[k]), acc);
+        acc = fmaf(bf16_hi(uw[k]), bf16_hi(vw[k]), acc);
+      }
+    }
+    for (int k = (nv << 3) + lane_id(); k < K; k += 32)
+      acc = fmaf(__bfloat162float(x[(int64_t)row * ldx + k]),
+                 __bfloat162float(a[(int64_t)e * a_e + (int64_t)j * a_r + k]), acc);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  if (lane_id() == 0 && j < low_ld)
+    low[(int64_t)row * low_ld + j] =
+        __float2bfloat16_rn(has && j < rank ? acc * (scales != nullptr ? scales[e] : scale) : 0.f);
+}
+
+// Per block of 256 rows: the distinct adapters in order of first use, and
+// every row's place among them (-1: none).
+__global__ void __launch_bounds__(256)
+plan_kernel(const int* ids, int rows, int E, int* cnt, int* list, int* slot) {
+  __shared__ int id_s[256], rank_s[256], warp_s[8];
+  const int t = threadIdx.x, row = blockIdx.x * 256 + t;
+  int id = row < rows ? ids[row] : -1;
+  if (id < 0 || id >= E) id = -1;
+  id_s[t] = id;
+  __syncthreads();
+  int first = 0;
+  while (id_s[first] != id) ++first;  // ends at t
+  const bool head = id >= 0 && first == t;
+  const uint32_t m = __ballot_sync(0xffffffffu, head);
+  if (lane_id() == 0) warp_s[warp_id()] = __popc(m);
+  __syncthreads();
+  int before = __popc(m & ((1u << lane_id()) - 1u)), total = 0;
+  for (int w = 0; w < 8; ++w) {
+    if (w < warp_id()) before += warp_s[w];
+    total += warp_s[w];
+  }
+  rank_s[t] = before;
+  __syncthreads();
+  if (head) list[(int64_t)blockIdx.x * 256 + before] = id;
+  if (row < rows) slot[row] = id < 0 ? -1 : rank_s[first];
+  if (t == 0) cnt[blockIdx.x] = total;
+}
+
+template <bool BIG_MN, bool SMALL_MN, int OUT>
+static int go(const CUtensorMap& tbig, const CUtensorMap& tsmall, const SkinnyParams& p,
+              int passes, int kernel_id, bool early, cudaStream_t st) {
+  auto* fn = skinny_kernel<BIG_MN, SMALL_MN, OUT>;
+  const Layout l = layout_of(p.n, SMALL_MN);
+  // the largest layout's request, once per kernel
+  const int rc = ensure_smem_attr((const void*)fn, 232448, kernel_id);
+  if (rc) return rc;
+  const int tiles = (p.rows + 127) / 128, kbs = (p.K + 63) / 64;
+  // CTAs resident at one time: two an SM while the ring is the smaller one
+  const int slots = l.smem <= 113 * 1024 ? 296 : 148;
+  // contraction split: the one whose rounds of CTAs times blocks per CTA
+  // (and about two blocks' time for the exchange) is smallest
+  int split = 1;
+  int64_t best = INT64_MAX;
+  for (int c = 1; c <= 8 && c <= kbs; ++c) {
+    const int64_t rounds = ((int64_t)tiles * c * passes + slots - 1) / slots;
+    const int64_t cost = rounds * ((kbs + c - 1) / c + 2);
+    if (cost < best) best = cost, split = c;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(tiles * split), passes, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = l.smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = early ? 2 : 1;
+  const int bar_off = l.smem - kBarBytes - 1024;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, tbig, tsmall, p, split, l.stage, l.stages,
+                                           bar_off, l.cols);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return record_cuda_error(e);
+  }
+  return launch_status();
+}
+
+}  // namespace skinny
+
+int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool small_mn,
+                       SkinnyParams p, int out, bool early, cudaStream_t st) {
+  if (p.rows == 0) return FA_OK;
+  CUtensorMap tb, ts;
+  int passes = 1;
+  if (out == kSkinnyLow && p.list_cnt != nullptr) {
+    p.slots_per_pass = std::max(1, 128 / p.low_ld);
+    const int most = std::min(p.E, 256);
+    p.slots_per_pass = std::min(p.slots_per_pass, most);
+    p.n = p.slots_per_pass * p.low_ld;
+    passes = (most + p.slots_per_pass - 1) / p.slots_per_pass;
+  }
+  int rc = big_mn ? make_tmap_3d(&tb, big, 64, 64) : make_tmap_3d(&tb, big, 64, 128);
+  const int box = out == kSkinnyLow ? p.low_ld : p.n;
+  if (!rc) rc = small_mn ? make_tmap_3d(&ts, small, 64, 64) : make_tmap_3d(&ts, small, 64, box);
+  if (rc) return rc;
+  using namespace skinny;
+  if (out == kSkinnyCols && !big_mn && !small_mn)
+    return go<false, false, kSkinnyCols>(tb, ts, p, passes, kKernelSkinny, early, st);
+  if (out == kSkinnyCols && big_mn && !small_mn)
+    return go<true, false, kSkinnyCols>(tb, ts, p, passes, kKernelSkinny + 1, early, st);
+  if (out == kSkinnyLow && !big_mn && !small_mn)
+    return go<false, false, kSkinnyLow>(tb, ts, p, passes, kKernelSkinny + 2, early, st);
+  if (out == kSkinnyLow && !big_mn && small_mn)
+    return go<false, true, kSkinnyLow>(tb, ts, p, passes, kKernelSkinny + 3, early, st);
+  if (out == kSkinnyGrad && big_mn && small_mn)
+    return go<true, true, kSkinnyGrad>(tb, ts, p, passes, kKernelSkinny + 4, early, st);
+  return FA_ERR_UNSUPPORTED;
+}
+
+int launch_low_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int64_t a_e,
+                    int64_t a_r, const int* ids, int E, const float* scales, float scale, int rows,
+                    int K, int rank, int low_ld, __nv_bfloat16* low, cudaStream_t st) {
+  skinny::low_rows_kernel<<<(unsigned)(rows * (low_ld / 8)), 256, 0, st>>>(
+      x, ldx, a, a_e, a_r, ids, E, scales, scale, K, rank, low_ld, low);
+  return launch_status();
+}
+
+int launch_adapter_plan(const int* ids, int rows, int E, int* cnt, int* list, int* slot,
+                        cudaStream_t st) {
+  skinny::plan_kernel<<<(unsigned)((rows + 255) / 256), 256, 0, st>>>(ids, rows, E, cnt, list, slot);
+  return launch_status();
+}
+
+int skinny_device_status() { return tu_device_status(); }
+
+}  // namespace fa

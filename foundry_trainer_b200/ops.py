@@ -11,12 +11,13 @@ from __future__ import annotations
 import ctypes as C
 import math
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import FA_DTYPE_BF16, FA_DTYPE_F32, check, fa_rope_t, fa_tensor_t
+from ._lib import (FA_DTYPE_BF16, FA_DTYPE_F32, check, fa_matrix_t, fa_rope_t,
+                   fa_tensor_t)
 
 ROPE_AXES = (32, 32, 32, 32)  # lib.rs:20
 ROPE_THETA = 10000.0          # lib.rs:21
@@ -224,6 +225,271 @@ def qk_norm_rope_bwd(x_txt, x_img, w_txt, w_img, rope: Optional[Rope], dy: torch
         dw_img.data_ptr() if dw_img is not None else None, _stream_ptr(stream)),
         "fa_qk_norm_rope_bwd")
     return dx_t, dx_i, dw_txt, dw_img
+
+
+# --------------------------------------------------------- block operators
+
+def _on(t: torch.Tensor, stream) -> int:
+    """The stream to launch on: `stream`, or the current one of t's device."""
+    return (stream if stream is not None else torch.cuda.current_stream(t.device)).cuda_stream
+
+
+def _same_device(ref: torch.Tensor, **tensors) -> None:
+    if not ref.is_cuda:
+        raise ValueError("tensor must live on a CUDA device")
+    for name, t in tensors.items():
+        if t is not None and t.device != ref.device:
+            raise ValueError(f"{name} is on {t.device}, x on {ref.device}")
+
+
+def _norm_desc(t: torch.Tensor) -> fa_tensor_t:
+    """(rows, D) or (groups, rows, D) as the C ABI's (groups, rows, 1, D)."""
+    sg = t.stride(0) if t.dim() == 3 else 0
+    sd = t.stride(-1) if t.shape[-1] > 1 else 1
+    return fa_tensor_t(t.data_ptr(), sg, t.stride(-2), 0, sd)
+
+
+def _norm_params(x: torch.Tensor, weight, bias):
+    """Checked (weight, bias, dtype code, stride between groups)."""
+    given = [p for p in (weight, bias) if p is not None]
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if p.dim() == 2 and x.dim() != 3:
+            raise ValueError(f"{name} (groups, D) needs x (groups, rows, D)")
+        want = (x.shape[-1],) if p.dim() == 1 else (x.shape[0], x.shape[-1])
+        if tuple(p.shape) != want:
+            raise ValueError(f"{name} has shape {tuple(p.shape)}, expected {want}")
+    if len(given) == 2 and (weight.dim() != bias.dim() or weight.dtype != bias.dtype):
+        raise ValueError("weight and bias must share one layout and dtype")
+    if not given:
+        return None, None, FA_DTYPE_F32, 0
+    if given[0].dim() == 1:
+        weight, bias = (p.contiguous() if p is not None else None for p in (weight, bias))
+        return weight, bias, _dtype_code(given[0]), 0
+    # rows of two modulation chunks share a stride; others are copied (D values each)
+    st = {p.stride(0) for p in given}
+    if len(st) != 1 or 0 in st or any(p.stride(1) != 1 for p in given) or x.shape[0] == 1:
+        weight, bias = (p.contiguous() if p is not None else None for p in (weight, bias))
+        st = {x.shape[-1]}
+    return weight, bias, _dtype_code(given[0]), st.pop()
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return t.data_ptr() if t is not None else None
+
+
+def _check_norm_x(x: torch.Tensor, **like) -> Tuple[int, int, int]:
+    if x.dim() not in (2, 3):
+        raise ValueError(f"expected (rows, D) or (groups, rows, D), got {tuple(x.shape)}")
+    for name, t in like.items():
+        if t.shape != x.shape or t.dtype != x.dtype:
+            raise ValueError(f"{name} must have x's shape and dtype")
+    return (x.shape[0] if x.dim() == 3 else 1), x.shape[-2], x.shape[-1]
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, *, unit_offset: bool = False,
+               eps: float = NORM_EPS, out: Optional[torch.Tensor] = None, stream=None):
+    """Layer norm over the last dimension of x (rows, D) or (groups, rows, D),
+    bf16 or f32: y = h * weight + bias, h = (x - mean) / sqrt(var + eps); with
+    unit_offset the gain is 1 + weight (the modulation of layer_norm_mod,
+    lib.rs:60-71). weight and bias: (D,), or (groups, D) for one pair per
+    group; None: no gain or no bias. Returns (y, stats), stats the fp32
+    (2, groups * rows) means and reciprocal deviations layer_norm_bwd reads."""
+    G, R, D = _check_norm_x(x)
+    _same_device(x, weight=weight, bias=bias, out=out)
+    dt = _dtype_code(x)
+    w, b, pdt, ps = _norm_params(x, weight, bias)
+    y = torch.empty_like(x) if out is None else out
+    _check_norm_x(x, out=y)
+    stats = torch.empty((2, G * R), device=x.device, dtype=torch.float32)
+    with torch.cuda.device(x.device):
+        check(_lib.load().fa_layer_norm_fwd(
+            dt, G, R, D, C.byref(_norm_desc(x)), _ptr(w), _ptr(b), pdt, ps, int(unit_offset),
+            float(eps), C.byref(_norm_desc(y)), stats.data_ptr(), _on(x, stream)),
+            "fa_layer_norm_fwd")
+    return y, stats
+
+
+def layer_norm_bwd(x: torch.Tensor, weight: Optional[torch.Tensor], dy: torch.Tensor,
+                   stats: torch.Tensor, *, unit_offset: bool = False, params: bool = True,
+                   stream=None):
+    """Gradients of layer_norm: (dx, dweight, dbias), the last two fp32 with
+    weight's shape (of a (D,) pair when weight is None), or None with
+    params=False. Identical bits across repeats."""
+    G, R, D = _check_norm_x(x, dy=dy)
+    _same_device(x, weight=weight, dy=dy, stats=stats)
+    if (stats.dtype != torch.float32 or tuple(stats.shape) != (2, G * R)
+            or not stats.is_contiguous()):
+        raise ValueError("stats must be layer_norm's (2, rows) float32 tensor")
+    dt = _dtype_code(x)
+    w, _, pdt, ps = _norm_params(x, weight, None)
+    dx = torch.empty_like(x)
+    lead = () if ps == 0 else (G,)
+    dw = torch.empty(lead + (D,), device=x.device, dtype=torch.float32) if params else None
+    db = torch.empty_like(dw) if params else None
+    lib = _lib.load()
+    nb = lib.fa_layer_norm_bwd_workspace_bytes(G, R, D)
+    ws = torch.empty(nb, device=x.device, dtype=torch.uint8) if nb else None
+    with torch.cuda.device(x.device):
+        check(lib.fa_layer_norm_bwd(
+            dt, G, R, D, C.byref(_norm_desc(x)), _ptr(w), pdt, ps, int(unit_offset),
+            C.byref(_norm_desc(dy)), stats.data_ptr(), C.byref(_norm_desc(dx)), _ptr(dw), _ptr(db),
+            _ptr(ws), nb, _on(x, stream)), "fa_layer_norm_bwd")
+    return dx, dw, db
+
+
+def _matrix(t: torch.Tensor, name: str) -> fa_matrix_t:
+    """A 2-D or (batch, rows, cols) tensor for the C ABI."""
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    # a stride that no element uses may be anything: give it a legal one
+    sr = t.stride(-2) if t.shape[-2] > 1 else -(-t.shape[-1] // 8) * 8
+    sb = 0
+    if t.dim() == 3:
+        sb = t.stride(0) if t.shape[0] > 1 else t.shape[1] * sr
+    return fa_matrix_t(t.data_ptr(), sb, sr)
+
+
+def _rows2d(t: torch.Tensor, name: str) -> torch.Tensor:
+    """(..., K) as one (rows, K) matrix, without a copy."""
+    if t.dim() == 2:
+        return t
+    if t.dim() < 2:
+        raise ValueError(f"{name}: expected (..., features), got {tuple(t.shape)}")
+    try:
+        return t.view(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
+    except RuntimeError:
+        raise ValueError(f"{name}: the leading dimensions must be one strided set of rows; "
+                         "reshape it first") from None
+
+
+def _aligned_rows(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
+    """An uninitialised (rows, cols) bf16 matrix whose rows start on 16 bytes."""
+    ld = -(-cols // 8) * 8
+    return torch.empty((rows, ld), device=like.device, dtype=torch.bfloat16)[:, :cols]
+
+
+def _pad_rank(a: torch.Tensor, b: torch.Tensor):
+    """The factors with the rank a multiple of 8 (zero rows of a, columns of b)."""
+    p = -a.shape[-2] % 8
+    if p:
+        a, b = torch.nn.functional.pad(a, (0, 0, 0, p)), torch.nn.functional.pad(b, (0, p))
+    return a, b
+
+
+def _check_lora(x2, w, a, b, bias, stacked: bool) -> None:
+    for name, t in (("x", x2), ("w", w), ("a", a), ("b", b), ("bias", bias)):
+        if t is not None and t.dtype != torch.bfloat16:
+            raise TypeError(f"{name}: the linear with adapters computes in bf16, got {t.dtype}")
+    _same_device(x2, w=w, a=a, b=b, bias=bias)
+    nd = 3 if stacked else 2
+    if w.dim() != 2 or a.dim() != nd or b.dim() != nd:
+        raise ValueError("expected w (out, in) and factors a (..., rank, in), b (..., out, rank)")
+    K, M = w.shape[1], w.shape[0]
+    if x2.shape[1] != K or a.shape[-1] != K or b.shape[-2] != M or a.shape[-2] != b.shape[-1]:
+        raise ValueError(f"shapes do not fit: x (..., {x2.shape[1]}), w {tuple(w.shape)}, "
+                         f"a {tuple(a.shape)}, b {tuple(b.shape)}")
+    if stacked and a.shape[0] != b.shape[0]:
+        raise ValueError("a and b must hold as many adapters")
+    if bias is not None and (tuple(bias.shape) != (M,) or not bias.is_contiguous()):
+        raise ValueError("bias must be a contiguous (out,) vector")
+
+
+def _low_dim(rank: int) -> int:
+    return -(-rank // 16) * 16
+
+
+def lora_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor, *,
+                scale: float = 1.0, bias: Optional[torch.Tensor] = None, stream=None):
+    """y = x w^T + bias + scale (x a^T) b^T in one product (the reference's
+    linear with LoRA factors, lib.rs:270-287): x (..., in), w (out, in),
+    a (rank, in), b (out, rank), bf16, fp32 sums. Rows of x, w and a must
+    start on 16 bytes; a rank that is no multiple of 8 costs a padded copy of
+    the factors, rank <= 256. Returns (y, low), low = scale x a^T as
+    lora_linear_bwd reads it."""
+    x2 = _rows2d(x, "x")
+    _check_lora(x2, w, a, b, bias, False)
+    a, b = _pad_rank(a, b)
+    N, K, M, r = x2.shape[0], w.shape[1], w.shape[0], a.shape[0]
+    y = _aligned_rows(N, M, x)
+    low = torch.empty((N, _low_dim(r)), device=x.device, dtype=torch.bfloat16)
+    ms = [_matrix(t, n) for t, n in ((x2, "x"), (w, "w"), (a, "a"), (b, "b"), (y, "y"))]
+    with torch.cuda.device(x.device):
+        check(_lib.load().fa_lora_linear_fwd(
+            FA_DTYPE_BF16, N, K, M, r, *[C.byref(m) for m in ms[:4]], float(scale), _ptr(bias),
+            C.byref(ms[4]), low.data_ptr(), _on(x, stream)), "fa_lora_linear_fwd")
+    return y.view(*x.shape[:-1], M) if x.dim() != 2 else y, low
+
+
+def lora_linear_bwd(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+                    dy: torch.Tensor, low: torch.Tensor, *, scale: float = 1.0,
+                    need_dx: bool = True, need_factors: bool = True, stream=None):
+    """Gradients of lora_linear with w frozen: (dx, da, db) in bf16, each None
+    when not needed. `low` is what the forward returned for the same x, a and
+    scale. Identical bits across repeats. (The bias's gradient, where it
+    trains, is dy summed over its rows.)"""
+    x2, dy2 = _rows2d(x, "x"), _rows2d(dy, "dy")
+    _check_lora(x2, w, a, b, None, False)
+    _same_device(x, dy=dy, low=low)
+    if dy2.dtype != torch.bfloat16 or tuple(dy2.shape) != (x2.shape[0], w.shape[0]):
+        raise ValueError(f"dy must be bf16 (..., {w.shape[0]}) with x's rows")
+    rank = a.shape[0]
+    a, b = _pad_rank(a, b)
+    N, K, M, r = x2.shape[0], w.shape[1], w.shape[0], a.shape[0]
+    if (low.dtype != torch.bfloat16 or tuple(low.shape) != (N, _low_dim(r))
+            or not low.is_contiguous()):
+        raise ValueError("low must be the tensor lora_linear returned for these rows")
+    dx = _aligned_rows(N, K, x) if need_dx else None
+    da = torch.empty((r, K), device=x.device, dtype=torch.bfloat16) if need_factors else None
+    db = torch.empty((M, r), device=x.device, dtype=torch.bfloat16) if need_factors else None
+    lib = _lib.load()
+    nb = lib.fa_lora_linear_bwd_workspace_bytes(N, r)
+    ws = torch.empty(nb, device=x.device, dtype=torch.uint8) if nb else None
+    ms = [_matrix(t, n) for t, n in ((x2, "x"), (w, "w"), (a, "a"), (b, "b"), (dy2, "dy"))]
+    mdx = _matrix(dx, "dx") if need_dx else None
+    with torch.cuda.device(x.device):
+        check(lib.fa_lora_linear_bwd(
+            FA_DTYPE_BF16, N, K, M, r, *[C.byref(m) for m in ms[:4]], float(scale), low.data_ptr(),
+            C.byref(ms[4]), _ref(mdx), _ptr(da), _ptr(db), _ptr(ws), nb, _on(x, stream)),
+            "fa_lora_linear_bwd")
+    if need_dx and x.dim() != 2:
+        dx = dx.view(*x.shape)
+    if need_factors and r != rank:
+        da, db = da[:rank], db[:, :rank]
+    return dx, da, db
+
+
+def lora_linear_many(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+                     ids: torch.Tensor, scales: torch.Tensor, *,
+                     bias: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """lora_linear for rows of many requests at once: a (E, rank, in),
+    b (E, out, rank), scales (E,) fp32, ids (rows,) int32 on the device; row i
+    uses adapter ids[i], and an id outside [0, E) means w alone. From one
+    token to packed prompts; ids in any order. Returns y."""
+    x2 = _rows2d(x, "x")
+    _check_lora(x2, w, a, b, bias, True)
+    _same_device(x, ids=ids, scales=scales)
+    if ids.dtype != torch.int32 or tuple(ids.shape) != (x2.shape[0],) or not ids.is_contiguous():
+        raise ValueError(f"ids must be a contiguous int32 ({x2.shape[0]},) tensor")
+    if (scales.dtype != torch.float32 or tuple(scales.shape) != (a.shape[0],)
+            or not scales.is_contiguous()):
+        raise ValueError(f"scales must be a contiguous float32 ({a.shape[0]},) tensor")
+    a, b = _pad_rank(a, b)
+    E, r = a.shape[0], a.shape[1]
+    N, K, M = x2.shape[0], w.shape[1], w.shape[0]
+    y = _aligned_rows(N, M, x)
+    lib = _lib.load()
+    nb = lib.fa_lora_linear_many_workspace_bytes(N, r)
+    ws = torch.empty(nb, device=x.device, dtype=torch.uint8) if nb else None
+    ms = [_matrix(t, n) for t, n in ((x2, "x"), (w, "w"), (a, "a"), (b, "b"), (y, "y"))]
+    with torch.cuda.device(x.device):
+        check(lib.fa_lora_linear_many(
+            FA_DTYPE_BF16, N, K, M, r, E, *[C.byref(m) for m in ms[:4]], ids.data_ptr(),
+            scales.data_ptr(), _ptr(bias), C.byref(ms[4]), _ptr(ws), nb, _on(x, stream)),
+            "fa_lora_linear_many")
+    return y.view(*x.shape[:-1], M) if x.dim() != 2 else y
 
 
 def device_status() -> int:

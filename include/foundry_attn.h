@@ -334,6 +334,79 @@ int fa_bwd_noalloc(int B, int S, int H, int D, const fa_tensor_t* q,
                    void* stream);
 
 /*
+ * Layer norm with an affine or adaptive output (bf16 or f32): the reference's
+ * layer_norm_mod (crates/foundry-spike/src/lib.rs:60-71) and its gradient.
+ * x, y, dy, dx are (groups, rows, 1, dim) tensors (stride_h unused; any group
+ * and row strides, dim contiguous). Per row, statistics in fp32:
+ *   h = (x - mean) / sqrt(var + eps),  y = h (off + weight) + bias,
+ * off = 1 with unit_offset (a modulation's scale), else 0. weight and bias
+ * (par_dtype; either may be NULL: 1 or 0 in place of off + weight or bias)
+ * hold `dim` entries per group, param_stride elements apart; 0: one for all
+ * groups. stats (may be NULL in the forward): fp32 (2, groups * rows), the
+ * means and 1 / sqrt(var + eps), which the backward reads. dim <= 16384.
+ * The backward writes dx and, when not NULL, dweight and dbias: fp32, (dim)
+ * when param_stride is 0, else (groups, dim), contiguous; identical bits
+ * across repeats. workspace: fa_layer_norm_bwd_workspace_bytes().
+ * Zero rows: dweight and dbias are zero.
+ */
+int fa_layer_norm_fwd(int dtype, int groups, int rows, int dim, const fa_tensor_t* x,
+                      const void* weight, const void* bias, int par_dtype, int64_t param_stride,
+                      int unit_offset, float eps, const fa_tensor_t* y, float* stats,
+                      void* stream);
+int fa_layer_norm_bwd(int dtype, int groups, int rows, int dim, const fa_tensor_t* x,
+                      const void* weight, int par_dtype, int64_t param_stride, int unit_offset,
+                      const fa_tensor_t* dy, const float* stats, const fa_tensor_t* dx,
+                      float* dweight, float* dbias, void* workspace, size_t workspace_bytes,
+                      void* stream);
+size_t fa_layer_norm_bwd_workspace_bytes(int groups, int rows, int dim);
+
+/* A strided (batch, rows, cols) bf16 device matrix with contiguous columns.
+ * Strides are in elements, multiples of 16 bytes; data is 16-byte aligned. */
+typedef struct {
+  void* data;
+  int64_t stride_batch;
+  int64_t stride_row;
+} fa_matrix_t;
+
+/*
+ * Linear with a low-rank adapter (bf16, fp32 sums; the reference's linear,
+ * crates/foundry-spike/src/lib.rs:270-287):
+ *   y = x W^T + bias + scale (x A^T) B^T
+ * x (rows, in_dim), w (out_dim, in_dim), a (rank, in_dim), b (out_dim, rank),
+ * y (rows, out_dim); bias (out_dim) bf16 or NULL. rank is a multiple of 8 up
+ * to 256 (pad smaller ones with zeros). `low` receives scale x A^T as bf16
+ * (rows, rank rounded up to 16), 16-byte aligned; the backward reads it.
+ * The backward, with W frozen, writes (each may be NULL, da and db together)
+ *   dx = dy W + U A,  da = U^T x (rank, in_dim),  db = dy^T low (out_dim, rank),
+ * U = scale dy B, in bf16, da and db contiguous; identical bits across
+ * repeats. workspace: fa_lora_linear_bwd_workspace_bytes(), 16-byte aligned.
+ */
+int fa_lora_linear_fwd(int dtype, int rows, int in_dim, int out_dim, int rank,
+                       const fa_matrix_t* x, const fa_matrix_t* w, const fa_matrix_t* a,
+                       const fa_matrix_t* b, float scale, const void* bias,
+                       const fa_matrix_t* y, void* low, void* stream);
+int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
+                       const fa_matrix_t* x, const fa_matrix_t* w, const fa_matrix_t* a,
+                       const fa_matrix_t* b, float scale, const void* low,
+                       const fa_matrix_t* dy, const fa_matrix_t* dx, void* da, void* db,
+                       void* workspace, size_t workspace_bytes, void* stream);
+size_t fa_lora_linear_bwd_workspace_bytes(int rows, int rank);
+
+/*
+ * The same forward for rows of many requests, each with its own adapter:
+ * a (n_adapters, rank, in_dim), b (n_adapters, out_dim, rank), `ids` (rows)
+ * int32 on the device: row i uses adapter ids[i] with scales[ids[i]] (fp32,
+ * n_adapters); an id outside [0, n_adapters) means the shared projection
+ * alone. The ids may be in any order; runs of equal ids are cheaper.
+ */
+int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, int n_adapters,
+                        const fa_matrix_t* x, const fa_matrix_t* w, const fa_matrix_t* a,
+                        const fa_matrix_t* b, const int32_t* ids, const float* scales,
+                        const void* bias, const fa_matrix_t* y, void* workspace,
+                        size_t workspace_bytes, void* stream);
+size_t fa_lora_linear_many_workspace_bytes(int rows, int rank);
+
+/*
  * Measurement hooks (no counterpart in the reference, which only wall-clocks
  * whole steps, bin/throughput.rs:868-873). While enabled, every launch of the
  * main forward (FA_TIMER_FWD) and backward (FA_TIMER_BWD) kernel is bracketed
