@@ -126,6 +126,11 @@ SIGNATURES = {
                                       _M, _M, C.c_void_p, _F, C.c_void_p, _M, C.c_void_p,
                                       C.c_size_t, C.c_void_p]),
     "fa_lora_linear_many_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "fa_orthogonalize": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int64,
+                                   C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_float,
+                                   C.c_float, C.c_float, C.c_float, C.c_void_p, C.c_size_t,
+                                   C.c_void_p]),
+    "fa_orthogonalize_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
     "fa_timing_enable": (C.c_int, [C.c_int]),
     "fa_timing_read": (C.c_int, [C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_int)]),
     "fa_status_string": (C.c_char_p, [C.c_int]),

@@ -32,7 +32,8 @@ NVCC_FLAGS = ARCH + [
 
 LIB_SOURCES = ["capi.cu", "attn_fwd_sm100.cu", "attn_bwd_sm100.cu", "attn_f32.cu", "misc.cu", "peer.cu",
                "qk_prologue.cu",
-               "layer_norm.cu", "gemm_wide_sm100.cu", "gemm_skinny_sm100.cu", "block_capi.cu",
+               "layer_norm.cu", "gemm_wide_sm100.cu", "gemm_skinny_sm100.cu",
+               "orthogonalize.cu", "block_capi.cu",
                "noalloc.cu"]
 # test infrastructure: the descriptor / operand-layout known-answer kernels
 SELFTEST_SOURCES = [ROOT / "tests" / "csrc" / "umma_selftest.cu"]

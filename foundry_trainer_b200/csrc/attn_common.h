@@ -30,9 +30,10 @@ enum KernelId {
   kKernelBwdBf16 = 1,
   kKernelF32Fwd = 2,
   kKernelF32Bwd = 3,
-  kKernelWide = 4,     // + 0..11: the wide product by operand layout, epilogue and tile
-  kKernelSkinny = 16,  // + 0..7
-  kKernelCount = 24
+  kKernelWide = 4,     // + 0..5: the wide product by operand layout and epilogue
+  kKernelSkinny = 10,  // + 0..4
+  kKernelThin = 15,    // + 0..11: the thin orthogonalisation by type, side and rank
+  kKernelCount = 27
 };
 
 // FA_OK when the last CUDA runtime call / launch on this thread succeeded;
@@ -172,6 +173,13 @@ int launch_layer_norm_bwd(int dtype, int groups, int rows, int dim, const fa_ten
                           const void* w, int par_dtype, int64_t par_stride, int unit_offset,
                           const fa_tensor_t* dy, const float* stats, const fa_tensor_t* dx,
                           float* dw, float* db, int shared, void* ws, cudaStream_t st);
+
+// Newton-Schulz orthogonalisation (orthogonalize.cu): g (batch, rows, cols)
+// in `dtype`, o bf16; strides in elements; c = (a, b, c)
+size_t orthogonalize_workspace(int batch, int rows, int cols, int steps);
+int launch_orthogonalize(int dtype, int batch, int rows, int cols, const void* g, int64_t gb,
+                         int64_t gr, void* o, int64_t ob, int64_t orow, int steps, const float* c,
+                         float eps, void* ws, cudaStream_t st);
 
 // Sequence-parallel exchange (peer.cu): bounded barrier over the ranks' flag
 // blocks, the owner's sum of received dK/dV contributions (dK un-rotated and

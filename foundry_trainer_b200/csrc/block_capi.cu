@@ -46,6 +46,7 @@ static int check_matrix(const fa_matrix_t* m) {
 }
 
 constexpr int kMaxRank = 256;
+constexpr int kMaxSteps = 64;
 
 static int check_lora(int dtype, int rows, int in_dim, int out_dim, int rank, float scale) {
   if (dtype != FA_DTYPE_BF16) return FA_ERR_UNSUPPORTED;
@@ -391,8 +392,47 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
   p.list_cnt = cnt;
   p.list_ids = list;
   p.slot = slot;
+  p.raw_x = bfp(x->data);
+  p.raw_ldx = x->stride_row;
+  p.raw_w = bfp(w->data);
+  p.raw_ldw = w->stride_row;
+  p.raw_f = bfp(b->data);
+  p.raw_fe = b->stride_batch;
+  p.raw_ldf = b->stride_row;
   p.bias = bfp(bias);
   return launch_gemm_wide(o, p, kEpiLinear, st);
+}
+
+size_t fa_orthogonalize_workspace_bytes(int batch, int rows, int cols, int steps) {
+  if (batch <= 0 || rows <= 0 || cols <= 0 || steps < 1 || steps > kMaxSteps) return 0;
+  return orthogonalize_workspace(batch, rows, cols, steps);
+}
+
+int fa_orthogonalize(int dtype, int batch, int rows, int cols, const void* g, int64_t g_stride_batch,
+                     int64_t g_stride_row, void* o, int64_t o_stride_batch, int64_t o_stride_row,
+                     int steps, float a, float b, float c, float eps, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  FA_TRY(check_dtype(dtype));
+  if (batch < 0 || rows <= 0 || cols <= 0 || steps < 1) return FA_ERR_INVALID_ARG;
+  if (steps > kMaxSteps || batch > 65535 || rows > (1 << 20) || cols > (1 << 20) ||
+      (int64_t)batch * ((rows + 255) / 256) * ((cols + 255) / 256) >= INT32_MAX)
+    return FA_ERR_TOO_LARGE;
+  if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c) || !(eps >= 0.f) ||
+      !std::isfinite(eps))
+    return FA_ERR_INVALID_ARG;
+  if (batch == 0) return FA_OK;
+  if (g == nullptr || o == nullptr) return FA_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(g) % (dtype == FA_DTYPE_BF16 ? 2 : 4) != 0 ||
+      reinterpret_cast<uintptr_t>(o) % 16 != 0 || o_stride_row % 8 != 0 || o_stride_batch % 8 != 0)
+    return FA_ERR_ALIGNMENT;
+  const size_t need = fa_orthogonalize_workspace_bytes(batch, rows, cols, steps);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return FA_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return FA_ERR_ALIGNMENT;
+  FA_TRY(check_sm100());
+  const float coef[3] = {a, b, c};
+  return launch_orthogonalize(dtype, batch, rows, cols, g, g_stride_batch, g_stride_row, o,
+                              o_stride_batch, o_stride_row, steps, coef, eps, workspace,
+                              reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

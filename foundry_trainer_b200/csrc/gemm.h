@@ -45,6 +45,11 @@ struct WideParams {
   const int* list_cnt = nullptr;
   const int* list_ids = nullptr;
   const int* slot = nullptr;
+  // plain views of A, B and the adapters (E, N, rank), for blocks of several
+  const __nv_bfloat16* raw_x = nullptr;
+  const __nv_bfloat16* raw_w = nullptr;
+  const __nv_bfloat16* raw_f = nullptr;
+  int64_t raw_ldx = 0, raw_ldw = 0, raw_fe = 0, raw_ldf = 0;
   const __nv_bfloat16* bias = nullptr;
   // orthogonalisation
   float alpha = 1.f;

@@ -127,6 +127,15 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
       : "memory");
 }
 
+// Warp-wide forms (sm100_ptx.cuh says why): one elected lane issues.
+__device__ __forceinline__ void umma_ss_pair_w(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                               uint32_t idesc, uint32_t accumulate) {
+  if (elect_one()) umma_ss_pair(d_tmem, a_desc, b_desc, idesc, accumulate);
+}
+__device__ __forceinline__ void umma_commit_pair_w(uint64_t* bar) {
+  if (elect_one()) umma_commit_pair(bar);
+}
+
 // Instruction descriptor, kind::f16, fp32 D: idesc_bf16's bits with the
 // element format of A and B (0 fp16, 1 bf16).
 __host__ __device__ constexpr uint32_t idesc_f16(int fmt, int M, int N, bool a_mn, bool b_mn) {

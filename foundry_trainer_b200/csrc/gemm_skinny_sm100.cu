@@ -135,22 +135,23 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
     }
   } else if (warp == 5) {
     const uint32_t idesc = idesc_f16(1, 128, n, BIG_MN, SMALL_MN);
+    const uint32_t base = smem_u32(smem);
+    const uint64_t a0 = BIG_MN ? mnmajor_desc(base, 0, 8192) : kmajor_desc(base, 0, 0);
+    const uint64_t b0 = SMALL_MN ? mnmajor_desc(base + kBig, 0, 8192)
+                                 : kmajor_desc(base + kBig, 0, 0);
     int s = 0;
     uint32_t ph = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
       if (!(ok = mbar_wait_w(&full[s], ph))) break;
       tc_fence_after();
-      const uint32_t a = smem_u32(smem + s * stage_bytes), b = a + kBig;
-      if (elect_one()) {
+      const uint64_t a = a0 + (uint32_t)(s * (stage_bytes >> 4));
+      const uint64_t b = b0 + (uint32_t)(s * (stage_bytes >> 4));
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          umma_ss(tmem, BIG_MN ? mnmajor_desc(a, kk, 8192) : kmajor_desc(a, kk, 0),
-                  SMALL_MN ? mnmajor_desc(b, kk, 8192) : kmajor_desc(b, kk, 0), idesc,
+      for (int kk = 0; kk < 4; ++kk)
+        umma_ss_w(tmem, a + (BIG_MN ? 128 : 2) * kk, b + (SMALL_MN ? 128 : 2) * kk, idesc,
                   kb > kb0 || kk > 0);
-        umma_commit(&empty[s]);
-        if (kb == kb1 - 1) umma_commit(done);
-      }
-      __syncwarp();
+      umma_commit_w(&empty[s]);
+      if (kb == kb1 - 1) umma_commit_w(done);
       if (++s == stages) { s = 0; ph ^= 1; }
     }
     if (!ok) *abort_flag = 1;
@@ -247,6 +248,10 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
           for (int q = 0; q < split; ++q) acc += recv[(q * own + j - j0) * 128 + r];
           p.out[(int64_t)i * p.out_ld + j - sl * p.low_ld] = __float2bfloat16_rn(acc * sc);
         }
+      } else if (p.slot != nullptr && p.slot[i] < 0 && s0 == 0 && part == 0) {
+        // a row without an adapter: zeros (a block whose other rows share one
+        // adapter is multiplied whole)
+        for (int j = 0; j < p.low_ld; ++j) p.out[(int64_t)i * p.out_ld + j] = __float2bfloat16_rn(0.f);
       }
     } else {
       for (int j = j0; j < min(j1, p.cols); ++j) {

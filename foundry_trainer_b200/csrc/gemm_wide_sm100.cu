@@ -7,13 +7,15 @@
 // symmetric matrix) or N-contiguous (B_MN: a weight in the backward, the
 // iterate of the orthogonalisation). fp32 accumulation, 16-bit operands.
 //
-// Bound by the tensor cores. A pair of CTAs (cta_group::2) owns a 256 x BN
-// tile: each stages its 128 rows of A and half of B's BN columns per 64-wide
+// Bound by the tensor cores. A pair of CTAs (cta_group::2) owns a 256 x kBN
+// tile: each stages its 128 rows of A and half of B's kBN columns per 64-wide
 // K block, so every staged byte of B feeds both SMs: per K block 32 KB land
-// and 16 KB + 16 KB are read per SM for 512 cycles of tensor work (BN = 256), below the
-// 128 bytes a cycle of shared memory that a single-CTA 128 x 256 tile exceeds.
+// and 32 KB are read per SM for 512 cycles of tensor work, within the 128
+// bytes a cycle of shared memory that a single-CTA 128 x 256 tile exceeds. A
+// 256 x 128 tile was measured to take as long as the 256 x 256 one, so there
+// is no narrower form.
 // The pair is persistent over tiles; the accumulator is double-buffered in
-// tensor memory (2 BN columns), so a tile's epilogue runs under the next
+// tensor memory (2 kBN columns), so a tile's epilogue runs under the next
 // tile's products.
 //   warps 0-3  epilogue: one row per thread
 //   warp 4     producer: TMA loads (one lane); builds the adapters' A operand
@@ -22,7 +24,8 @@
 // Adapters: a row's low-rank term is one more K block per adapter present in
 // the tile's 256 rows. Its A operand holds low[m, :] in the rows that use the
 // adapter and zeros elsewhere (written by the producer warp in the swizzled
-// layout TMA would have written); its B operand is the adapter's own matrix,
+// layout TMA would have written; by TMA itself where the block has one
+// adapter); its B operand is the adapter's own matrix,
 // loaded by TMA with zero fill past the rank. So the low-rank product costs
 // ceil(r / 16) tensor instructions a tile and no pass over D.
 #include <algorithm>
@@ -39,37 +42,34 @@ constexpr int kStageA = 16384;    // 128 rows x 64 elements
 constexpr int kStaging = 16384;   // epilogue tile: 128 rows x 64 elements
 constexpr int kBarBytes = 512;
 
-template <int BN>
-struct Cfg {
-  static constexpr int kStageB = BN / 2 * 128;
-  static constexpr int kStage = kStageA + kStageB;
-  static constexpr int kStages = BN == 256 ? 6 : 8;
-  static constexpr int kOffStaging = kStages * kStage;
-  static constexpr int kOffBar = kOffStaging + 2 * kStaging;
-  static constexpr int kSmem = kOffBar + kBarBytes + 1024;  // + alignment slack
-  static constexpr uint32_t kTmemCols = 2 * BN;
-};
-static_assert(Cfg<256>::kSmem <= 232448 && Cfg<128>::kSmem <= 232448, "shared memory");
+constexpr int kBN = 256;                     // columns of a tile
+constexpr int kStageB = kBN / 2 * 128;
+constexpr int kStage = kStageA + kStageB;
+constexpr int kStages = 6;
+constexpr int kOffStaging = kStages * kStage;
+constexpr int kOffBar = kOffStaging + 2 * kStaging;
+constexpr int kSmem = kOffBar + kBarBytes + 1024;  // + alignment slack
+constexpr uint32_t kTmemCols = 2 * kBN;
+static_assert(kSmem <= 232448, "shared memory");
 
 struct Tile {
-  int m, n, b;  // 256-row block, BN-column block, batch
+  int m, n, b;  // 256-row block, kBN-column block, batch
 };
 
 // Tile t of the walk: eight row blocks high columns first, so that the pairs
 // at work at one time share their A rows and B columns in L2. Products with a
 // symmetric result visit only the tiles on or below the diagonal.
-__device__ __forceinline__ Tile tile_of(int64_t t, const WideParams& p, int BN) {
+__device__ __forceinline__ Tile tile_of(int64_t t, const WideParams& p) {
   Tile o;
   o.b = (int)(t / p.tiles_per_batch);
   int i = (int)(t - (int64_t)o.b * p.tiles_per_batch);
   if (p.symmetric) {
-    // row block m has (m + 1) * (256 / BN) column blocks (cut at tiles_n)
-    const int per = 256 / BN;
-    int m = (int)((sqrtf(8.f * (float)(i / per) + 1.f) - 1.f) * 0.5f);
-    while ((int64_t)per * (m + 1) * (m + 2) / 2 <= i) ++m;
-    while ((int64_t)per * m * (m + 1) / 2 > i) --m;
+    // row block m has the column blocks 0 .. m
+    int m = (int)((sqrtf(8.f * (float)i + 1.f) - 1.f) * 0.5f);
+    while ((int64_t)(m + 1) * (m + 2) / 2 <= i) ++m;
+    while ((int64_t)m * (m + 1) / 2 > i) --m;
     o.m = m;
-    o.n = i - per * (m * (m + 1) / 2);
+    o.n = i - m * (m + 1) / 2;
     return o;
   }
   constexpr int kHigh = 8;
@@ -87,19 +87,37 @@ __device__ __forceinline__ int slots_of(const WideParams& p, int m) {
   return p.list_cnt != nullptr ? p.list_cnt[m] : 1;
 }
 
-template <int BN, bool B_MN, int EPI>
+// One output value from its own row's operands alone. Only for values that a
+// block of several adapters left non-finite: there a row's zeros in another
+// adapter's K block met a NaN or infinity of that adapter (0 x inf = NaN).
+__device__ __noinline__ float one_value(const WideParams& p, int row, int col, int m) {
+  const __nv_bfloat16* x = p.raw_x + (int64_t)row * p.raw_ldx;
+  const __nv_bfloat16* w = p.raw_w + (int64_t)col * p.raw_ldw;
+  float acc = 0.f;
+  for (int k = 0; k < p.K; ++k) acc = fmaf(__bfloat162float(x[k]), __bfloat162float(w[k]), acc);
+  const int s = p.slot[row];
+  if (s >= 0) {
+    const __nv_bfloat16* f = p.raw_f + (int64_t)p.list_ids[(int64_t)m * 256 + s] * p.raw_fe +
+                             (int64_t)col * p.raw_ldf;
+    const __nv_bfloat16* l = p.low + (int64_t)row * p.low_ld;
+    for (int k = 0; k < p.rank; ++k) acc = fmaf(__bfloat162float(l[k]), __bfloat162float(f[k]), acc);
+  }
+  return acc;
+}
+
+template <bool B_MN, int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
-            const __grid_constant__ CUtensorMap te, const __grid_constant__ CUtensorMap td,
+            const __grid_constant__ CUtensorMap te, const __grid_constant__ CUtensorMap tl_low,
+            const __grid_constant__ CUtensorMap td,
             const __grid_constant__ CUtensorMap td2, const __grid_constant__ WideParams p) {
-  using C = Cfg<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
   uint64_t* full = bars;                      // leader's is used
-  uint64_t* empty = bars + C::kStages;        // both
-  uint64_t* accfull = bars + 2 * C::kStages;  // both
+  uint64_t* empty = bars + kStages;        // both
+  uint64_t* accfull = bars + 2 * kStages;  // both
   uint64_t* accempty = accfull + 2;           // leader's is used
   uint32_t* slot = reinterpret_cast<uint32_t*>(accempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
@@ -108,7 +126,7 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
   const bool leader = rank == 0;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::kStages; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 2);
       mbar_init(&empty[i], 1);
     }
@@ -123,7 +141,7 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
     tma_prefetch_desc(&td);
   }
   if (warp == 5) {
-    tmem_alloc_pair(slot, C::kTmemCols);
+    tmem_alloc_pair(slot, kTmemCols);
     tmem_relinquish_pair();
   }
   tc_fence_before();
@@ -136,7 +154,7 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
   const int pairs = gridDim.x >> 1;
   const int kb_main = (p.K + 63) >> 6;
   const int kb_ext = (p.rank + 63) >> 6;  // per slot
-  constexpr int kHalfN = BN / 2;
+  constexpr int kHalfN = kBN / 2;
 
   if (warp == 4) {
     // ------------------------------------------------------------- producer
@@ -144,18 +162,38 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
     int s = 0;
     uint32_t ph = 0;
     for (int64_t t = blockIdx.x >> 1; t < tiles && ok; t += pairs) {
-      const Tile tl = tile_of(t, p, BN);
+      const Tile tl = tile_of(t, p);
       const int row0 = tl.m * 256 + (int)rank * 128;
-      const int col0 = tl.n * BN + (int)rank * kHalfN;
+      const int col0 = tl.n * kBN + (int)rank * kHalfN;
+      // A tile of several adapters: this CTA's rows of low and their slots are
+      // fetched now, under the main blocks, and kept while the rank is at most
+      // 32 (16 registers of 16 bytes a lane); each adapter's operand is then
+      // stores alone. Fetched per adapter instead they cost 14 us a tile.
+      const int ns = EPI == kEpiLinear ? slots_of(p, tl.m) : 0;
+      constexpr int kHold = EPI == kEpiLinear ? 16 : 1;
+      uint4 hold[kHold];
+      int hold_slot[kHold];
+      const int chunks = p.low_ld >> 3, lg = chunks == 4 ? 2 : 1;
+      const bool held = EPI == kEpiLinear && (chunks == 2 || chunks == 4);
+      if (ns > 1 && held) {
+#pragma unroll
+        for (int i = 0; i < kHold; ++i) {
+          const int r = (i * 32 + lane) >> lg, c = lane & (chunks - 1), row = row0 + r;
+          const bool in = r < 128 && row < p.M;
+          hold_slot[i] = in ? p.slot[row] : -1;
+          hold[i] = in ? __ldcg(reinterpret_cast<const uint4*>(p.low + (int64_t)row * p.low_ld + c * 8))
+                       : make_uint4(0, 0, 0, 0);
+        }
+      }
       for (int kb = 0; kb < kb_main; ++kb) {
-        if (!(ok = mbar_wait_cluster_w(&empty[s], ph ^ 1))) break;
-        uint8_t* sa = smem + s * C::kStage;
+        if (!(ok = mbar_wait_w(&empty[s], ph ^ 1))) break;
+        uint8_t* sa = smem + s * kStage;
         uint8_t* sb = sa + kStageA;
         if (lane == 0) {
           const uint32_t fb = mapa(smem_u32(&full[s]), 0);
           if (leader) {
-            mbar_arrive_expect_tx(&full[s], 2 * C::kStage);
-            mbar_arrive(&full[s]);  // the second arrival is the other CTA's in adapter blocks
+            mbar_arrive_expect_tx(&full[s], 2 * kStage);
+            mbar_arrive(&full[s]);  // the second arrival: the other CTA's where it builds A
           }
           tma_load_3d_pair(sa, &ta, fb, kb * 64, row0, tl.b);
           if constexpr (B_MN) {
@@ -166,33 +204,52 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
             tma_load_3d_pair(sb, &tb, fb, kb * 64, col0, tl.b);
           }
         }
-        if (++s == C::kStages) { s = 0; ph ^= 1; }
+        if (++s == kStages) { s = 0; ph ^= 1; }
       }
-      if (!ok || p.low == nullptr) continue;
-      const int ns = slots_of(p, tl.m);
+      if (!ok || ns == 0) continue;
       for (int q = 0; q < ns && ok; ++q) {
         const int e = p.list_ids != nullptr ? p.list_ids[(int64_t)tl.m * 256 + q] : 0;
         for (int j = 0; j < kb_ext; ++j) {
-          if (!(ok = mbar_wait_cluster_w(&empty[s], ph ^ 1))) break;
-          uint8_t* sa = smem + s * C::kStage;
+          if (!(ok = mbar_wait_w(&empty[s], ph ^ 1))) break;
+          uint8_t* sa = smem + s * kStage;
           uint8_t* sb = sa + kStageA;
-          // rows that use adapter e: their low values; the others: zeros
-          const int cols = min(64, p.low_ld - j * 64);
-#pragma unroll 4
-          for (int i = lane; i < 1024; i += 32) {
-            const int r = i >> 3, c = i & 7, row = row0 + r;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (row < p.M && c * 8 < cols && (p.slot == nullptr || p.slot[row] == q))
-              v = __ldcg(reinterpret_cast<const uint4*>(p.low + (int64_t)row * p.low_ld + j * 64 +
-                                                        c * 8));
-            *reinterpret_cast<uint4*>(sa + sw128_offset(r, c)) = v;
+          if (ns > 1) {
+            // rows that use adapter e: their low values; the others: zeros
+            if (held) {
+#pragma unroll
+              for (int i = 0; i < kHold; ++i) {
+                const int r = (i * 32 + lane) >> lg, c = lane & (chunks - 1);
+                if (r < 128)
+                  *reinterpret_cast<uint4*>(sa + sw128_offset(r, c)) =
+                      hold_slot[i] == q ? hold[i] : make_uint4(0, 0, 0, 0);
+              }
+            } else {
+#pragma unroll 8
+              for (int i = lane; i < 1024; i += 32) {
+                const int r = i >> 3, c = i & 7, row = row0 + r;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (row < p.M && j * 64 + c * 8 < p.low_ld && p.slot[row] == q)
+                  v = __ldcg(reinterpret_cast<const uint4*>(p.low + (int64_t)row * p.low_ld +
+                                                            j * 64 + c * 8));
+                *reinterpret_cast<uint4*>(sa + sw128_offset(r, c)) = v;
+              }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
           }
-          fence_proxy_async_smem();
-          __syncwarp();
           if (lane == 0) {
             const uint32_t fb = mapa(smem_u32(&full[s]), 0);
-            if (leader) mbar_arrive_expect_tx(&full[s], 2 * C::kStageB);
-            else mbar_arrive_cluster(fb);
+            if (ns > 1) {
+              if (leader) mbar_arrive_expect_tx(&full[s], 2 * kStageB);
+              else mbar_arrive_cluster(fb);
+            } else {
+              // one adapter: rows without it hold zeros in low already
+              if (leader) {
+                mbar_arrive_expect_tx(&full[s], 2 * kStage);
+                mbar_arrive(&full[s]);
+              }
+              tma_load_3d_pair(sa, &tl_low, fb, j * 64, row0, 0);
+            }
             if constexpr (B_MN) {
 #pragma unroll
               for (int i = 0; i < kHalfN / 64; ++i)
@@ -201,7 +258,7 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
               tma_load_3d_pair(sb, &te, fb, j * 64, col0, e);
             }
           }
-          if (++s == C::kStages) { s = 0; ph ^= 1; }
+          if (++s == kStages) { s = 0; ph ^= 1; }
         }
       }
     }
@@ -209,33 +266,42 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
   } else if (warp == 5) {
     // ------------------------------------------------------------ tcgen05
     if (leader) {
-      const uint32_t idesc = idesc_f16(p.fmt, 256, BN, false, B_MN);
+      const uint32_t idesc = idesc_f16(p.fmt, 256, kBN, false, B_MN);
+      const uint64_t a0 = kmajor_desc(smem_u32(smem), 0, 0);
+      const uint64_t b0 = B_MN ? mnmajor_desc(smem_u32(smem) + kStageA, 0, 8192)
+                               : kmajor_desc(smem_u32(smem) + kStageA, 0, 0);
+      constexpr uint32_t kStepB = B_MN ? 128 : 2;  // 16 K rows of 128 bytes, or 32 bytes
       bool ok = true;
       int s = 0, it = 0;
       uint32_t ph = 0;
       for (int64_t t = blockIdx.x >> 1; t < tiles && ok; t += pairs, ++it) {
-        const Tile tl = tile_of(t, p, BN);
+        const Tile tl = tile_of(t, p);
         const int buf = it & 1;
-        const uint32_t d = tmem + buf * BN;
-        if (!(ok = mbar_wait_cluster_w(&accempty[buf], ((it >> 1) & 1) ^ 1))) break;
+        const uint32_t d = tmem + buf * kBN;
+        if (!(ok = mbar_wait_w(&accempty[buf], ((it >> 1) & 1) ^ 1))) break;
         tc_fence_after();
         const int nkb = kb_main + slots_of(p, tl.m) * kb_ext;
         for (int kb = 0; kb < nkb; ++kb) {
-          if (!(ok = mbar_wait_cluster_w(&full[s], ph))) break;
+          // cluster scope where the other CTA may have built its operand
+          if (!(ok = kb < kb_main ? mbar_wait_w(&full[s], ph) : mbar_wait_cluster_w(&full[s], ph)))
+            break;
           tc_fence_after();
-          const uint32_t a = smem_u32(smem + s * C::kStage), b = a + kStageA;
-          int steps = 4;
-          if (kb >= kb_main) steps = min(4, (p.rank - ((kb - kb_main) % kb_ext) * 64 + 15) >> 4);
-          if (elect_one()) {
+          // the whole warp runs the loop with uniform descriptors: stage and
+          // K slice are additions to their 16-byte address fields
+          const uint64_t a = a0 + (uint32_t)(s * (kStage >> 4));
+          const uint64_t b = b0 + (uint32_t)(s * (kStage >> 4));
+          if (kb < kb_main) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_ss_pair_w(d, a + 2 * kk, b + kStepB * kk, idesc, kb > 0 || kk > 0);
+          } else {
+            const int steps = min(4, (p.rank - ((kb - kb_main) % kb_ext) * 64 + 15) >> 4);
             for (int kk = 0; kk < steps; ++kk)
-              umma_ss_pair(d, kmajor_desc(a, kk, 0),
-                           B_MN ? mnmajor_desc(b, kk, 8192) : kmajor_desc(b, kk, 0), idesc,
-                           kb > 0 || kk > 0);
-            umma_commit_pair(&empty[s]);
-            if (kb == nkb - 1) umma_commit_pair(&accfull[buf]);
+              umma_ss_pair_w(d, a + 2 * kk, b + kStepB * kk, idesc, 1);
           }
-          __syncwarp();
-          if (++s == C::kStages) { s = 0; ph ^= 1; }
+          umma_commit_pair_w(&empty[s]);
+          if (kb == nkb - 1) umma_commit_pair_w(&accfull[buf]);
+          if (++s == kStages) { s = 0; ph ^= 1; }
         }
       }
       if (!ok) *abort_flag = 1;
@@ -246,10 +312,11 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
     int it = 0;
     const int r = threadIdx.x;  // 0..127: the tile row and tensor-memory lane
     const uint32_t lane_off = (uint32_t)(warp * 32) << 16;
-    uint8_t* stg = smem + C::kOffStaging;
+    uint8_t* stg = smem + kOffStaging;
     float ca = 0.f, cb = 0.f;
+    const bool bias_vec = (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0;
     for (int64_t t = blockIdx.x >> 1; t < tiles; t += pairs, ++it) {
-      const Tile tl = tile_of(t, p, BN);
+      const Tile tl = tile_of(t, p);
       const int buf = it & 1;
       const int row0 = tl.m * 256 + (int)rank * 128, row = row0 + r;
       const bool live = row < p.M;
@@ -261,21 +328,48 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
       ok = mbar_wait_w(&accfull[buf], (it >> 1) & 1);
       if (!ok) break;
       tc_fence_after();
-      const bool mirror = p.symmetric && tl.n * BN + BN <= tl.m * 256;
+      // a block of several adapters: its rows must not see each other's
+      const bool mixed = EPI == kEpiLinear && p.raw_x != nullptr && slots_of(p, tl.m) > 1;
+      const bool mirror = p.symmetric && tl.n < tl.m;
 #pragma unroll 1
-      for (int c = 0; c < BN / 64; ++c) {
-        const int col0 = tl.n * BN + c * 64;
+      for (int c = 0; c < kBN / 64; ++c) {
+        const int col0 = tl.n * kBN + c * 64;
         uint32_t acc[64];
-        tmem_ld32(tmem + lane_off + buf * BN + c * 64, acc);
-        tmem_ld32(tmem + lane_off + buf * BN + c * 64 + 32, acc + 32);
+        tmem_ld32(tmem + lane_off + buf * kBN + c * 64, acc);
+        tmem_ld32(tmem + lane_off + buf * kBN + c * 64 + 32, acc + 32);
         float* v = reinterpret_cast<float*>(acc);
         uint32_t lo[EPI == kEpiUpdate ? 32 : 1];
         if constexpr (EPI == kEpiLinear) {
           tmem_wait_ld();
-          if (p.bias != nullptr) {
+          if (mixed) {
+            // zero times a non-finite entry of another row's adapter
+            float z = 0.f;
 #pragma unroll
-            for (int i = 0; i < 64; ++i)
-              if (col0 + i < p.N) v[i] += __bfloat162float(p.bias[col0 + i]);
+            for (int i = 0; i < 64; ++i) z = fmaf(v[i], 0.f, z);
+            if (z != 0.f && live) {
+#pragma unroll
+              for (int i = 0; i < 64; ++i)
+                if (!isfinite(v[i]) && col0 + i < p.N) v[i] = one_value(p, row, col0 + i, tl.m);
+            }
+          }
+          if (p.bias != nullptr) {
+            if (bias_vec && col0 + 64 <= p.N) {
+              const uint4* b4 = reinterpret_cast<const uint4*>(p.bias + col0);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const uint4 w = __ldg(b4 + i);
+                const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                  v[8 * i + 2 * u] += bf16_lo(ww[u]);
+                  v[8 * i + 2 * u + 1] += bf16_hi(ww[u]);
+                }
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 64; ++i)
+                if (col0 + i < p.N) v[i] += __bfloat162float(p.bias[col0 + i]);
+            }
           }
 #pragma unroll
           for (int i = 0; i < 32; ++i) acc[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
@@ -396,63 +490,53 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
   if (warp == 5) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc_pair(tmem, C::kTmemCols);
+    tmem_dealloc_pair(tmem, kTmemCols);
   }
 }
 
-template <int BN, bool B_MN, int EPI>
+template <bool B_MN, int EPI>
 static int go(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& te,
-              const CUtensorMap& td, const CUtensorMap& td2, const WideParams& p, int kernel_id,
+              const CUtensorMap& tlow, const CUtensorMap& td, const CUtensorMap& td2, const WideParams& p, int kernel_id,
               cudaStream_t st) {
-  auto* fn = wide_kernel<BN, B_MN, EPI>;
-  const int rc = ensure_smem_attr((const void*)fn, Cfg<BN>::kSmem, kernel_id);
+  auto* fn = wide_kernel<B_MN, EPI>;
+  const int rc = ensure_smem_attr((const void*)fn, kSmem, kernel_id);
   if (rc) return rc;
   const int64_t tiles = (int64_t)p.tiles_per_batch * p.batch;
   const int pairs = (int)std::min<int64_t>(tiles, 74);
-  fn<<<2 * pairs, kThreads, Cfg<BN>::kSmem, st>>>(ta, tb, te, td, td2, p);
+  fn<<<2 * pairs, kThreads, kSmem, st>>>(ta, tb, te, tlow, td, td2, p);
   return launch_status();
 }
 
 }  // namespace wide
 
 int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t st) {
+  using wide::kBN;
   if (p.M == 0 || p.N == 0 || p.batch == 0) return FA_OK;
-  // 256-wide tiles, unless 128-wide ones fill the 74 SM pairs better: the
-  // cost of a walk is its rounds over the pairs times the tile's width
-  auto count = [&](int bn) -> int64_t {
-    const int tm = (p.M + 255) / 256, tn = (p.N + bn - 1) / bn;
-    if (!p.symmetric) return (int64_t)tm * tn;
-    const int per = 256 / bn;
-    int64_t n = 0;
-    for (int m = 0; m < tm; ++m) n += std::min((m + 1) * per, tn);
-    return n;
-  };
-  const int64_t r256 = (count(256) * p.batch + 73) / 74, r128 = (count(128) * p.batch + 73) / 74;
-  const int bn = r128 < 2 * r256 ? 128 : 256;
   p.tiles_m = (p.M + 255) / 256;
-  p.tiles_n = (p.N + bn - 1) / bn;
-  p.tiles_per_batch = (int)count(bn);
-  CUtensorMap ta, tb, te, td, td2;
+  p.tiles_n = (p.N + kBN - 1) / kBN;
+  p.tiles_per_batch = p.symmetric ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
+  CUtensorMap ta, tb, te, tlow, td, td2;
   int rc = make_tmap_3d(&ta, o.a, 64, 128);
-  if (!rc) rc = o.b_mn ? make_tmap_3d(&tb, o.b, 64, 64) : make_tmap_3d(&tb, o.b, 64, bn / 2);
+  if (!rc) rc = o.b_mn ? make_tmap_3d(&tb, o.b, 64, 64) : make_tmap_3d(&tb, o.b, 64, kBN / 2);
   te = tb;
   if (!rc && p.low != nullptr)
-    rc = o.b_mn ? make_tmap_3d(&te, o.e, 64, 64) : make_tmap_3d(&te, o.e, 64, bn / 2);
+    rc = o.b_mn ? make_tmap_3d(&te, o.e, 64, 64) : make_tmap_3d(&te, o.e, 64, kBN / 2);
+  tlow = ta;
+  if (!rc && p.low != nullptr)
+    rc = make_tmap_3d(&tlow, Mat3{p.low, 1, p.M, p.low_ld, 0, p.low_ld, 1}, 64, 128);
   td = ta;
   if (!rc && o.d.p != nullptr) rc = make_tmap_3d(&td, o.d, 64, 128);
   td2 = td;
   if (!rc && o.d2.p != nullptr) rc = make_tmap_3d(&td2, o.d2, 64, 128);
   if (rc) return rc;
 #define FA_WIDE(EPI, MN, ID)                                                                  \
-  if (epi == EPI && o.b_mn == MN)                                                             \
-    return bn == 256 ? wide::go<256, MN, EPI>(ta, tb, te, td, td2, p, ID, st)                 \
-                     : wide::go<128, MN, EPI>(ta, tb, te, td, td2, p, ID + 1, st);
+  if (epi == EPI && o.b_mn == MN) return wide::go<MN, EPI>(ta, tb, te, tlow, td, td2, p, ID, st);
   FA_WIDE(kEpiLinear, false, kKernelWide)
-  FA_WIDE(kEpiLinear, true, kKernelWide + 2)
-  FA_WIDE(kEpiGram, false, kKernelWide + 4)
-  FA_WIDE(kEpiPoly, false, kKernelWide + 6)
-  FA_WIDE(kEpiUpdate, true, kKernelWide + 8)
-  FA_WIDE(kEpiLast, true, kKernelWide + 10)
+  FA_WIDE(kEpiLinear, true, kKernelWide + 1)
+  FA_WIDE(kEpiGram, false, kKernelWide + 2)
+  FA_WIDE(kEpiPoly, false, kKernelWide + 3)
+  FA_WIDE(kEpiUpdate, true, kKernelWide + 4)
+  FA_WIDE(kEpiLast, true, kKernelWide + 5)
 #undef FA_WIDE
   return FA_ERR_UNSUPPORTED;
 }

@@ -1,0 +1,588 @@
+// orthogonalize.cu — Newton-Schulz orthogonalisation of an update matrix.
+//
+//   X_0 = G / (|G|_F + eps),   X_{k+1} = a X_k + (b Q + c Q^2) X_k,  Q = X_k X_k^T
+//
+// pushes every singular value of G towards one: the result approximates the
+// orthogonal factor of G's polar decomposition, the step direction of an
+// optimiser that treats a weight as a linear map. Two forms, by the short
+// side r of the matrix:
+//
+// r <= 64 (the factors of adapters), thin_kernel. All X_k are X_k = P_k X_0
+// with P_k a polynomial in the r x r Gram matrix Q_0 of X_0, and everything
+// commutes: with M = a + b Q + c Q^2, P <- M P and Q <- M Q M. So the long
+// side is read for Q_0 and once more (from L2) for P X_0, and all steps stay
+// on chip. Forming Q_0 squares the singular values, so it, and the steps, are
+// in fp64: a direction of relative strength 1e-3 is 1e-6 in Q_0, of which fp32
+// sums would leave a digit, while P amplifies it 485-fold. One cluster per
+// matrix: its CTAs sum their parts of Q_0, exchange them through distributed
+// shared memory in CTA order, run the same steps, and each applies P to its
+// own part of the long side.
+//
+// r > 64: three tensor-core products a step (gemm_wide_sm100.cu; both Gram
+// products compute the tiles on and below the diagonal and mirror them).
+// Operands are fp16, not bf16: after the normalisation every quantity is
+// bounded by about one, so eleven bits are worth more than range (a factor
+// 256 on X and 64 on Q keep small entries clear of fp16's subnormals). What
+// must not be rounded to 11 bits is X itself, since a rounding of X is noise
+// in all directions and the following steps amplify it up to 485-fold where
+// G has no strength. X is therefore kept as the sum of two fp16 matrices, hi
+// and lo (22 bits); the products read hi, and the epilogue adds a (hi + lo)
+// in fp32. Errors of the products stay within G's own directions, where the
+// steps contract. Against 64 bits: 2.3e-3 of the result's norm on Gaussian
+// noise, 1.7e-3 on a few strong directions over noise; the final rounding to
+// bf16 alone is 1.7e-3.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "attn_common.h"
+#include "gemm.h"
+#include "gemm_ptx.cuh"
+
+namespace fa {
+namespace ns {
+
+constexpr int kThinThreads = 512;
+
+template <typename T>
+__device__ __forceinline__ float ld_f(const T* p);
+template <>
+__device__ __forceinline__ float ld_f<float>(const float* p) { return __ldg(p); }
+template <>
+__device__ __forceinline__ float ld_f<__nv_bfloat16>(const __nv_bfloat16* p) {
+  return __bfloat162float(*p);
+}
+
+__device__ __forceinline__ double ld_cluster_f64(uint32_t addr) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// Tile t of the upper triangle of an n x n tile grid, row-major: (i, j), i <= j
+__device__ __forceinline__ void upper_tile(int t, int n, int& i, int& j) {
+  i = 0;
+  while (t >= n - i) t -= n - i++;
+  j = i + t;
+}
+
+template <int R>
+struct Thin {
+  static constexpr int kLong = 4096 / R;              // long positions staged at a time
+  static constexpr int kStage = kLong * (R + 1) * 8;  // padded: no 32-way bank conflicts
+  static constexpr int kMat = R * R * 8;
+  static constexpr int kSmem = 4 * kMat + kStage + 16;
+  static constexpr int kTs = R / 16;                  // Gram tile a thread: kTs x kTs
+  static constexpr int kTiles = 136;                  // 16 * 17 / 2
+  static constexpr int kGroups = kThinThreads / kTiles;
+  static constexpr int kTm = R == 64 ? 2 : 1;         // tile of the r x r products
+};
+
+// dst = alpha X Y + beta Z + gamma I for symmetric commuting R x R matrices:
+// the upper triangle is summed and mirrored.
+template <int R>
+__device__ __forceinline__ void sym_product(double* dst, const double* X, const double* Y,
+                                            double alpha, const double* Z, double beta,
+                                            double gamma) {
+  constexpr int TM = Thin<R>::kTm, N = R / TM;
+  for (int t = threadIdx.x; t < N * (N + 1) / 2; t += kThinThreads) {
+    int i, j;
+    upper_tile(t, N, i, j);
+    i *= TM;
+    j *= TM;
+    double acc[TM][TM];
+#pragma unroll
+    for (int u = 0; u < TM; ++u)
+#pragma unroll
+      for (int v = 0; v < TM; ++v) acc[u][v] = 0.0;
+#pragma unroll 8
+    for (int k = 0; k < R; ++k) {
+      double x[TM], y[TM];
+#pragma unroll
+      for (int u = 0; u < TM; ++u) x[u] = X[k * R + i + u], y[u] = Y[k * R + j + u];
+#pragma unroll
+      for (int u = 0; u < TM; ++u)
+#pragma unroll
+        for (int v = 0; v < TM; ++v) acc[u][v] = fma(x[u], y[v], acc[u][v]);
+    }
+#pragma unroll
+    for (int u = 0; u < TM; ++u)
+#pragma unroll
+      for (int v = 0; v < TM; ++v) {
+        const int p = i + u, q = j + v;
+        double d = alpha * acc[u][v];
+        if (Z != nullptr) d += beta * Z[p * R + q];
+        if (p == q) d += gamma;
+        if (p <= q) {
+          dst[p * R + q] = d;
+          dst[q * R + p] = d;
+        }
+      }
+  }
+}
+
+// One cluster per matrix (blockIdx.x / parts). TALL: the long side is the rows.
+template <typename T, int R, bool TALL>
+__global__ void __launch_bounds__(kThinThreads, 1)
+thin_kernel(const T* g, int64_t g_batch, int64_t g_row, __nv_bfloat16* o, int64_t o_batch,
+            int64_t o_row, int r, int len, int parts, int steps, double ca, double cb, double cc,
+            double eps) {
+  using C = Thin<R>;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  double* A = reinterpret_cast<double*>(smem_raw);
+  double* M = A + R * R;
+  double* P = M + R * R;
+  double* Q = P + R * R;
+  double* stage = Q + R * R;
+  const int mat = blockIdx.x / parts, part = blockIdx.x - mat * parts;
+  const T* gm = g + (int64_t)mat * g_batch;
+  // this CTA's share of the long side
+  const int l0 = (int)((int64_t)len * part / parts), l1 = (int)((int64_t)len * (part + 1) / parts);
+  const int tid = threadIdx.x;
+
+  // ---- Gram matrix of the share: kGroups sets of threads take every
+  // kGroups-th position, each thread a kTs x kTs tile of the upper triangle
+  const int grp = tid / C::kTiles, tile = tid - grp * C::kTiles;
+  int ti, tj;
+  upper_tile(tile, 16, ti, tj);
+  ti *= C::kTs;
+  tj *= C::kTs;
+  double acc[C::kTs][C::kTs];
+#pragma unroll
+  for (int u = 0; u < C::kTs; ++u)
+#pragma unroll
+    for (int v = 0; v < C::kTs; ++v) acc[u][v] = 0.0;
+  for (int l = l0; l < l1; l += C::kLong) {
+    const int n = min(C::kLong, l1 - l);
+#pragma unroll
+    for (int k = 0; k < 4096 / kThinThreads; ++k) {
+      const int idx = tid + k * kThinThreads;
+      const int ll = TALL ? idx / R : idx % C::kLong, j = TALL ? idx % R : idx / C::kLong;
+      float v = 0.f;
+      if (ll < n && j < r)
+        v = ld_f<T>(TALL ? gm + (int64_t)(l + ll) * g_row + j : gm + (int64_t)j * g_row + l + ll);
+      stage[ll * (R + 1) + j] = (double)v;
+    }
+    __syncthreads();
+    if (grp < C::kGroups) {
+#pragma unroll 4
+      for (int k = grp; k < n; k += C::kGroups) {
+        const double* row = stage + k * (R + 1);
+        double x[C::kTs], y[C::kTs];
+#pragma unroll
+        for (int u = 0; u < C::kTs; ++u) x[u] = row[ti + u], y[u] = row[tj + u];
+#pragma unroll
+        for (int u = 0; u < C::kTs; ++u)
+#pragma unroll
+          for (int v = 0; v < C::kTs; ++v) acc[u][v] = fma(x[u], y[v], acc[u][v]);
+      }
+    }
+    __syncthreads();
+  }
+  // groups join in order (their tiles pass through M and P), then the CTAs
+  // of the cluster (through Q)
+  constexpr int kTt = C::kTs * C::kTs;
+  static_assert(C::kGroups * C::kTiles * kTt <= 2 * R * R, "group sums fit M and P");
+  if (grp < C::kGroups) {
+#pragma unroll
+    for (int u = 0; u < kTt; ++u)
+      M[(grp * C::kTiles + tile) * kTt + u] = acc[u / C::kTs][u % C::kTs];
+  }
+  __syncthreads();
+  for (int i = tid; i < C::kTiles * kTt; i += kThinThreads) {
+    double s = 0.0;
+    for (int k = 0; k < C::kGroups; ++k) s += M[k * C::kTiles * kTt + i];
+    Q[i] = s;
+  }
+  if (parts > 1) cluster_sync();
+  else __syncthreads();
+  for (int i = tid; i < C::kTiles * kTt; i += kThinThreads) {
+    double s = 0.0;
+    if (parts > 1) {
+      const uint32_t at = smem_u32(Q + i);
+      for (int k = 0; k < parts; ++k) s += ld_cluster_f64(mapa(at, k));
+    } else {
+      s = Q[i];
+    }
+    int p, q;
+    upper_tile(i / kTt, 16, p, q);
+    p = p * C::kTs + (i % kTt) / C::kTs;
+    q = q * C::kTs + (i % kTt) % C::kTs;
+    if (p <= q) A[p * R + q] = A[q * R + p] = s;
+  }
+  if (parts > 1) cluster_sync();  // nobody reads another CTA's memory after this
+  else __syncthreads();
+  double tr = 0.0;
+  for (int i = 0; i < R; ++i) tr += A[i * R + i];
+  const double inv = 1.0 / (sqrt(tr) + eps);
+  __syncthreads();
+  for (int i = tid; i < R * R; i += kThinThreads) A[i] *= inv * inv;
+  __syncthreads();
+
+  // ---- the steps
+  for (int s = 0; s < steps; ++s) {
+    sym_product<R>(M, A, A, cc, A, cb, ca);
+    __syncthreads();
+    if (s == 0) {
+      for (int i = tid; i < R * R; i += kThinThreads) P[i] = M[i];
+    } else {
+      sym_product<R>(Q, M, P, 1.0, nullptr, 0.0, 0.0);
+      double* t = P;
+      P = Q;
+      Q = t;
+    }
+    if (s + 1 == steps) break;
+    __syncthreads();
+    sym_product<R>(Q, A, M, 1.0, nullptr, 0.0, 0.0);
+    __syncthreads();
+    sym_product<R>(A, Q, M, 1.0, nullptr, 0.0, 0.0);
+    __syncthreads();
+  }
+  __syncthreads();
+  // P / |G| in fp32 (its largest entries are a few hundred times the
+  // result's: 24 bits leave the bf16 result its own rounding)
+  float* pf = reinterpret_cast<float*>(stage);
+  for (int i = tid; i < R * R; i += kThinThreads) pf[i] = (float)(P[i] * inv);
+  __syncthreads();
+
+  // ---- O = P G over the share, a long position per thread
+  __nv_bfloat16* om = o + (int64_t)mat * o_batch;
+  for (int l = l0 + tid; l < l1; l += kThinThreads) {
+    uint64_t sum[R / 2];
+#pragma unroll
+    for (int i = 0; i < R / 2; ++i) sum[i] = 0;
+#pragma unroll 4
+    for (int j = 0; j < r; ++j) {
+      const float x = ld_f<T>(TALL ? gm + (int64_t)l * g_row + j : gm + (int64_t)j * g_row + l);
+      const uint64_t xx = f2_pack(x, x);
+      const ulonglong2* pr = reinterpret_cast<const ulonglong2*>(pf + j * R);
+#pragma unroll
+      for (int i = 0; i < R / 4; ++i) {
+        const ulonglong2 w = pr[i];
+        sum[2 * i] = ffma2(w.x, xx, sum[2 * i]);
+        sum[2 * i + 1] = ffma2(w.y, xx, sum[2 * i + 1]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R / 2; ++i) {
+      float u, v;
+      f2_unpack(sum[i], u, v);
+      if constexpr (TALL) {
+        if (2 * i < r) om[(int64_t)l * o_row + 2 * i] = __float2bfloat16_rn(u);
+        if (2 * i + 1 < r) om[(int64_t)l * o_row + 2 * i + 1] = __float2bfloat16_rn(v);
+      } else {
+        if (2 * i < r) om[(int64_t)(2 * i) * o_row + l] = __float2bfloat16_rn(u);
+        if (2 * i + 1 < r) om[(int64_t)(2 * i + 1) * o_row + l] = __float2bfloat16_rn(v);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------ the wide form
+
+constexpr int kNormBlocks = 256;  // partial sums of squares per matrix
+
+// part[mat][block] = sum of squares over every kNormBlocks-th row, in fp64 (the
+// squares of fp32 values may leave fp32's range). `vec`: 16-byte loads.
+template <typename T>
+__global__ void __launch_bounds__(256)
+norm_kernel(const T* g, int64_t g_batch, int64_t g_row, int m, int n, int vec, double* part) {
+  __shared__ double red[8];
+  constexpr int E = 16 / sizeof(T);
+  const int mat = blockIdx.y;
+  const T* gm = g + (int64_t)mat * g_batch;
+  double s = 0.0;
+  for (int i = blockIdx.x; i < m; i += kNormBlocks) {
+    const T* row = gm + (int64_t)i * g_row;
+    int done = 0;
+    if (vec) {
+      done = n / E * E;
+#pragma unroll 4
+      for (int j = threadIdx.x * E; j < done; j += 256 * E) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(row + j));
+        const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+          const double v = (double)(float)e[k];
+          s = fma(v, v, s);
+        }
+      }
+    }
+    for (int j = done + threadIdx.x; j < n; j += 256) {
+      const double v = (double)ld_f<T>(row + j);
+      s = fma(v, v, s);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane_id() == 0) red[warp_id()] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) s += red[i];
+    part[(int64_t)mat * kNormBlocks + blockIdx.x] = s;
+  }
+}
+
+// |G| + eps = nu 2^e, 1 <= nu < 2, from the partial sums (256 threads)
+__device__ __forceinline__ double norm_of(const double* part, double eps, int* e) {
+  __shared__ double red[8];
+  double s = part[threadIdx.x];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (lane_id() == 0) red[warp_id()] = s;
+  __syncthreads();
+  s = red[0];
+  for (int i = 1; i < 8; ++i) s += red[i];
+  const double v = sqrt(s) + eps;
+  *e = isfinite(v) && v > 0.0 ? ilogb(v) : 0;
+  return scalbn(v, -*e);
+}
+
+// X_0 nu 256 = G 2^(8 - e) as fp16 hi + lo / 2048 (a power of two: exact for
+// bf16 inputs in range), transposed when the input is tall. 64 x 64 tiles.
+// Block (0, 0) of a matrix also writes its coefficients: the division by nu is
+// folded into the first step's. coef: (steps, 2 (Q then X), batch, 2).
+template <typename T, bool TALL>
+__global__ void __launch_bounds__(256)
+split_kernel(const T* g, int64_t g_batch, int64_t g_row, int m, int n, const double* part,
+             double eps, __half* hi, __half* lo, int ld, int64_t x_batch, float* coef, int batch,
+             int steps, double ca, double cb, double cc) {
+  __shared__ float tile[64][65];
+  const int mat = blockIdx.z;
+  int e;
+  const double nu = norm_of(part + (int64_t)mat * kNormBlocks, eps, &e);
+  const float scale = (float)scalbn(1.0, 8 - e);
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < steps) {
+    const int s = threadIdx.x;
+    const double v = s == 0 ? nu : 1.0;
+    float* q = coef + ((int64_t)(2 * s) * batch + mat) * 2;
+    q[0] = (float)(cb / (v * v * v));
+    q[1] = (float)(cc / (v * v * v * v * v) / 64.0);
+    float* x = coef + ((int64_t)(2 * s + 1) * batch + mat) * 2;
+    x[0] = (float)(ca / v);
+    x[1] = 1.f / 64.f;
+  }
+  const T* gm = g + (int64_t)mat * g_batch;
+  const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
+  const int c = threadIdx.x & 63;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int r = (threadIdx.x >> 6) + 4 * k;
+    float v = 0.f;
+    if (i0 + r < m && j0 + c < n) v = ld_f<T>(gm + (int64_t)(i0 + r) * g_row + j0 + c);
+    tile[r][c] = v * scale;
+  }
+  __syncthreads();
+  // two columns a thread
+  const int rows = TALL ? n : m, cols = TALL ? m : n;  // of X
+  const int r0 = TALL ? j0 : i0, c0 = TALL ? i0 : j0;
+  const int cp = (threadIdx.x & 31) * 2;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int r = (threadIdx.x >> 5) + 8 * k;
+    if (r0 + r < rows && c0 + cp < cols) {
+      const float u = TALL ? tile[cp][r] : tile[r][cp], v = TALL ? tile[cp + 1][r] : tile[r][cp + 1];
+      const uint32_t h = pack_f16(u, v);
+      const float2 hf = unpack_f16(h);
+      const int64_t at = (int64_t)mat * x_batch + (int64_t)(r0 + r) * ld + c0 + cp;
+      *reinterpret_cast<uint32_t*>(hi + at) = h;  // ld is even: a last odd column has its pad
+      *reinterpret_cast<uint32_t*>(lo + at) = pack_f16((u - hf.x) * 2048.f, (v - hf.y) * 2048.f);
+    }
+  }
+}
+
+static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+static int ld8(int n) { return (n + 7) / 8 * 8; }
+
+struct Space {  // workspace of the wide form
+  size_t part, coef, x, q, total;
+};
+
+static Space space_of(int batch, int m, int n, int steps) {
+  Space s{};
+  s.part = align256((size_t)batch * kNormBlocks * 8);
+  s.coef = align256((size_t)batch * steps * 4 * 4);
+  s.x = align256((size_t)batch * m * ld8(n) * 2);
+  s.q = align256((size_t)batch * m * ld8(m) * 2);
+  s.total = s.part + s.coef + 3 * s.x + 2 * s.q;
+  return s;
+}
+
+template <typename T, int R, bool TALL>
+static int thin_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, int64_t orow,
+                   int batch, int r, int len, int steps, const float* c, float eps, int kid,
+                   cudaStream_t st) {
+  auto* fn = thin_kernel<T, R, TALL>;
+  const int rc = ensure_smem_attr((const void*)fn, Thin<R>::kSmem, kid);
+  if (rc) return rc;
+  // a CTA for every 256 positions, eight at most
+  const int parts = std::max(1, std::min(8, (len + 255) / 256));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(batch * parts));
+  cfg.blockDim = dim3(kThinThreads);
+  cfg.dynamicSmemBytes = Thin<R>::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = parts;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(
+      &cfg, fn, reinterpret_cast<const T*>(g), gb, gr, reinterpret_cast<__nv_bfloat16*>(o), ob,
+      orow, r, len, parts, steps, (double)c[0], (double)c[1], (double)c[2], (double)eps);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return record_cuda_error(e);
+  }
+  return launch_status();
+}
+
+template <typename T, bool TALL>
+static int thin_pick(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, int64_t orow,
+                     int batch, int r, int len, int steps, const float* c, float eps, int kid,
+                     cudaStream_t st) {
+  if (r <= 16)
+    return thin_go<T, 16, TALL>(g, gb, gr, o, ob, orow, batch, r, len, steps, c, eps, kid, st);
+  if (r <= 32)
+    return thin_go<T, 32, TALL>(g, gb, gr, o, ob, orow, batch, r, len, steps, c, eps, kid + 1, st);
+  return thin_go<T, 64, TALL>(g, gb, gr, o, ob, orow, batch, r, len, steps, c, eps, kid + 2, st);
+}
+
+template <typename T>
+static int wide_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, int64_t orow,
+                   int batch, int rows, int cols, int steps, const float* c, float eps, void* ws,
+                   cudaStream_t st) {
+  const bool tall = rows > cols;
+  const int m = std::min(rows, cols), n = std::max(rows, cols);
+  const Space sp = space_of(batch, m, n, steps);
+  uint8_t* w = reinterpret_cast<uint8_t*>(ws);
+  double* part = reinterpret_cast<double*>(w);
+  w += sp.part;
+  float* coef = reinterpret_cast<float*>(w);
+  w += sp.coef;
+  __half* hi[2];
+  hi[0] = reinterpret_cast<__half*>(w);
+  w += sp.x;
+  hi[1] = reinterpret_cast<__half*>(w);
+  w += sp.x;
+  __half* lo = reinterpret_cast<__half*>(w);
+  w += sp.x;
+  __half* q = reinterpret_cast<__half*>(w);
+  w += sp.q;
+  __half* pq = reinterpret_cast<__half*>(w);
+  const int ldx = ld8(n), ldq = ld8(m);
+  const int64_t xb = (int64_t)m * ldx, qb = (int64_t)m * ldq;
+  const T* gp = reinterpret_cast<const T*>(g);
+  const int vec = reinterpret_cast<uintptr_t>(g) % 16 == 0 && gb * (int)sizeof(T) % 16 == 0 &&
+                  gr * (int)sizeof(T) % 16 == 0;
+  norm_kernel<T><<<dim3(kNormBlocks, batch), 256, 0, st>>>(gp, gb, gr, rows, cols, vec, part);
+  int rc = launch_status();
+  if (rc) return rc;
+  const dim3 tiles((cols + 63) / 64, (rows + 63) / 64, batch);
+  if (tall)
+    split_kernel<T, true><<<tiles, 256, 0, st>>>(gp, gb, gr, rows, cols, part, eps, hi[0], lo, ldx,
+                                                 xb, coef, batch, steps, c[0], c[1], c[2]);
+  else
+    split_kernel<T, false><<<tiles, 256, 0, st>>>(gp, gb, gr, rows, cols, part, eps, hi[0], lo, ldx,
+                                                  xb, coef, batch, steps, c[0], c[1], c[2]);
+  rc = launch_status();
+  if (rc) return rc;
+  auto x_mat = [&](const __half* p) { return Mat3{p, batch, m, n, xb, ldx, 0}; };
+  auto q_mat = [&](const __half* p) { return Mat3{p, batch, m, m, qb, ldq, 0}; };
+  for (int s = 0; s < steps; ++s) {
+    const __half* h = hi[s & 1];
+    {  // Q 64 = (256 X)(256 X)^T / 1024
+      WideOperands op;
+      op.a = op.b = x_mat(h);
+      op.d = q_mat(q);
+      WideParams p;
+      p.M = p.N = m;
+      p.K = n;
+      p.batch = batch;
+      p.fmt = 0;
+      p.symmetric = 1;
+      p.alpha = 1.f / 1024.f;
+      p.sym_out = q;
+      p.sym_batch = qb;
+      p.sym_ld = ldq;
+      if ((rc = launch_gemm_wide(op, p, kEpiGram, st))) return rc;
+    }
+    {  // (b Q + c Q^2) 64
+      WideOperands op;
+      op.a = op.b = q_mat(q);
+      op.d = q_mat(pq);
+      WideParams p;
+      p.M = p.N = p.K = m;
+      p.batch = batch;
+      p.fmt = 0;
+      p.symmetric = 1;
+      p.coef = coef + (int64_t)(2 * s) * batch * 2;
+      p.in_hi = q;
+      p.in_batch = qb;
+      p.in_ld = ldq;
+      p.sym_out = pq;
+      p.sym_batch = qb;
+      p.sym_ld = ldq;
+      if ((rc = launch_gemm_wide(op, p, kEpiPoly, st))) return rc;
+    }
+    const bool last = s + 1 == steps;
+    WideOperands op;
+    op.b_mn = true;
+    op.a = q_mat(pq);
+    op.b = x_mat(h);
+    WideParams p;
+    p.M = p.K = m;
+    p.N = n;
+    p.batch = batch;
+    p.fmt = 0;
+    p.coef = coef + (int64_t)(2 * s + 1) * batch * 2;
+    p.in_hi = h;
+    p.in_lo = lo;
+    p.in_batch = xb;
+    p.in_ld = ldx;
+    if (!last) {
+      op.d = x_mat(hi[(s + 1) & 1]);
+      op.d2 = x_mat(lo);
+    } else {
+      p.alpha = 1.f / 256.f;
+      if (tall) {
+        p.out_t = reinterpret_cast<uint16_t*>(o);
+        p.out_t_batch = ob;
+        p.out_t_ld = orow;
+      } else {
+        op.d = Mat3{o, batch, m, n, ob, orow, 1};
+      }
+    }
+    if ((rc = launch_gemm_wide(op, p, last ? kEpiLast : kEpiUpdate, st))) return rc;
+  }
+  return FA_OK;
+}
+
+constexpr int kThinMost = 64;
+
+}  // namespace ns
+
+size_t orthogonalize_workspace(int batch, int rows, int cols, int steps) {
+  const int m = std::min(rows, cols), n = std::max(rows, cols);
+  return m <= ns::kThinMost ? 0 : ns::space_of(batch, m, n, steps).total;
+}
+
+int launch_orthogonalize(int dtype, int batch, int rows, int cols, const void* g, int64_t gb,
+                         int64_t gr, void* o, int64_t ob, int64_t orow, int steps, const float* c,
+                         float eps, void* ws, cudaStream_t st) {
+  const bool bf = dtype == FA_DTYPE_BF16, tall = rows > cols;
+  const int m = std::min(rows, cols), n = std::max(rows, cols);
+  if (m > ns::kThinMost)
+    return bf ? ns::wide_go<__nv_bfloat16>(g, gb, gr, o, ob, orow, batch, rows, cols, steps, c, eps, ws, st)
+              : ns::wide_go<float>(g, gb, gr, o, ob, orow, batch, rows, cols, steps, c, eps, ws, st);
+  const int kid = kKernelThin + (bf ? 0 : 6) + (tall ? 3 : 0);
+#define FA_THIN(T, TALL) \
+  ns::thin_pick<T, TALL>(g, gb, gr, o, ob, orow, batch, m, n, steps, c, eps, kid, st)
+  if (bf) return tall ? FA_THIN(__nv_bfloat16, true) : FA_THIN(__nv_bfloat16, false);
+  return tall ? FA_THIN(float, true) : FA_THIN(float, false);
+#undef FA_THIN
+}
+
+}  // namespace fa

@@ -229,9 +229,25 @@ def qk_norm_rope_bwd(x_txt, x_img, w_txt, w_img, rope: Optional[Rope], dy: torch
 
 # --------------------------------------------------------- block operators
 
-def _on(t: torch.Tensor, stream) -> int:
-    """The stream to launch on: `stream`, or the current one of t's device."""
-    return (stream if stream is not None else torch.cuda.current_stream(t.device)).cuda_stream
+def _launch(fn, where: str, t: torch.Tensor, stream, temps, *args) -> None:
+    """fn(*args, stream) with t's device current, on `stream` or the current
+    stream of that device. `temps` are the call's own buffers: on a stream of
+    the caller's they are kept until it has passed them."""
+    dev = t.get_device()
+    if stream is None:
+        ptr = torch._C._cuda_getCurrentRawStream(dev)
+    else:
+        ptr = stream.cuda_stream
+        for b in temps:
+            if b is not None:
+                b.record_stream(stream)
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, ptr)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, ptr)
+    if rc:
+        check(rc, where)
 
 
 def _same_device(ref: torch.Tensor, **tensors) -> None:
@@ -304,11 +320,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     y = torch.empty_like(x) if out is None else out
     _check_norm_x(x, out=y)
     stats = torch.empty((2, G * R), device=x.device, dtype=torch.float32)
-    with torch.cuda.device(x.device):
-        check(_lib.load().fa_layer_norm_fwd(
-            dt, G, R, D, C.byref(_norm_desc(x)), _ptr(w), _ptr(b), pdt, ps, int(unit_offset),
-            float(eps), C.byref(_norm_desc(y)), stats.data_ptr(), _on(x, stream)),
-            "fa_layer_norm_fwd")
+    _launch(_lib.load().fa_layer_norm_fwd, "fa_layer_norm_fwd", x, stream, (w, b), dt, G, R, D,
+            C.byref(_norm_desc(x)), _ptr(w), _ptr(b), pdt, ps, int(unit_offset), float(eps),
+            C.byref(_norm_desc(y)), stats.data_ptr())
     return y, stats
 
 
@@ -332,11 +346,9 @@ def layer_norm_bwd(x: torch.Tensor, weight: Optional[torch.Tensor], dy: torch.Te
     lib = _lib.load()
     nb = lib.fa_layer_norm_bwd_workspace_bytes(G, R, D)
     ws = torch.empty(nb, device=x.device, dtype=torch.uint8) if nb else None
-    with torch.cuda.device(x.device):
-        check(lib.fa_layer_norm_bwd(
-            dt, G, R, D, C.byref(_norm_desc(x)), _ptr(w), pdt, ps, int(unit_offset),
-            C.byref(_norm_desc(dy)), stats.data_ptr(), C.byref(_norm_desc(dx)), _ptr(dw), _ptr(db),
-            _ptr(ws), nb, _on(x, stream)), "fa_layer_norm_bwd")
+    _launch(lib.fa_layer_norm_bwd, "fa_layer_norm_bwd", x, stream, (w, ws), dt, G, R, D,
+            C.byref(_norm_desc(x)), _ptr(w), pdt, ps, int(unit_offset), C.byref(_norm_desc(dy)),
+            stats.data_ptr(), C.byref(_norm_desc(dx)), _ptr(dw), _ptr(db), _ptr(ws), nb)
     return dx, dw, db
 
 
@@ -416,10 +428,9 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.Tens
     y = _aligned_rows(N, M, x)
     low = torch.empty((N, _low_dim(r)), device=x.device, dtype=torch.bfloat16)
     ms = [_matrix(t, n) for t, n in ((x2, "x"), (w, "w"), (a, "a"), (b, "b"), (y, "y"))]
-    with torch.cuda.device(x.device):
-        check(_lib.load().fa_lora_linear_fwd(
-            FA_DTYPE_BF16, N, K, M, r, *[C.byref(m) for m in ms[:4]], float(scale), _ptr(bias),
-            C.byref(ms[4]), low.data_ptr(), _on(x, stream)), "fa_lora_linear_fwd")
+    _launch(_lib.load().fa_lora_linear_fwd, "fa_lora_linear_fwd", x, stream, (a, b), FA_DTYPE_BF16,
+            N, K, M, r, *[C.byref(m) for m in ms[:4]], float(scale), _ptr(bias), C.byref(ms[4]),
+            low.data_ptr())
     return y.view(*x.shape[:-1], M) if x.dim() != 2 else y, low
 
 
@@ -449,11 +460,9 @@ def lora_linear_bwd(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.
     ws = torch.empty(nb, device=x.device, dtype=torch.uint8) if nb else None
     ms = [_matrix(t, n) for t, n in ((x2, "x"), (w, "w"), (a, "a"), (b, "b"), (dy2, "dy"))]
     mdx = _matrix(dx, "dx") if need_dx else None
-    with torch.cuda.device(x.device):
-        check(lib.fa_lora_linear_bwd(
-            FA_DTYPE_BF16, N, K, M, r, *[C.byref(m) for m in ms[:4]], float(scale), low.data_ptr(),
-            C.byref(ms[4]), _ref(mdx), _ptr(da), _ptr(db), _ptr(ws), nb, _on(x, stream)),
-            "fa_lora_linear_bwd")
+    _launch(lib.fa_lora_linear_bwd, "fa_lora_linear_bwd", x, stream, (a, b, ws), FA_DTYPE_BF16, N, K,
+            M, r, *[C.byref(m) for m in ms[:4]], float(scale), low.data_ptr(), C.byref(ms[4]),
+            _ref(mdx), _ptr(da), _ptr(db), _ptr(ws), nb)
     if need_dx and x.dim() != 2:
         dx = dx.view(*x.shape)
     if need_factors and r != rank:
@@ -484,12 +493,52 @@ def lora_linear_many(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch
     nb = lib.fa_lora_linear_many_workspace_bytes(N, r)
     ws = torch.empty(nb, device=x.device, dtype=torch.uint8) if nb else None
     ms = [_matrix(t, n) for t, n in ((x2, "x"), (w, "w"), (a, "a"), (b, "b"), (y, "y"))]
-    with torch.cuda.device(x.device):
-        check(lib.fa_lora_linear_many(
-            FA_DTYPE_BF16, N, K, M, r, E, *[C.byref(m) for m in ms[:4]], ids.data_ptr(),
-            scales.data_ptr(), _ptr(bias), C.byref(ms[4]), _ptr(ws), nb, _on(x, stream)),
-            "fa_lora_linear_many")
+    _launch(lib.fa_lora_linear_many, "fa_lora_linear_many", x, stream, (a, b, ws), FA_DTYPE_BF16, N,
+            K, M, r, E, *[C.byref(m) for m in ms[:4]], ids.data_ptr(), scales.data_ptr(),
+            _ptr(bias), C.byref(ms[4]), _ptr(ws), nb)
     return y.view(*x.shape[:-1], M) if x.dim() != 2 else y
+
+
+NS_COEFFS = (3.4445, -4.7750, 2.0315)  # five steps take [0.005, 1] to about [0.7, 1.2]
+
+
+def orthogonalize(g: torch.Tensor, *, steps: int = 5, coeffs=NS_COEFFS, eps: float = 1e-7,
+                  out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """Newton-Schulz orthogonalisation of the matrices g (..., m, n), bf16 or
+    f32: X = g / (|g|_F + eps), then `steps` times X = a X + (b Q + c Q^2) X
+    with Q = X X^T (of the transpose when m > n). Returns bf16, (..., m, n):
+    a step's direction, whose singular values the iteration itself leaves
+    spread by some 20 percent. Identical bits across repeats."""
+    if g.dim() < 2:
+        raise ValueError(f"expected (..., m, n), got {tuple(g.shape)}")
+    _same_device(g, out=out)
+    dt = _dtype_code(g)
+    m, n = g.shape[-2:]
+    try:
+        g3 = g.view(-1, m, n) if g.numel() else g.reshape(-1, m, n)
+    except RuntimeError:
+        raise ValueError("the leading dimensions must be one strided set of matrices; "
+                         "reshape g first") from None
+    if n > 1 and g3.stride(-1) != 1:
+        raise ValueError("g's last dimension must be contiguous")
+    B = g3.shape[0]
+    if out is None:
+        o3 = _aligned_rows(B * m, n, g).unflatten(0, (B, m))
+    else:
+        if out.shape != g.shape or out.dtype != torch.bfloat16:
+            raise ValueError("out must be bf16 with g's shape")
+        o3 = out.view(-1, m, n)
+        if n > 1 and o3.stride(-1) != 1:
+            raise ValueError("out's last dimension must be contiguous")
+    mo = _matrix(o3, "out")
+    a, b, c = (float(v) for v in coeffs)
+    lib = _lib.load()
+    nb = lib.fa_orthogonalize_workspace_bytes(B, m, n, int(steps))
+    ws = torch.empty(nb, device=g.device, dtype=torch.uint8) if nb else None
+    _launch(lib.fa_orthogonalize, "fa_orthogonalize", g, stream, (ws,), dt, B, m, n, g3.data_ptr(),
+            g3.stride(0), g3.stride(1), mo.data, mo.stride_batch, mo.stride_row, int(steps), a, b,
+            c, float(eps), _ptr(ws), nb)
+    return o3.view(g.shape) if out is None else out
 
 
 def device_status() -> int:

@@ -407,6 +407,23 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
 size_t fa_lora_linear_many_workspace_bytes(int rows, int rank);
 
 /*
+ * Newton-Schulz orthogonalisation of update matrices: for each of `batch`
+ * (rows, cols) matrices G in `dtype` (f32 or bf16; columns contiguous),
+ *   X = G / (|G|_F + eps);  steps times: X = a X + (b Q + c Q^2) X, Q = X X^T
+ * (on the transposed matrix when rows > cols), written to o as bf16 (columns
+ * contiguous, 16-byte aligned, strides multiples of 8). Singular values have
+ * to stay below about 100 for the given a, b, c (fp16 operands); 1 <= steps
+ * <= 64. Identical bits across repeats. workspace:
+ * fa_orthogonalize_workspace_bytes() (0 while the short side is at most 64),
+ * 16-byte aligned. No counterpart in the reference, whose optimiser is AdamW.
+ */
+int fa_orthogonalize(int dtype, int batch, int rows, int cols, const void* g,
+                     int64_t g_stride_batch, int64_t g_stride_row, void* o,
+                     int64_t o_stride_batch, int64_t o_stride_row, int steps, float a, float b,
+                     float c, float eps, void* workspace, size_t workspace_bytes, void* stream);
+size_t fa_orthogonalize_workspace_bytes(int batch, int rows, int cols, int steps);
+
+/*
  * Measurement hooks (no counterpart in the reference, which only wall-clocks
  * whole steps, bin/throughput.rs:868-873). While enabled, every launch of the
  * main forward (FA_TIMER_FWD) and backward (FA_TIMER_BWD) kernel is bracketed
