@@ -33,7 +33,8 @@ enum KernelId {
   kKernelWide = 4,     // + 0..5: the wide product by operand layout and epilogue
   kKernelSkinny = 10,  // + 0..4
   kKernelThin = 15,    // + 0..11: the thin orthogonalisation by type, side and rank
-  kKernelCount = 27
+  kKernelNorm = 27,    // + 0..11: the ring layer norm by direction, type and width
+  kKernelCount = 39
 };
 
 // FA_OK when the last CUDA runtime call / launch on this thread succeeded;
@@ -204,5 +205,6 @@ int f32_device_status();
 int misc_device_status();
 int qkp_device_status();
 int peer_device_status();
+int norm_device_status();
 
 }  // namespace fa

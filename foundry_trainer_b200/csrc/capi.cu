@@ -279,7 +279,7 @@ int fa_device_status(void) {
   int first = 0;
   for (int v : {fwd_device_status(), bwd_device_status(), f32_device_status(),
                 misc_device_status(), qkp_device_status(), peer_device_status(),
-                wide_device_status(), skinny_device_status()}) {
+                norm_device_status(), wide_device_status(), skinny_device_status()}) {
     if (v < 0) return FA_ERR_LAUNCH;
     if (first == 0) first = v;
   }

@@ -15,12 +15,21 @@
 // once. dw and db are summed in registers by the thread that owns the column,
 // over the rows of its block, and joined in block order by a second kernel:
 // the same bits every time. All sums are fp32.
+//
+// Two forms of each. The ring form (rows of at least 1 KB whose starts are
+// 16-byte aligned) keeps the next rows on their way while a block reduces the
+// present ones: one thread copies whole rows into a ring in shared memory
+// (cp.async.bulk), every thread takes its columns of R rows from there, and
+// the block barrier of the rows' sums also tells that thread that the slot is
+// free. Loads straight into registers were latency-bound: at 4608 x 2048 bf16
+// forward 18.5 us, backward 24 us. The direct form serves every other width,
+// stride and alignment, and the forward's smallest calls.
 #include <cuda_bf16.h>
 
 #include <algorithm>
 
 #include "attn_common.h"
-#include "sm100_ptx.cuh"
+#include "gemm_ptx.cuh"
 
 namespace fa {
 namespace ln {
@@ -100,6 +109,27 @@ __device__ __forceinline__ void load_par(const void* base, int64_t at, int bf16,
   }
 }
 
+// V vectors of E parameters from column c on, `step` columns apart. One branch
+// on the type around all the loads, so that they are in flight together.
+template <int E, int V>
+__device__ __forceinline__ void load_pars(const void* base, int64_t at, int bf16, float none, int c,
+                                          int step, int dim, float (*e)[E]) {
+  if (base != nullptr && bf16) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (c + v * step < dim) load_par<E>(base, at + c + v * step, 1, none, e[v]);
+  } else if (base != nullptr) {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (c + v * step < dim) load_par<E>(base, at + c + v * step, 0, none, e[v]);
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int i = 0; i < E; ++i) e[v][i] = none;
+  }
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -144,6 +174,9 @@ fwd_kernel(Mat x, Mat y, Par par, int64_t n_rows, int rows, int dim, float eps, 
       for (int i = 0; i < E; ++i) e[v][i] = 0.f;
     }
   }
+  float w[V][E], b[V][E];
+  load_pars<E, V>(par.w, g * par.stride, par.bf16, 1.f - par.off, t * E, team * E, dim, w);
+  load_pars<E, V>(par.b, g * par.stride, par.bf16, 0.f, t * E, team * E, dim, b);
   float s = 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v)
@@ -171,11 +204,9 @@ fwd_kernel(Mat x, Mat y, Par par, int64_t n_rows, int rows, int dim, float eps, 
   for (int v = 0; v < V; ++v) {
     const int c = (t + v * team) * E;
     if (c < dim) {
-      float w[E], b[E], o[E];
-      load_par<E>(par.w, g * par.stride + c, par.bf16, 1.f - par.off, w);
-      load_par<E>(par.b, g * par.stride + c, par.bf16, 0.f, b);
+      float o[E];
 #pragma unroll
-      for (int i = 0; i < E; ++i) o[i] = fmaf(e[v][i] * rstd, par.off + w[i], b[i]);
+      for (int i = 0; i < E; ++i) o[i] = fmaf(e[v][i] * rstd, par.off + w[v][i], b[v][i]);
       store_e<T, E>(yr + c, o);
     }
   }
@@ -353,24 +384,388 @@ bwd_kernel(Mat x, Mat dy, Mat dx, Par par, const float* stats, int64_t n_rows, i
   }
 }
 
+// ------------------------------------------------------------- ring form
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// The 16 bytes of a row as E / 2 pairs of fp32, for the two-lane arithmetic:
+// the kernels' instructions, not memory, set the pace of scalar code here
+// (0.6 instructions issued a cycle at 4.0 TB/s; forward 162 us and backward
+// 211 us at 36864 x 4096 bf16).
+template <int E>
+__device__ __forceinline__ void pairs_of(const uint4& v, uint64_t* e) {
+  if constexpr (E == 4) {
+    e[0] = f2_pack(__uint_as_float(v.x), __uint_as_float(v.y));
+    e[1] = f2_pack(__uint_as_float(v.z), __uint_as_float(v.w));
+  } else {
+    e[0] = f2_pack(bf16_lo(v.x), bf16_hi(v.x));
+    e[1] = f2_pack(bf16_lo(v.y), bf16_hi(v.y));
+    e[2] = f2_pack(bf16_lo(v.z), bf16_hi(v.z));
+    e[3] = f2_pack(bf16_lo(v.w), bf16_hi(v.w));
+  }
+}
+__device__ __forceinline__ uint64_t twice(float v) { return f2_pack(v, v); }
+__device__ __forceinline__ float f2_sum(uint64_t v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a + b;
+}
+template <typename T, int E>
+__device__ __forceinline__ void store_pairs(T* p, const uint64_t* e) {
+  float f[E];
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) f2_unpack(e[i], f[2 * i], f[2 * i + 1]);
+  store_e<T, E>(p, f);
+}
+
+constexpr int kMaxStages = 4;
+
+// A ring of `stages` slots of R rows of each of NT tensors; row bytes `rb`.
+template <int R, int NT>
+struct Ring {
+  uint8_t* base;
+  uint64_t* full;
+  int stages, rb, nb, r0, r1;
+  const uint8_t* src[NT];
+  int64_t step[NT];  // bytes from row to row
+
+  __device__ __forceinline__ int rows(int it) const { return min(R, r1 - r0 - it * R); }
+  __device__ __forceinline__ const uint8_t* slot(int s) const { return base + s * NT * R * rb; }
+  // one thread: turn `it` into slot s
+  __device__ __forceinline__ void issue(int it, int s) const {
+    const int n = rows(it);
+    mbar_arrive_expect_tx(&full[s], (uint32_t)(NT * n * rb));
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      for (int k = 0; k < n; ++k)
+        bulk_load(base + ((s * NT + t) * R + k) * rb, src[t] + (int64_t)(r0 + it * R + k) * step[t],
+                  (uint32_t)rb, &full[s]);
+  }
+  __device__ __forceinline__ void start() const {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < stages; ++i) mbar_init(&full[i], 1);
+      fence_mbar_init();
+      for (int it = 0; it < min(stages, nb); ++it) issue(it, it);
+    }
+    __syncthreads();
+  }
+};
+
+// K block-wide sums (K = 1, 2, 4, 8). Within a warp the lanes halve the set
+// they carry with every exchange; across warps a lane takes every 32nd of the
+// (warp, value) partials. `red` is one of two buffers used in turn, so one
+// barrier a call suffices.
+template <int K>
+__device__ __forceinline__ void block_sums(float* s, float* red) {
+  const int lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  float v[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = s[k];
+  int which = 0;
+#pragma unroll
+  for (int off = 16, n = K; off > 0; off >>= 1) {
+    if (n > 1) {
+      n >>= 1;
+      const bool up = (lane & off) != 0;
+      which = 2 * which + (up ? 1 : 0);
+#pragma unroll
+      for (int k = 0; k < K / 2; ++k) {
+        if (k < n) {
+          const float send = up ? v[k] : v[k + n], keep = up ? v[k + n] : v[k];
+          v[k] = keep + __shfl_xor_sync(0xffffffffu, send, off);
+        }
+      }
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
+    }
+  }
+  if ((lane & (32 / K - 1)) == 0) red[(threadIdx.x >> 5) * K + which] = v[0];
+  __syncthreads();
+  float a = 0.f;
+#pragma unroll
+  for (int i = 0; i < K / 2 + (K == 1); ++i)  // at most 16 warps: 16 K partials
+    if (lane + 32 * i < nw * K) a += red[lane + 32 * i];
+#pragma unroll
+  for (int off = 16; off >= K; off >>= 1) a += __shfl_xor_sync(0xffffffffu, a, off);
+#pragma unroll
+  for (int k = 0; k < K; ++k) s[k] = __shfl_sync(0xffffffffu, a, k);
+}
+
+template <typename T, int E, int V, int R>
+__global__ void __launch_bounds__(V == 1 ? 256 : 512, V == 1 ? 3 : 1)
+fwd_ring_kernel(Mat x, Mat y, Par par, int64_t n_rows, int rows, int dim, float eps, float* stats,
+                int per, int chunks, int stages) {
+  extern __shared__ __align__(128) uint8_t ring_mem[];
+  __shared__ float red[2][16 * R];
+  constexpr int P = E / 2;
+  const int g = blockIdx.x / chunks, chunk = blockIdx.x - g * chunks;
+  Ring<R, 1> q;
+  q.rb = dim * (int)sizeof(T);
+  q.stages = stages;
+  q.r0 = chunk * per;
+  q.r1 = min(rows, q.r0 + per);
+  q.nb = (q.r1 - q.r0 + R - 1) / R;
+  q.base = ring_mem;
+  q.full = reinterpret_cast<uint64_t*>(ring_mem + stages * R * q.rb);
+  q.src[0] = reinterpret_cast<const uint8_t*>(reinterpret_cast<const T*>(x.p) + (int64_t)g * x.sg);
+  q.step[0] = x.sr * (int64_t)sizeof(T);
+  q.start();
+  const int t = threadIdx.x, team = blockDim.x;
+  uint64_t w[V][P], b[V][P];
+  {
+    float wf[V][E], bf[V][E];
+    load_pars<E, V>(par.w, (int64_t)g * par.stride, par.bf16, 1.f - par.off, t * E, team * E, dim, wf);
+    load_pars<E, V>(par.b, (int64_t)g * par.stride, par.bf16, 0.f, t * E, team * E, dim, bf);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        w[v][i] = f2_pack(wf[v][2 * i] + par.off, wf[v][2 * i + 1] + par.off);
+        b[v][i] = f2_pack(bf[v][2 * i], bf[v][2 * i + 1]);
+      }
+  }
+  bool in[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) in[v] = (t + v * team) * E < dim;
+  T* yr = reinterpret_cast<T*>(y.p) + (int64_t)g * y.sg + (int64_t)q.r0 * y.sr + t * E;
+  const float inv = 1.f / (float)dim;
+  bool alive = true;  // false once a wait has run out: the block goes on
+                      // without waiting, its barriers stay matched
+  int s = 0;
+  uint32_t ph = 0;
+  for (int it = 0; it < q.nb; ++it) {
+    const int n = q.rows(it);
+    if (alive) alive = mbar_wait(&q.full[s], ph);
+    const uint8_t* slot = q.slot(s) + t * 16;
+    uint4 raw[R][V];
+    float sum[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      uint64_t a = 0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        raw[k][v] = make_uint4(0, 0, 0, 0);
+        if (k < n && in[v]) raw[k][v] = *reinterpret_cast<const uint4*>(slot + k * q.rb + v * team * 16);
+        uint64_t e[P];
+        pairs_of<E>(raw[k][v], e);
+#pragma unroll
+        for (int i = 0; i < P; ++i) a = fadd2(a, e[i]);
+      }
+      sum[k] = f2_sum(a);
+    }
+    block_sums<R>(sum, red[0]);
+    if (t == 0 && it + stages < q.nb) q.issue(it + stages, s);
+    if (++s == stages) s = 0, ph ^= 1;
+    float mean[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      mean[k] = sum[k] * inv;
+      const uint64_t m = twice(-mean[k]);
+      uint64_t a = 0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (in[v]) {
+          uint64_t e[P];
+          pairs_of<E>(raw[k][v], e);
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            const uint64_t d = fadd2(e[i], m);
+            a = ffma2(d, d, a);
+          }
+        }
+      }
+      sum[k] = f2_sum(a);
+    }
+    block_sums<R>(sum, red[1]);
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      if (k < n) {
+        const float rstd = rsqrtf(sum[k] * inv + eps);
+        if (t == 0 && stats != nullptr) {
+          const int64_t row = (int64_t)g * rows + q.r0 + it * R + k;
+          stats[row] = mean[k];
+          stats[n_rows + row] = rstd;
+        }
+        const uint64_t m = twice(-mean[k]), r = twice(rstd);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          if (in[v]) {
+            uint64_t e[P];
+            pairs_of<E>(raw[k][v], e);
+#pragma unroll
+            for (int i = 0; i < P; ++i) e[i] = ffma2(fmul2(fadd2(e[i], m), r), w[v][i], b[v][i]);
+            store_pairs<T, E>(yr + v * team * E, e);
+          }
+        }
+        yr += y.sr;
+      }
+    }
+  }
+  if (!alive) drain_delay();
+}
+
+template <typename T, int E, int V, int R>
+__global__ void __launch_bounds__(V == 1 ? 256 : 512, V == 1 ? 2 : 1)
+bwd_ring_kernel(Mat x, Mat dy, Mat dx, Par par, const float* stats, int64_t n_rows, int rows,
+                int dim, int per, int chunks, int stages, float* part) {
+  extern __shared__ __align__(128) uint8_t ring_mem[];
+  __shared__ float red[2][16 * 2 * R];
+  constexpr int P = E / 2;
+  pdl_launch_next();
+  const int g = blockIdx.x / chunks, chunk = blockIdx.x - g * chunks;
+  Ring<R, 2> q;
+  q.rb = dim * (int)sizeof(T);
+  q.stages = stages;
+  q.r0 = chunk * per;
+  q.r1 = min(rows, q.r0 + per);
+  q.nb = (q.r1 - q.r0 + R - 1) / R;
+  q.base = ring_mem;
+  q.full = reinterpret_cast<uint64_t*>(ring_mem + stages * 2 * R * q.rb);
+  q.src[0] = reinterpret_cast<const uint8_t*>(reinterpret_cast<const T*>(x.p) + (int64_t)g * x.sg);
+  q.src[1] = reinterpret_cast<const uint8_t*>(reinterpret_cast<const T*>(dy.p) + (int64_t)g * dy.sg);
+  q.step[0] = x.sr * (int64_t)sizeof(T);
+  q.step[1] = dy.sr * (int64_t)sizeof(T);
+  q.start();
+  const int t = threadIdx.x, team = blockDim.x;
+  uint64_t w[V][P], aw[V][P], ab[V][P];
+  bool in[V];
+  {
+    float wf[V][E];
+    load_pars<E, V>(par.w, (int64_t)g * par.stride, par.bf16, 1.f - par.off, t * E, team * E, dim, wf);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      in[v] = (t + v * team) * E < dim;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        w[v][i] = f2_pack(wf[v][2 * i] + par.off, wf[v][2 * i + 1] + par.off);
+        aw[v][i] = ab[v][i] = 0;
+      }
+    }
+  }
+  T* dxr = reinterpret_cast<T*>(dx.p) + (int64_t)g * dx.sg + (int64_t)q.r0 * dx.sr + t * E;
+  const float inv = 1.f / (float)dim;
+  const float* st = stats + (int64_t)g * rows + q.r0;
+  // a row's statistics are read one turn ahead
+  float mean[R], rs[R];
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    const bool live = k < q.r1 - q.r0;
+    mean[k] = live ? st[k] : 0.f;
+    rs[k] = live ? st[n_rows + k] : 0.f;
+  }
+  bool alive = true;
+  int s = 0;
+  uint32_t ph = 0;
+  for (int it = 0; it < q.nb; ++it) {
+    const int n = q.rows(it);
+    float mean_n[R], rs_n[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const bool live = q.r0 + (it + 1) * R + k < q.r1;
+      mean_n[k] = live ? st[(it + 1) * R + k] : 0.f;
+      rs_n[k] = live ? st[n_rows + (it + 1) * R + k] : 0.f;
+    }
+    if (alive) alive = mbar_wait(&q.full[s], ph);
+    const uint8_t* slot = q.slot(s) + t * 16;
+    uint4 rx[R][V], rd[R][V];
+    float sum[2 * R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      uint64_t s1 = 0, s2 = 0;
+      const uint64_t r = twice(rs[k]), m = twice(-mean[k]);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        rx[k][v] = rd[k][v] = make_uint4(0, 0, 0, 0);
+        if (k < n && in[v]) {
+          rx[k][v] = *reinterpret_cast<const uint4*>(slot + k * q.rb + v * team * 16);
+          rd[k][v] = *reinterpret_cast<const uint4*>(slot + (R + k) * q.rb + v * team * 16);
+          uint64_t e[P], d[P];
+          pairs_of<E>(rx[k][v], e);
+          pairs_of<E>(rd[k][v], d);
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            const uint64_t h = fmul2(fadd2(e[i], m), r), tt = fmul2(d[i], w[v][i]);
+            ab[v][i] = fadd2(ab[v][i], d[i]);
+            aw[v][i] = ffma2(d[i], h, aw[v][i]);
+            s1 = fadd2(s1, tt);
+            s2 = ffma2(tt, h, s2);
+          }
+        }
+      }
+      sum[2 * k] = f2_sum(s1);
+      sum[2 * k + 1] = f2_sum(s2);
+    }
+    block_sums<2 * R>(sum, red[it & 1]);
+    if (t == 0 && it + stages < q.nb) q.issue(it + stages, s);
+    if (++s == stages) s = 0, ph ^= 1;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      if (k < n) {
+        const float c1 = sum[2 * k] * inv, c2 = sum[2 * k + 1] * inv * rs[k];
+        // dx = rs (dy w - c1 - (x - mean) c2)
+        const uint64_t r = twice(rs[k]), m = twice(-mean[k]), k1 = twice(-c1 * rs[k]),
+                       k2 = twice(-c2 * rs[k]);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          if (in[v]) {
+            uint64_t e[P], d[P];
+            pairs_of<E>(rx[k][v], e);
+            pairs_of<E>(rd[k][v], d);
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+              e[i] = ffma2(d[i], fmul2(w[v][i], r), ffma2(fadd2(e[i], m), k2, k1));
+            store_pairs<T, E>(dxr + v * team * E, e);
+          }
+        }
+        dxr += dx.sr;
+      }
+      mean[k] = mean_n[k];
+      rs[k] = rs_n[k];
+    }
+  }
+  float* dst = part + (int64_t)blockIdx.x * 2 * dim;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = (t + v * team) * E;
+    if (in[v]) {
+#pragma unroll
+      for (int i = 0; i < P; i += 2) {
+        *reinterpret_cast<ulonglong2*>(dst + c + 2 * i) = make_ulonglong2(aw[v][i], aw[v][i + 1]);
+        *reinterpret_cast<ulonglong2*>(dst + dim + c + 2 * i) =
+            make_ulonglong2(ab[v][i], ab[v][i + 1]);
+      }
+    }
+  }
+  if (!alive) drain_delay();
+}
+
 // out[j][i] = sum over p < parts of part[(j * parts + p)][i], i < 2 dim: one
-// column per thread of x, eight threads of y share the parts, joined in order.
-__global__ void __launch_bounds__(256)
+// column per thread of x, sixteen threads of y share the parts, joined in order.
+__global__ void __launch_bounds__(512)
 join_kernel(const float* part, int parts, int dim, float* dw, float* db) {
-  __shared__ float s[8][33];
+  __shared__ float s[16][33];
   const int tiles = (2 * dim + 31) / 32, j = blockIdx.x / tiles;
   const int col = (blockIdx.x - j * tiles) * 32 + threadIdx.x;
   float a = 0.f;
+  pdl_wait_previous();
   if (col < 2 * dim) {
     const float* p = part + (int64_t)j * parts * 2 * dim + col;
-    for (int i = threadIdx.y; i < parts; i += 8) a += p[(int64_t)i * 2 * dim];
+#pragma unroll 8
+    for (int i = threadIdx.y; i < parts; i += 16) a += p[(int64_t)i * 2 * dim];
   }
   s[threadIdx.y][threadIdx.x] = a;
   __syncthreads();
   if (threadIdx.y == 0 && col < 2 * dim) {
     a = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a += s[i][threadIdx.x];
+    for (int i = 0; i < 16; ++i) a += s[i][threadIdx.x];
     float* dst = col < dim ? dw : db;
     const int c = col < dim ? col : col - dim;
     if (dst != nullptr) dst[(int64_t)j * dim + c] = a;
@@ -398,6 +793,43 @@ static bool can_vector(int es, int dim, const Mat* m, int nm, const Par& par) {
   return true;
 }
 
+// Rows of a ring kernel's turn, threads and ring depth for a row of nv
+// vectors: 256 threads while two vectors each suffice, R V = 4 vectors of
+// every tensor in registers a turn.
+struct RingPlan {
+  int V, R, threads, stages, smem, per_sm;
+};
+
+static RingPlan ring_plan(int nv, int tensors) {
+  RingPlan p{};
+  p.V = nv <= 256 ? 1 : (nv <= 1024 ? 2 : 4);
+  p.R = 4 / p.V;
+  p.threads = ((nv + p.V - 1) / p.V + 31) / 32 * 32;
+  const int stage = tensors * p.R * nv * 16;
+  // resident blocks by registers (forward at most 85 a thread at V = 1, the
+  // others up to 128), all within the SM's 227 KB
+  p.per_sm = std::max(1, std::min(8, (tensors == 1 && p.V == 1 ? 768 : 512) / p.threads));
+  p.stages = std::max(2, std::min(kMaxStages, 220 * 1024 / p.per_sm / stage));
+  p.smem = p.stages * stage + kMaxStages * 8;
+  return p;
+}
+
+// A ring needs rows of a kilobyte for its copies to pay, and holds 32 KB ones
+static bool use_ring(int nv) { return nv >= 64 && nv <= 2048; }
+
+struct Split {
+  int chunks, per;
+};
+
+// blocks per group: `slots` over all groups, at least `least` rows each
+static Split split_of(int groups, int rows, int slots, int least) {
+  Split s{};
+  const int want = std::max(1, slots / std::max(1, groups));
+  s.per = std::max(least, (rows + want - 1) / want);
+  s.chunks = std::max(1, (rows + s.per - 1) / s.per);
+  return s;
+}
+
 template <typename T, int E, int V, bool WARP>
 static int fwd_go(const Mat& x, const Mat& y, const Par& par, int64_t n, int rows, int dim,
                   float eps, float* stats, int threads, cudaStream_t st) {
@@ -407,47 +839,86 @@ static int fwd_go(const Mat& x, const Mat& y, const Par& par, int64_t n, int row
   return launch_status();
 }
 
+template <typename T, int E, int V>
+static int fwd_ring_go(const Mat& x, const Mat& y, const Par& par, int groups, int rows, int dim,
+                       float eps, float* stats, const RingPlan& p, int kid, cudaStream_t st) {
+  auto* fn = fwd_ring_kernel<T, E, V, 4 / V>;
+  const int rc = ensure_smem_attr((const void*)fn, 225 * 1024, kid);
+  if (rc) return rc;
+  const Split s = split_of(groups, rows, p.per_sm * kSms, 4 / V);
+  fn<<<(unsigned)((int64_t)groups * s.chunks), p.threads, p.smem, st>>>(
+      x, y, par, (int64_t)groups * rows, rows, dim, eps, stats, s.per, s.chunks, p.stages);
+  return launch_status();
+}
+
 template <typename T, int E>
-static int fwd_pick(const Mat& x, const Mat& y, const Par& par, int64_t n, int rows, int dim,
+static int fwd_pick(const Mat& x, const Mat& y, const Par& par, int groups, int rows, int dim,
                     float eps, float* stats, cudaStream_t st) {
   const int nv = (dim + E - 1) / E;
-  // a warp per row while a lane's share stays at 64 values or below
-  constexpr int kMost = 64 / E;
+  const int64_t n = (int64_t)groups * rows;
+  if constexpr (E > 1) {
+    // a few rows a block at least, or the ring's set-up is all there is
+    if (use_ring(nv) && n >= 8 * kSms) {
+      const RingPlan p = ring_plan(nv, 1);
+      const int kid = kKernelNorm + (sizeof(T) == 2 ? 0 : 3);
+      if (p.V == 1) return fwd_ring_go<T, E, 1>(x, y, par, groups, rows, dim, eps, stats, p, kid, st);
+      if (p.V == 2)
+        return fwd_ring_go<T, E, 2>(x, y, par, groups, rows, dim, eps, stats, p, kid + 1, st);
+      return fwd_ring_go<T, E, 4>(x, y, par, groups, rows, dim, eps, stats, p, kid + 2, st);
+    }
+  }
+  // a warp per row while a lane's share stays at 32 values or below and the
+  // rows are many; few rows take a block each
+  constexpr int kMost = 32 / E;
   const int need = (nv + 31) / 32;
-  if (need <= kMost) {
-    // few rows: small blocks, so that they spread over the SMs
+  if (need <= 1 || (need <= kMost && n >= 2 * kSms)) {
     const int th = n >= 8 * kSms ? 256 : (n >= 2 * kSms ? 128 : 32);
-    if (need <= kMost / 8) return fwd_go<T, E, kMost / 8, true>(x, y, par, n, rows, dim, eps, stats, th, st);
-    if (need <= kMost / 4) return fwd_go<T, E, kMost / 4, true>(x, y, par, n, rows, dim, eps, stats, th, st);
-    if (need <= kMost / 2) return fwd_go<T, E, kMost / 2, true>(x, y, par, n, rows, dim, eps, stats, th, st);
+    if (need <= 1) return fwd_go<T, E, 1, true>(x, y, par, n, rows, dim, eps, stats, th, st);
+    if constexpr (kMost >= 8)
+      if (need <= kMost / 4)
+        return fwd_go<T, E, kMost / 4, true>(x, y, par, n, rows, dim, eps, stats, th, st);
     return fwd_go<T, E, kMost, true>(x, y, par, n, rows, dim, eps, stats, th, st);
   }
-  constexpr int kV = 32 / E;  // dim <= 16384: 512 threads at most
-  const int th = (((nv + kV - 1) / kV) + 31) / 32 * 32;
-  return fwd_go<T, E, kV, false>(x, y, par, n, rows, dim, eps, stats, th, st);
+  auto th = [&](int v) { return ((nv + v - 1) / v + 31) / 32 * 32; };
+  if (nv <= 512) return fwd_go<T, E, 1, false>(x, y, par, n, rows, dim, eps, stats, th(1), st);
+  return fwd_go<T, E, kMost, false>(x, y, par, n, rows, dim, eps, stats, th(kMost), st);
 }
 
 struct BwdPlan {
-  int chunks, per, threads;
-  bool warp;
+  Split s;
+  bool ring;
 };
 
-// blocks per group: two per SM over all groups, at least eight rows each
-static BwdPlan bwd_plan(int groups, int rows) {
+// The backward's blocks, each of which leaves one partial sum of dw and db:
+// with the ring as many as are resident, else four an SM.
+static BwdPlan bwd_plan(int es, bool vec, int groups, int rows, int dim) {
+  const int nv = dim / (16 / es);
   BwdPlan p{};
-  const int want = std::max(1, 2 * kSms / std::max(1, groups));
-  p.per = std::max(8, (rows + want - 1) / want);
-  p.chunks = std::max(1, (rows + p.per - 1) / p.per);
+  p.ring = vec && use_ring(nv);
+  p.s = p.ring ? split_of(groups, rows, ring_plan(nv, 2).per_sm * kSms, 4)
+               : split_of(groups, rows, 4 * kSms, 4);
   return p;
 }
 
 template <typename T, int E, int V, int R, bool WARP>
 static int bwd_go(const Mat& x, const Mat& dy, const Mat& dx, const Par& par, const float* stats,
-                  int groups, int rows, int dim, const BwdPlan& pl, int threads, float* part,
+                  int groups, int rows, int dim, const Split& s, int threads, float* part,
                   cudaStream_t st) {
   const int smem = WARP ? threads / 32 * 2 * dim * 4 : 0;
-  bwd_kernel<T, E, V, R, WARP><<<(unsigned)((int64_t)groups * pl.chunks), threads, smem, st>>>(
-      x, dy, dx, par, stats, (int64_t)groups * rows, rows, dim, pl.per, pl.chunks, part);
+  bwd_kernel<T, E, V, R, WARP><<<(unsigned)((int64_t)groups * s.chunks), threads, smem, st>>>(
+      x, dy, dx, par, stats, (int64_t)groups * rows, rows, dim, s.per, s.chunks, part);
+  return launch_status();
+}
+
+template <typename T, int E, int V>
+static int bwd_ring_go(const Mat& x, const Mat& dy, const Mat& dx, const Par& par,
+                       const float* stats, int groups, int rows, int dim, const Split& s,
+                       const RingPlan& p, int kid, float* part, cudaStream_t st) {
+  auto* fn = bwd_ring_kernel<T, E, V, 4 / V>;
+  const int rc = ensure_smem_attr((const void*)fn, 225 * 1024, kid);
+  if (rc) return rc;
+  fn<<<(unsigned)((int64_t)groups * s.chunks), p.threads, p.smem, st>>>(
+      x, dy, dx, par, stats, (int64_t)groups * rows, rows, dim, s.per, s.chunks, p.stages, part);
   return launch_status();
 }
 
@@ -456,19 +927,28 @@ static int bwd_pick(const Mat& x, const Mat& dy, const Mat& dx, const Par& par,
                     const float* stats, int groups, int rows, int dim, const BwdPlan& pl,
                     float* part, cudaStream_t st) {
   const int nv = (dim + E - 1) / E;
+  const Split& s = pl.s;
+  if constexpr (E > 1) {
+    if (pl.ring) {
+      const RingPlan p = ring_plan(nv, 2);
+      const int kid = kKernelNorm + 6 + (sizeof(T) == 2 ? 0 : 3);
+      if (p.V == 1) return bwd_ring_go<T, E, 1>(x, dy, dx, par, stats, groups, rows, dim, s, p, kid, part, st);
+      if (p.V == 2) return bwd_ring_go<T, E, 2>(x, dy, dx, par, stats, groups, rows, dim, s, p, kid + 1, part, st);
+      return bwd_ring_go<T, E, 4>(x, dy, dx, par, stats, groups, rows, dim, s, p, kid + 2, part, st);
+    }
+  }
   if (nv <= 32)  // a warp holds the row (dim <= 256): 8 teams, 16 KB of shared memory at most
-    return bwd_go<T, E, 1, 4, true>(x, dy, dx, par, stats, groups, rows, dim, pl, 256, part, st);
+    return bwd_go<T, E, 1, 4, true>(x, dy, dx, par, stats, groups, rows, dim, s, 256, part, st);
   auto th = [&](int v) { return ((nv + v - 1) / v + 31) / 32 * 32; };
   if constexpr (E == 1) {
     if (nv <= 4 * 512)
-      return bwd_go<T, E, 4, 2, false>(x, dy, dx, par, stats, groups, rows, dim, pl, th(4), part, st);
-    return bwd_go<T, E, 32, 1, false>(x, dy, dx, par, stats, groups, rows, dim, pl, th(32), part, st);
-  } else {
-    if (nv <= 512)
-      return bwd_go<T, E, 1, 4, false>(x, dy, dx, par, stats, groups, rows, dim, pl, th(1), part, st);
-    if (nv <= 2 * 512)
-      return bwd_go<T, E, 2, 2, false>(x, dy, dx, par, stats, groups, rows, dim, pl, th(2), part, st);
-    return bwd_go<T, E, 32 / E, 1, false>(x, dy, dx, par, stats, groups, rows, dim, pl, th(32 / E), part, st);
+      return bwd_go<T, E, 4, 2, false>(x, dy, dx, par, stats, groups, rows, dim, s, th(4), part, st);
+    return bwd_go<T, E, 32, 1, false>(x, dy, dx, par, stats, groups, rows, dim, s, th(32), part, st);
+  } else {  // 33 to 63 vectors, or fp32 rows of more than 32 KB
+    if constexpr (E == 4)
+      if (nv > 2048)
+        return bwd_go<T, E, 8, 1, false>(x, dy, dx, par, stats, groups, rows, dim, s, th(8), part, st);
+    return bwd_go<T, E, 1, 4, false>(x, dy, dx, par, stats, groups, rows, dim, s, th(1), part, st);
   }
 }
 
@@ -486,17 +966,21 @@ int launch_layer_norm_fwd(int dtype, int groups, int rows, int dim, const fa_ten
   const ln::Par par{w, b, par_stride, par_dtype == FA_DTYPE_BF16, unit_offset ? 1.f : 0.f};
   if (dtype == FA_DTYPE_BF16) {
     return ln::can_vector(2, dim, m, 2, par)
-               ? ln::fwd_pick<__nv_bfloat16, 8>(m[0], m[1], par, n, rows, dim, eps, stats, st)
-               : ln::fwd_pick<__nv_bfloat16, 1>(m[0], m[1], par, n, rows, dim, eps, stats, st);
+               ? ln::fwd_pick<__nv_bfloat16, 8>(m[0], m[1], par, groups, rows, dim, eps, stats, st)
+               : ln::fwd_pick<__nv_bfloat16, 1>(m[0], m[1], par, groups, rows, dim, eps, stats, st);
   }
   return ln::can_vector(4, dim, m, 2, par)
-             ? ln::fwd_pick<float, 4>(m[0], m[1], par, n, rows, dim, eps, stats, st)
-             : ln::fwd_pick<float, 1>(m[0], m[1], par, n, rows, dim, eps, stats, st);
+             ? ln::fwd_pick<float, 4>(m[0], m[1], par, groups, rows, dim, eps, stats, st)
+             : ln::fwd_pick<float, 1>(m[0], m[1], par, groups, rows, dim, eps, stats, st);
 }
 
 size_t layer_norm_bwd_workspace(int groups, int rows, int dim) {
-  const ln::BwdPlan pl = ln::bwd_plan(groups, rows);
-  return (size_t)groups * pl.chunks * 2 * dim * sizeof(float);
+  // the most that any type and alignment takes
+  int64_t parts = 0;
+  for (int es : {2, 4})
+    for (bool vec : {false, true})
+      parts = std::max<int64_t>(parts, ln::bwd_plan(es, vec, groups, rows, dim).s.chunks);
+  return (size_t)groups * parts * 2 * dim * sizeof(float);
 }
 
 int launch_layer_norm_bwd(int dtype, int groups, int rows, int dim, const fa_tensor_t* x,
@@ -504,26 +988,42 @@ int launch_layer_norm_bwd(int dtype, int groups, int rows, int dim, const fa_ten
                           const fa_tensor_t* dy, const float* stats, const fa_tensor_t* dx,
                           float* dw, float* db, int shared, void* ws, cudaStream_t st) {
   if (groups == 0 && !shared) return FA_OK;
-  const ln::BwdPlan pl = ln::bwd_plan(groups, rows);
   float* part = reinterpret_cast<float*>(ws);
+  const int es = dtype == FA_DTYPE_BF16 ? 2 : 4;
+  const ln::Mat m[3] = {ln_mat(x), ln_mat(dy), ln_mat(dx)};
+  const ln::Par par{w, nullptr, par_stride, par_dtype == FA_DTYPE_BF16, unit_offset ? 1.f : 0.f};
+  const bool vec = ln::can_vector(es, dim, m, 3, par);
+  const ln::BwdPlan pl = ln::bwd_plan(es, vec, groups, rows, dim);
   if (groups > 0) {
-    const ln::Mat m[3] = {ln_mat(x), ln_mat(dy), ln_mat(dx)};
-    const ln::Par par{w, nullptr, par_stride, par_dtype == FA_DTYPE_BF16, unit_offset ? 1.f : 0.f};
     int rc;
-    if (dtype == FA_DTYPE_BF16)
-      rc = ln::can_vector(2, dim, m, 3, par)
-               ? ln::bwd_pick<__nv_bfloat16, 8>(m[0], m[1], m[2], par, stats, groups, rows, dim, pl, part, st)
+    if (es == 2)
+      rc = vec ? ln::bwd_pick<__nv_bfloat16, 8>(m[0], m[1], m[2], par, stats, groups, rows, dim, pl, part, st)
                : ln::bwd_pick<__nv_bfloat16, 1>(m[0], m[1], m[2], par, stats, groups, rows, dim, pl, part, st);
     else
-      rc = ln::can_vector(4, dim, m, 3, par)
-               ? ln::bwd_pick<float, 4>(m[0], m[1], m[2], par, stats, groups, rows, dim, pl, part, st)
+      rc = vec ? ln::bwd_pick<float, 4>(m[0], m[1], m[2], par, stats, groups, rows, dim, pl, part, st)
                : ln::bwd_pick<float, 1>(m[0], m[1], m[2], par, stats, groups, rows, dim, pl, part, st);
     if (rc != FA_OK) return rc;
   }
   if (dw == nullptr && db == nullptr) return FA_OK;
-  const int outs = shared ? 1 : groups, parts = shared ? groups * pl.chunks : pl.chunks;
-  ln::join_kernel<<<(unsigned)((int64_t)(2 * dim + 31) / 32 * outs), dim3(32, 8), 0, st>>>(part, parts, dim, dw, db);
+  const int outs = shared ? 1 : groups, parts = shared ? groups * pl.s.chunks : pl.s.chunks;
+  // may start while the backward's last blocks run, and waits for them
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((int64_t)(2 * dim + 31) / 32 * outs));
+  cfg.blockDim = dim3(32, 16);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = groups > 0 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, ln::join_kernel, (const float*)part, parts, dim, dw, db);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return record_cuda_error(e);
+  }
   return launch_status();
 }
+
+int norm_device_status() { return tu_device_status(); }
 
 }  // namespace fa

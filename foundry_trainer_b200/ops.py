@@ -251,57 +251,61 @@ def _launch(fn, where: str, t: torch.Tensor, stream, temps, *args) -> None:
 
 
 def _same_device(ref: torch.Tensor, **tensors) -> None:
-    if not ref.is_cuda:
+    dev = ref.get_device()
+    if dev < 0:
         raise ValueError("tensor must live on a CUDA device")
     for name, t in tensors.items():
-        if t is not None and t.device != ref.device:
-            raise ValueError(f"{name} is on {t.device}, x on {ref.device}")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name} is on {t.device}, the first operand on {ref.device}")
 
 
 def _norm_desc(t: torch.Tensor) -> fa_tensor_t:
     """(rows, D) or (groups, rows, D) as the C ABI's (groups, rows, 1, D)."""
-    sg = t.stride(0) if t.dim() == 3 else 0
-    sd = t.stride(-1) if t.shape[-1] > 1 else 1
-    return fa_tensor_t(t.data_ptr(), sg, t.stride(-2), 0, sd)
+    st = t.stride()
+    sd = st[-1] if t.shape[-1] > 1 else 1
+    return fa_tensor_t(t.data_ptr(), st[0] if len(st) == 3 else 0, st[-2], 0, sd)
 
 
 def _norm_params(x: torch.Tensor, weight, bias):
     """Checked (weight, bias, dtype code, stride between groups)."""
-    given = [p for p in (weight, bias) if p is not None]
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        if p.dim() == 2 and x.dim() != 3:
-            raise ValueError(f"{name} (groups, D) needs x (groups, rows, D)")
-        want = (x.shape[-1],) if p.dim() == 1 else (x.shape[0], x.shape[-1])
-        if tuple(p.shape) != want:
-            raise ValueError(f"{name} has shape {tuple(p.shape)}, expected {want}")
-    if len(given) == 2 and (weight.dim() != bias.dim() or weight.dtype != bias.dtype):
-        raise ValueError("weight and bias must share one layout and dtype")
-    if not given:
+    first = weight if weight is not None else bias
+    if first is None:
         return None, None, FA_DTYPE_F32, 0
-    if given[0].dim() == 1:
+    want = x.shape[-1:] if first.dim() == 1 else (x.shape[0] if x.dim() == 3 else -1, x.shape[-1])
+    if first.shape != want or (weight is not None and bias is not None
+                               and (bias.shape != want or bias.dtype != first.dtype)):
+        raise ValueError("weight and bias must be (D,), or (groups, D) with x (groups, rows, D), "
+                         f"and of one dtype: got {[tuple(p.shape) for p in (weight, bias) if p is not None]}"
+                         f" for x {tuple(x.shape)}")
+    code = _dtype_code(first)
+    if first.dim() == 1:
+        return (weight.contiguous() if weight is not None else None,
+                bias.contiguous() if bias is not None else None, code, 0)
+    # two modulation chunks share the stride of their rows; others are copied (D values each)
+    ps, unit = first.stride()
+    if (ps <= 0 or unit != 1 or x.shape[0] == 1
+            or (weight is not None and bias is not None and bias.stride() != (ps, 1))):
         weight, bias = (p.contiguous() if p is not None else None for p in (weight, bias))
-        return weight, bias, _dtype_code(given[0]), 0
-    # rows of two modulation chunks share a stride; others are copied (D values each)
-    st = {p.stride(0) for p in given}
-    if len(st) != 1 or 0 in st or any(p.stride(1) != 1 for p in given) or x.shape[0] == 1:
-        weight, bias = (p.contiguous() if p is not None else None for p in (weight, bias))
-        st = {x.shape[-1]}
-    return weight, bias, _dtype_code(given[0]), st.pop()
+        ps = x.shape[-1]
+    return weight, bias, code, ps
 
 
 def _ptr(t: Optional[torch.Tensor]):
     return t.data_ptr() if t is not None else None
 
 
-def _check_norm_x(x: torch.Tensor, **like) -> Tuple[int, int, int]:
-    if x.dim() not in (2, 3):
-        raise ValueError(f"expected (rows, D) or (groups, rows, D), got {tuple(x.shape)}")
-    for name, t in like.items():
-        if t.shape != x.shape or t.dtype != x.dtype:
-            raise ValueError(f"{name} must have x's shape and dtype")
-    return (x.shape[0] if x.dim() == 3 else 1), x.shape[-2], x.shape[-1]
+def _check_norm_x(x: torch.Tensor) -> Tuple[int, int, int]:
+    s = x.shape
+    if len(s) == 3:
+        return s
+    if len(s) != 2:
+        raise ValueError(f"expected (rows, D) or (groups, rows, D), got {tuple(s)}")
+    return 1, s[0], s[1]
+
+
+def _check_like(x: torch.Tensor, name: str, t: torch.Tensor) -> None:
+    if t.shape != x.shape or t.dtype != x.dtype:
+        raise ValueError(f"{name} must have x's shape and dtype")
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -318,8 +322,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     dt = _dtype_code(x)
     w, b, pdt, ps = _norm_params(x, weight, bias)
     y = torch.empty_like(x) if out is None else out
-    _check_norm_x(x, out=y)
-    stats = torch.empty((2, G * R), device=x.device, dtype=torch.float32)
+    if out is not None:
+        _check_like(x, "out", out)
+    stats = x.new_empty((2, G * R), dtype=torch.float32)
     _launch(_lib.load().fa_layer_norm_fwd, "fa_layer_norm_fwd", x, stream, (w, b), dt, G, R, D,
             C.byref(_norm_desc(x)), _ptr(w), _ptr(b), pdt, ps, int(unit_offset), float(eps),
             C.byref(_norm_desc(y)), stats.data_ptr())
@@ -332,7 +337,8 @@ def layer_norm_bwd(x: torch.Tensor, weight: Optional[torch.Tensor], dy: torch.Te
     """Gradients of layer_norm: (dx, dweight, dbias), the last two fp32 with
     weight's shape (of a (D,) pair when weight is None), or None with
     params=False. Identical bits across repeats."""
-    G, R, D = _check_norm_x(x, dy=dy)
+    G, R, D = _check_norm_x(x)
+    _check_like(x, "dy", dy)
     _same_device(x, weight=weight, dy=dy, stats=stats)
     if (stats.dtype != torch.float32 or tuple(stats.shape) != (2, G * R)
             or not stats.is_contiguous()):
@@ -354,13 +360,14 @@ def layer_norm_bwd(x: torch.Tensor, weight: Optional[torch.Tensor], dy: torch.Te
 
 def _matrix(t: torch.Tensor, name: str) -> fa_matrix_t:
     """A 2-D or (batch, rows, cols) tensor for the C ABI."""
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    s, st = t.shape, t.stride()
+    if s[-1] > 1 and st[-1] != 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
     # a stride that no element uses may be anything: give it a legal one
-    sr = t.stride(-2) if t.shape[-2] > 1 else -(-t.shape[-1] // 8) * 8
+    sr = st[-2] if s[-2] > 1 else -(-s[-1] // 8) * 8
     sb = 0
-    if t.dim() == 3:
-        sb = t.stride(0) if t.shape[0] > 1 else t.shape[1] * sr
+    if len(s) == 3:
+        sb = st[0] if s[0] > 1 else s[1] * sr
     return fa_matrix_t(t.data_ptr(), sb, sr)
 
 
@@ -380,7 +387,8 @@ def _rows2d(t: torch.Tensor, name: str) -> torch.Tensor:
 def _aligned_rows(rows: int, cols: int, like: torch.Tensor) -> torch.Tensor:
     """An uninitialised (rows, cols) bf16 matrix whose rows start on 16 bytes."""
     ld = -(-cols // 8) * 8
-    return torch.empty((rows, ld), device=like.device, dtype=torch.bfloat16)[:, :cols]
+    t = torch.empty((rows, ld), device=like.device, dtype=torch.bfloat16)
+    return t if ld == cols else t[:, :cols]
 
 
 def _pad_rank(a: torch.Tensor, b: torch.Tensor):

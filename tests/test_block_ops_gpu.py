@@ -52,6 +52,13 @@ NORM_CASES = [
     (2, 9, 16384, BF, True, False),
     (1, 3, 16381, F32, False, False),
     (300, 1, 128, BF, True, True),
+    (1, 1300, 520, BF, True, True),
+    (2, 700, 2048, BF, True, True),
+    (1, 1203, 2568, F32, False, False),
+    (3, 411, 4104, BF, False, True),
+    (1, 1201, 8200, BF, True, True),
+    (1, 5, 16384, F32, False, False),
+    (1, 1200, 300, F32, True, True),
 ]
 
 
