@@ -67,183 +67,253 @@ __device__ __forceinline__ void upper_tile(int t, int n, int& i, int& j) {
   j = i + t;
 }
 
+// D (8 x 8) += A (8 x 4) B (4 x 8) in fp64. Lane (g, q) = (lane / 4, lane % 4)
+// holds A[g][q], B[q][g], and D[g][2 q], D[g][2 q + 1]: a lane's value of a
+// symmetric matrix's 8 x 4 block is the same as A and as B.
+__device__ __forceinline__ void dmma(double* d, double a, double b) {
+  asm volatile(
+      "mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
+      : "+d"(d[0]), "+d"(d[1])
+      : "d"(a), "d"(b));
+}
+
 template <int R>
 struct Thin {
-  static constexpr int kLong = 4096 / R;              // long positions staged at a time
-  static constexpr int kStage = kLong * (R + 1) * 8;  // padded: no 32-way bank conflicts
-  static constexpr int kMat = R * R * 8;
-  static constexpr int kSmem = 4 * kMat + kStage + 16;
-  static constexpr int kTs = R / 16;                  // Gram tile a thread: kTs x kTs
-  static constexpr int kTiles = 136;                  // 16 * 17 / 2
-  static constexpr int kGroups = kThinThreads / kTiles;
-  static constexpr int kTm = R == 64 ? 2 : 1;         // tile of the r x r products
+  static constexpr int kLd = R + 4;  // doubles: an 8 x 4 block has no bank conflicts
+  static constexpr int kMat = R * kLd;
+  static constexpr int kN = R / 8;
+  static constexpr int kTiles = kN * (kN + 1) / 2;
+  // Gram sums: warps that split the positions, and per set of 8 x 8 tiles
+  static constexpr int kSplit = R == 64 ? 4 : 16;
+  static constexpr int kPart = kSplit * kTiles * 64;
+  static constexpr int kRest = 5 * kMat > kPart ? 5 * kMat : kPart;
+  static constexpr int kSmem = (kMat + kTiles * 64 + kRest) * 8;
 };
+static_assert(Thin<64>::kSmem <= 232448, "shared memory");
 
-// dst = alpha X Y + beta Z + gamma I for symmetric commuting R x R matrices:
-// the upper triangle is summed and mirrored.
-template <int R>
-__device__ __forceinline__ void sym_product(double* dst, const double* X, const double* Y,
-                                            double alpha, const double* Z, double beta,
-                                            double gamma) {
-  constexpr int TM = Thin<R>::kTm, N = R / TM;
-  for (int t = threadIdx.x; t < N * (N + 1) / 2; t += kThinThreads) {
-    int i, j;
-    upper_tile(t, N, i, j);
-    i *= TM;
-    j *= TM;
-    double acc[TM][TM];
+// The values of 8 rows (8 * tile + g) at the positions of one turn: lane q
+// takes the EB positions l + EB q .. (wide) or l + q, l + 4 + q, .. (tall);
+// the sum over positions does not ask for their order.
+template <typename T, bool TALL>
+struct Turn {
+  static constexpr int EB = 16 / sizeof(T);
+  T e[EB];
+
+  __device__ __forceinline__ void load(const T* g, int64_t row, int r, int j, int l, int l1, bool vec,
+                                       int q) {
+    if constexpr (TALL) {
 #pragma unroll
-    for (int u = 0; u < TM; ++u)
-#pragma unroll
-      for (int v = 0; v < TM; ++v) acc[u][v] = 0.0;
-#pragma unroll 8
-    for (int k = 0; k < R; ++k) {
-      double x[TM], y[TM];
-#pragma unroll
-      for (int u = 0; u < TM; ++u) x[u] = X[k * R + i + u], y[u] = Y[k * R + j + u];
-#pragma unroll
-      for (int u = 0; u < TM; ++u)
-#pragma unroll
-        for (int v = 0; v < TM; ++v) acc[u][v] = fma(x[u], y[v], acc[u][v]);
-    }
-#pragma unroll
-    for (int u = 0; u < TM; ++u)
-#pragma unroll
-      for (int v = 0; v < TM; ++v) {
-        const int p = i + u, q = j + v;
-        double d = alpha * acc[u][v];
-        if (Z != nullptr) d += beta * Z[p * R + q];
-        if (p == q) d += gamma;
-        if (p <= q) {
-          dst[p * R + q] = d;
-          dst[q * R + p] = d;
-        }
+      for (int u = 0; u < EB; ++u) {
+        const int p = l + 4 * u + q;
+        e[u] = j < r && p < l1 ? g[(int64_t)p * row + j] : T(0.f);
       }
+    } else {
+      const int p = l + EB * q;
+      if (vec && j < r && p + EB <= l1) {
+        *reinterpret_cast<uint4*>(e) = __ldg(reinterpret_cast<const uint4*>(g + (int64_t)j * row + p));
+      } else {
+#pragma unroll
+        for (int u = 0; u < EB; ++u)
+          e[u] = j < r && p + u < l1 ? g[(int64_t)j * row + p + u] : T(0.f);
+      }
+    }
   }
-}
+  __device__ __forceinline__ double at(int u) const { return (double)(float)e[u]; }
+};
 
 // One cluster per matrix (blockIdx.x / parts). TALL: the long side is the rows.
 template <typename T, int R, bool TALL>
-__global__ void __launch_bounds__(kThinThreads, 1)
+__global__ void __launch_bounds__(kThinThreads, R == 64 ? 1 : 2)
 thin_kernel(const T* g, int64_t g_batch, int64_t g_row, __nv_bfloat16* o, int64_t o_batch,
-            int64_t o_row, int r, int len, int parts, int steps, double ca, double cb, double cc,
-            double eps) {
+            int64_t o_row, int r, int len, int parts, int steps, int vec, int ovec, double ca,
+            double cb, double cc, double eps) {
   using C = Thin<R>;
+  constexpr int LD = C::kLd, NT = C::kTiles;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   double* A = reinterpret_cast<double*>(smem_raw);
-  double* M = A + R * R;
-  double* P = M + R * R;
-  double* Q = P + R * R;
-  double* stage = Q + R * R;
+  double* mine = A + C::kMat;  // this CTA's Gram sums, (tile, 8, 8)
+  double* rest = mine + NT * 64;
   const int mat = blockIdx.x / parts, part = blockIdx.x - mat * parts;
   const T* gm = g + (int64_t)mat * g_batch;
-  // this CTA's share of the long side
-  const int l0 = (int)((int64_t)len * part / parts), l1 = (int)((int64_t)len * (part + 1) / parts);
-  const int tid = threadIdx.x;
+  // this CTA's share of the long side, in whole turns
+  const int turns = (len + 31) / 32;
+  const int l0 = (int)((int64_t)turns * part / parts) * 32;
+  const int l1 = min(len, (int)((int64_t)turns * (part + 1) / parts) * 32);
+  const int tid = threadIdx.x, warp = warp_id(), lane = lane_id(), gg = lane >> 2, qq = lane & 3;
 
-  // ---- Gram matrix of the share: kGroups sets of threads take every
-  // kGroups-th position, each thread a kTs x kTs tile of the upper triangle
-  const int grp = tid / C::kTiles, tile = tid - grp * C::kTiles;
-  int ti, tj;
-  upper_tile(tile, 16, ti, tj);
-  ti *= C::kTs;
-  tj *= C::kTs;
-  double acc[C::kTs][C::kTs];
+  // ---- Gram matrix of the share
+  {
+    constexpr int EB = Turn<T, TALL>::EB, kTurn = 4 * EB;
+    // tiles of a warp: all, or at R = 64 a quarter: rows 0-3 or 4-7 of the
+    // tile triangle (10 tiles), or rows 0-3 with columns 4-5 or 6-7 (8)
+    constexpr int NF = R == 64 ? 4 : C::kN;
+    constexpr int ND = NF * (NF + 1) / 2;
+    const int role = R == 64 ? warp & 3 : 0, set = R == 64 ? warp >> 2 : warp;
+    const int base = role == 1 ? 4 : 0;
+    double acc[ND][2];
 #pragma unroll
-  for (int u = 0; u < C::kTs; ++u)
+    for (int i = 0; i < ND; ++i) acc[i][0] = acc[i][1] = 0.0;
+    if (R < 64 || role < 2) {
+      for (int l = l0 + set * kTurn; l < l1; l += C::kSplit * kTurn) {
+        Turn<T, TALL> f[NF];
 #pragma unroll
-    for (int v = 0; v < C::kTs; ++v) acc[u][v] = 0.0;
-  for (int l = l0; l < l1; l += C::kLong) {
-    const int n = min(C::kLong, l1 - l);
+        for (int i = 0; i < NF; ++i)
+          f[i].load(gm, g_row, r, (base + i) * 8 + gg, l, l1, vec, qq);
 #pragma unroll
-    for (int k = 0; k < 4096 / kThinThreads; ++k) {
-      const int idx = tid + k * kThinThreads;
-      const int ll = TALL ? idx / R : idx % C::kLong, j = TALL ? idx % R : idx / C::kLong;
-      float v = 0.f;
-      if (ll < n && j < r)
-        v = ld_f<T>(TALL ? gm + (int64_t)(l + ll) * g_row + j : gm + (int64_t)j * g_row + l + ll);
-      stage[ll * (R + 1) + j] = (double)v;
-    }
-    __syncthreads();
-    if (grp < C::kGroups) {
-#pragma unroll 4
-      for (int k = grp; k < n; k += C::kGroups) {
-        const double* row = stage + k * (R + 1);
-        double x[C::kTs], y[C::kTs];
+        for (int u = 0; u < EB; ++u) {
+          double x[NF];
 #pragma unroll
-        for (int u = 0; u < C::kTs; ++u) x[u] = row[ti + u], y[u] = row[tj + u];
+          for (int i = 0; i < NF; ++i) x[i] = f[i].at(u);
+          int k = 0;
 #pragma unroll
-        for (int u = 0; u < C::kTs; ++u)
+          for (int i = 0; i < NF; ++i)
 #pragma unroll
-          for (int v = 0; v < C::kTs; ++v) acc[u][v] = fma(x[u], y[v], acc[u][v]);
+            for (int j = i; j < NF; ++j) dmma(acc[k++], x[i], x[j]);
+        }
+      }
+    } else {
+      const int cols = role == 2 ? 4 : 6;
+      for (int l = l0 + set * kTurn; l < l1; l += C::kSplit * kTurn) {
+        Turn<T, TALL> f[4], h[2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i].load(gm, g_row, r, i * 8 + gg, l, l1, vec, qq);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) h[i].load(gm, g_row, r, (cols + i) * 8 + gg, l, l1, vec, qq);
+#pragma unroll
+        for (int u = 0; u < EB; ++u) {
+          const double y0 = h[0].at(u), y1 = h[1].at(u);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const double x = f[i].at(u);
+            if constexpr (ND >= 8) {
+              dmma(acc[2 * i], x, y0);
+              dmma(acc[2 * i + 1], x, y1);
+            }
+          }
+        }
       }
     }
-    __syncthreads();
-  }
-  // groups join in order (their tiles pass through M and P), then the CTAs
-  // of the cluster (through Q)
-  constexpr int kTt = C::kTs * C::kTs;
-  static_assert(C::kGroups * C::kTiles * kTt <= 2 * R * R, "group sums fit M and P");
-  if (grp < C::kGroups) {
+    // the sets' sums join in order
+    double* p = rest + (int64_t)set * NT * 64;
+    auto put = [&](int ti, int tj, const double* d) {
+      int at = 0;  // place of (ti, tj) in the upper triangle
+      for (int i = 0; i < ti; ++i) at += C::kN - i;
+      double* w = p + (at + tj - ti) * 64 + gg * 8 + 2 * qq;
+      w[0] = d[0];
+      w[1] = d[1];
+    };
+    if (R < 64 || role < 2) {
+      int k = 0;
 #pragma unroll
-    for (int u = 0; u < kTt; ++u)
-      M[(grp * C::kTiles + tile) * kTt + u] = acc[u / C::kTs][u % C::kTs];
+      for (int i = 0; i < NF; ++i)
+#pragma unroll
+        for (int j = i; j < NF; ++j) put(base + i, base + j, acc[k++]);
+    } else if constexpr (ND >= 8) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) put(i, (role == 2 ? 4 : 6) + j, acc[2 * i + j]);
+    }
   }
   __syncthreads();
-  for (int i = tid; i < C::kTiles * kTt; i += kThinThreads) {
+  for (int i = tid; i < NT * 64; i += kThinThreads) {
     double s = 0.0;
-    for (int k = 0; k < C::kGroups; ++k) s += M[k * C::kTiles * kTt + i];
-    Q[i] = s;
+    for (int k = 0; k < C::kSplit; ++k) s += rest[k * NT * 64 + i];
+    mine[i] = s;
   }
+  // and the CTAs' in order
   if (parts > 1) cluster_sync();
   else __syncthreads();
-  for (int i = tid; i < C::kTiles * kTt; i += kThinThreads) {
+  for (int i = tid; i < NT * 64; i += kThinThreads) {
     double s = 0.0;
     if (parts > 1) {
-      const uint32_t at = smem_u32(Q + i);
+      const uint32_t at = smem_u32(mine + i);
       for (int k = 0; k < parts; ++k) s += ld_cluster_f64(mapa(at, k));
     } else {
-      s = Q[i];
+      s = mine[i];
     }
-    int p, q;
-    upper_tile(i / kTt, 16, p, q);
-    p = p * C::kTs + (i % kTt) / C::kTs;
-    q = q * C::kTs + (i % kTt) % C::kTs;
-    if (p <= q) A[p * R + q] = A[q * R + p] = s;
+    int ti, tj;
+    upper_tile(i >> 6, C::kN, ti, tj);
+    const int p = ti * 8 + ((i >> 3) & 7), c = tj * 8 + (i & 7);
+    A[p * LD + c] = s;
+    if (ti != tj) A[c * LD + p] = s;
   }
   if (parts > 1) cluster_sync();  // nobody reads another CTA's memory after this
   else __syncthreads();
   double tr = 0.0;
-  for (int i = 0; i < R; ++i) tr += A[i * R + i];
+#pragma unroll 8
+  for (int i = 0; i < R; ++i) tr += A[i * LD + i];
   const double inv = 1.0 / (sqrt(tr) + eps);
   __syncthreads();
-  for (int i = tid; i < R * R; i += kThinThreads) A[i] *= inv * inv;
+  for (int i = tid; i < R * R; i += kThinThreads) A[(i / R) * LD + i % R] *= inv * inv;
   __syncthreads();
 
-  // ---- the steps
-  for (int s = 0; s < steps; ++s) {
-    sym_product<R>(M, A, A, cc, A, cb, ca);
-    __syncthreads();
-    if (s == 0) {
-      for (int i = tid; i < R * R; i += kThinThreads) P[i] = M[i];
-    } else {
-      sym_product<R>(Q, M, P, 1.0, nullptr, 0.0, 0.0);
-      double* t = P;
-      P = Q;
-      Q = t;
+  // ---- the steps. With S = A^2: M = a + b A + c S, P <- M P, and A <- A M^2 =
+  // a^2 A + S U, U = c^2 A S + 2 b c S + (b^2 + 2 a c) A + 2 a b; the products
+  // of one line below are independent and share the warps.
+  double *S = rest, *M = S + C::kMat, *U = M + C::kMat, *P = U + C::kMat, *P2 = P + C::kMat;
+  // tile (ti, tj) of X Y for symmetric commuting X, Y; f(row, column, value)
+  auto product = [&](int tile, const double* X, const double* Y, auto&& f) {
+    int ti, tj;
+    upper_tile(tile, C::kN, ti, tj);
+    const double* x = X + (ti * 8 + gg) * LD + qq;
+    const double* y = Y + (tj * 8 + gg) * LD + qq;
+    double d[2][2] = {};
+#pragma unroll
+    for (int k = 0; k < R; k += 8) {
+      dmma(d[0], x[k], y[k]);
+      dmma(d[1], x[k + 4], y[k + 4]);
     }
-    if (s + 1 == steps) break;
+    const int p = ti * 8 + gg, c = tj * 8 + 2 * qq;
+    f(p, c, d[0][0] + d[1][0], ti != tj);
+    f(p, c + 1, d[0][1] + d[1][1], ti != tj);
+  };
+  constexpr int kWarps = kThinThreads / 32;
+  for (int s = 0; s < steps; ++s) {
+    const bool last = s + 1 == steps;
+    double* M0 = s == 0 ? P : M;  // the first step's M is P
+    for (int t = warp; t < NT; t += kWarps)
+      product(t, A, A, [&](int p, int c, double v, bool mirror) {
+        const double m = cc * v + cb * A[p * LD + c] + (p == c ? ca : 0.0);
+        S[p * LD + c] = v;
+        M0[p * LD + c] = m;
+        if (mirror) S[c * LD + p] = v, M0[c * LD + p] = m;
+      });
     __syncthreads();
-    sym_product<R>(Q, A, M, 1.0, nullptr, 0.0, 0.0);
+    const int n_u = last ? 0 : NT, n_p = s == 0 ? 0 : NT;
+    for (int t = warp; t < n_u + n_p; t += kWarps) {
+      if (t < n_u)
+        product(t, A, S, [&](int p, int c, double v, bool mirror) {
+          const double u = cc * cc * v + 2.0 * cb * cc * S[p * LD + c] +
+                           (cb * cb + 2.0 * ca * cc) * A[p * LD + c] + (p == c ? 2.0 * ca * cb : 0.0);
+          U[p * LD + c] = u;
+          if (mirror) U[c * LD + p] = u;
+        });
+      else
+        product(t - n_u, M, P, [&](int p, int c, double v, bool mirror) {
+          P2[p * LD + c] = v;
+          if (mirror) P2[c * LD + p] = v;
+        });
+    }
     __syncthreads();
-    sym_product<R>(A, Q, M, 1.0, nullptr, 0.0, 0.0);
+    if (s > 0) {
+      double* w = P;
+      P = P2;
+      P2 = w;
+    }
+    if (last) break;
+    for (int t = warp; t < NT; t += kWarps)
+      product(t, S, U, [&](int p, int c, double v, bool mirror) {
+        const double n = v + ca * ca * A[p * LD + c];
+        A[p * LD + c] = n;
+        if (mirror) A[c * LD + p] = n;
+      });
     __syncthreads();
   }
-  __syncthreads();
   // P / |G| in fp32 (its largest entries are a few hundred times the
-  // result's: 24 bits leave the bf16 result its own rounding)
-  float* pf = reinterpret_cast<float*>(stage);
-  for (int i = tid; i < R * R; i += kThinThreads) pf[i] = (float)(P[i] * inv);
+  // result's: 24 bits leave the bf16 result its own rounding), in A's place
+  float* pf = reinterpret_cast<float*>(A);
+  for (int i = tid; i < R * R; i += kThinThreads) pf[i] = (float)(P[(i / R) * LD + i % R] * inv);
   __syncthreads();
 
   // ---- O = P G over the share, a long position per thread
@@ -252,9 +322,7 @@ thin_kernel(const T* g, int64_t g_batch, int64_t g_row, __nv_bfloat16* o, int64_
     uint64_t sum[R / 2];
 #pragma unroll
     for (int i = 0; i < R / 2; ++i) sum[i] = 0;
-#pragma unroll 4
-    for (int j = 0; j < r; ++j) {
-      const float x = ld_f<T>(TALL ? gm + (int64_t)l * g_row + j : gm + (int64_t)j * g_row + l);
+    auto add = [&](int j, float x) {
       const uint64_t xx = f2_pack(x, x);
       const ulonglong2* pr = reinterpret_cast<const ulonglong2*>(pf + j * R);
 #pragma unroll
@@ -263,17 +331,42 @@ thin_kernel(const T* g, int64_t g_batch, int64_t g_row, __nv_bfloat16* o, int64_
         sum[2 * i] = ffma2(w.x, xx, sum[2 * i]);
         sum[2 * i + 1] = ffma2(w.y, xx, sum[2 * i + 1]);
       }
-    }
+    };
+    constexpr int EB = 16 / sizeof(T);
+    if (TALL && vec) {  // a row of r values, EB at a time
+      const T* row = gm + (int64_t)l * g_row;
+#pragma unroll 1
+      for (int j = 0; j < r; j += EB) {
+        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(row + j));
+        const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-    for (int i = 0; i < R / 2; ++i) {
-      float u, v;
-      f2_unpack(sum[i], u, v);
-      if constexpr (TALL) {
-        if (2 * i < r) om[(int64_t)l * o_row + 2 * i] = __float2bfloat16_rn(u);
-        if (2 * i + 1 < r) om[(int64_t)l * o_row + 2 * i + 1] = __float2bfloat16_rn(v);
-      } else {
-        if (2 * i < r) om[(int64_t)(2 * i) * o_row + l] = __float2bfloat16_rn(u);
-        if (2 * i + 1 < r) om[(int64_t)(2 * i + 1) * o_row + l] = __float2bfloat16_rn(v);
+        for (int u = 0; u < EB; ++u) add(j + u, (float)e[u]);
+      }
+    } else {
+#pragma unroll 8
+      for (int j = 0; j < r; ++j)
+        add(j, ld_f<T>(TALL ? gm + (int64_t)l * g_row + j : gm + (int64_t)j * g_row + l));
+    }
+    if (TALL && ovec) {
+#pragma unroll
+      for (int i = 0; i < R / 8; ++i) {
+        if (8 * i < r) {
+          float f[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) f2_unpack(sum[4 * i + k], f[2 * k], f[2 * k + 1]);
+          *reinterpret_cast<uint4*>(om + (int64_t)l * o_row + 8 * i) =
+              make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]),
+                         pack_bf16(f[6], f[7]));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < R / 2; ++i) {
+        float u, v;
+        f2_unpack(sum[i], u, v);
+        __nv_bfloat16* w = TALL ? om + (int64_t)l * o_row + 2 * i : om + (int64_t)(2 * i) * o_row + l;
+        if (2 * i < r) w[0] = __float2bfloat16_rn(u);
+        if (2 * i + 1 < r) w[TALL ? 1 : o_row] = __float2bfloat16_rn(v);
       }
     }
   }
@@ -416,8 +509,24 @@ static int thin_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, i
   auto* fn = thin_kernel<T, R, TALL>;
   const int rc = ensure_smem_attr((const void*)fn, Thin<R>::kSmem, kid);
   if (rc) return rc;
-  // a CTA for every 256 positions, eight at most
-  const int parts = std::max(1, std::min(8, (len + 255) / 256));
+  // a CTA for every 256 positions, eight at most (a portable cluster); 16
+  // while that leaves SMs free
+  int parts = std::max(1, std::min(16, (len + 255) / 256));
+  if (parts > 8 && batch * parts > 128) parts = 8;
+  if (parts > 8) {
+    const cudaError_t e =
+        cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      parts = 8;
+    }
+  }
+  const int es = (int)sizeof(T);
+  // 16-byte reads of rows: wide rows start anywhere in a share of whole
+  // turns; tall ones hold a multiple of a vector
+  const int vec = reinterpret_cast<uintptr_t>(g) % 16 == 0 && gb * es % 16 == 0 && gr * es % 16 == 0 &&
+                  (!TALL || r % (16 / es) == 0);
+  const int ovec = r % 8 == 0;  // o's rows start on 16 bytes
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(batch * parts));
   cfg.blockDim = dim3(kThinThreads);
@@ -431,7 +540,7 @@ static int thin_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, i
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(
       &cfg, fn, reinterpret_cast<const T*>(g), gb, gr, reinterpret_cast<__nv_bfloat16*>(o), ob,
-      orow, r, len, parts, steps, (double)c[0], (double)c[1], (double)c[2], (double)eps);
+      orow, r, len, parts, steps, vec, ovec, (double)c[0], (double)c[1], (double)c[2], (double)eps);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return record_cuda_error(e);
