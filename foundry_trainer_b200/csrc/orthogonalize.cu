@@ -34,7 +34,9 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <cstdint>
 
 #include "attn_common.h"
 #include "gemm.h"
@@ -221,17 +223,32 @@ thin_kernel(const T* g, int64_t g_batch, int64_t g_row, __nv_bfloat16* o, int64_
     for (int k = 0; k < C::kSplit; ++k) s += rest[k * NT * 64 + i];
     mine[i] = s;
   }
-  // and the CTAs' in order
-  if (parts > 1) cluster_sync();
-  else __syncthreads();
-  for (int i = tid; i < NT * 64; i += kThinThreads) {
-    double s = 0.0;
-    if (parts > 1) {
+  // and the CTAs' in CTA order: each CTA sums its share of the entries over
+  // the cluster, then takes the other shares from their owners (all reading
+  // all took 14 us of a 38 us call at 64 x 4096)
+  double* sums = rest;  // (the sets' sums are done with)
+  constexpr int kAll = NT * 64;
+  const int share = (kAll + parts - 1) / parts;
+  if (parts > 1) {
+    cluster_sync();
+    const int i1 = min(kAll, (part + 1) * share);
+    for (int i = part * share + tid; i < i1; i += kThinThreads) {
       const uint32_t at = smem_u32(mine + i);
-      for (int k = 0; k < parts; ++k) s += ld_cluster_f64(mapa(at, k));
-    } else {
-      s = mine[i];
+      double v[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[k] = k < parts ? ld_cluster_f64(mapa(at, k)) : 0.0;
+      double s = 0.0;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) s += v[k];
+      sums[i] = s;
     }
+    cluster_sync();
+  } else {
+    __syncthreads();
+  }
+#pragma unroll 5
+  for (int i = tid; i < kAll; i += kThinThreads) {
+    const double s = parts > 1 ? ld_cluster_f64(mapa(smem_u32(sums + i), i / share)) : mine[i];
     int ti, tj;
     upper_tile(i >> 6, C::kN, ti, tj);
     const int p = ti * 8 + ((i >> 3) & 7), c = tj * 8 + (i & 7);
@@ -502,6 +519,42 @@ static Space space_of(int batch, int m, int n, int steps) {
   return s;
 }
 
+// Resident clusters of `c` CTAs, asked of the driver once per kernel and size.
+static int clusters_that_fit(const void* fn, int smem, int c, int slot, int* fit) {
+  static std::atomic<int> known[64][60];  // 0: not asked yet, else fit + 1
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FA_ERR_NO_DEVICE;
+  int v = known[dev][slot].load(std::memory_order_acquire);
+  if (v == 0) {
+    if (c > 8) {
+      const cudaError_t e =
+          cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return record_cuda_error(e);
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(c);
+    cfg.blockDim = dim3(kThinThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = c;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, fn, &cfg);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      if (c == 1) return record_cuda_error(e);
+      n = 0;  // no cluster of this size here
+    }
+    v = n + 1;
+    known[dev][slot].store(v, std::memory_order_release);
+  }
+  *fit = v - 1;
+  return FA_OK;
+}
+
 template <typename T, int R, bool TALL>
 static int thin_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, int64_t orow,
                    int batch, int r, int len, int steps, const float* c, float eps, int kid,
@@ -509,17 +562,20 @@ static int thin_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, i
   auto* fn = thin_kernel<T, R, TALL>;
   const int rc = ensure_smem_attr((const void*)fn, Thin<R>::kSmem, kid);
   if (rc) return rc;
-  // a CTA for every 256 positions, eight at most (a portable cluster); 16
-  // while that leaves SMs free
-  int parts = std::max(1, std::min(16, (len + 255) / 256));
-  if (parts > 8 && batch * parts > 128) parts = 8;
-  if (parts > 8) {
-    const cudaError_t e =
-        cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) {
-      cudaGetLastError();
-      parts = 8;
-    }
+  // CTAs per matrix: of 1 .. 16, what is soonest done by the clusters of that
+  // size that are resident at once (a cluster stays within a GPC, so large ones
+  // leave SMs idle). A matrix costs about as much apart from its positions as
+  // 1500 positions do.
+  int parts = 1;
+  int64_t best = INT64_MAX;
+  for (int c = 1, k = 0; c <= 16; c *= 2, ++k) {
+    if (c > 1 && c * 128 > len) break;
+    int fit = 0;
+    const int rf = clusters_that_fit((const void*)fn, Thin<R>::kSmem, c, (kid - kKernelThin) * 5 + k, &fit);
+    if (rf) return rf;
+    if (fit <= 0) break;
+    const int64_t cost = (int64_t)((batch + fit - 1) / fit) * (1500 + (len + c - 1) / c);
+    if (cost < best) best = cost, parts = c;
   }
   const int es = (int)sizeof(T);
   // 16-byte reads of rows: wide rows start anywhere in a share of whole
