@@ -11,6 +11,7 @@ from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
 LIB_PATH = _PKG / "lib" / "libfoundry_attn.so"
+BINDING_PATH = _PKG / "lib" / "_fa_torch.so"
 
 FA_OK = 0
 FA_ERR_INVALID_ARG = 1
@@ -125,6 +126,8 @@ SIGNATURES = {
     "fa_lora_linear_many": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _M, _M,
                                       _M, _M, C.c_void_p, _F, C.c_void_p, _M, C.c_void_p,
                                       C.c_size_t, C.c_void_p]),
+    "fa_pad_rows": (C.c_int, [C.c_int64, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                              C.c_void_p]),
     "fa_lora_linear_many_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int]),
     "fa_orthogonalize": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int64,
                                    C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_float,
@@ -156,6 +159,29 @@ def load() -> C.CDLL:
             fn.argtypes = args
         _lib = lib
     return _lib
+
+
+_binding = None
+
+
+def binding():
+    """The compiled calls of the block operators over torch tensors (once).
+    Raises if they have not been built."""
+    global _binding
+    if _binding is None:
+        import importlib.util
+
+        import torch  # noqa: F401  (the module links against torch's libraries)
+        load()
+        if not BINDING_PATH.exists():
+            raise FaError(-1, "binding",
+                          f"{BINDING_PATH} is missing; run `python -m foundry_trainer_b200.build`")
+        spec = importlib.util.spec_from_file_location("_fa_torch", BINDING_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.set_check(check)
+        _binding = mod
+    return _binding
 
 
 def status_string(status: int) -> str:

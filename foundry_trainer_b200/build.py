@@ -5,6 +5,7 @@
 
 Outputs (git-ignored, shipped with the tree to the GPU box):
     foundry_trainer_b200/lib/libfoundry_attn.so   the C ABI of include/foundry_attn.h
+    foundry_trainer_b200/lib/_fa_torch.so          the block operators' calls over torch tensors
     foundry_trainer_b200/lib/test_attn_op         C++ host-mirror driver (tests only)
     tests/lib/libfa_selftest.so                   tcgen05 known-answer kernels of
                                                   tests/csrc/ (tests only)
@@ -99,6 +100,29 @@ def build_cpp_driver(force: bool = False) -> Path:
     return out
 
 
+def build_torch_binding(force: bool = False) -> Path:
+    """The compiled half of ops.py (csrc/torch_binding.cpp), linked against
+    the C ABI library beside it and this interpreter's torch."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension as ce
+    src = CSRC / "torch_binding.cpp"
+    out = LIB / "_fa_torch.so"
+    if force or _stale(out, [src, ROOT / "include" / "foundry_attn.h"]):
+        cmd = ["g++", "-std=c++17", "-O2", "-shared", "-fPIC", "-w",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               "-I", str(ROOT / "include"), "-I", sysconfig.get_paths()["include"],
+               "-I", "/usr/local/cuda/include"]
+        for d in ce.include_paths():
+            cmd += ["-I", d]
+        cmd += [str(src), "-o", str(out), "-L", str(LIB), "-lfoundry_attn", "-Wl,-rpath,$ORIGIN"]
+        for d in ce.library_paths():
+            cmd += ["-L", d, f"-Wl,-rpath,{d}"]
+        _run(cmd + ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"])
+    return out
+
+
 def build_all(force: bool = False, verbose_ptxas: bool = False) -> dict[str, Path]:
     OBJ.mkdir(exist_ok=True)
     LIB.mkdir(exist_ok=True)
@@ -118,7 +142,8 @@ def build_all(force: bool = False, verbose_ptxas: bool = False) -> dict[str, Pat
     _link([objs[s] for s in LIB_SOURCES], lib)
     _link([objs[s.name] for s in SELFTEST_SOURCES], st)
     drv = build_cpp_driver(force)
-    return {"lib": lib, "selftest": st, "cpp_driver": drv}
+    return {"lib": lib, "torch_binding": build_torch_binding(force), "selftest": st,
+            "cpp_driver": drv}
 
 
 if __name__ == "__main__":

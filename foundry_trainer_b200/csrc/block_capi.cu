@@ -51,7 +51,7 @@ constexpr int kMaxSteps = 64;
 static int check_lora(int dtype, int rows, int in_dim, int out_dim, int rank, float scale) {
   if (dtype != FA_DTYPE_BF16) return FA_ERR_UNSUPPORTED;
   if (rows < 0 || in_dim <= 0 || out_dim <= 0 || rank <= 0) return FA_ERR_INVALID_ARG;
-  if (rank % 8 != 0 || rank > kMaxRank) return FA_ERR_UNSUPPORTED;
+  if (rank > kMaxRank) return FA_ERR_UNSUPPORTED;
   if (!std::isfinite(scale)) return FA_ERR_INVALID_ARG;
   if (rows > (1 << 30) || in_dim > (1 << 24) || out_dim > (1 << 24)) return FA_ERR_TOO_LARGE;
   return FA_OK;
@@ -295,6 +295,19 @@ int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
   p.low_ld = ld;
   p.rank = rank;
   return launch_gemm_wide(o, p, kEpiLinear, st);
+}
+
+int fa_pad_rows(int64_t rows, int cols, const void* src, int64_t src_stride, void* dst,
+                int64_t dst_stride, void* stream) {
+  if (rows < 0 || cols <= 0 || src_stride < 0 || dst_stride < cols) return FA_ERR_INVALID_ARG;
+  if (rows == 0) return FA_OK;
+  if (src == nullptr || dst == nullptr) return FA_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(src) % 2 != 0 || reinterpret_cast<uintptr_t>(dst) % 2 != 0)
+    return FA_ERR_ALIGNMENT;
+  if (rows * cols >= (int64_t)1 << 38) return FA_ERR_TOO_LARGE;
+  FA_TRY(check_sm100());
+  return launch_pad_rows(rows, cols, src, src_stride, dst, dst_stride,
+                         reinterpret_cast<cudaStream_t>(stream));
 }
 
 // [low (rows, low_dim) bf16 | per-256-row counts | their adapters | slots]

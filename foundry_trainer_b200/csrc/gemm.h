@@ -101,6 +101,8 @@ int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool sma
 int launch_low_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int64_t a_e,
                     int64_t a_r, const int* ids, int E, const float* scales, float scale, int rows,
                     int K, int rank, int low_ld, __nv_bfloat16* low, cudaStream_t st);
+int launch_pad_rows(int64_t rows, int cols, const void* src, int64_t src_stride, void* dst,
+                    int64_t dst_stride, cudaStream_t st);
 int launch_adapter_plan(const int* ids, int rows, int E, int* cnt, int* list, int* slot,
                         cudaStream_t st);
 int skinny_device_status();

@@ -215,7 +215,8 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
             const __nv_bfloat16* lw = p.low + (int64_t)j * p.low_ld;
             const __nv_bfloat16* f = p.fac + (int64_t)e * p.fac_e + (int64_t)i * p.fac_i;
             if (p.fac_i != 1) {  // the adapter's row i, its rank contiguous (16-byte rows)
-              for (int k = 0; k < p.rank; k += 8) {
+              int k = 0;
+              for (; k + 8 <= p.rank; k += 8) {
                 const uint4 b4 = __ldg(reinterpret_cast<const uint4*>(f + k));
                 const uint4 l4 = __ldcg(reinterpret_cast<const uint4*>(lw + k));
                 const uint32_t bw[4] = {b4.x, b4.y, b4.z, b4.w}, xw[4] = {l4.x, l4.y, l4.z, l4.w};
@@ -225,6 +226,8 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
                   acc = fmaf(bf16_hi(bw[u]), bf16_hi(xw[u]), acc);
                 }
               }
+              for (; k < p.rank; ++k)
+                acc = fmaf(__bfloat162float(f[k]), __bfloat162float(lw[k]), acc);
             } else {  // its column i, consecutive over the threads
               for (int k = 0; k < p.rank; ++k)
                 acc = fmaf(__bfloat162float(f[(int64_t)k * p.fac_k]), __bfloat162float(lw[k]), acc);
@@ -298,6 +301,15 @@ low_rows_kernel(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int
   if (lane_id() == 0 && j < low_ld)
     low[(int64_t)row * low_ld + j] =
         __float2bfloat16_rn(has && j < rank ? acc * (scales != nullptr ? scales[e] : scale) : 0.f);
+}
+
+__global__ void __launch_bounds__(256)
+pad_rows_kernel(int64_t n, int cols, const uint16_t* src, int64_t ss, uint16_t* dst, int64_t ds) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int64_t r = i / cols;
+  const int c = (int)(i - r * cols);
+  dst[r * ds + c] = src[r * ss + c];
 }
 
 // Per block of 256 rows: the distinct adapters in order of first use, and
@@ -408,6 +420,15 @@ int launch_low_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a,
                     int K, int rank, int low_ld, __nv_bfloat16* low, cudaStream_t st) {
   skinny::low_rows_kernel<<<(unsigned)(rows * (low_ld / 8)), 256, 0, st>>>(
       x, ldx, a, a_e, a_r, ids, E, scales, scale, K, rank, low_ld, low);
+  return launch_status();
+}
+
+int launch_pad_rows(int64_t rows, int cols, const void* src, int64_t src_stride, void* dst,
+                    int64_t dst_stride, cudaStream_t st) {
+  const int64_t n = rows * cols;
+  skinny::pad_rows_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(
+      n, cols, reinterpret_cast<const uint16_t*>(src), src_stride,
+      reinterpret_cast<uint16_t*>(dst), dst_stride);
   return launch_status();
 }
 

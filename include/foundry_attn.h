@@ -373,8 +373,9 @@ typedef struct {
  * crates/foundry-spike/src/lib.rs:270-287):
  *   y = x W^T + bias + scale (x A^T) B^T
  * x (rows, in_dim), w (out_dim, in_dim), a (rank, in_dim), b (out_dim, rank),
- * y (rows, out_dim); bias (out_dim) bf16 or NULL. rank is a multiple of 8 up
- * to 256 (pad smaller ones with zeros). `low` receives scale x A^T as bf16
+ * y (rows, out_dim); bias (out_dim) bf16 or NULL; rank <= 256. (A dense b
+ * whose rank is no multiple of 8 breaks the 16-byte rule: fa_pad_rows makes
+ * an aligned copy.) `low` receives scale x A^T as bf16
  * (rows, rank rounded up to 16), 16-byte aligned; the backward reads it.
  * The backward, with W frozen, writes (each may be NULL, da and db together)
  *   dx = dy W + U A,  da = U^T x (rank, in_dim),  db = dy^T low (out_dim, rank),
@@ -391,6 +392,11 @@ int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
                        const fa_matrix_t* dy, const fa_matrix_t* dx, void* da, void* db,
                        void* workspace, size_t workspace_bytes, void* stream);
 size_t fa_lora_linear_bwd_workspace_bytes(int rows, int rank);
+
+/* Copies a (rows, cols) 16-bit matrix to rows of another stride (in elements);
+ * what lies between the copied columns is not written. */
+int fa_pad_rows(int64_t rows, int cols, const void* src, int64_t src_stride, void* dst,
+                int64_t dst_stride, void* stream);
 
 /*
  * The same forward for rows of many requests, each with its own adapter:
