@@ -31,10 +31,11 @@ enum KernelId {
   kKernelF32Fwd = 2,
   kKernelF32Bwd = 3,
   kKernelWide = 4,     // + 0..5: the wide product by operand layout and epilogue
-  kKernelSkinny = 10,  // + 0..4
+  kKernelSkinny = 10,  // + 0..4 by operand layout and output
   kKernelThin = 15,    // + 0..11: the thin orthogonalisation by type, side and rank
   kKernelNorm = 27,    // + 0..11: the ring layer norm by direction, type and width
-  kKernelCount = 39
+  kKernelSkinnyBig = 39,  // + 0..4: the same with one block an SM
+  kKernelCount = 44
 };
 
 // FA_OK when the last CUDA runtime call / launch on this thread succeeded;
@@ -54,6 +55,11 @@ int check_sm100();
 
 // Raises the dynamic shared-memory limit of `fn` once per (device, kernel).
 int ensure_smem_attr(const void* fn, int bytes, int kernel_id);
+
+// Resident clusters of `c` CTAs (of `threads` and `smem` bytes) on this device,
+// asked of the driver once per kernel_id and size: a cluster stays within a
+// GPC, so large ones leave SMs idle.
+int clusters_that_fit(const void* fn, int threads, int smem, int c, int kernel_id, int* fit);
 
 // bf16 sm_100a kernels
 // merge: 0 plain; 1 (o_acc, lse_acc) <- block; 2 fold block into them;

@@ -73,8 +73,9 @@ static const __nv_bfloat16* bfp(const void* p) { return reinterpret_cast<const _
 // Up to 256 rows the weight's bytes are the cost and its rows make the
 // 128-row side; beyond, the tokens do (measured at 4096 x 4096, rank 16).
 constexpr int kFewRows = 256;
-// Up to 64 rows a warp per inner product beats the tensor-core form's
-// fixed cost.
+// Up to 64 rows four warps per inner product beat the tensor-core form's fixed
+// cost (at 4096, rank 16: 64 rows 4.4 us against 8.3 us). With many adapters
+// the other form also needs a plan of the rows first: up to kFewRows there.
 constexpr int kDotRows = 64;
 
 }  // namespace fa
@@ -175,11 +176,8 @@ int fa_lora_linear_fwd(int dtype, int rows, int in_dim, int out_dim, int rank,
     s.low = lw;
     s.low_ld = ld;
     s.rank = rank;
-    s.fac = bfp(b->data);
-    s.fac_i = b->stride_row;
-    s.fac_k = 1;
     return launch_gemm_skinny(mat(w, 1, out_dim, in_dim), false, mat(x, 1, rows, in_dim), false, s,
-                              kSkinnyCols, early, st);
+                              kSkinnyCols, early, st, mat(b, 1, out_dim, rank));
   }
   WideOperands o;
   o.a = mat(x, 1, rows, in_dim);
@@ -275,11 +273,8 @@ int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
     s.low = u;
     s.low_ld = ld;
     s.rank = rank;
-    s.fac = bfp(a->data);
-    s.fac_i = 1;
-    s.fac_k = a->stride_row;
     return launch_gemm_skinny(mat(w, 1, out_dim, in_dim), true, mat(dy, 1, rows, out_dim), false, s,
-                              kSkinnyCols, false, st);
+                              kSkinnyCols, false, st, mat(a, 1, rank, in_dim));
   }
   WideOperands o;
   o.b_mn = true;
@@ -348,7 +343,7 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
   ws += align256(blocks * 256 * 4);
   int* slot = reinterpret_cast<int*>(ws);
   bool early = false;
-  if (rows <= kDotRows) {
+  if (rows <= kFewRows) {
     FA_TRY(launch_low_rows(bfp(x->data), x->stride_row, bfp(a->data), a->stride_batch,
                            a->stride_row, ids, n_adapters, scales, 1.f, rows, in_dim, rank, ld, low,
                            st));
@@ -383,12 +378,15 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
     s.rank = rank;
     s.E = n_adapters;
     s.ids = ids;
-    s.fac = bfp(b->data);
-    s.fac_e = b->stride_batch;
-    s.fac_i = b->stride_row;
-    s.fac_k = 1;
+    s.raw_x = bfp(x->data);
+    s.raw_ldx = x->stride_row;
+    s.raw_w = bfp(w->data);
+    s.raw_ldw = w->stride_row;
+    s.raw_f = bfp(b->data);
+    s.raw_fe = b->stride_batch;
+    s.raw_ldf = b->stride_row;
     return launch_gemm_skinny(mat(w, 1, out_dim, in_dim), false, mat(x, 1, rows, in_dim), false, s,
-                              kSkinnyCols, early, st);
+                              kSkinnyCols, early, st, mat(b, n_adapters, out_dim, rank));
   }
   WideOperands o;
   o.a = mat(x, 1, rows, in_dim);

@@ -127,6 +127,43 @@ int ensure_smem_attr(const void* fn, int bytes, int kernel_id) {
   return FA_OK;
 }
 
+int clusters_that_fit(const void* fn, int threads, int smem, int c, int kernel_id, int* fit) {
+  static std::atomic<int> known[64][kKernelCount][17];  // 0: not asked yet, else fit + 1
+  int dev = 0;
+  if (c < 1 || c > 16 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)
+    return FA_ERR_NO_DEVICE;
+  std::atomic<int>& k = known[dev][kernel_id][c];
+  int v = k.load(std::memory_order_acquire);
+  if (v == 0) {
+    if (c > 8) {
+      const cudaError_t e =
+          cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return record_cuda_error(e);
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(c);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = c;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, fn, &cfg);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      if (c == 1) return record_cuda_error(e);
+      n = 0;  // no cluster of this size here
+    }
+    v = n + 1;
+    k.store(v, std::memory_order_release);
+  }
+  *fit = v - 1;
+  return FA_OK;
+}
+
 RopeArgs make_rope_args(const fa_rope_t* rope, int round_bf16, int pos_offset) {
   RopeArgs r;
   std::memset(&r, 0, sizeof(r));

@@ -80,12 +80,15 @@ struct SkinnyParams {
   __nv_bfloat16* out = nullptr;
   int64_t out_ld = 0, out_j = 0;
   const __nv_bfloat16* bias = nullptr;
-  // adapters: as WideParams; `fac` (E, i, k) with element strides
+  // adapters: low as in WideParams; per token its adapter (none: 0 for all)
   const __nv_bfloat16* low = nullptr;
   int low_ld = 0, rank = 0, E = 1;
   const int* ids = nullptr;
-  const __nv_bfloat16* fac = nullptr;
-  int64_t fac_e = 0, fac_i = 0, fac_k = 0;
+  // plain views of Small, Big and the adapters, for tokens of several
+  const __nv_bfloat16* raw_x = nullptr;
+  const __nv_bfloat16* raw_w = nullptr;
+  const __nv_bfloat16* raw_f = nullptr;
+  int64_t raw_ldx = 0, raw_ldw = 0, raw_fe = 0, raw_ldf = 0;
   float scale = 1.f;
   const float* scales = nullptr;
   const int* list_cnt = nullptr;
@@ -94,10 +97,13 @@ struct SkinnyParams {
   int slots_per_pass = 1;
 };
 
+// fac: the adapters of a linear for tokens, (E, i, rank) as Big is stored, or
+// (E, rank, i) with big_mn.
 // early: the launch may start before its predecessor ends (programmatic
 // dependent launch); only `low` may then come from that predecessor.
 int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool small_mn,
-                       SkinnyParams p, int out, bool early, cudaStream_t st);
+                       SkinnyParams p, int out, bool early, cudaStream_t st,
+                       const Mat3& fac = Mat3{});
 int launch_low_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int64_t a_e,
                     int64_t a_r, const int* ids, int E, const float* scales, float scale, int rows,
                     int K, int rank, int low_ld, __nv_bfloat16* low, cudaStream_t st);

@@ -27,6 +27,9 @@ constexpr int kThreads = 192;
 constexpr int kBig = 16384;  // 128 x 64 elements
 constexpr int kMaxStages = 8;
 constexpr int kBarBytes = 256;
+constexpr int kTwoSmem = 109 * 1024;  // two CTAs an SM, beside their static 2.6 KB
+constexpr int kOneSmem = 220 * 1024;
+constexpr int kMaxTokens = 256;
 
 struct Layout {
   int stage, stages, smem, cols;  // stage bytes, ring depth, launch bytes, TMEM columns
@@ -38,7 +41,7 @@ static Layout layout_of(int n, bool small_mn) {
   Layout l{};
   const int small = small_mn ? (n + 63) / 64 * 8192 : (n * 128 + 1023) / 1024 * 1024;
   l.stage = kBig + small;
-  const int budget = n <= 128 ? 100 * 1024 : 200 * 1024;
+  const int budget = n <= 128 ? kTwoSmem - kBarBytes - 1024 : 200 * 1024;
   l.stages = std::min(kMaxStages, budget / l.stage);
   const int exchange = (n + 8) * 512;  // the columns' owner's partial sums
   l.smem = std::max(l.stage * l.stages, exchange) + kBarBytes + 1024;
@@ -47,10 +50,91 @@ static Layout layout_of(int n, bool small_mn) {
   return l;
 }
 
+// The adapters in use by up to 256 tokens, in order of first use, and every
+// token's place among them (-1: none).
+struct TokenPlan {
+  int id[kMaxTokens];
+  int list[kMaxTokens];
+  int16_t slot[kMaxTokens];
+  int heads[8];
+  int cnt;
+};
+
+// 128 threads (named barrier 1)
+__device__ __forceinline__ void plan_tokens(TokenPlan& pl, const SkinnyParams& p) {
+  const int t = threadIdx.x;
+  if (p.ids == nullptr) {
+    for (int j = t; j < kMaxTokens; j += 128) pl.slot[j] = j < p.cols ? 0 : -1;
+    if (t == 0) pl.cnt = 1, pl.list[0] = 0;
+    named_bar_sync(1, 128);
+    return;
+  }
+  for (int j = t; j < kMaxTokens; j += 128) {
+    const int e = j < p.cols ? p.ids[j] : -1;
+    pl.id[j] = e >= 0 && e < p.E ? e : -1;
+  }
+  named_bar_sync(1, 128);
+  int first[2], before[2];
+  bool head[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int j = t + 128 * h, e = pl.id[j];
+    int f = 0;
+    if (e >= 0 && j < p.cols)
+      while (pl.id[f] != e) ++f;  // ends at j
+    else
+      f = j;
+    first[h] = f;
+    head[h] = e >= 0 && f == j;
+    const uint32_t m = __ballot_sync(0xffffffffu, head[h]);
+    before[h] = __popc(m & ((1u << lane_id()) - 1u));
+    if (lane_id() == 0) pl.heads[4 * h + warp_id()] = __popc(m);
+  }
+  named_bar_sync(1, 128);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    int at = before[h];
+    for (int w = 0; w < 4 * h + warp_id(); ++w) at += pl.heads[w];
+    if (head[h]) {
+      pl.list[at] = pl.id[t + 128 * h];
+      pl.slot[t + 128 * h] = (int16_t)at;
+    }
+  }
+  if (t == 0) {
+    int n = 0;
+    for (int w = 0; w < 8; ++w) n += pl.heads[w];
+    pl.cnt = n;
+  }
+  named_bar_sync(1, 128);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int j = t + 128 * h;
+    if (!head[h]) pl.slot[j] = pl.id[j] >= 0 ? pl.slot[first[h]] : (int16_t)-1;
+  }
+  named_bar_sync(1, 128);
+}
+
+// One output value from its own token's operands alone, for values that a
+// block of several adapters left non-finite (zero times a NaN or infinity of
+// another token's adapter).
+__device__ __noinline__ float one_value(const SkinnyParams& p, int j, int i) {
+  const __nv_bfloat16* x = p.raw_x + (int64_t)j * p.raw_ldx;
+  const __nv_bfloat16* w = p.raw_w + (int64_t)i * p.raw_ldw;
+  float acc = 0.f;
+  for (int k = 0; k < p.K; ++k) acc = fmaf(__bfloat162float(x[k]), __bfloat162float(w[k]), acc);
+  const int e = p.ids[j];
+  if (e >= 0 && e < p.E) {
+    const __nv_bfloat16* f = p.raw_f + (int64_t)e * p.raw_fe + (int64_t)i * p.raw_ldf;
+    const __nv_bfloat16* l = p.low + (int64_t)j * p.low_ld;
+    for (int k = 0; k < p.rank; ++k) acc = fmaf(__bfloat162float(l[k]), __bfloat162float(f[k]), acc);
+  }
+  return acc;
+}
+
 template <bool BIG_MN, bool SMALL_MN, int OUT>
 __global__ void __launch_bounds__(kThreads, 2)
 skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ CUtensorMap tsmall,
-              const __grid_constant__ SkinnyParams p, int split, int stage_bytes, int stages,
+              const __grid_constant__ CUtensorMap tfac, const __grid_constant__ SkinnyParams p, int split, int stage_bytes, int stages,
               int bar_off, int tmem_cols) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -59,7 +143,10 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
   uint64_t* full = bars;
   uint64_t* empty = bars + kMaxStages;
   uint64_t* done = bars + 2 * kMaxStages;
-  uint32_t* slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* planned = done + 1;
+  uint64_t* grant = planned + 1;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(grant + kMaxStages);
+  __shared__ TokenPlan plan;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
   const int warp = warp_id(), lane = lane_id();
   const int tile = blockIdx.x / split, part = blockIdx.x - tile * split;
@@ -78,10 +165,12 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < stages; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], OUT == kSkinnyCols ? 2 : 1);
       mbar_init(&empty[i], 1);
+      mbar_init(&grant[i], 1);
     }
     mbar_init(done, 1);
+    mbar_init(planned, 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tbig);
@@ -98,6 +187,10 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
   const int kbs = (p.K + 63) >> 6;
   const int kb0 = (int)((int64_t)kbs * part / split), kb1 = (int)((int64_t)kbs * (part + 1) / split);
   bool ok = true;
+  // adapters (token columns): after its share of K, the CTA's share of the
+  // K blocks that hold (adapter, 64 ranks)
+  const bool adapters = OUT == kSkinnyCols && p.low != nullptr;
+  const int kbe = (p.rank + 63) >> 6;
 
   if (warp == 4) {
     if (lane == 0) {
@@ -112,6 +205,7 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
         uint8_t* sa = smem + s * stage_bytes;
         uint8_t* sb = sa + kBig;
         mbar_arrive_expect_tx(&full[s], bytes);
+        if constexpr (OUT == kSkinnyCols) mbar_arrive(&full[s]);  // else: the builders' arrival
         if constexpr (BIG_MN) {
           tma_load_3d(sa, &tbig, &full[s], i0, kb * 64, 0);
           tma_load_3d(sa + 8192, &tbig, &full[s], i0 + 64, kb * 64, 0);
@@ -130,6 +224,22 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
           tma_load_3d(sb, &tsmall, &full[s], kb * 64, 0, 0);
         }
         if (++s == stages) { s = 0; ph ^= 1; }
+      }
+      if (ok && adapters && (ok = mbar_wait(planned, 0))) {
+        for (int x = part; x < plan.cnt * kbe; x += split) {
+          if (!(ok = mbar_wait(&empty[s], ph ^ 1))) break;
+          uint8_t* sa = smem + s * stage_bytes;
+          const int e = plan.list[x / kbe], j = x % kbe;
+          mbar_arrive(&grant[s]);
+          mbar_arrive_expect_tx(&full[s], kBig);
+          if constexpr (BIG_MN) {
+            tma_load_3d(sa, &tfac, &full[s], i0, j * 64, e);
+            tma_load_3d(sa + 8192, &tfac, &full[s], i0 + 64, j * 64, e);
+          } else {
+            tma_load_3d(sa, &tfac, &full[s], j * 64, i0, e);
+          }
+          if (++s == stages) { s = 0; ph ^= 1; }
+        }
       }
       if (!ok) *abort_flag = 1;
     }
@@ -151,12 +261,60 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
         umma_ss_w(tmem, a + (BIG_MN ? 128 : 2) * kk, b + (SMALL_MN ? 128 : 2) * kk, idesc,
                   kb > kb0 || kk > 0);
       umma_commit_w(&empty[s]);
-      if (kb == kb1 - 1) umma_commit_w(done);
+      if (!adapters && kb == kb1 - 1) umma_commit_w(done);
       if (++s == stages) { s = 0; ph ^= 1; }
+    }
+    if (ok && adapters && (ok = mbar_wait_w(planned, 0))) {
+      const int blocks = plan.cnt * kbe;
+      for (int x = part; x < blocks; x += split) {
+        if (!(ok = mbar_wait_w(&full[s], ph))) break;
+        tc_fence_after();
+        const uint64_t a = a0 + (uint32_t)(s * (stage_bytes >> 4));
+        const uint64_t b = b0 + (uint32_t)(s * (stage_bytes >> 4));
+        const int steps = min(4, (p.rank - (x % kbe) * 64 + 15) >> 4);
+        for (int kk = 0; kk < steps; ++kk)
+          umma_ss_w(tmem, a + (BIG_MN ? 128 : 2) * kk, b + 2 * kk, idesc, 1);
+        umma_commit_w(&empty[s]);
+        if (++s == stages) { s = 0; ph ^= 1; }
+      }
+      if (ok) umma_commit_w(done);
     }
     if (!ok) *abort_flag = 1;
   } else {
-    ok = mbar_wait_w(done, 0);
+    if (adapters) {
+      // the tokens' operand of each adapter block: low[j, :] in the tokens that
+      // use the adapter, zeros in the others, in the layout TMA writes
+      const int t = threadIdx.x;
+      plan_tokens(plan, p);
+      if (t == 0) mbar_arrive(planned);
+      pdl_wait_previous();
+      // A slot is theirs when the producer, which has waited for every earlier
+      // use of it, grants it: a parity wait on `empty` from here would skip
+      // phases and could return for an earlier one.
+      const int blocks = plan.cnt * kbe;
+      int s = (kb1 - kb0) % stages;
+      uint32_t turns = 0;  // bit s: parity of the slot's next grant
+      for (int x = part; x < blocks; x += split) {
+        ok = mbar_wait(&grant[s], (turns >> s) & 1);
+        if (named_bar_any(1, 128, !ok)) { ok = false; break; }
+        const int q = x / kbe, k0 = (x - q * kbe) * 64, chunks = min(8, (p.low_ld - k0) >> 3);
+        uint8_t* sb = smem + s * stage_bytes + kBig;
+#pragma unroll 4
+        for (int i = t; i < n * chunks; i += 128) {
+          const int j = i / chunks, c = i - j * chunks;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (j < p.cols && plan.slot[j] == q)
+            v = *reinterpret_cast<const uint4*>(p.low + (int64_t)j * p.low_ld + k0 + c * 8);
+          *reinterpret_cast<uint4*>(sb + sw128_offset(j, c)) = v;
+        }
+        fence_proxy_async_smem();
+        named_bar_sync(1, 128);
+        if (t == 0) mbar_arrive(&full[s]);
+        turns ^= 1u << s;
+        if (++s == stages) s = 0;
+      }
+    }
+    if (ok) ok = mbar_wait_w(done, 0);
     if (!ok) *abort_flag = 1;
   }
   tc_fence_before();
@@ -202,39 +360,15 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
   const int i = i0 + r;
   if (warp < 4 && good && i < p.rows) {
     if constexpr (OUT == kSkinnyCols) {
-      // out[j, i] (+ bias[i] + the row's low-rank term), a column a token
-      if (p.low != nullptr) pdl_wait_previous();
+      // out[j, i], a column a token
       const float bias = p.bias != nullptr ? __bfloat162float(p.bias[i]) : 0.f;
-      for (int j = j0; j < j1; ++j) {
-        float acc = bias;
+      const bool mixed = adapters && plan.cnt > 1;
+#pragma unroll 4
+      for (int j = j0; j < min(j1, p.cols); ++j) {
+        float acc = 0.f;
         for (int q = 0; q < split; ++q) acc += recv[(q * own + j - j0) * 128 + r];
-        if (j >= p.cols) break;
-        if (p.low != nullptr) {
-          const int e = p.ids != nullptr ? p.ids[j] : 0;
-          if (e >= 0 && e < p.E) {
-            const __nv_bfloat16* lw = p.low + (int64_t)j * p.low_ld;
-            const __nv_bfloat16* f = p.fac + (int64_t)e * p.fac_e + (int64_t)i * p.fac_i;
-            if (p.fac_i != 1) {  // the adapter's row i, its rank contiguous (16-byte rows)
-              int k = 0;
-              for (; k + 8 <= p.rank; k += 8) {
-                const uint4 b4 = __ldg(reinterpret_cast<const uint4*>(f + k));
-                const uint4 l4 = __ldcg(reinterpret_cast<const uint4*>(lw + k));
-                const uint32_t bw[4] = {b4.x, b4.y, b4.z, b4.w}, xw[4] = {l4.x, l4.y, l4.z, l4.w};
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                  acc = fmaf(bf16_lo(bw[u]), bf16_lo(xw[u]), acc);
-                  acc = fmaf(bf16_hi(bw[u]), bf16_hi(xw[u]), acc);
-                }
-              }
-              for (; k < p.rank; ++k)
-                acc = fmaf(__bfloat162float(f[k]), __bfloat162float(lw[k]), acc);
-            } else {  // its column i, consecutive over the threads
-              for (int k = 0; k < p.rank; ++k)
-                acc = fmaf(__bfloat162float(f[(int64_t)k * p.fac_k]), __bfloat162float(lw[k]), acc);
-            }
-          }
-        }
-        p.out[(int64_t)j * p.out_ld + i] = __float2bfloat16_rn(acc);
+        if (mixed && !isfinite(acc)) acc = one_value(p, j, i);
+        p.out[(int64_t)j * p.out_ld + i] = __float2bfloat16_rn(acc + bias);
       }
     } else if constexpr (OUT == kSkinnyLow) {
       // out[i, j]: the columns of the row's own adapter, scaled, in bf16 (the
@@ -266,24 +400,27 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
   }
 }
 
-// Inner products of few rows with their own adapters: low[n, j] = s x[n] A_e[j],
-// a warp each; columns [rank, low_ld) are zero.
+// Inner products of few rows with their own adapters: low[n, j] = s x[n] A_e[j].
+// Four warps share one (a single token's 16 products of 4096 terms would keep
+// one SM's warps alone at work for 4 us); columns [rank, low_ld) are zero.
 __global__ void __launch_bounds__(256)
 low_rows_kernel(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int64_t a_e,
                 int64_t a_r, const int* ids, int E, const float* scales, float scale, int K,
                 int rank, int low_ld, __nv_bfloat16* low) {
+  __shared__ float red[8];
   pdl_launch_next();
-  const int groups = low_ld / 8;
-  const int row = blockIdx.x / groups, j = (blockIdx.x - row * groups) * 8 + warp_id();
+  const int groups = low_ld / 2;
+  const int row = blockIdx.x / groups, j = (blockIdx.x - row * groups) * 2 + (warp_id() >> 2);
+  const int t = threadIdx.x & 127;
   const int e = ids != nullptr ? ids[row] : 0;
-  const bool has = e >= 0 && e < E;
+  const bool has = e >= 0 && e < E && j < rank;
   float acc = 0.f;
-  if (has && j < rank) {
+  if (has) {
     const uint4* xr = reinterpret_cast<const uint4*>(x + (int64_t)row * ldx);
     const uint4* ar = reinterpret_cast<const uint4*>(a + (int64_t)e * a_e + (int64_t)j * a_r);
     const int nv = K >> 3;
-#pragma unroll 8
-    for (int i = lane_id(); i < nv; i += 32) {
+#pragma unroll 4
+    for (int i = t; i < nv; i += 128) {
       const uint4 u = __ldg(xr + i), v = __ldg(ar + i);
       const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -292,15 +429,21 @@ low_rows_kernel(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int
         acc = fmaf(bf16_hi(uw[k]), bf16_hi(vw[k]), acc);
       }
     }
-    for (int k = (nv << 3) + lane_id(); k < K; k += 32)
+    const int k = (nv << 3) + t;
+    if (k < K)
       acc = fmaf(__bfloat162float(x[(int64_t)row * ldx + k]),
                  __bfloat162float(a[(int64_t)e * a_e + (int64_t)j * a_r + k]), acc);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-  if (lane_id() == 0 && j < low_ld)
+  if (lane_id() == 0) red[warp_id()] = acc;
+  __syncthreads();
+  if (t == 0) {
+    const float* s = red + (warp_id() & 4);
+    acc = (s[0] + s[1]) + (s[2] + s[3]);
     low[(int64_t)row * low_ld + j] =
-        __float2bfloat16_rn(has && j < rank ? acc * (scales != nullptr ? scales[e] : scale) : 0.f);
+        __float2bfloat16_rn(has ? acc * (scales != nullptr ? scales[e] : scale) : 0.f);
+  }
 }
 
 __global__ void __launch_bounds__(256)
@@ -341,22 +484,28 @@ plan_kernel(const int* ids, int rows, int E, int* cnt, int* list, int* slot) {
 }
 
 template <bool BIG_MN, bool SMALL_MN, int OUT>
-static int go(const CUtensorMap& tbig, const CUtensorMap& tsmall, const SkinnyParams& p,
-              int passes, int kernel_id, bool early, cudaStream_t st) {
+static int go(const CUtensorMap& tbig, const CUtensorMap& tsmall, const CUtensorMap& tfac,
+              const SkinnyParams& p, int passes, int kernel_id, bool early, cudaStream_t st) {
   auto* fn = skinny_kernel<BIG_MN, SMALL_MN, OUT>;
   const Layout l = layout_of(p.n, SMALL_MN);
   // the largest layout's request, once per kernel
-  const int rc = ensure_smem_attr((const void*)fn, 232448, kernel_id);
+  const int rc = ensure_smem_attr((const void*)fn, kOneSmem, kernel_id);
   if (rc) return rc;
   const int tiles = (p.rows + 127) / 128, kbs = (p.K + 63) / 64;
-  // CTAs resident at one time: two an SM while the ring is the smaller one
-  const int slots = l.smem <= 113 * 1024 ? 296 : 148;
-  // contraction split: the one whose rounds of CTAs times blocks per CTA
-  // (and about two blocks' time for the exchange) is smallest
+  // contraction split: the one whose rounds of resident clusters times blocks
+  // per CTA (and about two blocks' time for the exchange) is smallest. A wave
+  // that spills over costs a whole round: with 72 clusters of 4 where 66 fit,
+  // 302 MB took 74 us.
+  const bool two = l.smem <= kTwoSmem;
   int split = 1;
   int64_t best = INT64_MAX;
   for (int c = 1; c <= 8 && c <= kbs; ++c) {
-    const int64_t rounds = ((int64_t)tiles * c * passes + slots - 1) / slots;
+    int fit = 0;
+    const int rf = clusters_that_fit((const void*)fn, kThreads, two ? kTwoSmem : kOneSmem, c,
+                                     kernel_id + (two ? 0 : kKernelSkinnyBig - kKernelSkinny), &fit);
+    if (rf) return rf;
+    if (fit <= 0) continue;
+    const int64_t rounds = ((int64_t)tiles * passes + fit - 1) / fit;
     const int64_t cost = rounds * ((kbs + c - 1) / c + 2);
     if (cost < best) best = cost, split = c;
   }
@@ -374,7 +523,7 @@ static int go(const CUtensorMap& tbig, const CUtensorMap& tsmall, const SkinnyPa
   cfg.attrs = at;
   cfg.numAttrs = early ? 2 : 1;
   const int bar_off = l.smem - kBarBytes - 1024;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, tbig, tsmall, p, split, l.stage, l.stages,
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, tbig, tsmall, tfac, p, split, l.stage, l.stages,
                                            bar_off, l.cols);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -386,9 +535,9 @@ static int go(const CUtensorMap& tbig, const CUtensorMap& tsmall, const SkinnyPa
 }  // namespace skinny
 
 int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool small_mn,
-                       SkinnyParams p, int out, bool early, cudaStream_t st) {
+                       SkinnyParams p, int out, bool early, cudaStream_t st, const Mat3& fac) {
   if (p.rows == 0) return FA_OK;
-  CUtensorMap tb, ts;
+  CUtensorMap tb, ts, tf;
   int passes = 1;
   if (out == kSkinnyLow && p.list_cnt != nullptr) {
     p.slots_per_pass = std::max(1, 128 / p.low_ld);
@@ -400,25 +549,28 @@ int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool sma
   int rc = big_mn ? make_tmap_3d(&tb, big, 64, 64) : make_tmap_3d(&tb, big, 64, 128);
   const int box = out == kSkinnyLow ? p.low_ld : p.n;
   if (!rc) rc = small_mn ? make_tmap_3d(&ts, small, 64, 64) : make_tmap_3d(&ts, small, 64, box);
+  tf = tb;
+  if (!rc && out == kSkinnyCols && p.low != nullptr)
+    rc = big_mn ? make_tmap_3d(&tf, fac, 64, 64) : make_tmap_3d(&tf, fac, 64, 128);
   if (rc) return rc;
   using namespace skinny;
   if (out == kSkinnyCols && !big_mn && !small_mn)
-    return go<false, false, kSkinnyCols>(tb, ts, p, passes, kKernelSkinny, early, st);
+    return go<false, false, kSkinnyCols>(tb, ts, tf, p, passes, kKernelSkinny, early, st);
   if (out == kSkinnyCols && big_mn && !small_mn)
-    return go<true, false, kSkinnyCols>(tb, ts, p, passes, kKernelSkinny + 1, early, st);
+    return go<true, false, kSkinnyCols>(tb, ts, tf, p, passes, kKernelSkinny + 1, early, st);
   if (out == kSkinnyLow && !big_mn && !small_mn)
-    return go<false, false, kSkinnyLow>(tb, ts, p, passes, kKernelSkinny + 2, early, st);
+    return go<false, false, kSkinnyLow>(tb, ts, tf, p, passes, kKernelSkinny + 2, early, st);
   if (out == kSkinnyLow && !big_mn && small_mn)
-    return go<false, true, kSkinnyLow>(tb, ts, p, passes, kKernelSkinny + 3, early, st);
+    return go<false, true, kSkinnyLow>(tb, ts, tf, p, passes, kKernelSkinny + 3, early, st);
   if (out == kSkinnyGrad && big_mn && small_mn)
-    return go<true, true, kSkinnyGrad>(tb, ts, p, passes, kKernelSkinny + 4, early, st);
+    return go<true, true, kSkinnyGrad>(tb, ts, tf, p, passes, kKernelSkinny + 4, early, st);
   return FA_ERR_UNSUPPORTED;
 }
 
 int launch_low_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int64_t a_e,
                     int64_t a_r, const int* ids, int E, const float* scales, float scale, int rows,
                     int K, int rank, int low_ld, __nv_bfloat16* low, cudaStream_t st) {
-  skinny::low_rows_kernel<<<(unsigned)(rows * (low_ld / 8)), 256, 0, st>>>(
+  skinny::low_rows_kernel<<<(unsigned)(rows * (low_ld / 2)), 256, 0, st>>>(
       x, ldx, a, a_e, a_r, ids, E, scales, scale, K, rank, low_ld, low);
   return launch_status();
 }

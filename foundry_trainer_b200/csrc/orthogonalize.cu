@@ -34,7 +34,6 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -519,42 +518,6 @@ static Space space_of(int batch, int m, int n, int steps) {
   return s;
 }
 
-// Resident clusters of `c` CTAs, asked of the driver once per kernel and size.
-static int clusters_that_fit(const void* fn, int smem, int c, int slot, int* fit) {
-  static std::atomic<int> known[64][60];  // 0: not asked yet, else fit + 1
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FA_ERR_NO_DEVICE;
-  int v = known[dev][slot].load(std::memory_order_acquire);
-  if (v == 0) {
-    if (c > 8) {
-      const cudaError_t e =
-          cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e != cudaSuccess) return record_cuda_error(e);
-    }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(c);
-    cfg.blockDim = dim3(kThinThreads);
-    cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = c;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    int n = 0;
-    const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, fn, &cfg);
-    if (e != cudaSuccess) {
-      cudaGetLastError();
-      if (c == 1) return record_cuda_error(e);
-      n = 0;  // no cluster of this size here
-    }
-    v = n + 1;
-    known[dev][slot].store(v, std::memory_order_release);
-  }
-  *fit = v - 1;
-  return FA_OK;
-}
-
 template <typename T, int R, bool TALL>
 static int thin_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, int64_t orow,
                    int batch, int r, int len, int steps, const float* c, float eps, int kid,
@@ -568,10 +531,10 @@ static int thin_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, i
   // 1500 positions do.
   int parts = 1;
   int64_t best = INT64_MAX;
-  for (int c = 1, k = 0; c <= 16; c *= 2, ++k) {
+  for (int c = 1; c <= 16; c *= 2) {
     if (c > 1 && c * 128 > len) break;
     int fit = 0;
-    const int rf = clusters_that_fit((const void*)fn, Thin<R>::kSmem, c, (kid - kKernelThin) * 5 + k, &fit);
+    const int rf = clusters_that_fit((const void*)fn, kThinThreads, Thin<R>::kSmem, c, kid, &fit);
     if (rf) return rf;
     if (fit <= 0) break;
     const int64_t cost = (int64_t)((batch + fit - 1) / fit) * (1500 + (len + c - 1) / c);

@@ -208,6 +208,13 @@ MANY_CASES = [
     (1500, 512, 768, 128, 9, "runs"),
     (2049, 256, 512, 8, 2, "runs"),
     (600, 256, 256, 16, 4, "none"),
+    # more turns of the ring than its slots before the adapters' blocks, more
+    # adapters' blocks than slots, several clusters an SM
+    (1, 4096, 4096, 16, 4, "one"),
+    (8, 4096, 4096, 16, 8, "random"),
+    (40, 8192, 128, 64, 40, "random"),
+    (64, 4096, 6144, 16, 48, "random"),
+    (200, 2048, 3000, 96, 200, "random"),
 ]
 
 
