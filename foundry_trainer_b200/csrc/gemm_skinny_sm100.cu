@@ -33,6 +33,7 @@ constexpr int kMaxTokens = 256;
 
 struct Layout {
   int stage, stages, smem, cols;  // stage bytes, ring depth, launch bytes, TMEM columns
+  int exchange;                   // offset of the partial sums: behind the ring, or 0: over it
 };
 
 // n: columns of the product (multiple of 16), small_mn: Small stored with its
@@ -41,10 +42,15 @@ static Layout layout_of(int n, bool small_mn) {
   Layout l{};
   const int small = small_mn ? (n + 63) / 64 * 8192 : (n * 128 + 1023) / 1024 * 1024;
   l.stage = kBig + small;
-  const int budget = n <= 128 ? kTwoSmem - kBarBytes - 1024 : 200 * 1024;
-  l.stages = std::min(kMaxStages, budget / l.stage);
-  const int exchange = (n + 8) * 512;  // the columns' owner's partial sums
-  l.smem = std::max(l.stage * l.stages, exchange) + kBarBytes + 1024;
+  const int budget = (n <= 128 ? kTwoSmem : kOneSmem) - kBarBytes - 1024;
+  // the columns' owner's partial sums, owners' shares rounded up to 4 columns.
+  // While they are small they get memory of their own, so that a CTA need not
+  // wait for the others' rings before it sends.
+  const int sums = (n + 32) * 512;
+  const bool own = n <= 16;
+  l.stages = std::min(kMaxStages, (budget - (own ? sums : 0)) / l.stage);
+  l.exchange = own ? l.stage * l.stages : 0;
+  l.smem = (own ? l.exchange + sums : std::max(l.stage * l.stages, sums)) + kBarBytes + 1024;
   l.cols = 32;
   while (l.cols < n) l.cols *= 2;
   return l;
@@ -135,7 +141,7 @@ template <bool BIG_MN, bool SMALL_MN, int OUT>
 __global__ void __launch_bounds__(kThreads, 2)
 skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ CUtensorMap tsmall,
               const __grid_constant__ CUtensorMap tfac, const __grid_constant__ SkinnyParams p, int split, int stage_bytes, int stages,
-              int bar_off, int tmem_cols) {
+              int bar_off, int exchange, int tmem_cols) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -183,6 +189,7 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  if (split > 1) cluster_arrive();  // this CTA has started: its memory may be written
   const uint32_t tmem = *slot;
   const int kbs = (p.K + 63) >> 6;
   const int kb0 = (int)((int64_t)kbs * part / split), kb1 = (int)((int64_t)kbs * (part + 1) / split);
@@ -320,18 +327,21 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
   tc_fence_before();
   __syncthreads();
   if (*abort_flag) drain_delay();
-  if (split > 1) cluster_sync();  // every ring of the cluster is idle: its memory takes the sums
+  if (split > 1) {
+    cluster_wait();  // all have started
+    if (exchange == 0) cluster_sync();  // and every ring is idle: its memory takes the sums
+  }
   tc_fence_after();
 
-  // columns of owner q: [q * own, (q + 1) * own)
-  const int own = (n + split - 1) / split;
+  // columns of owner q: [q * own, (q + 1) * own); sums (split, own / 4, 128, 4)
+  const int own = ((n + split - 1) / split + 3) & ~3;
   const int j0 = part * own, j1 = min(n, j0 + own);
   const int r = threadIdx.x;
-  float* recv = reinterpret_cast<float*>(smem);  // (split, own, 128)
+  float* recv = reinterpret_cast<float*>(smem + exchange);
   const bool good = *abort_flag == 0;
   if (warp < 4 && good) {
     const uint32_t taddr = tmem + ((uint32_t)(warp * 32) << 16);
-    const uint32_t mine = smem_u32(recv) + (uint32_t)(part * own * 128 + r) * 4u;
+    const uint32_t mine = smem_u32(recv) + (uint32_t)(part * own * 512 + r * 16);
     int q = 0, at = 0;  // owner of the column, its place there
     uint32_t dst = split > 1 ? mapa(mine, 0) : mine;
     for (int c = 0; c < n; c += 16) {
@@ -339,10 +349,14 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
       tmem_ld16(taddr + c, v);
       tmem_wait_ld();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (split > 1) st_cluster_f32(dst + (uint32_t)at * 512u, __uint_as_float(v[i]));
-        else recv[(c + i) * 128 + r] = __uint_as_float(v[i]);
-        if (++at == own && q + 1 < split) {
+      for (int i = 0; i < 16; i += 4) {
+        const uint32_t a = dst + (uint32_t)at * 512u;
+        if (split > 1) st_cluster_v4(a, v[i], v[i + 1], v[i + 2], v[i + 3]);
+        else
+          *reinterpret_cast<uint4*>(recv + (c + i) * 128 + r * 4) =
+              make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        at += 4;
+        if (at == own && q + 1 < split) {
           at = 0;
           dst = mapa(mine, ++q);
         }
@@ -358,17 +372,30 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
     tmem_dealloc(tmem, tmem_cols);
   }
   const int i = i0 + r;
+  // the four columns from j on, summed in CTA order
+  auto sum4 = [&](int j, float* acc) {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q = 0; q < split; ++q) {
+      const float4 v = *reinterpret_cast<const float4*>(recv + (q * own + j - j0) * 128 + r * 4);
+      a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+    }
+    acc[0] = a.x; acc[1] = a.y; acc[2] = a.z; acc[3] = a.w;
+  };
   if (warp < 4 && good && i < p.rows) {
     if constexpr (OUT == kSkinnyCols) {
       // out[j, i], a column a token
       const float bias = p.bias != nullptr ? __bfloat162float(p.bias[i]) : 0.f;
       const bool mixed = adapters && plan.cnt > 1;
-#pragma unroll 4
-      for (int j = j0; j < min(j1, p.cols); ++j) {
-        float acc = 0.f;
-        for (int q = 0; q < split; ++q) acc += recv[(q * own + j - j0) * 128 + r];
-        if (mixed && !isfinite(acc)) acc = one_value(p, j, i);
-        p.out[(int64_t)j * p.out_ld + i] = __float2bfloat16_rn(acc + bias);
+#pragma unroll 2
+      for (int j = j0; j < min(j1, p.cols); j += 4) {
+        float acc[4];
+        sum4(j, acc);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (j + k >= p.cols) break;
+          if (mixed && !isfinite(acc[k])) acc[k] = one_value(p, j + k, i);
+          p.out[(int64_t)(j + k) * p.out_ld + i] = __float2bfloat16_rn(acc[k] + bias);
+        }
       }
     } else if constexpr (OUT == kSkinnyLow) {
       // out[i, j]: the columns of the row's own adapter, scaled, in bf16 (the
@@ -380,10 +407,11 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
         sc = p.scales[p.list_ids[(int64_t)(i0 >> 8) * 256 + s0 + sl]];
       const int lo = max(j0, sl * p.low_ld), hi = min(j1, (sl + 1) * p.low_ld);
       if (sl >= 0 && sl < ns) {
-        for (int j = lo; j < hi; ++j) {
-          float acc = 0.f;
-          for (int q = 0; q < split; ++q) acc += recv[(q * own + j - j0) * 128 + r];
-          p.out[(int64_t)i * p.out_ld + j - sl * p.low_ld] = __float2bfloat16_rn(acc * sc);
+        for (int j = lo; j < hi; j += 4) {  // (all bounds are multiples of 4)
+          float acc[4];
+          sum4(j, acc);
+          *reinterpret_cast<uint2*>(p.out + (int64_t)i * p.out_ld + j - sl * p.low_ld) =
+              make_uint2(pack_bf16(acc[0] * sc, acc[1] * sc), pack_bf16(acc[2] * sc, acc[3] * sc));
         }
       } else if (p.slot != nullptr && p.slot[i] < 0 && s0 == 0 && part == 0) {
         // a row without an adapter: zeros (a block whose other rows share one
@@ -391,10 +419,13 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
         for (int j = 0; j < p.low_ld; ++j) p.out[(int64_t)i * p.out_ld + j] = __float2bfloat16_rn(0.f);
       }
     } else {
-      for (int j = j0; j < min(j1, p.cols); ++j) {
-        float acc = 0.f;
-        for (int q = 0; q < split; ++q) acc += recv[(q * own + j - j0) * 128 + r];
-        p.out[(int64_t)j * p.out_j + (int64_t)i * p.out_ld] = __float2bfloat16_rn(acc);
+      for (int j = j0; j < min(j1, p.cols); j += 4) {
+        float acc[4];
+        sum4(j, acc);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (j + k < p.cols)
+            p.out[(int64_t)(j + k) * p.out_j + (int64_t)i * p.out_ld] = __float2bfloat16_rn(acc[k]);
       }
     }
   }
@@ -524,7 +555,7 @@ static int go(const CUtensorMap& tbig, const CUtensorMap& tsmall, const CUtensor
   cfg.numAttrs = early ? 2 : 1;
   const int bar_off = l.smem - kBarBytes - 1024;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, tbig, tsmall, tfac, p, split, l.stage, l.stages,
-                                           bar_off, l.cols);
+                                           bar_off, l.exchange, l.cols);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return record_cuda_error(e);
