@@ -58,7 +58,7 @@ static Layout layout_of(int n, bool small_mn) {
 
 // The adapters in use by up to 256 tokens, in order of first use, and every
 // token's place among them (-1: none).
-struct TokenPlan {
+struct alignas(16) TokenPlan {
   int id[kMaxTokens];
   int list[kMaxTokens];
   int16_t slot[kMaxTokens];
@@ -85,11 +85,16 @@ __device__ __forceinline__ void plan_tokens(TokenPlan& pl, const SkinnyParams& p
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int j = t + 128 * h, e = pl.id[j];
-    int f = 0;
-    if (e >= 0 && j < p.cols)
-      while (pl.id[f] != e) ++f;  // ends at j
-    else
-      f = j;
+    int f = j;
+    if (e >= 0) {  // four at a time; ends at j at the latest
+      for (int b = 0;; b += 4) {
+        const int4 v = *reinterpret_cast<const int4*>(&pl.id[b]);
+        if (v.x == e) { f = b; break; }
+        if (v.y == e) { f = b + 1; break; }
+        if (v.z == e) { f = b + 2; break; }
+        if (v.w == e) { f = b + 3; break; }
+      }
+    }
     first[h] = f;
     head[h] = e >= 0 && f == j;
     const uint32_t m = __ballot_sync(0xffffffffu, head[h]);
@@ -295,30 +300,63 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
       plan_tokens(plan, p);
       if (t == 0) mbar_arrive(planned);
       pdl_wait_previous();
-      // A slot is theirs when the producer, which has waited for every earlier
-      // use of it, grants it: a parity wait on `empty` from here would skip
-      // phases and could return for an earlier one.
+      // A warp builds for every fourth slot of the ring. A slot is its when the
+      // producer, which has waited for every earlier use of it, grants it: a
+      // parity wait on `empty` from here would skip phases and could return
+      // for an earlier one.
       const int blocks = plan.cnt * kbe;
       int s = (kb1 - kb0) % stages;
       uint32_t turns = 0;  // bit s: parity of the slot's next grant
-      for (int x = part; x < blocks; x += split) {
-        ok = mbar_wait(&grant[s], (turns >> s) & 1);
-        if (named_bar_any(1, 128, !ok)) { ok = false; break; }
-        const int q = x / kbe, k0 = (x - q * kbe) * 64, chunks = min(8, (p.low_ld - k0) >> 3);
+      // A lane's 16-byte pieces of the operand are the same in every block
+      // while one block holds the rank: up to 16 are kept in registers (with
+      // their place, and the adapter's slot above it) and a block is stores
+      // alone.
+      constexpr int kHold = 16;
+      const int chunks0 = min(8, p.low_ld >> 3);
+      const bool held = kbe == 1 && n * chunks0 <= kHold * 32;
+      uint4 hold[kHold];
+      int at[kHold];
+      if (held) {
+#pragma unroll
+        for (int k = 0; k < kHold; ++k) {
+          const int i = lane + 32 * k, j = i / chunks0, c = i - j * chunks0;
+          at[k] = -1;
+          hold[k] = make_uint4(0, 0, 0, 0);
+          if (i < n * chunks0) {
+            at[k] = (int)sw128_offset(j, c) | 511 << 16;
+            if (j < p.cols && plan.slot[j] >= 0) {
+              at[k] = (int)sw128_offset(j, c) | plan.slot[j] << 16;
+              hold[k] = *reinterpret_cast<const uint4*>(p.low + (int64_t)j * p.low_ld + c * 8);
+            }
+          }
+        }
+      }
+      for (int x = part; x < blocks; x += split, s = s + 1 == stages ? 0 : s + 1) {
+        if ((s & 3) != warp) continue;
+        if (!(ok = mbar_wait_w(&grant[s], (turns >> s) & 1))) break;
+        turns ^= 1u << s;
+        const int q = x / kbe;
         uint8_t* sb = smem + s * stage_bytes + kBig;
-#pragma unroll 4
-        for (int i = t; i < n * chunks; i += 128) {
-          const int j = i / chunks, c = i - j * chunks;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (j < p.cols && plan.slot[j] == q)
-            v = *reinterpret_cast<const uint4*>(p.low + (int64_t)j * p.low_ld + k0 + c * 8);
-          *reinterpret_cast<uint4*>(sb + sw128_offset(j, c)) = v;
+        if (held) {
+#pragma unroll
+          for (int k = 0; k < kHold; ++k)
+            if (at[k] >= 0)
+              *reinterpret_cast<uint4*>(sb + (at[k] & 0xffff)) =
+                  (at[k] >> 16) == q ? hold[k] : make_uint4(0, 0, 0, 0);
+        } else {
+          const int k0 = (x - q * kbe) * 64, chunks = min(8, (p.low_ld - k0) >> 3);
+#pragma unroll 8
+          for (int i = lane; i < n * chunks; i += 32) {
+            const int j = i / chunks, c = i - j * chunks;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (j < p.cols && plan.slot[j] == q)
+              v = *reinterpret_cast<const uint4*>(p.low + (int64_t)j * p.low_ld + k0 + c * 8);
+            *reinterpret_cast<uint4*>(sb + sw128_offset(j, c)) = v;
+          }
         }
         fence_proxy_async_smem();
-        named_bar_sync(1, 128);
-        if (t == 0) mbar_arrive(&full[s]);
-        turns ^= 1u << s;
-        if (++s == stages) s = 0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[s]);
       }
     }
     if (ok) ok = mbar_wait_w(done, 0);
