@@ -70,13 +70,11 @@ static size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 static const __nv_bfloat16* bfp(const void* p) { return reinterpret_cast<const __nv_bfloat16*>(p); }
 
-// Up to 256 rows the weight's bytes are the cost and its rows make the
-// 128-row side; beyond, the tokens do (measured at 4096 x 4096, rank 16).
-constexpr int kFewRows = 256;
 // Up to 64 rows four warps per inner product beat the tensor-core form's fixed
 // cost (at 4096, rank 16: 64 rows 4.4 us against 8.3 us). With many adapters
-// the other form also needs a plan of the rows first: up to kFewRows there.
+// the other form also needs a plan of the rows first: up to 256 there.
 constexpr int kDotRows = 64;
+constexpr int kDotRowsMany = 256;
 
 }  // namespace fa
 
@@ -148,11 +146,11 @@ int fa_lora_linear_fwd(int dtype, int rows, int in_dim, int out_dim, int rank,
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int ld = low_dim(rank);
   __nv_bfloat16* lw = reinterpret_cast<__nv_bfloat16*>(low);
-  bool early = false;
+  // the product starts while the low-rank factor's kernel runs (which itself
+  // starts when all earlier work is done) and waits for it where it needs it
   if (rows <= kDotRows) {
     FA_TRY(launch_low_rows(bfp(x->data), x->stride_row, bfp(a->data), 0, a->stride_row, nullptr, 1,
                            nullptr, scale, rows, in_dim, rank, ld, lw, st));
-    early = true;
   } else {
     SkinnyParams s;
     s.rows = rows;
@@ -164,11 +162,10 @@ int fa_lora_linear_fwd(int dtype, int rows, int in_dim, int out_dim, int rank,
     FA_TRY(launch_gemm_skinny(mat(x, 1, rows, in_dim), false, mat(a, 1, rank, in_dim), false, s,
                               kSkinnyLow, false, st));
   }
-  if (rows <= kFewRows) {
+  if (linear_as_columns(out_dim, in_dim, rows)) {
     SkinnyParams s;
     s.rows = out_dim;
     s.cols = rows;
-    s.n = (rows + 15) / 16 * 16;
     s.K = in_dim;
     s.out = reinterpret_cast<__nv_bfloat16*>(y->data);
     s.out_ld = y->stride_row;
@@ -177,7 +174,7 @@ int fa_lora_linear_fwd(int dtype, int rows, int in_dim, int out_dim, int rank,
     s.low_ld = ld;
     s.rank = rank;
     return launch_gemm_skinny(mat(w, 1, out_dim, in_dim), false, mat(x, 1, rows, in_dim), false, s,
-                              kSkinnyCols, early, st, mat(b, 1, out_dim, rank));
+                              kSkinnyCols, true, st, mat(b, 1, out_dim, rank));
   }
   WideOperands o;
   o.a = mat(x, 1, rows, in_dim);
@@ -191,6 +188,7 @@ int fa_lora_linear_fwd(int dtype, int rows, int in_dim, int out_dim, int rank,
   p.low = lw;
   p.low_ld = ld;
   p.rank = rank;
+  p.early = 1;
   p.bias = bfp(bias);
   return launch_gemm_wide(o, p, kEpiLinear, st);
 }
@@ -232,6 +230,7 @@ int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
   FA_TRY(check_sm100());
   const int ld = low_dim(rank);
   __nv_bfloat16* u = reinterpret_cast<__nv_bfloat16*>(workspace);
+  // every kernel after the first starts early and waits for the one before it
   {  // U = scale dy B
     SkinnyParams s;
     s.rows = rows;
@@ -253,20 +252,19 @@ int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
     s.out_ld = 1;
     s.out_j = in_dim;
     FA_TRY(launch_gemm_skinny(mat(x, 1, rows, in_dim), true, dense(u, rows, ld, ld), true, s,
-                              kSkinnyGrad, false, st));
+                              kSkinnyGrad, true, st));
     s.rows = out_dim;  // db = dy^T low
     s.out = reinterpret_cast<__nv_bfloat16*>(db);
     s.out_ld = rank;
     s.out_j = 1;
     FA_TRY(launch_gemm_skinny(mat(dy, 1, rows, out_dim), true, dense(low, rows, ld, ld), true, s,
-                              kSkinnyGrad, false, st));
+                              kSkinnyGrad, true, st));
   }
   if (dx == nullptr) return FA_OK;
-  if (rows <= kFewRows) {
+  if (linear_as_columns(in_dim, out_dim, rows)) {
     SkinnyParams s;
     s.rows = in_dim;
     s.cols = rows;
-    s.n = (rows + 15) / 16 * 16;
     s.K = out_dim;
     s.out = reinterpret_cast<__nv_bfloat16*>(dx->data);
     s.out_ld = dx->stride_row;
@@ -274,7 +272,7 @@ int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
     s.low_ld = ld;
     s.rank = rank;
     return launch_gemm_skinny(mat(w, 1, out_dim, in_dim), true, mat(dy, 1, rows, out_dim), false, s,
-                              kSkinnyCols, false, st, mat(a, 1, rank, in_dim));
+                              kSkinnyCols, true, st, mat(a, 1, rank, in_dim));
   }
   WideOperands o;
   o.b_mn = true;
@@ -289,6 +287,7 @@ int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
   p.low = u;
   p.low_ld = ld;
   p.rank = rank;
+  p.early = 1;
   return launch_gemm_wide(o, p, kEpiLinear, st);
 }
 
@@ -342,14 +341,13 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
   int* list = reinterpret_cast<int*>(ws);
   ws += align256(blocks * 256 * 4);
   int* slot = reinterpret_cast<int*>(ws);
-  bool early = false;
-  if (rows <= kFewRows) {
+  const bool dots = rows <= kDotRowsMany, columns = linear_as_columns(out_dim, in_dim, rows);
+  if (!dots || !columns) FA_TRY(launch_adapter_plan(ids, rows, n_adapters, cnt, list, slot, st));
+  if (dots) {
     FA_TRY(launch_low_rows(bfp(x->data), x->stride_row, bfp(a->data), a->stride_batch,
                            a->stride_row, ids, n_adapters, scales, 1.f, rows, in_dim, rank, ld, low,
                            st));
-    early = true;
   } else {
-    FA_TRY(launch_adapter_plan(ids, rows, n_adapters, cnt, list, slot, st));
     SkinnyParams s;
     s.rows = rows;
     s.cols = s.n = s.low_ld = ld;
@@ -364,11 +362,10 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
     FA_TRY(launch_gemm_skinny(mat(x, 1, rows, in_dim), false, mat(a, n_adapters, rank, in_dim),
                               false, s, kSkinnyLow, false, st));
   }
-  if (rows <= kFewRows) {
+  if (columns) {
     SkinnyParams s;
     s.rows = out_dim;
     s.cols = rows;
-    s.n = (rows + 15) / 16 * 16;
     s.K = in_dim;
     s.out = reinterpret_cast<__nv_bfloat16*>(y->data);
     s.out_ld = y->stride_row;
@@ -386,7 +383,7 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
     s.raw_fe = b->stride_batch;
     s.raw_ldf = b->stride_row;
     return launch_gemm_skinny(mat(w, 1, out_dim, in_dim), false, mat(x, 1, rows, in_dim), false, s,
-                              kSkinnyCols, early, st, mat(b, n_adapters, out_dim, rank));
+                              kSkinnyCols, true, st, mat(b, n_adapters, out_dim, rank));
   }
   WideOperands o;
   o.a = mat(x, 1, rows, in_dim);
@@ -403,6 +400,7 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
   p.list_cnt = cnt;
   p.list_ids = list;
   p.slot = slot;
+  p.early = 1;
   p.raw_x = bfp(x->data);
   p.raw_ldx = x->stride_row;
   p.raw_w = bfp(w->data);

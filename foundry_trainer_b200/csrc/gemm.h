@@ -45,6 +45,10 @@ struct WideParams {
   const int* list_cnt = nullptr;
   const int* list_ids = nullptr;
   const int* slot = nullptr;
+  // Programmatic dependent launch. 1: of what this product reads only `low`
+  // may come from the previous kernel (all older work is complete when that
+  // one starts); 2: anything may.
+  int early = 0;
   // plain views of A, B and the adapters (E, N, rank), for blocks of several
   const __nv_bfloat16* raw_x = nullptr;
   const __nv_bfloat16* raw_w = nullptr;
@@ -65,7 +69,9 @@ struct WideParams {
   int64_t out_t_batch = 0, out_t_ld = 0;
 };
 
-// out[i, j] = sum_k Big[i, k] Small[j, k], j < n <= 256
+// out[i, j] = sum_k Big[i, k] Small[j, k], j < n <= 256 (token columns: any
+// number, in blocks)
+constexpr int kMaxColumns = 256;
 enum SkinnyOut {
   kSkinnyCols = 0,  // out[j, i] bf16 + bias[i] + the adapters' term of row j
   kSkinnyLow = 1,   // out[i, j] bf16, scaled: a row's own adapter's columns
@@ -104,6 +110,8 @@ struct SkinnyParams {
 int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool small_mn,
                        SkinnyParams p, int out, bool early, cudaStream_t st,
                        const Mat3& fac = Mat3{});
+// whether a linear of `rows` tokens runs as kSkinnyCols rather than wide
+bool linear_as_columns(int64_t out, int64_t K, int rows);
 int launch_low_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int64_t a_e,
                     int64_t a_r, const int* ids, int E, const float* scales, float scale, int rows,
                     int K, int rank, int low_ld, __nv_bfloat16* low, cudaStream_t st);

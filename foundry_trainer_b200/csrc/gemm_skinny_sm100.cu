@@ -29,7 +29,7 @@ constexpr int kMaxStages = 8;
 constexpr int kBarBytes = 256;
 constexpr int kTwoSmem = 109 * 1024;  // two CTAs an SM, beside their static 2.6 KB
 constexpr int kOneSmem = 220 * 1024;
-constexpr int kMaxTokens = 256;
+constexpr int kMaxTokens = kMaxColumns;
 
 struct Layout {
   int stage, stages, smem, cols;  // stage bytes, ring depth, launch bytes, TMEM columns
@@ -67,17 +67,17 @@ struct alignas(16) TokenPlan {
 };
 
 // 128 threads (named barrier 1)
-__device__ __forceinline__ void plan_tokens(TokenPlan& pl, const SkinnyParams& p) {
+__device__ __forceinline__ void plan_tokens(TokenPlan& pl, const int* ids, int cols, int E) {
   const int t = threadIdx.x;
-  if (p.ids == nullptr) {
-    for (int j = t; j < kMaxTokens; j += 128) pl.slot[j] = j < p.cols ? 0 : -1;
+  if (ids == nullptr) {
+    for (int j = t; j < kMaxTokens; j += 128) pl.slot[j] = j < cols ? 0 : -1;
     if (t == 0) pl.cnt = 1, pl.list[0] = 0;
     named_bar_sync(1, 128);
     return;
   }
   for (int j = t; j < kMaxTokens; j += 128) {
-    const int e = j < p.cols ? p.ids[j] : -1;
-    pl.id[j] = e >= 0 && e < p.E ? e : -1;
+    const int e = j < cols ? ids[j] : -1;
+    pl.id[j] = e >= 0 && e < E ? e : -1;
   }
   named_bar_sync(1, 128);
   int first[2], before[2];
@@ -163,8 +163,12 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
   const int tile = blockIdx.x / split, part = blockIdx.x - tile * split;
   const int i0 = tile * 128;
 
-  // columns of this pass: adapters [s0, s0 + ns) of the tile's list, or all
+  // columns of this pass: adapters [s0, s0 + ns) of the tile's list, or all;
+  // of a linear the tokens j_base .. j_base + cols
   int n = p.n, s0 = 0, ns = 1;
+  const int j_base = OUT == kSkinnyCols ? blockIdx.y * p.n : 0;
+  const int cols = min(p.n, p.cols - j_base);
+  const __nv_bfloat16* low = p.low != nullptr ? p.low + (int64_t)j_base * p.low_ld : nullptr;
   if constexpr (OUT == kSkinnyLow) {
     if (p.list_cnt != nullptr) {
       s0 = blockIdx.y * p.slots_per_pass;
@@ -204,6 +208,7 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
   const bool adapters = OUT == kSkinnyCols && p.low != nullptr;
   const int kbe = (p.rank + 63) >> 6;
 
+  pdl_launch_next();
   if (warp == 4) {
     if (lane == 0) {
       if constexpr (OUT != kSkinnyCols) pdl_wait_previous();
@@ -233,7 +238,7 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
             tma_load_3d(sb + q * p.low_ld * 128, &tsmall, &full[s], kb * 64, 0, e);
           }
         } else {
-          tma_load_3d(sb, &tsmall, &full[s], kb * 64, 0, 0);
+          tma_load_3d(sb, &tsmall, &full[s], kb * 64, j_base, 0);
         }
         if (++s == stages) { s = 0; ph ^= 1; }
       }
@@ -297,7 +302,7 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
       // the tokens' operand of each adapter block: low[j, :] in the tokens that
       // use the adapter, zeros in the others, in the layout TMA writes
       const int t = threadIdx.x;
-      plan_tokens(plan, p);
+      plan_tokens(plan, p.ids != nullptr ? p.ids + j_base : nullptr, cols, p.E);
       if (t == 0) mbar_arrive(planned);
       pdl_wait_previous();
       // A warp builds for every fourth slot of the ring. A slot is its when the
@@ -324,9 +329,9 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
           hold[k] = make_uint4(0, 0, 0, 0);
           if (i < n * chunks0) {
             at[k] = (int)sw128_offset(j, c) | 511 << 16;
-            if (j < p.cols && plan.slot[j] >= 0) {
+            if (j < cols && plan.slot[j] >= 0) {
               at[k] = (int)sw128_offset(j, c) | plan.slot[j] << 16;
-              hold[k] = *reinterpret_cast<const uint4*>(p.low + (int64_t)j * p.low_ld + c * 8);
+              hold[k] = *reinterpret_cast<const uint4*>(low + (int64_t)j * p.low_ld + c * 8);
             }
           }
         }
@@ -349,8 +354,8 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
           for (int i = lane; i < n * chunks; i += 32) {
             const int j = i / chunks, c = i - j * chunks;
             uint4 v = make_uint4(0, 0, 0, 0);
-            if (j < p.cols && plan.slot[j] == q)
-              v = *reinterpret_cast<const uint4*>(p.low + (int64_t)j * p.low_ld + k0 + c * 8);
+            if (j < cols && plan.slot[j] == q)
+              v = *reinterpret_cast<const uint4*>(low + (int64_t)j * p.low_ld + k0 + c * 8);
             *reinterpret_cast<uint4*>(sb + sw128_offset(j, c)) = v;
           }
         }
@@ -425,14 +430,14 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
       const float bias = p.bias != nullptr ? __bfloat162float(p.bias[i]) : 0.f;
       const bool mixed = adapters && plan.cnt > 1;
 #pragma unroll 2
-      for (int j = j0; j < min(j1, p.cols); j += 4) {
+      for (int j = j0; j < min(j1, cols); j += 4) {
         float acc[4];
         sum4(j, acc);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          if (j + k >= p.cols) break;
-          if (mixed && !isfinite(acc[k])) acc[k] = one_value(p, j + k, i);
-          p.out[(int64_t)(j + k) * p.out_ld + i] = __float2bfloat16_rn(acc[k] + bias);
+          if (j + k >= cols) break;
+          if (mixed && !isfinite(acc[k])) acc[k] = one_value(p, j_base + j + k, i);
+          p.out[(int64_t)(j_base + j + k) * p.out_ld + i] = __float2bfloat16_rn(acc[k] + bias);
         }
       }
     } else if constexpr (OUT == kSkinnyLow) {
@@ -608,6 +613,11 @@ int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool sma
   if (p.rows == 0) return FA_OK;
   CUtensorMap tb, ts, tf;
   int passes = 1;
+  if (out == kSkinnyCols) {  // even blocks of up to 256 tokens
+    passes = (p.cols + kMaxColumns - 1) / kMaxColumns;
+    p.n = ((p.cols + passes - 1) / passes + 15) / 16 * 16;
+    passes = (p.cols + p.n - 1) / p.n;
+  }
   if (out == kSkinnyLow && p.list_cnt != nullptr) {
     p.slots_per_pass = std::max(1, 128 / p.low_ld);
     const int most = std::min(p.E, 256);
@@ -634,6 +644,39 @@ int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool sma
   if (out == kSkinnyGrad && big_mn && small_mn)
     return go<true, true, kSkinnyGrad>(tb, ts, tf, p, passes, kKernelSkinny + 4, early, st);
   return FA_ERR_UNSUPPORTED;
+}
+
+// Estimated microseconds of a linear as token columns: rounds of resident CTAs
+// times K blocks of tensor work (0.45 us at 256 columns, shared by the CTAs of
+// an SM, 0.19 us at least), no less than the weight's way from memory; and
+// what does not depend on K: start, exchange, output. Within 20 percent of
+// 88 measured shapes (65 to 2048 rows, 1024 to 16384 wide).
+static float cols_time(int64_t out, int64_t K, int rows) {
+  const int blocks = (rows + kMaxColumns - 1) / kMaxColumns;
+  const int n = ((rows + blocks - 1) / blocks + 15) / 16 * 16;
+  const int64_t tiles = (out + 127) / 128 * blocks, kbs = (K + 63) / 64;
+  const int per_sm = n <= 128 ? 2 : 1;
+  const float kb = std::max(0.45f * n / 256.f, 0.19f) * per_sm;
+  float best = 1e30f;
+  for (int c = 1; c <= 8 && c <= kbs; ++c) {
+    const int fit = per_sm * (c <= 2 ? 148 : (c <= 4 ? 132 : 120)) / c;
+    const int64_t rounds = (tiles + fit - 1) / fit;
+    best = std::min(best, rounds * (((kbs + c - 1) / c) * kb + 7.5f * n / 256.f));
+  }
+  return std::max(best, (float)(out * K * 2) / 6e6f) + 7.f;
+}
+
+// The same as 256 x 256 tiles of the pair form: 0.29 us a K block, 7 us apart.
+static float wide_time(int64_t out, int64_t K, int rows) {
+  const int64_t tiles = (int64_t)((rows + 255) / 256) * ((out + 255) / 256), kbs = (K + 63) / 64;
+  return 7.f + (tiles + 73) / 74 * kbs * 0.29f;
+}
+
+// Few 256 x 256 tiles leave SM pairs idle, where token columns split the
+// contraction over clusters (256 rows, 16384 -> 4096: 42 us against 82); many
+// fill them at half the staged bytes (512 rows, 4096 -> 16384: 97 against 52).
+bool linear_as_columns(int64_t out, int64_t K, int rows) {
+  return rows <= 64 || cols_time(out, K, rows) < wide_time(out, K, rows);
 }
 
 int launch_low_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int64_t a_e,

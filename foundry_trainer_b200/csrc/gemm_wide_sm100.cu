@@ -150,6 +150,8 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
   tc_fence_after();
   const uint32_t tmem = *slot;
 
+  pdl_launch_next();
+  if (p.early == 2) pdl_wait_previous();
   const int64_t tiles = (int64_t)p.tiles_per_batch * p.batch;
   const int pairs = gridDim.x >> 1;
   const int kb_main = (p.K + 63) >> 6;
@@ -175,6 +177,8 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
       int hold_slot[kHold];
       const int chunks = p.low_ld >> 3, lg = chunks == 4 ? 2 : 1;
       const bool held = EPI == kEpiLinear && (chunks == 2 || chunks == 4);
+      // (its lists are older; low itself may be the previous kernel's)
+      if (ns > 1 && held && p.early == 1) pdl_wait_previous();
       if (ns > 1 && held) {
 #pragma unroll
         for (int i = 0; i < kHold; ++i) {
@@ -207,6 +211,7 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
         if (++s == kStages) { s = 0; ph ^= 1; }
       }
       if (!ok || ns == 0) continue;
+      if (p.early == 1) pdl_wait_previous();
       for (int q = 0; q < ns && ok; ++q) {
         const int e = p.list_ids != nullptr ? p.list_ids[(int64_t)tl.m * 256 + q] : 0;
         for (int j = 0; j < kb_ext; ++j) {
@@ -262,6 +267,9 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
         }
       }
     }
+    // (also where no tile had an adapter: this kernel's end stands for the
+    // previous one's)
+    if (p.early == 1) pdl_wait_previous();
     if (!ok) *abort_flag = 1;
   } else if (warp == 5) {
     // ------------------------------------------------------------ tcgen05
@@ -503,7 +511,21 @@ static int go(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& t
   if (rc) return rc;
   const int64_t tiles = (int64_t)p.tiles_per_batch * p.batch;
   const int pairs = (int)std::min<int64_t>(tiles, 74);
-  fn<<<2 * pairs, kThreads, kSmem, st>>>(ta, tb, te, tlow, td, td2, p);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * pairs);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.early ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, ta, tb, te, tlow, td, td2, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return record_cuda_error(e);
+  }
   return launch_status();
 }
 

@@ -630,6 +630,7 @@ static int wide_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, i
       p.K = n;
       p.batch = batch;
       p.fmt = 0;
+      p.early = 2;
       p.symmetric = 1;
       p.alpha = 1.f / 1024.f;
       p.sym_out = q;
@@ -645,6 +646,7 @@ static int wide_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, i
       p.M = p.N = p.K = m;
       p.batch = batch;
       p.fmt = 0;
+      p.early = 2;
       p.symmetric = 1;
       p.coef = coef + (int64_t)(2 * s) * batch * 2;
       p.in_hi = q;
@@ -665,6 +667,7 @@ static int wide_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, i
     p.N = n;
     p.batch = batch;
     p.fmt = 0;
+    p.early = 2;
     p.coef = coef + (int64_t)(2 * s + 1) * batch * 2;
     p.in_hi = h;
     p.in_lo = lo;
