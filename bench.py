@@ -320,7 +320,8 @@ def run_block(args, rank, world, local):
     t_img, t_txt = mk(1, grid * grid, dim), mk(1, txt_len, dim)
 
     tr = blocks.LoraTrainer(w, shape, blocks.joint_positions(txt_len, grid), lora_scale=1.0,
-                            grad_hook=blocks.allreduce_mean if world > 1 else None)
+                            grad_hook=blocks.allreduce_mean if world > 1 else None,
+                            kernels=blocks.FusedKernels() if args.fused_block else None)
     step = lambda: tr.step(img, txt, temb, t_img, t_txt)
     flush_buf = torch.empty(256 * 1024 * 1024 // 4, device=dev, dtype=torch.float32)
     lib = _lib.load()
@@ -418,6 +419,8 @@ def run_block(args, rank, world, local):
                                f"{txt_len} text + {grid}x{grid} image tokens, 4x GELU MLP, "
                                f"LoRA r{rank_lora} alpha 16 on q/k/v/out of both streams",
                    "parallelism": f"data-parallel x{world} (LoRA grads all-reduced)",
+                   "block_kernels": "fused norms and adapter linears" if args.fused_block
+                                    else "torch norms and linears",
                    "l2": "flushed between timed steps (256 MB write outside the step events)"},
         "roofline": {"kernel": "attn_bwd_kernel", "bound": "tensor",
                      "achieved": attn_bwd_flops / (kt["bwd"] / 1e3) / 1e12 if kt["bwd"] else None,
@@ -429,8 +432,9 @@ def run_block(args, rank, world, local):
         "cpu_baseline": cpu,
         "e2e": e2e,
         # per step: q, k prologues + v concat + fwd; dO concat + delta + bwd +
-        # dQ finish + q, k prologue backwards
-        "gpu_launches": 10 * K,
+        # dQ finish + q, k prologue backwards; fused: 4 norms of 3 launches and
+        # 8 adapter linears of 6
+        "gpu_launches": (10 + (60 if args.fused_block else 0)) * K,
         "clocks": clocks,
     }
     print(json.dumps(line), flush=True)
@@ -456,6 +460,9 @@ def main():
                          "kernel beside the attention CTAs (sm)")
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--no-e2e", action="store_true")
+    ap.add_argument("--fused-block", action="store_true",
+                    help="c3: the block's norms and adapter linears on this framework's kernels "
+                         "(blocks.FusedKernels) instead of torch's")
     ap.add_argument("--ncu-case", action="store_true",
                     help="run --warmup eager fwd+bwd steps of --config and exit (no timing): "
                          "the small case ncu captures")

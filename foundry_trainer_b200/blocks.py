@@ -21,7 +21,11 @@ B200 op with its fused q/k RMSNorm + RoPE prologue (`attn.JointAttention`
 for the double block, `SingleAttention` here for the single block), which
 take the per-stream projections before the norm and return the attention
 output. Everything else (the linears, norms, modulation, MLPs) is torch on
-the device: cuBLAS GEMMs and elementwise kernels.
+the device: cuBLAS GEMMs and elementwise kernels; with `kernels=FusedKernels()`
+the norms and the linears with LoRA factors run on the framework's own kernels
+(ops.layer_norm, ops.lora_linear), and the linears of a batch of requests on
+ops.lora_linear_many. Muon is the other optimiser of the factors
+(ops.orthogonalize).
 
 Two block variants share this code:
   * the reference's (its fixtures and klein harness): one modulation linear
@@ -36,7 +40,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import Callable, Dict, List, Optional, Tuple
+from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -69,16 +73,20 @@ def linear(w: Weights, name: str, x: torch.Tensor, lora_scale: float) -> torch.T
     return y
 
 
-def swiglu(w: Weights, name: str, x: torch.Tensor, lora_scale: float) -> torch.Tensor:
-    gate = F.silu(linear(w, f"{name}.gate", x, lora_scale))
-    up = linear(w, f"{name}.up", x, lora_scale)
-    return linear(w, f"{name}.down", gate * up, lora_scale)
+def swiglu(w: Weights, name: str, x: torch.Tensor, lora_scale: float,
+           kernels: Optional["FusedKernels"] = None) -> torch.Tensor:
+    lin = linear if kernels is None else kernels.linear
+    gate = F.silu(lin(w, f"{name}.gate", x, lora_scale))
+    up = lin(w, f"{name}.up", x, lora_scale)
+    return lin(w, f"{name}.down", gate * up, lora_scale)
 
 
-def gelu_mlp(w: Weights, name: str, x: torch.Tensor, lora_scale: float) -> torch.Tensor:
+def gelu_mlp(w: Weights, name: str, x: torch.Tensor, lora_scale: float,
+             kernels: Optional["FusedKernels"] = None) -> torch.Tensor:
     """The FLUX MLP: fc2(gelu_tanh(fc1(x))), hidden 4x."""
-    return linear(w, f"{name}.fc2", F.gelu(linear(w, f"{name}.fc1", x, lora_scale),
-                                           approximate="tanh"), lora_scale)
+    lin = linear if kernels is None else kernels.linear
+    return lin(w, f"{name}.fc2", F.gelu(lin(w, f"{name}.fc1", x, lora_scale),
+                                        approximate="tanh"), lora_scale)
 
 
 def layer_norm_mod(x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor,
@@ -96,10 +104,11 @@ def mse(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     return (d * d).mean()
 
 
-def _mlp(w: Weights, name: str, x: torch.Tensor, lora_scale: float) -> torch.Tensor:
+def _mlp(w: Weights, name: str, x: torch.Tensor, lora_scale: float,
+         kernels: Optional["FusedKernels"] = None) -> torch.Tensor:
     if f"weights/{name}.fc1.weight" in w:
-        return gelu_mlp(w, name, x, lora_scale)
-    return swiglu(w, name, x, lora_scale)
+        return gelu_mlp(w, name, x, lora_scale, kernels)
+    return swiglu(w, name, x, lora_scale, kernels)
 
 
 def modulation_sets(w: Weights, name: str, temb_silu: torch.Tensor, dim: int, sets: int,
@@ -116,6 +125,119 @@ def _modulation(w: Weights, name: str, temb: torch.Tensor, dim: int,
     """The six (dim,) chunks of linear(silu(temb)): shift1, scale1, gate1,
     shift2, scale2, gate2 (the reference feeds silu(temb), lib.rs:310-317)."""
     return modulation_sets(w, name, F.silu(temb), dim, 2, lora_scale)
+
+
+# ------------------------------------------- the block's own fused kernels
+
+class _LayerNormMod(torch.autograd.Function):
+    """ops.layer_norm with the modulation's gain 1 + scale, and its gradient."""
+
+    @staticmethod
+    def forward(ctx, x, shift, scale, eps):
+        y, stats = ops.layer_norm(x, scale, shift, unit_offset=True, eps=eps)
+        ctx.save_for_backward(x, scale, stats)
+        ctx.shift_dtype = shift.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, scale, stats = ctx.saved_tensors
+        if dy.stride(-1) != 1:
+            dy = dy.contiguous()
+        dx, dscale, dshift = ops.layer_norm_bwd(x, scale, dy, stats, unit_offset=True,
+                                                params=any(ctx.needs_input_grad[1:3]))
+        cast = lambda g, dt: g.to(dt) if g is not None else None
+        return dx, cast(dshift, ctx.shift_dtype), cast(dscale, scale.dtype), None
+
+
+def _aligned(x: torch.Tensor) -> torch.Tensor:
+    """x (rows, n) with contiguous rows that start on 16 bytes (a copy only
+    where they do not)."""
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        x = x.contiguous()
+    if x.shape[0] > 1 and x.stride(0) % 8 or x.data_ptr() % 16:
+        n = x.shape[-1]
+        x = F.pad(x, (0, -n % 8))[:, :n]
+    return x
+
+
+class _LoraLinear(torch.autograd.Function):
+    """ops.lora_linear over the rows of x, and its gradient; the base weight
+    is frozen."""
+
+    @staticmethod
+    def forward(ctx, x, weight, a, b, bias, scale):
+        if ctx.needs_input_grad[1]:
+            raise ValueError("the fused linear trains the LoRA factors (and its bias); "
+                             "its weight must not require a gradient")
+        x2 = _aligned(x.reshape(-1, x.shape[-1]))
+        y, low = ops.lora_linear(x2, weight, a, b, scale=scale, bias=bias)
+        ctx.save_for_backward(x2, weight, a, b, low)
+        ctx.scale, ctx.x_shape = scale, x.shape
+        return y.view(*x.shape[:-1], weight.shape[0])
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x2, weight, a, b, low = ctx.saved_tensors
+        need_x, _, need_a, need_b, need_bias, _ = ctx.needs_input_grad
+        dy2 = _aligned(dy.reshape(-1, dy.shape[-1]))
+        dx = da = db = None
+        if need_x or need_a or need_b:
+            dx, da, db = ops.lora_linear_bwd(x2, weight, a, b, dy2, low, scale=ctx.scale,
+                                             need_dx=need_x, need_factors=need_a or need_b)
+        if dx is not None:
+            dx = dx.view(ctx.x_shape)
+        dbias = dy2.float().sum(0).to(dy.dtype) if need_bias else None
+        return dx, None, da if need_a else None, db if need_b else None, dbias, None
+
+
+class FusedKernels:
+    """The norms and adapter linears of the blocks on the framework's kernels:
+    pass it as `kernels=` to the block functions or to LoraTrainer. Same
+    arithmetic as `layer_norm_mod` and `linear` with fewer roundings (y = x W^T
+    + b + s (x A^T) B^T is rounded once, the low-rank term before it once).
+    bf16 linears, bf16 or f32 norms; linears without LoRA factors stay
+    torch's. On the GPU only.
+
+    `adapters`: serving a batch of requests that each have their own LoRA.
+    Factors stacked over the E adapters ((E, rank, in), (E, out, rank)) apply
+    adapters[i] (int32, on the device; an id outside [0, E): none) to the rows
+    of sample i. Graph-free."""
+
+    def __init__(self, adapters: Optional[torch.Tensor] = None):
+        self.adapters = adapters
+
+    def linear(self, w: Weights, name: str, x: torch.Tensor, lora_scale: float) -> torch.Tensor:
+        a, b = w.get(f"weights/{name}.lora_a"), w.get(f"weights/{name}.lora_b")
+        if a is None or b is None:
+            return linear(w, name, x, lora_scale)
+        weight, bias = _get(w, f"weights/{name}.weight"), w.get(f"weights/{name}.bias")
+        if a.dim() == 2:
+            return _LoraLinear.apply(x, weight, a, b, bias, lora_scale)
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (x, weight, a, b)):
+            raise ValueError(f"{name}: stacked adapters serve without gradients (torch.no_grad)")
+        if self.adapters is None or self.adapters.shape != x.shape[:1]:
+            raise ValueError(f"{name}: stacked adapters need one adapter id per sample, "
+                             f"{x.shape[0]} of them")
+        x2 = _aligned(x.reshape(-1, x.shape[-1]))
+        per = x2.shape[0] // max(1, x.shape[0])
+        ids = self.adapters.to(torch.int32)[:, None].expand(-1, per).reshape(-1)
+        scales = torch.full((a.shape[0],), float(lora_scale), device=x.device)
+        y = ops.lora_linear_many(x2, weight, a, b, ids, scales, bias=bias)
+        return y.view(*x.shape[:-1], weight.shape[0])
+
+    def layer_norm_mod(self, x: torch.Tensor, shift: torch.Tensor, scale: torch.Tensor,
+                       eps: float = NORM_EPS) -> torch.Tensor:
+        """x (..., dim) with shift, scale (dim,) or, for x (B, len, dim), one
+        per sample: (B, dim) or (B, 1, dim)."""
+        if scale.dim() == 3 and scale.shape[1] == 1:
+            shift, scale = shift[:, 0], scale[:, 0]
+        if scale.dim() == 1 and x.dim() != 2:
+            y = _LayerNormMod.apply(x.reshape(-1, x.shape[-1]), shift, scale, eps)
+            return y.view(x.shape)
+        return _LayerNormMod.apply(x, shift, scale, eps)
 
 
 # ------------------------------------------------------ attention callables
@@ -211,11 +333,19 @@ class BlockShape:
     head_dim: int = 128
 
 
+def _kernels(kernels: Optional[FusedKernels]):
+    """(linear, layer_norm_mod) of the block functions."""
+    if kernels is None:
+        return linear, layer_norm_mod
+    return kernels.linear, kernels.layer_norm_mod
+
+
 def double_block(w: Weights, img: torch.Tensor, txt: torch.Tensor, temb: torch.Tensor,
                  attention: JointFn, shape: BlockShape, *, prefix: str = "double",
                  lora_scale: float = 1.0,
                  acts: Optional[Dict[str, torch.Tensor]] = None,
-                 mods: Optional[Tuple[List[torch.Tensor], List[torch.Tensor]]] = None
+                 mods: Optional[Tuple[List[torch.Tensor], List[torch.Tensor]]] = None,
+                 kernels: Optional[FusedKernels] = None
                  ) -> Tuple[torch.Tensor, torch.Tensor]:
     """One double-stream block (lib.rs:301-392). img (B, I, dim), txt (B, T,
     dim), temb (dim,). `attention(q_t, k_t, v_t, q_i, k_i, v_i, wq_t, wk_t,
@@ -223,8 +353,10 @@ def double_block(w: Weights, img: torch.Tensor, txt: torch.Tensor, temb: torch.T
     RMSNorm and returns the (o_t, o_i) attention outputs. `mods` = the
     image and text streams' six modulation chunks when they are computed once
     for a whole stack (bin/throughput.rs:480-572); otherwise they come from
-    this block's modulation linear(s)."""
+    this block's modulation linear(s). `kernels`: FusedKernels, or None for
+    torch's norms and linears."""
     d, h, hd = shape.dim, shape.heads, shape.head_dim
+    lin, norm = _kernels(kernels)
     if mods is not None:
         mi, mt = mods
     elif f"weights/{prefix}.mod.weight" in w:
@@ -234,13 +366,13 @@ def double_block(w: Weights, img: torch.Tensor, txt: torch.Tensor, temb: torch.T
         mt = _modulation(w, f"{prefix}.txt.mod", temb, d, lora_scale)
     B, I, T = img.shape[0], img.shape[1], txt.shape[1]
 
-    ih = layer_norm_mod(img, mi[0], mi[1])
-    th = layer_norm_mod(txt, mt[0], mt[1])
+    ih = norm(img, mi[0], mi[1])
+    th = norm(txt, mt[0], mt[1])
     if acts is not None:
         acts[f"{prefix}.img_norm1"], acts[f"{prefix}.txt_norm1"] = ih, th
 
     def proj(stream, x, n, which):
-        return linear(w, f"{prefix}.{stream}.to_{which}", x, lora_scale).reshape(B, n, h, hd)
+        return lin(w, f"{prefix}.{stream}.to_{which}", x, lora_scale).reshape(B, n, h, hd)
 
     q_i, k_i, v_i = (proj("img", ih, I, c) for c in ("q", "k", "v"))
     q_t, k_t, v_t = (proj("txt", th, T, c) for c in ("q", "k", "v"))
@@ -252,15 +384,15 @@ def double_block(w: Weights, img: torch.Tensor, txt: torch.Tensor, temb: torch.T
     if acts is not None:
         acts[f"{prefix}.attn_img"] = a_i
 
-    img = img + mi[2] * linear(w, f"{prefix}.img.to_out", a_i.reshape(B, I, d), lora_scale)
-    txt = txt + mt[2] * linear(w, f"{prefix}.txt.to_out", a_t.reshape(B, T, d), lora_scale)
+    img = img + mi[2] * lin(w, f"{prefix}.img.to_out", a_i.reshape(B, I, d), lora_scale)
+    txt = txt + mt[2] * lin(w, f"{prefix}.txt.to_out", a_t.reshape(B, T, d), lora_scale)
     if acts is not None:
         acts[f"{prefix}.img_post_attn"] = img
 
-    ih2 = layer_norm_mod(img, mi[3], mi[4])
-    th2 = layer_norm_mod(txt, mt[3], mt[4])
-    img = img + mi[5] * _mlp(w, f"{prefix}.img.mlp", ih2, lora_scale)
-    txt = txt + mt[5] * _mlp(w, f"{prefix}.txt.mlp", th2, lora_scale)
+    ih2 = norm(img, mi[3], mi[4])
+    th2 = norm(txt, mt[3], mt[4])
+    img = img + mi[5] * _mlp(w, f"{prefix}.img.mlp", ih2, lora_scale, kernels)
+    txt = txt + mt[5] * _mlp(w, f"{prefix}.txt.mlp", th2, lora_scale, kernels)
     if acts is not None:
         acts[f"{prefix}.img_out"], acts[f"{prefix}.txt_out"] = img, txt
     return img, txt
@@ -268,26 +400,28 @@ def double_block(w: Weights, img: torch.Tensor, txt: torch.Tensor, temb: torch.T
 
 def single_block(w: Weights, x: torch.Tensor, temb: torch.Tensor, attention: SingleFn,
                  shape: BlockShape, *, prefix: str = "single", lora_scale: float = 1.0,
-                 acts: Optional[Dict[str, torch.Tensor]] = None) -> torch.Tensor:
+                 acts: Optional[Dict[str, torch.Tensor]] = None,
+                 kernels: Optional[FusedKernels] = None) -> torch.Tensor:
     """One single-stream block (lib.rs:394-456): fused QKV with LoRA, q/k
     RMSNorm + RoPE, attention, SwiGLU from the same normed input, gated
     residuals (x + g_at * attn + g_mlp * mlp; this block has no output
     projection and no second adaLN). x (B, S, dim); `attention(q, k, v, wq,
     wk)` gets the projections before the norm."""
     d, h, hd = shape.dim, shape.heads, shape.head_dim
+    lin, norm = _kernels(kernels)
     sh1, sc1, g_at, _, _, g_mlp = _modulation(w, f"{prefix}.mod", temb, d, lora_scale)
     B, S = x.shape[0], x.shape[1]
-    nh = layer_norm_mod(x, sh1, sc1)
+    nh = norm(x, sh1, sc1)
     if acts is not None:
         acts[f"{prefix}.norm1"] = nh
-    qkv = linear(w, f"{prefix}.to_qkv", nh, lora_scale).reshape(B, S, 3, h, hd)
+    qkv = lin(w, f"{prefix}.to_qkv", nh, lora_scale).reshape(B, S, 3, h, hd)
     q, k, v = qkv.unbind(2)
     o = attention(q, k, v, _get(w, f"weights/{prefix}.q_norm.weight"),
                   _get(w, f"weights/{prefix}.k_norm.weight"))
     a = o.reshape(B, S, d)
     if acts is not None:
         acts[f"{prefix}.attn"] = a
-    m = _mlp(w, f"{prefix}.mlp", nh, lora_scale)
+    m = _mlp(w, f"{prefix}.mlp", nh, lora_scale, kernels)
     if acts is not None:
         acts[f"{prefix}.mlp"] = m
     out = x + g_at * a + g_mlp * m
@@ -298,7 +432,8 @@ def single_block(w: Weights, x: torch.Tensor, temb: torch.Tensor, attention: Sin
 
 def single_block_fused(w: Weights, x: torch.Tensor, mod3: List[torch.Tensor],
                        attention: SingleFn, shape: BlockShape, *, mlp_ratio: int = 3,
-                       prefix: str = "single", lora_scale: float = 1.0) -> torch.Tensor:
+                       prefix: str = "single", lora_scale: float = 1.0,
+                       kernels: Optional[FusedKernels] = None) -> torch.Tensor:
     """The single-stream block in the klein layout (bin/throughput.rs:577-629):
     one fused in-projection `<prefix>.to_in` (dim -> (3 + 2*mlp_ratio)*dim:
     Q, K, V, then the SwiGLU gate and up of mlp_ratio*dim each), attention,
@@ -306,17 +441,18 @@ def single_block_fused(w: Weights, x: torch.Tensor, mod3: List[torch.Tensor],
     [attention | activation] (dim + mlp_ratio*dim -> dim); one gate on its
     output: x + g * out. mod3 = (shift, scale, gate)."""
     d, h, hd = shape.dim, shape.heads, shape.head_dim
+    lin, norm = _kernels(kernels)
     sh, sc, g = mod3
     B, S = x.shape[0], x.shape[1]
-    nh = layer_norm_mod(x, sh, sc)
-    fused = linear(w, f"{prefix}.to_in", nh, lora_scale).reshape(B, S, 3 + 2 * mlp_ratio, d)
+    nh = norm(x, sh, sc)
+    fused = lin(w, f"{prefix}.to_in", nh, lora_scale).reshape(B, S, 3 + 2 * mlp_ratio, d)
     q, k, v = (fused[:, :, c].reshape(B, S, h, hd) for c in range(3))
     gate = fused[:, :, 3:3 + mlp_ratio].reshape(B, S, mlp_ratio * d)
     up = fused[:, :, 3 + mlp_ratio:].reshape(B, S, mlp_ratio * d)
     o = attention(q, k, v, _get(w, f"weights/{prefix}.q_norm.weight"),
                   _get(w, f"weights/{prefix}.k_norm.weight"))
     joined = torch.cat([o.reshape(B, S, d), F.silu(gate) * up], dim=-1)
-    return x + g * linear(w, f"{prefix}.to_out", joined, lora_scale)
+    return x + g * lin(w, f"{prefix}.to_out", joined, lora_scale)
 
 
 # ------------------------------------------ checkpointed forward/backward
@@ -396,6 +532,51 @@ class AdamW:
             p.copy_((p.float() - (m / bc1) / denom * self.lr).to(p.dtype))
 
 
+@dataclass
+class Muon:
+    """Momentum with orthogonalised updates (ops.orthogonalize) for matrix
+    parameters, with AdamW's interface:
+      m <- momentum m + (1 - momentum) g,  u = m, or with nesterov
+      momentum m + (1 - momentum) g;  p <- (1 - lr weight_decay) p
+      - lr sqrt(max(1, rows / cols)) orthogonalize(u).
+    fp32 momentum; matrices of one shape are orthogonalised in one call. The
+    reference has no counterpart."""
+    lr: float = 0.02
+    momentum: float = 0.95
+    nesterov: bool = True
+    weight_decay: float = 0.0
+    ns_steps: int = 5
+    ns_coeffs: Tuple[float, float, float] = ops.NS_COEFFS
+    eps: float = 1e-7
+
+    def init(self, params: Sequence[torch.Tensor]) -> List[torch.Tensor]:
+        for p in params:
+            if p.dim() != 2:
+                raise ValueError(f"Muon steps matrices; got a parameter of shape {tuple(p.shape)}")
+        return [torch.zeros_like(p, dtype=torch.float32) for p in params]
+
+    @torch.no_grad()
+    def step(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
+             state: Sequence[torch.Tensor], t: int) -> None:
+        same: Dict[tuple, List[int]] = {}
+        for i, p in enumerate(params):
+            same.setdefault((tuple(p.shape), p.device), []).append(i)
+        for (shape, _), at in same.items():
+            u = torch.stack([grads[i].float() for i in at])
+            for row, i in zip(u, at):
+                state[i].lerp_(row, 1.0 - self.momentum)
+                if self.nesterov:
+                    row.lerp_(state[i], self.momentum)
+                else:
+                    row.copy_(state[i])
+            o = ops.orthogonalize(u, steps=self.ns_steps, coeffs=self.ns_coeffs, eps=self.eps)
+            lr = self.lr * math.sqrt(max(1.0, shape[0] / shape[1]))
+            for row, i in zip(o, at):
+                p = params[i]
+                p.copy_((p.float() * (1.0 - self.lr * self.weight_decay)
+                         - row.float() * lr).to(p.dtype))
+
+
 # ------------------------------------------- the benchmark configuration
 
 def make_c3_weights(dim: int = 3072, heads: int = 24, rank: int = 16, seed: int = 0,
@@ -457,11 +638,14 @@ def allreduce_mean(grads, group=None):
 class LoraTrainer:
     """One LoRA training step of a double block: forward, MSE loss against
     targets, backward to the LoRA factors only, AdamW. `attention` defaults
-    to the B200 op (JointAttention at `positions`)."""
+    to the B200 op (JointAttention at `positions`), `opt` to AdamW (Muon is the
+    other), `kernels` to torch's norms and linears (FusedKernels)."""
 
     def __init__(self, w: Weights, shape: BlockShape, positions: torch.Tensor, *,
-                 lora_scale: float = 1.0, opt: Optional[AdamW] = None,
-                 attention: Optional[JointFn] = None, grad_hook=None):
+                 lora_scale: float = 1.0, opt=None,
+                 attention: Optional[JointFn] = None, grad_hook=None,
+                 kernels: Optional[FusedKernels] = None):
+        self.kernels = kernels
         self.w = dict(w)
         self.shape = shape
         self.lora_scale = lora_scale
@@ -478,7 +662,7 @@ class LoraTrainer:
 
     def loss(self, img, txt, temb, target_img, target_txt):
         o_i, o_t = double_block(self.w, img, txt, temb, self.attention, self.shape,
-                                lora_scale=self.lora_scale)
+                                lora_scale=self.lora_scale, kernels=self.kernels)
         return mse(o_i, target_img) + mse(o_t, target_txt)
 
     def step(self, img, txt, temb, target_img, target_txt) -> torch.Tensor:

@@ -8,7 +8,6 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
-#include <c10/cuda/CUDACachingAllocator.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -92,18 +91,17 @@ void same_device(const Tensor& ref, const Tensor& t, const char* name) {
            ref.device().str());
 }
 
-// The device of the first operand made current, and the stream: the caller's
-// torch.cuda.Stream, or the current one of that device. On a caller's stream
-// the call's own buffers are kept until it has passed them.
+// The device of the first operand made current, with the caller's
+// torch.cuda.Stream as its current stream where one is given: outputs,
+// workspaces and copies belong to the stream that the kernels run on.
 struct Place {
   c10::cuda::CUDAGuard guard;
+  c10::cuda::OptionalCUDAStreamGuard on;
   c10::cuda::CUDAStream stream;
-  bool given;
 
   Place(const Tensor& t, PyObject* s)
-      : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index())),
-        given(s != Py_None) {
-    if (!given) return;
+      : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index())) {
+    if (s == Py_None) return;
     auto field = [&](const char* n) {
       PyObject* v = PyObject_GetAttrString(s, n);
       if (v == nullptr) throw Raised{};
@@ -116,11 +114,9 @@ struct Place {
                                             (c10::DeviceIndex)field("device_index"),
                                             (c10::DeviceType)field("device_type"));
     if (stream.device() != t.device()) refuse("the stream is on another device than the tensors");
+    on.reset_stream(stream);
   }
   void* ptr() const { return stream.stream(); }
-  void keep(const Tensor& t) const {
-    if (given && t.defined()) c10::cuda::CUDACachingAllocator::recordStream(t.storage().data_ptr(), stream);
-  }
 };
 
 Tensor scratch(size_t bytes, const Tensor& like) {
@@ -156,6 +152,16 @@ struct NormParams {
   Tensor w, b;  // undefined: none
   int dtype = FA_DTYPE_F32;
   int64_t stride = 0;
+  bool copy = false;
+
+  // two modulation chunks share the stride of their rows; others are copied
+  // (D values a group)
+  void settle(int64_t dim) {
+    if (!copy) return;
+    if (w.defined()) w = w.contiguous();
+    if (b.defined()) b = b.contiguous();
+    if (stride != 0) stride = dim;
+  }
 };
 
 NormParams norm_params(const Tensor& x, const Tensor& w, const Tensor& b) {
@@ -175,21 +181,15 @@ NormParams norm_params(const Tensor& x, const Tensor& w, const Tensor& b) {
   p.dtype = dtype_code(first);
   p.w = w;
   p.b = b;
-  // two modulation chunks share the stride of their rows; others are copied
-  // (D values a group)
-  bool copy = false;
   if (!shared) {
     p.stride = first.stride(0);
-    copy = p.stride <= 0 || x.size(0) == 1;
+    p.copy = p.stride <= 0 || x.size(0) == 1;
   }
   for (const Tensor* t : {&w, &b})
     if (t->defined())
-      copy = copy || t->stride(-1) != 1 || (!shared && t->stride(0) != p.stride);
-  if (copy) {
-    if (w.defined()) p.w = w.contiguous();
-    if (b.defined()) p.b = b.contiguous();
-    if (!shared) p.stride = x.size(-1);
-  }
+      p.copy = p.copy || (t->stride(-1) != 1 && t->size(-1) > 1) ||
+               (!shared && t->stride(0) != p.stride);
+  if (!shared && p.stride <= 0) p.stride = 1;  // (settle gives it the copy's)
   return p;
 }
 
@@ -221,21 +221,20 @@ PyObject* layer_norm(PyObject* const* a) {
   const float eps = (float)number(a[4]);
   const NormShape s = norm_shape(x);
   const int dt = dtype_code(x);
+  NormParams p = norm_params(x, w, b);
+  if (out.defined()) like_x(x, out, "out");
   need_cuda(x);
   same_device(x, w, "weight");
   same_device(x, b, "bias");
   same_device(x, out, "out");
   const Place at(x, a[6]);
-  const NormParams p = norm_params(x, w, b);
-  if (out.defined()) like_x(x, out, "out");
+  p.settle(s.dim);
   Tensor y = out.defined() ? out : at::empty_like(x);
   Tensor stats = at::empty({2, (int64_t)s.groups * s.rows}, x.options().dtype(at::kFloat));
   const fa_tensor_t dx = norm_desc(x), dy = norm_desc(y);
   checked(fa_layer_norm_fwd(dt, s.groups, s.rows, s.dim, &dx, ptr(p.w), ptr(p.b), p.dtype, p.stride,
                             unit, eps, &dy, stats.data_ptr<float>(), at.ptr()),
           "fa_layer_norm_fwd");
-  at.keep(p.w);
-  at.keep(p.b);
   return pair(y, stats);
 }
 
@@ -246,8 +245,9 @@ PyObject* layer_norm_bwd(PyObject* const* a) {
   const bool unit = truth(a[4]), params = truth(a[5]);
   const NormShape s = norm_shape(x);
   const int dt = dtype_code(x);
-  need_cuda(x);
   like_x(x, dy, "dy");
+  NormParams p = norm_params(x, w, Tensor());
+  need_cuda(x);
   same_device(x, w, "weight");
   same_device(x, dy, "dy");
   same_device(x, stats, "stats");
@@ -256,7 +256,7 @@ PyObject* layer_norm_bwd(PyObject* const* a) {
       stats.size(1) != n || !stats.is_contiguous())
     refuse("stats must be layer_norm's (2, rows) float32 tensor");
   const Place at(x, a[6]);
-  const NormParams p = norm_params(x, w, Tensor());
+  p.settle(s.dim);
   Tensor dx = at::empty_like(x), dw, db;
   if (params) {
     const auto o = x.options().dtype(at::kFloat);
@@ -270,8 +270,6 @@ PyObject* layer_norm_bwd(PyObject* const* a) {
                             &tdy, stats.data_ptr<float>(), &tdx, (float*)ptr(dw), (float*)ptr(db),
                             ptr(ws), nb, at.ptr()),
           "fa_layer_norm_bwd");
-  at.keep(p.w);
-  at.keep(ws);
   return triple(dx, dw, db);
 }
 
@@ -343,8 +341,6 @@ void check_lora(const Tensor& x2, const Tensor& w, const Tensor& a, const Tensor
       refuse_type(std::string(names[i]) + ": the linear with adapters computes in bf16, got " +
                   c10::toString(ts[i]->scalar_type()));
   }
-  need_cuda(x2);
-  for (int i = 1; i < 5; ++i) same_device(x2, *ts[i], names[i]);
   const int64_t nd = stacked ? 3 : 2;
   if (w.dim() != 2 || a.dim() != nd || b.dim() != nd)
     refuse("expected w (out, in) and factors a (..., rank, in), b (..., out, rank)");
@@ -356,6 +352,8 @@ void check_lora(const Tensor& x2, const Tensor& w, const Tensor& a, const Tensor
     refuse("bias must be a contiguous (out,) vector");
   for (const Tensor* t : {&x2, &w, &a})
     for (int64_t n : t->sizes()) to_int(n, "x, w or a");
+  need_cuda(x2);
+  for (int i = 1; i < 5; ++i) same_device(x2, *ts[i], names[i]);
 }
 
 int64_t low_dim(int64_t rank) { return (rank + 15) / 16 * 16; }
@@ -373,7 +371,6 @@ Tensor aligned_b(const Tensor& b, const Place& at) {
   checked(fa_pad_rows((int64_t)rows.size(0), (int)r, rows.data_ptr(), rows.stride(0), t.data_ptr(),
                       ld, at.ptr()),
           "fa_pad_rows");
-  at.keep(t);
   t = t.narrow(1, 0, r);
   return b.dim() == 2 ? t : t.as_strided(b.sizes(), {b.size(1) * ld, ld, 1});
 }
@@ -431,7 +428,6 @@ PyObject* lora_linear_bwd(PyObject* const* a_) {
                              scale, low.data_ptr(), &mdy, need_dx ? &mdx : nullptr, ptr(da), ptr(db),
                              ptr(ws), nb, at.ptr()),
           "fa_lora_linear_bwd");
-  at.keep(ws);
   return triple(need_dx ? shaped_like(dx, x) : dx, da, db);
 }
 
@@ -461,7 +457,6 @@ PyObject* lora_linear_many(PyObject* const* a_) {
                               &mb, ids.data_ptr<int32_t>(), scales.data_ptr<float>(), ptr(bias), &my,
                               ptr(ws), nb, at.ptr()),
           "fa_lora_linear_many");
-  at.keep(ws);
   return THPVariable_Wrap(shaped_like(y, x));
 }
 
@@ -526,7 +521,6 @@ PyObject* orthogonalize(PyObject* const* a_) {
                            mo.stride_batch, mo.stride_row, steps, a, b, c, eps, ptr(ws), nb,
                            at.ptr()),
           "fa_orthogonalize");
-  at.keep(ws);
   return THPVariable_Wrap(o);
 }
 
