@@ -432,9 +432,10 @@ def run_block(args, rank, world, local):
         "cpu_baseline": cpu,
         "e2e": e2e,
         # per step: q, k prologues + v concat + fwd; dO concat + delta + bwd +
-        # dQ finish + q, k prologue backwards; fused: 4 norms of 3 launches and
-        # 8 adapter linears of 6
-        "gpu_launches": (10 + (60 if args.fused_block else 0)) * K,
+        # dQ finish + q, k prologue backwards; fused: 4 norms and the backward
+        # of two; 8 adapter linears of 2 forward, 3 backward and the input
+        # gradient of two
+        "gpu_launches": (10 + (48 if args.fused_block else 0)) * K,
         "clocks": clocks,
     }
     print(json.dumps(line), flush=True)

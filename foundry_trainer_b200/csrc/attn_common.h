@@ -29,13 +29,13 @@ enum KernelId {
   kKernelFwdBf16 = 0,
   kKernelBwdBf16 = 1,
   kKernelF32Fwd = 2,
-  kKernelF32Bwd = 3,
-  kKernelWide = 4,     // + 0..5: the wide product by operand layout and epilogue
-  kKernelSkinny = 10,  // + 0..4 by operand layout and output
-  kKernelThin = 15,    // + 0..11: the thin orthogonalisation by type, side and rank
-  kKernelNorm = 27,    // + 0..11: the ring layer norm by direction, type and width
-  kKernelSkinnyBig = 39,  // + 0..4: the same with one block an SM
-  kKernelCount = 44
+  kKernelF32Bwd = 3,   // + 0..1: dK/dV and dQ
+  kKernelWide = 5,     // + 0..5: the wide product by operand layout and epilogue
+  kKernelSkinny = 11,  // + 0..4 by operand layout and output
+  kKernelThin = 16,    // + 0..11: the thin orthogonalisation by type, side and rank
+  kKernelNorm = 28,    // + 0..11: the ring layer norm by direction, type and width
+  kKernelSkinnyBig = 40,  // + 0..4: the same with one block an SM
+  kKernelCount = 45
 };
 
 // FA_OK when the last CUDA runtime call / launch on this thread succeeded;
