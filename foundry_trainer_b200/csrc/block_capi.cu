@@ -150,14 +150,15 @@ int fa_lora_linear_fwd(int dtype, int rows, int in_dim, int out_dim, int rank,
   // starts when all earlier work is done) and waits for it where it needs it
   if (rows <= kDotRows) {
     FA_TRY(launch_low_rows(bfp(x->data), x->stride_row, bfp(a->data), 0, a->stride_row, nullptr, 1,
-                           nullptr, scale, rows, in_dim, rank, ld, lw, st));
+                           nullptr, scale, rows, in_dim, rank, ld, lw, 2 * ld, ld, st));
   } else {
     SkinnyParams s;
     s.rows = rows;
     s.cols = s.n = s.low_ld = ld;
     s.K = in_dim;
     s.out = lw;
-    s.out_ld = ld;
+    s.out_ld = 2 * ld;
+    s.lo_at = ld;
     s.scale = scale;
     FA_TRY(launch_gemm_skinny(mat(x, 1, rows, in_dim), false, mat(a, 1, rank, in_dim), false, s,
                               kSkinnyLow, false, st));
@@ -172,6 +173,7 @@ int fa_lora_linear_fwd(int dtype, int rows, int in_dim, int out_dim, int rank,
     s.bias = bfp(bias);
     s.low = lw;
     s.low_ld = ld;
+    s.low_stride = 2 * ld;
     s.rank = rank;
     return launch_gemm_skinny(mat(w, 1, out_dim, in_dim), false, mat(x, 1, rows, in_dim), false, s,
                               kSkinnyCols, true, st, mat(b, 1, out_dim, rank));
@@ -187,6 +189,7 @@ int fa_lora_linear_fwd(int dtype, int rows, int in_dim, int out_dim, int rank,
   p.K = in_dim;
   p.low = lw;
   p.low_ld = ld;
+  p.low_stride = 2 * ld;
   p.rank = rank;
   p.early = 1;
   p.bias = bfp(bias);
@@ -195,7 +198,7 @@ int fa_lora_linear_fwd(int dtype, int rows, int in_dim, int out_dim, int rank,
 
 size_t fa_lora_linear_bwd_workspace_bytes(int rows, int rank) {
   if (rows <= 0 || rank <= 0) return 0;
-  return (size_t)rows * low_dim(rank) * 2;
+  return (size_t)rows * low_dim(rank) * 4;
 }
 
 int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
@@ -237,7 +240,8 @@ int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
     s.cols = s.n = s.low_ld = ld;
     s.K = out_dim;
     s.out = u;
-    s.out_ld = ld;
+    s.out_ld = 2 * ld;
+    s.lo_at = ld;
     s.scale = scale;
     FA_TRY(launch_gemm_skinny(mat(dy, 1, rows, out_dim), false, mat(b, 1, out_dim, rank), true, s,
                               kSkinnyLow, false, st));
@@ -247,18 +251,19 @@ int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
     s.cols = rank;
     s.n = ld;
     s.K = rows;
+    s.has_lo = 1;
     s.rows = in_dim;  // da = (x^T U)^T
     s.out = reinterpret_cast<__nv_bfloat16*>(da);
     s.out_ld = 1;
     s.out_j = in_dim;
-    FA_TRY(launch_gemm_skinny(mat(x, 1, rows, in_dim), true, dense(u, rows, ld, ld), true, s,
-                              kSkinnyGrad, true, st));
+    FA_TRY(launch_gemm_skinny(mat(x, 1, rows, in_dim), true, dense(u, rows, ld, 2 * ld), true, s,
+                              kSkinnyGrad, true, st, dense(u + ld, rows, ld, 2 * ld)));
     s.rows = out_dim;  // db = dy^T low
     s.out = reinterpret_cast<__nv_bfloat16*>(db);
     s.out_ld = rank;
     s.out_j = 1;
-    FA_TRY(launch_gemm_skinny(mat(dy, 1, rows, out_dim), true, dense(low, rows, ld, ld), true, s,
-                              kSkinnyGrad, true, st));
+    FA_TRY(launch_gemm_skinny(mat(dy, 1, rows, out_dim), true, dense(low, rows, ld, 2 * ld), true, s,
+                              kSkinnyGrad, true, st, dense(bfp(low) + ld, rows, ld, 2 * ld)));
   }
   if (dx == nullptr) return FA_OK;
   if (linear_as_columns(in_dim, out_dim, rows)) {
@@ -270,6 +275,7 @@ int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
     s.out_ld = dx->stride_row;
     s.low = u;
     s.low_ld = ld;
+    s.low_stride = 2 * ld;
     s.rank = rank;
     return launch_gemm_skinny(mat(w, 1, out_dim, in_dim), true, mat(dy, 1, rows, out_dim), false, s,
                               kSkinnyCols, true, st, mat(a, 1, rank, in_dim));
@@ -286,6 +292,7 @@ int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
   p.K = out_dim;
   p.low = u;
   p.low_ld = ld;
+  p.low_stride = 2 * ld;
   p.rank = rank;
   p.early = 1;
   return launch_gemm_wide(o, p, kEpiLinear, st);
@@ -346,7 +353,7 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
   if (dots) {
     FA_TRY(launch_low_rows(bfp(x->data), x->stride_row, bfp(a->data), a->stride_batch,
                            a->stride_row, ids, n_adapters, scales, 1.f, rows, in_dim, rank, ld, low,
-                           st));
+                           ld, 0, st));
   } else {
     SkinnyParams s;
     s.rows = rows;
@@ -372,6 +379,7 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
     s.bias = bfp(bias);
     s.low = low;
     s.low_ld = ld;
+    s.low_stride = ld;
     s.rank = rank;
     s.E = n_adapters;
     s.ids = ids;
@@ -396,6 +404,7 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
   p.K = in_dim;
   p.low = low;
   p.low_ld = ld;
+  p.low_stride = ld;
   p.rank = rank;
   p.list_cnt = cnt;
   p.list_ids = list;

@@ -37,11 +37,13 @@ struct WideParams {
   int M = 0, N = 0, K = 0, batch = 1;
   int fmt = 1;  // 0 fp16, 1 bf16 operands
   int tiles_m = 0, tiles_n = 0, tiles_per_batch = 0, symmetric = 0;
-  // adapters: low (M, low_ld) bf16, low_ld = the rank rounded up to 16;
+  // adapters: low (M, low_ld) bf16 of rows low_stride apart, low_ld = the rank
+  // rounded up to 16;
   // per 256-row block the adapters in use and their count, per row its slot
   // (no lists: adapter 0 for every row)
   const __nv_bfloat16* low = nullptr;
   int low_ld = 0, rank = 0;
+  int64_t low_stride = 0;  // elements from row to row of low
   const int* list_cnt = nullptr;
   const int* list_ids = nullptr;
   const int* slot = nullptr;
@@ -89,6 +91,12 @@ struct SkinnyParams {
   // adapters: low as in WideParams; per token its adapter (none: 0 for all)
   const __nv_bfloat16* low = nullptr;
   int low_ld = 0, rank = 0, E = 1;
+  int64_t low_stride = 0;
+  // kSkinnyLow: where each row's remainders (what rounding to bf16 dropped, as
+  // bf16) go behind its values; 0: nowhere. kSkinnyGrad: Small's remainders
+  // are `fac`, multiplied too.
+  int lo_at = 0;
+  int has_lo = 0;
   const int* ids = nullptr;
   // plain views of Small, Big and the adapters, for tokens of several
   const __nv_bfloat16* raw_x = nullptr;
@@ -114,7 +122,8 @@ int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool sma
 bool linear_as_columns(int64_t out, int64_t K, int rows);
 int launch_low_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int64_t a_e,
                     int64_t a_r, const int* ids, int E, const float* scales, float scale, int rows,
-                    int K, int rank, int low_ld, __nv_bfloat16* low, cudaStream_t st);
+                    int K, int rank, int low_ld, __nv_bfloat16* low, int64_t low_stride, int lo_at,
+                    cudaStream_t st);
 int launch_pad_rows(int64_t rows, int cols, const void* src, int64_t src_stride, void* dst,
                     int64_t dst_stride, cudaStream_t st);
 int launch_adapter_plan(const int* ids, int rows, int E, int* cnt, int* list, int* slot,

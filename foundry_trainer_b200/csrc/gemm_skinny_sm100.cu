@@ -38,9 +38,9 @@ struct Layout {
 
 // n: columns of the product (multiple of 16), small_mn: Small stored with its
 // short side contiguous (64-wide blocks)
-static Layout layout_of(int n, bool small_mn) {
+static Layout layout_of(int n, bool small_mn, bool two) {
   Layout l{};
-  const int small = small_mn ? (n + 63) / 64 * 8192 : (n * 128 + 1023) / 1024 * 1024;
+  const int small = small_mn ? (n + 63) / 64 * 8192 * (two ? 2 : 1) : (n * 128 + 1023) / 1024 * 1024;
   l.stage = kBig + small;
   const int budget = (n <= 128 ? kTwoSmem : kOneSmem) - kBarBytes - 1024;
   // the columns' owner's partial sums, owners' shares rounded up to 4 columns.
@@ -136,7 +136,7 @@ __device__ __noinline__ float one_value(const SkinnyParams& p, int j, int i) {
   const int e = p.ids[j];
   if (e >= 0 && e < p.E) {
     const __nv_bfloat16* f = p.raw_f + (int64_t)e * p.raw_fe + (int64_t)i * p.raw_ldf;
-    const __nv_bfloat16* l = p.low + (int64_t)j * p.low_ld;
+    const __nv_bfloat16* l = p.low + (int64_t)j * p.low_stride;
     for (int k = 0; k < p.rank; ++k) acc = fmaf(__bfloat162float(l[k]), __bfloat162float(f[k]), acc);
   }
   return acc;
@@ -168,7 +168,7 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
   int n = p.n, s0 = 0, ns = 1;
   const int j_base = OUT == kSkinnyCols ? blockIdx.y * p.n : 0;
   const int cols = min(p.n, p.cols - j_base);
-  const __nv_bfloat16* low = p.low != nullptr ? p.low + (int64_t)j_base * p.low_ld : nullptr;
+  const __nv_bfloat16* low = p.low != nullptr ? p.low + (int64_t)j_base * p.low_stride : nullptr;
   if constexpr (OUT == kSkinnyLow) {
     if (p.list_cnt != nullptr) {
       s0 = blockIdx.y * p.slots_per_pass;
@@ -213,7 +213,8 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
     if (lane == 0) {
       if constexpr (OUT != kSkinnyCols) pdl_wait_previous();
       const int small_blocks = (n + 63) >> 6;
-      const uint32_t bytes = kBig + (SMALL_MN ? small_blocks * 8192
+      const bool two = OUT == kSkinnyGrad && p.has_lo;
+      const uint32_t bytes = kBig + (SMALL_MN ? (two ? 2 : 1) * small_blocks * 8192
                                               : (OUT == kSkinnyCols ? p.n * 128 : n * 128));
       int s = 0;
       uint32_t ph = 0;
@@ -232,6 +233,9 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
         if constexpr (SMALL_MN) {
           for (int j = 0; j < small_blocks; ++j)
             tma_load_3d(sb + j * 8192, &tsmall, &full[s], j * 64, kb * 64, 0);
+          if (two)
+            for (int j = 0; j < small_blocks; ++j)
+              tma_load_3d(sb + (small_blocks + j) * 8192, &tfac, &full[s], j * 64, kb * 64, 0);
         } else if constexpr (OUT == kSkinnyLow) {
           for (int q = 0; q < ns; ++q) {
             const int e = p.list_ids != nullptr ? p.list_ids[(int64_t)(i0 >> 8) * 256 + s0 + q] : 0;
@@ -277,6 +281,12 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
       for (int kk = 0; kk < 4; ++kk)
         umma_ss_w(tmem, a + (BIG_MN ? 128 : 2) * kk, b + (SMALL_MN ? 128 : 2) * kk, idesc,
                   kb > kb0 || kk > 0);
+      if (OUT == kSkinnyGrad && p.has_lo) {
+        const uint64_t b2 = b + (uint32_t)(((n + 63) >> 6) * (8192 >> 4));
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          umma_ss_w(tmem, a + (BIG_MN ? 128 : 2) * kk, b2 + 128 * kk, idesc, 1);
+      }
       umma_commit_w(&empty[s]);
       if (!adapters && kb == kb1 - 1) umma_commit_w(done);
       if (++s == stages) { s = 0; ph ^= 1; }
@@ -331,7 +341,7 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
             at[k] = (int)sw128_offset(j, c) | 511 << 16;
             if (j < cols && plan.slot[j] >= 0) {
               at[k] = (int)sw128_offset(j, c) | plan.slot[j] << 16;
-              hold[k] = *reinterpret_cast<const uint4*>(low + (int64_t)j * p.low_ld + c * 8);
+              hold[k] = *reinterpret_cast<const uint4*>(low + (int64_t)j * p.low_stride + c * 8);
             }
           }
         }
@@ -355,7 +365,7 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
             const int j = i / chunks, c = i - j * chunks;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (j < cols && plan.slot[j] == q)
-              v = *reinterpret_cast<const uint4*>(low + (int64_t)j * p.low_ld + k0 + c * 8);
+              v = *reinterpret_cast<const uint4*>(low + (int64_t)j * p.low_stride + k0 + c * 8);
             *reinterpret_cast<uint4*>(sb + sw128_offset(j, c)) = v;
           }
         }
@@ -441,9 +451,11 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
         }
       }
     } else if constexpr (OUT == kSkinnyLow) {
-      // out[i, j]: the columns of the row's own adapter, scaled, in bf16 (the
-      // operand type of the product that follows; one rounding of a term that
-      // is added to the fp32 sum)
+      // out[i, j]: the columns of the row's own adapter, scaled, in bf16, the
+      // operand type of the products that follow: one rounding of a term that
+      // is added to the output's fp32 sum. The factors' gradients have no
+      // other term, so they also multiply the remainders (16 bits in all; with
+      // bf16 alone they were 2.4e-3 off, now 1.7e-3, their own rounding).
       const int sl = p.slot != nullptr ? p.slot[i] - s0 : 0;
       float sc = p.scale;
       if (p.scales != nullptr && sl >= 0 && sl < ns)
@@ -453,8 +465,15 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
         for (int j = lo; j < hi; j += 4) {  // (all bounds are multiples of 4)
           float acc[4];
           sum4(j, acc);
-          *reinterpret_cast<uint2*>(p.out + (int64_t)i * p.out_ld + j - sl * p.low_ld) =
-              make_uint2(pack_bf16(acc[0] * sc, acc[1] * sc), pack_bf16(acc[2] * sc, acc[3] * sc));
+          __nv_bfloat16* o = p.out + (int64_t)i * p.out_ld + j - sl * p.low_ld;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[k] *= sc;
+          const uint2 v = make_uint2(pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3]));
+          *reinterpret_cast<uint2*>(o) = v;
+          if (p.lo_at != 0)
+            *reinterpret_cast<uint2*>(o + p.lo_at) =
+                make_uint2(pack_bf16(acc[0] - bf16_lo(v.x), acc[1] - bf16_hi(v.x)),
+                           pack_bf16(acc[2] - bf16_lo(v.y), acc[3] - bf16_hi(v.y)));
         }
       } else if (p.slot != nullptr && p.slot[i] < 0 && s0 == 0 && part == 0) {
         // a row without an adapter: zeros (a block whose other rows share one
@@ -480,7 +499,7 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
 __global__ void __launch_bounds__(256)
 low_rows_kernel(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int64_t a_e,
                 int64_t a_r, const int* ids, int E, const float* scales, float scale, int K,
-                int rank, int low_ld, __nv_bfloat16* low) {
+                int rank, int low_ld, __nv_bfloat16* low, int64_t low_stride, int lo_at) {
   __shared__ float red[8];
   pdl_launch_next();
   const int groups = low_ld / 2;
@@ -515,8 +534,11 @@ low_rows_kernel(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int
   if (t == 0) {
     const float* s = red + (warp_id() & 4);
     acc = (s[0] + s[1]) + (s[2] + s[3]);
-    low[(int64_t)row * low_ld + j] =
-        __float2bfloat16_rn(has ? acc * (scales != nullptr ? scales[e] : scale) : 0.f);
+    acc = has ? acc * (scales != nullptr ? scales[e] : scale) : 0.f;
+    const __nv_bfloat16 hi = __float2bfloat16_rn(acc);
+    low[row * low_stride + j] = hi;
+    if (lo_at != 0)
+      low[row * low_stride + lo_at + j] = __float2bfloat16_rn(acc - __bfloat162float(hi));
   }
 }
 
@@ -561,7 +583,7 @@ template <bool BIG_MN, bool SMALL_MN, int OUT>
 static int go(const CUtensorMap& tbig, const CUtensorMap& tsmall, const CUtensorMap& tfac,
               const SkinnyParams& p, int passes, int kernel_id, bool early, cudaStream_t st) {
   auto* fn = skinny_kernel<BIG_MN, SMALL_MN, OUT>;
-  const Layout l = layout_of(p.n, SMALL_MN);
+  const Layout l = layout_of(p.n, SMALL_MN, OUT == kSkinnyGrad && p.has_lo);
   // the largest layout's request, once per kernel
   const int rc = ensure_smem_attr((const void*)fn, kOneSmem, kernel_id);
   if (rc) return rc;
@@ -629,6 +651,7 @@ int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool sma
   const int box = out == kSkinnyLow ? p.low_ld : p.n;
   if (!rc) rc = small_mn ? make_tmap_3d(&ts, small, 64, 64) : make_tmap_3d(&ts, small, 64, box);
   tf = tb;
+  if (!rc && out == kSkinnyGrad && p.has_lo) rc = make_tmap_3d(&tf, fac, 64, 64);
   if (!rc && out == kSkinnyCols && p.low != nullptr)
     rc = big_mn ? make_tmap_3d(&tf, fac, 64, 64) : make_tmap_3d(&tf, fac, 64, 128);
   if (rc) return rc;
@@ -681,9 +704,10 @@ bool linear_as_columns(int64_t out, int64_t K, int rows) {
 
 int launch_low_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int64_t a_e,
                     int64_t a_r, const int* ids, int E, const float* scales, float scale, int rows,
-                    int K, int rank, int low_ld, __nv_bfloat16* low, cudaStream_t st) {
+                    int K, int rank, int low_ld, __nv_bfloat16* low, int64_t low_stride, int lo_at,
+                    cudaStream_t st) {
   skinny::low_rows_kernel<<<(unsigned)(rows * (low_ld / 2)), 256, 0, st>>>(
-      x, ldx, a, a_e, a_r, ids, E, scales, scale, K, rank, low_ld, low);
+      x, ldx, a, a_e, a_r, ids, E, scales, scale, K, rank, low_ld, low, low_stride, lo_at);
   return launch_status();
 }
 

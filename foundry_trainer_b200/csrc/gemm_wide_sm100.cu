@@ -99,7 +99,7 @@ __device__ __noinline__ float one_value(const WideParams& p, int row, int col, i
   if (s >= 0) {
     const __nv_bfloat16* f = p.raw_f + (int64_t)p.list_ids[(int64_t)m * 256 + s] * p.raw_fe +
                              (int64_t)col * p.raw_ldf;
-    const __nv_bfloat16* l = p.low + (int64_t)row * p.low_ld;
+    const __nv_bfloat16* l = p.low + (int64_t)row * p.low_stride;
     for (int k = 0; k < p.rank; ++k) acc = fmaf(__bfloat162float(l[k]), __bfloat162float(f[k]), acc);
   }
   return acc;
@@ -185,7 +185,7 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
           const int r = (i * 32 + lane) >> lg, c = lane & (chunks - 1), row = row0 + r;
           const bool in = r < 128 && row < p.M;
           hold_slot[i] = in ? p.slot[row] : -1;
-          hold[i] = in ? __ldcg(reinterpret_cast<const uint4*>(p.low + (int64_t)row * p.low_ld + c * 8))
+          hold[i] = in ? __ldcg(reinterpret_cast<const uint4*>(p.low + (int64_t)row * p.low_stride + c * 8))
                        : make_uint4(0, 0, 0, 0);
         }
       }
@@ -234,7 +234,7 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
                 const int r = i >> 3, c = i & 7, row = row0 + r;
                 uint4 v = make_uint4(0, 0, 0, 0);
                 if (row < p.M && j * 64 + c * 8 < p.low_ld && p.slot[row] == q)
-                  v = __ldcg(reinterpret_cast<const uint4*>(p.low + (int64_t)row * p.low_ld +
+                  v = __ldcg(reinterpret_cast<const uint4*>(p.low + (int64_t)row * p.low_stride +
                                                             j * 64 + c * 8));
                 *reinterpret_cast<uint4*>(sa + sw128_offset(r, c)) = v;
               }
@@ -545,7 +545,7 @@ int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t 
     rc = o.b_mn ? make_tmap_3d(&te, o.e, 64, 64) : make_tmap_3d(&te, o.e, 64, kBN / 2);
   tlow = ta;
   if (!rc && p.low != nullptr)
-    rc = make_tmap_3d(&tlow, Mat3{p.low, 1, p.M, p.low_ld, 0, p.low_ld, 1}, 64, 128);
+    rc = make_tmap_3d(&tlow, Mat3{p.low, 1, p.M, p.low_ld, 0, p.low_stride, 1}, 64, 128);
   td = ta;
   if (!rc && o.d.p != nullptr) rc = make_tmap_3d(&td, o.d, 64, 128);
   td2 = td;

@@ -356,7 +356,7 @@ void check_lora(const Tensor& x2, const Tensor& w, const Tensor& a, const Tensor
   for (int i = 1; i < 5; ++i) same_device(x2, *ts[i], names[i]);
 }
 
-int64_t low_dim(int64_t rank) { return (rank + 15) / 16 * 16; }
+int64_t low_dim(int64_t rank) { return (rank + 15) / 16 * 32; }
 
 // b with rows that start on 16 bytes: itself, or a copy (a rank that is no
 // multiple of 8)

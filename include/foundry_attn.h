@@ -375,8 +375,9 @@ typedef struct {
  * x (rows, in_dim), w (out_dim, in_dim), a (rank, in_dim), b (out_dim, rank),
  * y (rows, out_dim); bias (out_dim) bf16 or NULL; rank <= 256. (A dense b
  * whose rank is no multiple of 8 breaks the 16-byte rule: fa_pad_rows makes
- * an aligned copy.) `low` receives scale x A^T as bf16
- * (rows, rank rounded up to 16), 16-byte aligned; the backward reads it.
+ * an aligned copy.) `low` receives scale x A^T: bf16
+ * (rows, 2, rank rounded up to 16), the values and the remainders of their
+ * rounding, 16-byte aligned; the backward reads it.
  * The backward, with W frozen, writes (each may be NULL, da and db together)
  *   dx = dy W + U A,  da = U^T x (rank, in_dim),  db = dy^T low (out_dim, rank),
  * U = scale dy B, in bf16, da and db contiguous; identical bits across

@@ -61,14 +61,18 @@ def lora_ref(x, w, a, b, scale, bias):
 
 
 def lora_bwd_ref(x, w, a, b, dy, scale):
-    """((dx, tol), (da, tol), (db, tol))."""
-    N, M, r = x.shape[0], w.shape[0], a.shape[0]
+    """((dx, tol), (da, tol), (db, tol)). The factors' gradients multiply the
+    inner products as two bf16 numbers: 2^-16 of a value is dropped."""
+    N, M, K, r = x.shape[0], w.shape[0], x.shape[1], a.shape[0]
     u = scale * (dy @ b)
-    u_err = U16 * u.abs() + M * STEP32 * abs(scale) * (dy.abs() @ b.abs())
-    _, _, low, low_err = lora_ref(x, w, a, b, scale, None)
+    u_sum = M * STEP32 * abs(scale) * (dy.abs() @ b.abs())
+    u_err = U16 * u.abs() + u_sum
+    low = scale * (x @ a.T)
+    low_sum = K * STEP32 * abs(scale) * (x.abs() @ a.abs().T)
     dx = dy @ w + u @ a
     tx = (u_err + (r + 1) * STEP32 * u.abs()) @ a.abs() \
         + (M + r + 2) * STEP32 * (dy.abs() @ w.abs())
-    da, ta = u.T @ x, (u_err + N * STEP32 * u.abs()).T @ x.abs()
-    db, tb = dy.T @ low, dy.abs().T @ (low_err + N * STEP32 * low.abs())
+    two = U16 * U16 + 2 * N * STEP32  # the remainder's rounding; two sums' steps
+    da, ta = u.T @ x, (u_sum + two * u.abs()).T @ x.abs()
+    db, tb = dy.T @ low, dy.abs().T @ (low_sum + two * low.abs())
     return tuple((v, U16 * (v.abs() + t) + t) for v, t in ((dx, tx), (da, ta), (db, tb)))

@@ -135,7 +135,7 @@ def test_c_abi_lora_validates_without_a_gpu():
     assert bwd(low=None) == INV and bwd(dy=None) == INV
     assert bwd(ws=None) == _lib.FA_ERR_WORKSPACE and bwd(nb=8) == _lib.FA_ERR_WORKSPACE
     assert bwd(ws=4104) == ALI
-    assert lib.fa_lora_linear_bwd_workspace_bytes(10, 12) == 10 * 16 * 2
+    assert lib.fa_lora_linear_bwd_workspace_bytes(10, 12) == 10 * 2 * 16 * 2
 
     def many(E=3, ids=4096, scales=4096, ws=4096, nb=1 << 20):
         return lib.fa_lora_linear_many(1, 4, 64, 64, 16, E, C.byref(m), C.byref(m), C.byref(m),
