@@ -35,7 +35,8 @@ enum KernelId {
   kKernelThin = 16,    // + 0..11: the thin orthogonalisation by type, side and rank
   kKernelNorm = 28,    // + 0..11: the ring layer norm by direction, type and width
   kKernelSkinnyBig = 40,  // + 0..4: the same with one block an SM
-  kKernelCount = 45
+  kKernelNarrow = 45,  // + 0..3: the narrow product by epilogue
+  kKernelCount = 49
 };
 
 // FA_OK when the last CUDA runtime call / launch on this thread succeeded;

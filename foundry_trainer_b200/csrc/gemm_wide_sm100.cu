@@ -56,6 +56,82 @@ struct Tile {
   int m, n, b;  // 256-row block, kBN-column block, batch
 };
 
+// 32 columns of an orthogonalisation product at (row, col) as they are stored:
+// out (16-bit pairs) and, for X, the remainders lo. What is read back is on
+// its way before the accumulator is waited for.
+template <int EPI>
+__device__ __forceinline__ void ns_values(const WideParams& p, int b, int row, bool live, int col,
+                                          float ca, float cb, uint32_t taddr, uint32_t* out,
+                                          uint32_t* lo) {
+  constexpr bool kReadX = EPI == kEpiUpdate || EPI == kEpiLast;
+  uint4 q[4], l[kReadX ? 4 : 1];
+  if constexpr (EPI != kEpiGram) {
+    const int64_t at = (int64_t)b * p.in_batch + (int64_t)row * p.in_ld + col;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = live && col + 8 * i < p.in_ld;
+      q[i] = in ? *reinterpret_cast<const uint4*>(p.in_hi + at + 8 * i) : make_uint4(0, 0, 0, 0);
+      if constexpr (kReadX)
+        l[i] = in ? *reinterpret_cast<const uint4*>(p.in_lo + at + 8 * i) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  uint32_t acc[32];
+  tmem_ld32(taddr, acc);
+  tmem_wait_ld();
+  const float* v = reinterpret_cast<const float*>(acc);
+  const uint32_t* qw = reinterpret_cast<const uint32_t*>(q);
+  const uint32_t* lw = reinterpret_cast<const uint32_t*>(l);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if constexpr (EPI == kEpiGram) {
+      out[i] = pack_f16(v[2 * i] * p.alpha, v[2 * i + 1] * p.alpha);
+    } else if constexpr (EPI == kEpiPoly) {  // b Q + c Q^2
+      const float2 x = unpack_f16(qw[i]);
+      out[i] = pack_f16(fmaf(cb, v[2 * i], ca * x.x), fmaf(cb, v[2 * i + 1], ca * x.y));
+    } else {  // a X + P X, X = hi + lo / 2048
+      const float2 h = unpack_f16(qw[i]), w = unpack_f16(lw[i]);
+      const float x0 = fmaf(ca, fmaf(w.x, 1.f / 2048.f, h.x), v[2 * i] * cb);
+      const float x1 = fmaf(ca, fmaf(w.y, 1.f / 2048.f, h.y), v[2 * i + 1] * cb);
+      if constexpr (EPI == kEpiUpdate) {
+        out[i] = pack_f16(x0, x1);
+        const float2 n = unpack_f16(out[i]);
+        lo[i] = pack_f16((x0 - n.x) * 2048.f, (x1 - n.y) * 2048.f);
+      } else {
+        out[i] = pack_bf16(x0 * p.alpha, x1 * p.alpha);
+      }
+    }
+  }
+}
+
+// The same 32 values to the mirrored place of a symmetric result, or of the
+// last product of a tall input to their place in the transpose: a column of 32
+// consecutive rows per warp store.
+__device__ __forceinline__ void store_columns(uint16_t* o, int64_t ld, int col, int n,
+                                              const uint32_t* out) {
+  const uint16_t* h = reinterpret_cast<const uint16_t*>(out);
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (col + i < n) o[(int64_t)(col + i) * ld] = h[i];
+}
+
+// The staged tiles of 128 rows x 64 columns: columns [32 half, 32 half + 32) of
+// this thread's row.
+__device__ __forceinline__ void stage_half(uint8_t* buf, int r, int half, const uint32_t* v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    *reinterpret_cast<uint4*>(buf + sw128_offset(r, 4 * half + i)) =
+        make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+}
+
+// Row block m of a symmetric walk, tiles_of(m) = per (m + 1) column tiles:
+// the place of walk position i.
+__device__ __forceinline__ void triangle(int i, int per, int& m, int& n) {
+  m = (int)((sqrtf(8.f * (float)(i / per) + 1.f) - 1.f) * 0.5f);
+  while ((int64_t)per * (m + 1) * (m + 2) / 2 <= i) ++m;
+  while ((int64_t)per * m * (m + 1) / 2 > i) --m;
+  n = i - per * (m * (m + 1) / 2);
+}
+
 // Tile t of the walk: eight row blocks high columns first, so that the pairs
 // at work at one time share their A rows and B columns in L2. Products with a
 // symmetric result visit only the tiles on or below the diagonal.
@@ -64,12 +140,7 @@ __device__ __forceinline__ Tile tile_of(int64_t t, const WideParams& p) {
   o.b = (int)(t / p.tiles_per_batch);
   int i = (int)(t - (int64_t)o.b * p.tiles_per_batch);
   if (p.symmetric) {
-    // row block m has the column blocks 0 .. m
-    int m = (int)((sqrtf(8.f * (float)i + 1.f) - 1.f) * 0.5f);
-    while ((int64_t)(m + 1) * (m + 2) / 2 <= i) ++m;
-    while ((int64_t)m * (m + 1) / 2 > i) --m;
-    o.m = m;
-    o.n = i - m * (m + 1) / 2;
+    triangle(i, 1, o.m, o.n);
     return o;
   }
   constexpr int kHigh = 8;
@@ -342,12 +413,16 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
 #pragma unroll 1
       for (int c = 0; c < kBN / 64; ++c) {
         const int col0 = tl.n * kBN + c * 64;
-        uint32_t acc[64];
-        tmem_ld32(tmem + lane_off + buf * kBN + c * 64, acc);
-        tmem_ld32(tmem + lane_off + buf * kBN + c * 64 + 32, acc + 32);
-        float* v = reinterpret_cast<float*>(acc);
-        uint32_t lo[EPI == kEpiUpdate ? 32 : 1];
+        const uint32_t taddr = tmem + lane_off + buf * kBN + c * 64;
+        // stage the 128 x 64 tile and store it with TMA (two buffers in turn,
+        // or one each for hi and lo)
+        constexpr bool kTwo = EPI == kEpiUpdate;
+        uint8_t* b0 = kTwo ? stg : stg + (c & 1) * kStaging;
         if constexpr (EPI == kEpiLinear) {
+          uint32_t acc[64];
+          tmem_ld32(taddr, acc);
+          tmem_ld32(taddr + 32, acc + 32);
+          float* v = reinterpret_cast<float*>(acc);
           tmem_wait_ld();
           if (mixed) {
             // zero times a non-finite entry of another row's adapter
@@ -381,97 +456,36 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
           }
 #pragma unroll
           for (int i = 0; i < 32; ++i) acc[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
-        } else if constexpr (EPI == kEpiGram) {
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            acc[i] = pack_f16(v[2 * i] * p.alpha, v[2 * i + 1] * p.alpha);
-        } else if constexpr (EPI == kEpiPoly) {
-          // b Q + c Q^2, Q read back at this tile
-          uint4 q[8];
-          const uint4* src = reinterpret_cast<const uint4*>(
-              p.in_hi + (int64_t)tl.b * p.in_batch + (int64_t)row * p.in_ld + col0);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            q[i] = live && col0 + 8 * i < p.in_ld ? src[i] : make_uint4(0, 0, 0, 0);
-          tmem_wait_ld();
-          const uint32_t* qw = reinterpret_cast<const uint32_t*>(q);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float2 x = unpack_f16(qw[i]);
-            acc[i] = pack_f16(fmaf(cb, v[2 * i], ca * x.x), fmaf(cb, v[2 * i + 1], ca * x.y));
-          }
+          if (threadIdx.x == 0) bulk_wait_group_read1();
+          named_bar_sync(1, 128);
+          stage_half(b0, r, 0, acc);
+          stage_half(b0, r, 1, acc + 16);
         } else {
-          // a X + P X: X read back as hi + lo / 2048
-          uint4 q[8], l[8];
-          const int64_t at = (int64_t)tl.b * p.in_batch + (int64_t)row * p.in_ld + col0;
-          const uint4* sh = reinterpret_cast<const uint4*>(p.in_hi + at);
-          const uint4* sl = reinterpret_cast<const uint4*>(p.in_lo + at);
+          const bool direct = EPI == kEpiLast && p.out_t != nullptr;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const bool in = live && col0 + 8 * i < p.in_ld;
-            q[i] = in ? sh[i] : make_uint4(0, 0, 0, 0);
-            l[i] = in ? sl[i] : make_uint4(0, 0, 0, 0);
-          }
-          tmem_wait_ld();
-          const uint32_t* qw = reinterpret_cast<const uint32_t*>(q);
-          const uint32_t* lw = reinterpret_cast<const uint32_t*>(l);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float2 h = unpack_f16(qw[i]), w = unpack_f16(lw[i]);
-            const float x0 = fmaf(ca, fmaf(w.x, 1.f / 2048.f, h.x), v[2 * i] * cb);
-            const float x1 = fmaf(ca, fmaf(w.y, 1.f / 2048.f, h.y), v[2 * i + 1] * cb);
-            if constexpr (EPI == kEpiUpdate) {
-              acc[i] = pack_f16(x0, x1);
-              const float2 n = unpack_f16(acc[i]);
-              lo[i] = pack_f16((x0 - n.x) * 2048.f, (x1 - n.y) * 2048.f);
-            } else {
-              acc[i] = pack_bf16(x0 * p.alpha, x1 * p.alpha);
+          for (int h = 0; h < 2; ++h) {
+            uint32_t out[16], lo[16];
+            ns_values<EPI>(p, tl.b, row, live, col0 + 32 * h, ca, cb, taddr + 32 * h, out, lo);
+            if (direct) {
+              if (live)
+                store_columns(p.out_t + (int64_t)tl.b * p.out_t_batch + row, p.out_t_ld,
+                              col0 + 32 * h, p.N, out);
+              continue;
             }
-          }
-        }
-        if constexpr (EPI == kEpiLast) {
-          if (p.out_t != nullptr) {
-            // tall input: the result is stored transposed, a column of 32
-            // consecutive rows per warp store
-            if (live) {
-              const uint16_t* h = reinterpret_cast<const uint16_t*>(acc);
-#pragma unroll
-              for (int i = 0; i < 64; ++i)
-                if (col0 + i < p.N)
-                  p.out_t[(int64_t)tl.b * p.out_t_batch + (int64_t)(col0 + i) * p.out_t_ld + row] =
-                      h[i];
+            if (mirror && live)
+              store_columns(reinterpret_cast<uint16_t*>(p.sym_out) + (int64_t)tl.b * p.sym_batch + row,
+                            p.sym_ld, col0 + 32 * h, p.N, out);
+            if (h == 0) {
+              if (threadIdx.x == 0) {
+                if constexpr (kTwo) bulk_wait_group_read0();
+                else bulk_wait_group_read1();
+              }
+              named_bar_sync(1, 128);
             }
-            continue;
+            stage_half(b0, r, h, out);
+            if constexpr (kTwo) stage_half(stg + kStaging, r, h, lo);
           }
-        }
-        if constexpr (EPI == kEpiGram || EPI == kEpiPoly) {
-          if (mirror && live) {
-            const uint16_t* h = reinterpret_cast<const uint16_t*>(acc);
-            uint16_t* o = reinterpret_cast<uint16_t*>(p.sym_out) + (int64_t)tl.b * p.sym_batch + row;
-#pragma unroll
-            for (int i = 0; i < 64; ++i)
-              if (col0 + i < p.N) o[(int64_t)(col0 + i) * p.sym_ld] = h[i];
-          }
-        }
-        // stage the 128 x 64 tile and store it with TMA (two buffers in turn,
-        // or one each for hi and lo)
-        constexpr bool kTwo = EPI == kEpiUpdate;
-        uint8_t* b0 = kTwo ? stg : stg + (c & 1) * kStaging;
-        if (threadIdx.x == 0) {
-          if constexpr (kTwo) bulk_wait_group_read0();
-          else bulk_wait_group_read1();
-        }
-        named_bar_sync(1, 128);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<uint4*>(b0 + sw128_offset(r, i)) =
-              make_uint4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
-        if constexpr (kTwo) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<uint4*>(stg + kStaging + sw128_offset(r, i)) =
-                make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+          if (direct) continue;
         }
         fence_proxy_async_smem();
         named_bar_sync(1, 128);
@@ -487,7 +501,7 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(mapa(smem_u32(&accempty[buf]), 0));
     }
-    if (threadIdx.x == 0) bulk_wait_group0();
+    if (threadIdx.x == 0) bulk_wait_group_read0();  // (the grid's end completes the stores)
     if (!ok) *abort_flag = 1;
   }
 
@@ -529,20 +543,214 @@ static int go(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& t
   return launch_status();
 }
 
+// ------------------------------------------------------------ narrow form
+// The orthogonalisation's products of matrices too small to fill the SM pairs:
+// one 128 x 64 tile per CTA (cta_group::1), two CTAs an SM, so that a 1024 x
+// 1024 product has 72 to 128 CTAs instead of 10 to 16 pairs. Its time is start,
+// latency and epilogue; the next product's CTAs are set up meanwhile
+// (programmatic dependent launch). The staging tiles lie over the ring.
+constexpr int kNarrowBN = 64;
+constexpr int kNarrowStage = kStageA + kNarrowBN * 128;
+constexpr int kNarrowStages = 4;
+constexpr int kNarrowBar = kNarrowStages * kNarrowStage;
+constexpr int kNarrowSmem = kNarrowBar + 256 + 1024;
+
+template <bool B_MN, int EPI>
+__global__ void __launch_bounds__(kThreads, 2)
+narrow_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
+              const __grid_constant__ CUtensorMap td, const __grid_constant__ CUtensorMap td2,
+              const __grid_constant__ WideParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kNarrowBar);
+  uint64_t* empty = full + kNarrowStages;
+  uint64_t* done = empty + kNarrowStages;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
+  const int warp = warp_id(), lane = lane_id();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kNarrowStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&ta);
+    tma_prefetch_desc(&tb);
+    tma_prefetch_desc(&td);
+  }
+  if (warp == 5) {
+    tmem_alloc(slot, kNarrowBN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+  pdl_launch_next();
+  pdl_wait_previous();
+
+  const int b = blockIdx.x / p.tiles_per_batch;
+  const int i = blockIdx.x - b * p.tiles_per_batch;
+  int tm, tn;
+  if (p.symmetric) {
+    triangle(i, 2, tm, tn);  // 128-row block m: column tiles 0 .. 2 m + 1
+  } else {
+    tn = i / p.tiles_m;
+    tm = i - tn * p.tiles_m;
+  }
+  const int row0 = tm * 128, col0 = tn * kNarrowBN;
+  const int kbs = (p.K + 63) >> 6;
+  bool ok = true;
+  if (warp == 4) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      for (int kb = 0; kb < kbs; ++kb) {
+        if (!(ok = mbar_wait(&empty[s], ph ^ 1))) break;
+        uint8_t* sa = smem + s * kNarrowStage;
+        mbar_arrive_expect_tx(&full[s], kNarrowStage);
+        tma_load_3d(sa, &ta, &full[s], kb * 64, row0, b);
+        if constexpr (B_MN) tma_load_3d(sa + kStageA, &tb, &full[s], col0, kb * 64, b);
+        else tma_load_3d(sa + kStageA, &tb, &full[s], kb * 64, col0, b);
+        if (++s == kNarrowStages) { s = 0; ph ^= 1; }
+      }
+      if (!ok) *abort_flag = 1;
+    }
+  } else if (warp == 5) {
+    const uint32_t idesc = idesc_f16(p.fmt, 128, kNarrowBN, false, B_MN);
+    const uint32_t base = smem_u32(smem);
+    const uint64_t a0 = kmajor_desc(base, 0, 0);
+    const uint64_t b0 = B_MN ? mnmajor_desc(base + kStageA, 0, 8192) : kmajor_desc(base + kStageA, 0, 0);
+    int s = 0;
+    uint32_t ph = 0;
+    for (int kb = 0; kb < kbs; ++kb) {
+      if (!(ok = mbar_wait_w(&full[s], ph))) break;
+      tc_fence_after();
+      const uint64_t a = a0 + (uint32_t)(s * (kNarrowStage >> 4));
+      const uint64_t bb = b0 + (uint32_t)(s * (kNarrowStage >> 4));
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        umma_ss_w(tmem, a + 2 * kk, bb + (B_MN ? 128 : 2) * kk, idesc, kb > 0 || kk > 0);
+      umma_commit_w(&empty[s]);
+      if (kb == kbs - 1) umma_commit_w(done);
+      if (++s == kNarrowStages) { s = 0; ph ^= 1; }
+    }
+    if (!ok) *abort_flag = 1;
+  } else {
+    const int r = threadIdx.x, row = row0 + r;
+    const bool live = row < p.M;
+    float ca = 0.f, cb = 0.f;
+    if constexpr (EPI != kEpiGram) {
+      ca = p.coef[2 * b];
+      cb = p.coef[2 * b + 1];
+    }
+    ok = mbar_wait_w(done, 0);
+    if (!named_bar_any(1, 128, !ok)) {
+      tc_fence_after();
+      const uint32_t taddr = tmem + ((uint32_t)(warp * 32) << 16);
+      const bool mirror = p.symmetric && tn < 2 * tm;
+      const bool direct = EPI == kEpiLast && p.out_t != nullptr;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t out[16], lo[16];
+        ns_values<EPI>(p, b, row, live, col0 + 32 * h, ca, cb, taddr + 32 * h, out, lo);
+        if (direct) {
+          if (live)
+            store_columns(p.out_t + (int64_t)b * p.out_t_batch + row, p.out_t_ld, col0 + 32 * h, p.N,
+                          out);
+          continue;
+        }
+        if (mirror && live)
+          store_columns(reinterpret_cast<uint16_t*>(p.sym_out) + (int64_t)b * p.sym_batch + row,
+                        p.sym_ld, col0 + 32 * h, p.N, out);
+        stage_half(smem, r, h, out);
+        if constexpr (EPI == kEpiUpdate) stage_half(smem + kStaging, r, h, lo);
+      }
+      if (!direct) {
+        fence_proxy_async_smem();
+        named_bar_sync(1, 128);
+        if (threadIdx.x == 0) {
+          if (row0 < p.M && col0 < p.N) {
+            tma_store_3d(&td, smem, col0, row0, b);
+            if constexpr (EPI == kEpiUpdate) tma_store_3d(&td2, smem + kStaging, col0, row0, b);
+          }
+          bulk_commit_group();
+          bulk_wait_group_read0();
+        }
+      }
+    } else {
+      *abort_flag = 1;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) drain_delay();
+  if (warp == 5) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, kNarrowBN);
+  }
+}
+
+template <bool B_MN, int EPI>
+static int narrow_go(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td,
+                     const CUtensorMap& td2, const WideParams& p, int kernel_id, cudaStream_t st) {
+  auto* fn = narrow_kernel<B_MN, EPI>;
+  const int rc = ensure_smem_attr((const void*)fn, kNarrowSmem, kernel_id);
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((int64_t)p.tiles_per_batch * p.batch));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kNarrowSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.early ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, ta, tb, td, td2, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return record_cuda_error(e);
+  }
+  return launch_status();
+}
+
+// Which form is sooner done: rounds of 296 resident tiles of 128 x 64, 0.4 us a
+// K block while an SM holds two (0.2 us one), or of 74 pairs' tiles of 256 x
+// 256, 0.29 us a K block.
+static bool use_narrow(const WideParams& p) {
+  const int64_t m1 = (p.M + 127) / 128, n1 = (p.N + 63) / 64;
+  const int64_t m2 = (p.M + 255) / 256, n2 = (p.N + 255) / 256;
+  const int64_t t1 = (p.symmetric ? m1 * (m1 + 1) : m1 * n1) * p.batch;
+  const int64_t t2 = (p.symmetric ? m2 * (m2 + 1) / 2 : m2 * n2) * p.batch;
+  const int64_t kbs = (p.K + 63) / 64;
+  const float narrow = 4.f + (t1 <= 148 ? 0.2f * kbs : (t1 + 295) / 296 * kbs * 0.4f);
+  const float pairs = 9.f + (t2 + 73) / 74 * kbs * 0.29f;
+  return narrow < pairs;
+}
+
 }  // namespace wide
 
 int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t st) {
-  using wide::kBN;
-  if (p.M == 0 || p.N == 0 || p.batch == 0) return FA_OK;
-  p.tiles_m = (p.M + 255) / 256;
-  p.tiles_n = (p.N + kBN - 1) / kBN;
-  p.tiles_per_batch = p.symmetric ? p.tiles_m * (p.tiles_m + 1) / 2 : p.tiles_m * p.tiles_n;
+  const bool narrow = epi != kEpiLinear && wide::use_narrow(p);
+  const int tile_n = narrow ? wide::kNarrowBN : wide::kBN, tile_m = narrow ? 128 : 256;
+  p.tiles_m = (p.M + tile_m - 1) / tile_m;
+  p.tiles_n = (p.N + tile_n - 1) / tile_n;
+  p.tiles_per_batch = !p.symmetric ? p.tiles_m * p.tiles_n
+                      : narrow     ? p.tiles_m * (p.tiles_m + 1)
+                                   : p.tiles_m * (p.tiles_m + 1) / 2;
+  // a pair's CTA loads half of the tile's columns
+  const int load_n = narrow ? tile_n : tile_n / 2;
   CUtensorMap ta, tb, te, tlow, td, td2;
   int rc = make_tmap_3d(&ta, o.a, 64, 128);
-  if (!rc) rc = o.b_mn ? make_tmap_3d(&tb, o.b, 64, 64) : make_tmap_3d(&tb, o.b, 64, kBN / 2);
+  if (!rc) rc = o.b_mn ? make_tmap_3d(&tb, o.b, 64, 64) : make_tmap_3d(&tb, o.b, 64, load_n);
   te = tb;
   if (!rc && p.low != nullptr)
-    rc = o.b_mn ? make_tmap_3d(&te, o.e, 64, 64) : make_tmap_3d(&te, o.e, 64, kBN / 2);
+    rc = o.b_mn ? make_tmap_3d(&te, o.e, 64, 64) : make_tmap_3d(&te, o.e, 64, load_n);
   tlow = ta;
   if (!rc && p.low != nullptr)
     rc = make_tmap_3d(&tlow, Mat3{p.low, 1, p.M, p.low_ld, 0, p.low_stride, 1}, 64, 128);
@@ -551,8 +759,15 @@ int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t 
   td2 = td;
   if (!rc && o.d2.p != nullptr) rc = make_tmap_3d(&td2, o.d2, 64, 128);
   if (rc) return rc;
-#define FA_WIDE(EPI, MN, ID)                                                                  \
+#define FA_WIDE(EPI, MN, ID) \
   if (epi == EPI && o.b_mn == MN) return wide::go<MN, EPI>(ta, tb, te, tlow, td, td2, p, ID, st);
+#define FA_NARROW(EPI, MN, ID)                    \
+  if (narrow && epi == EPI && o.b_mn == MN)       \
+    return wide::narrow_go<MN, EPI>(ta, tb, td, td2, p, ID, st);
+  FA_NARROW(kEpiGram, false, kKernelNarrow)
+  FA_NARROW(kEpiPoly, false, kKernelNarrow + 1)
+  FA_NARROW(kEpiUpdate, true, kKernelNarrow + 2)
+  FA_NARROW(kEpiLast, true, kKernelNarrow + 3)
   FA_WIDE(kEpiLinear, false, kKernelWide)
   FA_WIDE(kEpiLinear, true, kKernelWide + 1)
   FA_WIDE(kEpiGram, false, kKernelWide + 2)
@@ -560,6 +775,7 @@ int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t 
   FA_WIDE(kEpiUpdate, true, kKernelWide + 4)
   FA_WIDE(kEpiLast, true, kKernelWide + 5)
 #undef FA_WIDE
+#undef FA_NARROW
   return FA_ERR_UNSUPPORTED;
 }
 
