@@ -130,7 +130,20 @@ int launch_adapter_plan(const int* ids, int rows, int E, int* cnt, int* list, in
                         cudaStream_t st);
 int skinny_device_status();
 
-int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t st);
+// The descriptors of one call's matrices (each pointer has one shape in it),
+// for a sequence of products over the same few: encoding five per launch costs
+// as much as the launch.
+struct TmapMemo {
+  static constexpr int kMost = 12;
+  const void* p[kMost];
+  int box[kMost];
+  CUtensorMap maps[kMost];
+  int n = 0;
+  int get(CUtensorMap* map, const Mat3& m, int rows);
+};
+
+int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t st,
+                     TmapMemo* maps = nullptr);
 int wide_device_status();
 
 }  // namespace fa

@@ -56,31 +56,39 @@ struct Tile {
   int m, n, b;  // 256-row block, kBN-column block, batch
 };
 
-// 32 columns of an orthogonalisation product at (row, col) as they are stored:
-// out (16-bit pairs) and, for X, the remainders lo. What is read back is on
-// its way before the accumulator is waited for.
+// What an orthogonalisation product reads back for 32 columns of its result:
+// Q, or X as hi and lo.
 template <int EPI>
-__device__ __forceinline__ void ns_values(const WideParams& p, int b, int row, bool live, int col,
-                                          float ca, float cb, uint32_t taddr, uint32_t* out,
-                                          uint32_t* lo) {
-  constexpr bool kReadX = EPI == kEpiUpdate || EPI == kEpiLast;
-  uint4 q[4], l[kReadX ? 4 : 1];
-  if constexpr (EPI != kEpiGram) {
-    const int64_t at = (int64_t)b * p.in_batch + (int64_t)row * p.in_ld + col;
+struct Back {
+  static constexpr bool kX = EPI == kEpiUpdate || EPI == kEpiLast;
+  static constexpr bool kNone = EPI == kEpiGram || EPI == kEpiLinear;
+  uint4 q[kNone ? 1 : 4], l[kX ? 4 : 1];
+
+  __device__ __forceinline__ void load(const WideParams& p, int b, int row, bool live, int col) {
+    if constexpr (!kNone) {
+      const int64_t at = (int64_t)b * p.in_batch + (int64_t)row * p.in_ld + col;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool in = live && col + 8 * i < p.in_ld;
-      q[i] = in ? *reinterpret_cast<const uint4*>(p.in_hi + at + 8 * i) : make_uint4(0, 0, 0, 0);
-      if constexpr (kReadX)
-        l[i] = in ? *reinterpret_cast<const uint4*>(p.in_lo + at + 8 * i) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < 4; ++i) {
+        const bool in = live && col + 8 * i < p.in_ld;
+        q[i] = in ? *reinterpret_cast<const uint4*>(p.in_hi + at + 8 * i) : make_uint4(0, 0, 0, 0);
+        if constexpr (kX)
+          l[i] = in ? *reinterpret_cast<const uint4*>(p.in_lo + at + 8 * i) : make_uint4(0, 0, 0, 0);
+      }
     }
   }
+};
+
+// These 32 columns as they are stored: out (16-bit pairs) and, for X, the
+// remainders lo.
+template <int EPI>
+__device__ __forceinline__ void ns_values(const WideParams& p, const Back<EPI>& back, float ca,
+                                          float cb, uint32_t taddr, uint32_t* out, uint32_t* lo) {
   uint32_t acc[32];
   tmem_ld32(taddr, acc);
   tmem_wait_ld();
   const float* v = reinterpret_cast<const float*>(acc);
-  const uint32_t* qw = reinterpret_cast<const uint32_t*>(q);
-  const uint32_t* lw = reinterpret_cast<const uint32_t*>(l);
+  const uint32_t* qw = reinterpret_cast<const uint32_t*>(back.q);
+  const uint32_t* lw = reinterpret_cast<const uint32_t*>(back.l);
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     if constexpr (EPI == kEpiGram) {
@@ -404,6 +412,9 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
         ca = p.coef[2 * tl.b];
         cb = p.coef[2 * tl.b + 1];
       }
+      // what a product reads back is fetched 32 columns ahead
+      Back<EPI> back[2];
+      if constexpr (EPI != kEpiLinear) back[0].load(p, tl.b, row, live, tl.n * kBN);
       ok = mbar_wait_w(&accfull[buf], (it >> 1) & 1);
       if (!ok) break;
       tc_fence_after();
@@ -465,7 +476,9 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t out[16], lo[16];
-            ns_values<EPI>(p, tl.b, row, live, col0 + 32 * h, ca, cb, taddr + 32 * h, out, lo);
+            // (past the tile's last columns: loads that are not used)
+            back[1 - h].load(p, tl.b, row, live && (h == 0 || c + 1 < kBN / 64), col0 + 32 * h + 32);
+            ns_values<EPI>(p, back[h], ca, cb, taddr + 32 * h, out, lo);
             if (direct) {
               if (live)
                 store_columns(p.out_t + (int64_t)tl.b * p.out_t_batch + row, p.out_t_ld,
@@ -647,6 +660,9 @@ narrow_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
       ca = p.coef[2 * b];
       cb = p.coef[2 * b + 1];
     }
+    Back<EPI> back[2];  // on its way under the products
+    back[0].load(p, b, row, live, col0);
+    back[1].load(p, b, row, live, col0 + 32);
     ok = mbar_wait_w(done, 0);
     if (!named_bar_any(1, 128, !ok)) {
       tc_fence_after();
@@ -656,7 +672,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t out[16], lo[16];
-        ns_values<EPI>(p, b, row, live, col0 + 32 * h, ca, cb, taddr + 32 * h, out, lo);
+        ns_values<EPI>(p, back[h], ca, cb, taddr + 32 * h, out, lo);
         if (direct) {
           if (live)
             store_columns(p.out_t + (int64_t)b * p.out_t_batch + row, p.out_t_ld, col0 + 32 * h, p.N,
@@ -735,7 +751,23 @@ static bool use_narrow(const WideParams& p) {
 
 }  // namespace wide
 
-int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t st) {
+int TmapMemo::get(CUtensorMap* map, const Mat3& m, int rows) {
+  for (int i = 0; i < n; ++i)
+    if (p[i] == m.p && box[i] == rows) {
+      *map = maps[i];
+      return FA_OK;
+    }
+  const int rc = make_tmap_3d(map, m, 64, rows);
+  if (rc == FA_OK && n < kMost) {
+    p[n] = m.p;
+    box[n] = rows;
+    maps[n++] = *map;
+  }
+  return rc;
+}
+
+int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t st,
+                     TmapMemo* maps) {
   const bool narrow = epi != kEpiLinear && wide::use_narrow(p);
   const int tile_n = narrow ? wide::kNarrowBN : wide::kBN, tile_m = narrow ? 128 : 256;
   p.tiles_m = (p.M + tile_m - 1) / tile_m;
@@ -746,8 +778,11 @@ int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t 
   // a pair's CTA loads half of the tile's columns
   const int load_n = narrow ? tile_n : tile_n / 2;
   CUtensorMap ta, tb, te, tlow, td, td2;
-  int rc = make_tmap_3d(&ta, o.a, 64, 128);
-  if (!rc) rc = o.b_mn ? make_tmap_3d(&tb, o.b, 64, 64) : make_tmap_3d(&tb, o.b, 64, load_n);
+  auto encode = [&](CUtensorMap* m, const Mat3& x, int rows) {
+    return maps != nullptr ? maps->get(m, x, rows) : make_tmap_3d(m, x, 64, rows);
+  };
+  int rc = encode(&ta, o.a, 128);
+  if (!rc) rc = encode(&tb, o.b, o.b_mn ? 64 : load_n);
   te = tb;
   if (!rc && p.low != nullptr)
     rc = o.b_mn ? make_tmap_3d(&te, o.e, 64, 64) : make_tmap_3d(&te, o.e, 64, load_n);
@@ -755,9 +790,9 @@ int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t 
   if (!rc && p.low != nullptr)
     rc = make_tmap_3d(&tlow, Mat3{p.low, 1, p.M, p.low_ld, 0, p.low_stride, 1}, 64, 128);
   td = ta;
-  if (!rc && o.d.p != nullptr) rc = make_tmap_3d(&td, o.d, 64, 128);
+  if (!rc && o.d.p != nullptr) rc = encode(&td, o.d, 128);
   td2 = td;
-  if (!rc && o.d2.p != nullptr) rc = make_tmap_3d(&td2, o.d2, 64, 128);
+  if (!rc && o.d2.p != nullptr) rc = encode(&td2, o.d2, 128);
   if (rc) return rc;
 #define FA_WIDE(EPI, MN, ID) \
   if (epi == EPI && o.b_mn == MN) return wide::go<MN, EPI>(ta, tb, te, tlow, td, td2, p, ID, st);

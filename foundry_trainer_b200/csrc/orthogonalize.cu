@@ -619,6 +619,7 @@ static int wide_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, i
   if (rc) return rc;
   auto x_mat = [&](const __half* p) { return Mat3{p, batch, m, n, xb, ldx, 0}; };
   auto q_mat = [&](const __half* p) { return Mat3{p, batch, m, m, qb, ldq, 0}; };
+  TmapMemo maps;
   for (int s = 0; s < steps; ++s) {
     const __half* h = hi[s & 1];
     {  // Q 64 = (256 X)(256 X)^T / 1024
@@ -636,7 +637,7 @@ static int wide_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, i
       p.sym_out = q;
       p.sym_batch = qb;
       p.sym_ld = ldq;
-      if ((rc = launch_gemm_wide(op, p, kEpiGram, st))) return rc;
+      if ((rc = launch_gemm_wide(op, p, kEpiGram, st, &maps))) return rc;
     }
     {  // (b Q + c Q^2) 64
       WideOperands op;
@@ -655,7 +656,7 @@ static int wide_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, i
       p.sym_out = pq;
       p.sym_batch = qb;
       p.sym_ld = ldq;
-      if ((rc = launch_gemm_wide(op, p, kEpiPoly, st))) return rc;
+      if ((rc = launch_gemm_wide(op, p, kEpiPoly, st, &maps))) return rc;
     }
     const bool last = s + 1 == steps;
     WideOperands op;
@@ -686,7 +687,7 @@ static int wide_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, i
         op.d = Mat3{o, batch, m, n, ob, orow, 1};
       }
     }
-    if ((rc = launch_gemm_wide(op, p, last ? kEpiLast : kEpiUpdate, st))) return rc;
+    if ((rc = launch_gemm_wide(op, p, last ? kEpiLast : kEpiUpdate, st, &maps))) return rc;
   }
   return FA_OK;
 }
