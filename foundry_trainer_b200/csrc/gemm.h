@@ -28,6 +28,8 @@ enum WideEpi {
   kEpiLast = 4     // the same, as bf16 alpha D, straight or transposed
 };
 
+// e: the adapters, or the X that an update reads back as hi (d2: its lo, read
+// back and written).
 struct WideOperands {
   Mat3 a, b, e, d, d2;
   bool b_mn = false;
@@ -64,9 +66,6 @@ struct WideParams {
   const __half* in_lo = nullptr;
   int64_t in_batch = 0;
   int in_ld = 0;
-  void* sym_out = nullptr;
-  int64_t sym_batch = 0;
-  int sym_ld = 0;
   uint16_t* out_t = nullptr;
   int64_t out_t_batch = 0, out_t_ld = 0;
 };

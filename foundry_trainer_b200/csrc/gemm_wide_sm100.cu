@@ -45,19 +45,21 @@ constexpr int kBarBytes = 512;
 constexpr int kBN = 256;                     // columns of a tile
 constexpr int kStageB = kBN / 2 * 128;
 constexpr int kStage = kStageA + kStageB;
-constexpr int kStages = 6;
-constexpr int kOffStaging = kStages * kStage;
-constexpr int kOffBar = kOffStaging + 2 * kStaging;
-constexpr int kSmem = kOffBar + kBarBytes + 1024;  // + alignment slack
+// Ring slots and 16 KB epilogue buffers: the orthogonalisation's epilogues read
+// and write two matrices, twice buffered.
+constexpr int stages_of(int epi) { return epi == kEpiLinear ? 6 : 5; }
+constexpr int buffers_of(int epi) { return epi == kEpiLinear ? 2 : 4; }
+constexpr int bar_off_of(int epi) { return stages_of(epi) * kStage + buffers_of(epi) * kStaging; }
+constexpr int smem_of(int epi) { return bar_off_of(epi) + kBarBytes + 1024; }  // + alignment slack
 constexpr uint32_t kTmemCols = 2 * kBN;
-static_assert(kSmem <= 232448, "shared memory");
+static_assert(smem_of(kEpiLinear) <= 232448 && smem_of(kEpiUpdate) <= 232448, "shared memory");
 
 struct Tile {
   int m, n, b;  // 256-row block, kBN-column block, batch
 };
 
 // What an orthogonalisation product reads back for 32 columns of its result:
-// Q, or X as hi and lo.
+// Q, or X as hi and lo; from memory, or from the row's staged tiles.
 template <int EPI>
 struct Back {
   static constexpr bool kX = EPI == kEpiUpdate || EPI == kEpiLast;
@@ -76,16 +78,23 @@ struct Back {
       }
     }
   }
+  __device__ __forceinline__ void take(const uint8_t* hi, const uint8_t* lo, int r, int half) {
+    if constexpr (!kNone) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        q[i] = *reinterpret_cast<const uint4*>(hi + sw128_offset(r, 4 * half + i));
+        if constexpr (kX) l[i] = *reinterpret_cast<const uint4*>(lo + sw128_offset(r, 4 * half + i));
+      }
+    }
+  }
 };
 
 // These 32 columns as they are stored: out (16-bit pairs) and, for X, the
 // remainders lo.
 template <int EPI>
 __device__ __forceinline__ void ns_values(const WideParams& p, const Back<EPI>& back, float ca,
-                                          float cb, uint32_t taddr, uint32_t* out, uint32_t* lo) {
-  uint32_t acc[32];
-  tmem_ld32(taddr, acc);
-  tmem_wait_ld();
+                                          float cb, const uint32_t* acc, uint32_t* out,
+                                          uint32_t* lo) {
   const float* v = reinterpret_cast<const float*>(acc);
   const uint32_t* qw = reinterpret_cast<const uint32_t*>(back.q);
   const uint32_t* lw = reinterpret_cast<const uint32_t*>(back.l);
@@ -111,9 +120,8 @@ __device__ __forceinline__ void ns_values(const WideParams& p, const Back<EPI>& 
   }
 }
 
-// The same 32 values to the mirrored place of a symmetric result, or of the
-// last product of a tall input to their place in the transpose: a column of 32
-// consecutive rows per warp store.
+// The same 32 values of the last product of a tall input to their place in the
+// transpose (any alignment): a column of 32 consecutive rows per warp store.
 __device__ __forceinline__ void store_columns(uint16_t* o, int64_t ld, int col, int n,
                                               const uint32_t* out) {
   const uint16_t* h = reinterpret_cast<const uint16_t*>(out);
@@ -129,6 +137,23 @@ __device__ __forceinline__ void stage_half(uint8_t* buf, int r, int half, const 
   for (int i = 0; i < 4; ++i)
     *reinterpret_cast<uint4*>(buf + sw128_offset(r, 4 * half + i)) =
         make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+}
+
+// The same tile transposed, for the mirrored place of a symmetric result: two
+// blocks of 64 rows (the tile's columns) x 64 columns.
+__device__ __forceinline__ void stage_mirror(uint8_t* buf, int r, int half, const uint32_t* v) {
+  const uint16_t* h = reinterpret_cast<const uint16_t*>(v);
+  uint8_t* b = buf + (r >> 6) * 8192 + (r & 7) * 2;
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    *reinterpret_cast<uint16_t*>(b + sw128_offset(32 * half + i, (r & 63) >> 3)) = h[i];
+}
+
+// and its store by one thread: rows col0 .., columns row0 .. of the result
+__device__ __forceinline__ void store_mirror(const CUtensorMap* map, const uint8_t* buf, int row0,
+                                             int col0, int b, const WideParams& p) {
+  tma_store_3d(map, buf, row0, col0, b);
+  if (row0 + 64 < p.M) tma_store_3d(map, buf + 8192, row0 + 64, col0, b);
 }
 
 // Row block m of a symmetric walk, tiles_of(m) = per (m + 1) column tiles:
@@ -193,12 +218,14 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOffBar);
+  constexpr int kStages = stages_of(EPI), kOffStaging = kStages * kStage;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + bar_off_of(EPI));
   uint64_t* full = bars;                      // leader's is used
   uint64_t* empty = bars + kStages;        // both
   uint64_t* accfull = bars + 2 * kStages;  // both
   uint64_t* accempty = accfull + 2;           // leader's is used
-  uint32_t* slot = reinterpret_cast<uint32_t*>(accempty + 2);
+  uint64_t* back = accempty + 2;              // what the epilogue reads back landed
+  uint32_t* slot = reinterpret_cast<uint32_t*>(back + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
   const int warp = warp_id(), lane = lane_id();
   const uint32_t rank = cluster_rank();
@@ -212,6 +239,7 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
     for (int i = 0; i < 2; ++i) {
       mbar_init(&accfull[i], 1);
       mbar_init(&accempty[i], 8);
+      mbar_init(&back[i], 1);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -412,11 +440,20 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
         ca = p.coef[2 * tl.b];
         cb = p.coef[2 * tl.b + 1];
       }
-      // what a product reads back is fetched 32 columns ahead
-      Back<EPI> back[2];
-      if constexpr (EPI != kEpiLinear) back[0].load(p, tl.b, row, live, tl.n * kBN);
+      constexpr bool kReads = EPI == kEpiPoly || EPI == kEpiUpdate || EPI == kEpiLast;
+      constexpr bool kX = EPI == kEpiUpdate || EPI == kEpiLast;
+      // chunk g of this CTA's walk uses buffer pair g & 1; thread 0 requests the
+      // pair of the next one, whose last store has been read
+      auto request = [&](const Tile& o, int c, int g) {
+        uint8_t* b = stg + (g & 1) * 2 * kStaging;
+        const int row = o.m * 256 + (int)rank * 128, col = o.n * kBN + c * 64;
+        mbar_arrive_expect_tx(&back[g & 1], (kX ? 2 : 1) * kStaging);
+        tma_load_3d(b, kX ? &te : &ta, &back[g & 1], col, row, o.b);
+        if constexpr (kX) tma_load_3d(b + kStaging, &td2, &back[g & 1], col, row, o.b);
+      };
+      if (kReads && it == 0 && threadIdx.x == 0) request(tl, 0, 0);
       ok = mbar_wait_w(&accfull[buf], (it >> 1) & 1);
-      if (!ok) break;
+      if (named_bar_any(1, 128, !ok)) { ok = false; break; }
       tc_fence_after();
       // a block of several adapters: its rows must not see each other's
       const bool mixed = EPI == kEpiLinear && p.raw_x != nullptr && slots_of(p, tl.m) > 1;
@@ -425,11 +462,9 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
       for (int c = 0; c < kBN / 64; ++c) {
         const int col0 = tl.n * kBN + c * 64;
         const uint32_t taddr = tmem + lane_off + buf * kBN + c * 64;
-        // stage the 128 x 64 tile and store it with TMA (two buffers in turn,
-        // or one each for hi and lo)
-        constexpr bool kTwo = EPI == kEpiUpdate;
-        uint8_t* b0 = kTwo ? stg : stg + (c & 1) * kStaging;
         if constexpr (EPI == kEpiLinear) {
+          // stage the 128 x 64 tile and store it with TMA, two buffers in turn
+          uint8_t* b0 = stg + (c & 1) * kStaging;
           uint32_t acc[64];
           tmem_ld32(taddr, acc);
           tmem_ld32(taddr + 32, acc + 32);
@@ -471,45 +506,62 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
           named_bar_sync(1, 128);
           stage_half(b0, r, 0, acc);
           stage_half(b0, r, 1, acc + 16);
+          fence_proxy_async_smem();
+          named_bar_sync(1, 128);
+          if (threadIdx.x == 0) {
+            if (row0 < p.M && col0 < p.N) tma_store_3d(&td, b0, col0, row0, tl.b);
+            bulk_commit_group();
+          }
         } else {
+          const int g = it * (kBN / 64) + c;
           const bool direct = EPI == kEpiLast && p.out_t != nullptr;
+          uint8_t* b0 = stg + (g & 1) * 2 * kStaging;  // in: Q or hi; out: the tile
+          uint8_t* b1 = b0 + kStaging;                 // in and out: lo; out: the mirrored tile
+          if (threadIdx.x == 0) {
+            if constexpr (kReads) {
+              bulk_wait_group_read0();
+              const int64_t tn = t + pairs;
+              if (c + 1 < kBN / 64) request(tl, c + 1, g + 1);
+              else if (tn < tiles) request(tile_of(tn, p), 0, g + 1);
+            } else {
+              bulk_wait_group_read1();
+            }
+          }
+          if constexpr (kReads) ok = mbar_wait_w(&back[g & 1], (g >> 1) & 1);
+          if (named_bar_any(1, 128, !ok)) { ok = false; break; }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            uint32_t out[16], lo[16];
-            // (past the tile's last columns: loads that are not used)
-            back[1 - h].load(p, tl.b, row, live && (h == 0 || c + 1 < kBN / 64), col0 + 32 * h + 32);
-            ns_values<EPI>(p, back[h], ca, cb, taddr + 32 * h, out, lo);
+            uint32_t acc[32], out[16], lo[16];
+            Back<EPI> bk;
+            tmem_ld32(taddr + 32 * h, acc);
+            bk.take(b0, b1, r, h);
+            tmem_wait_ld();
+            ns_values<EPI>(p, bk, ca, cb, acc, out, lo);
             if (direct) {
               if (live)
                 store_columns(p.out_t + (int64_t)tl.b * p.out_t_batch + row, p.out_t_ld,
                               col0 + 32 * h, p.N, out);
               continue;
             }
-            if (mirror && live)
-              store_columns(reinterpret_cast<uint16_t*>(p.sym_out) + (int64_t)tl.b * p.sym_batch + row,
-                            p.sym_ld, col0 + 32 * h, p.N, out);
-            if (h == 0) {
-              if (threadIdx.x == 0) {
-                if constexpr (kTwo) bulk_wait_group_read0();
-                else bulk_wait_group_read1();
-              }
-              named_bar_sync(1, 128);
-            }
             stage_half(b0, r, h, out);
-            if constexpr (kTwo) stage_half(stg + kStaging, r, h, lo);
+            if constexpr (EPI == kEpiUpdate) stage_half(b1, r, h, lo);
+            if constexpr (!kX)
+              if (mirror) stage_mirror(b1, r, h, out);
           }
-          if (direct) continue;
-        }
-        fence_proxy_async_smem();
-        named_bar_sync(1, 128);
-        if (threadIdx.x == 0) {
-          if (row0 < p.M && col0 < p.N) {
-            tma_store_3d(&td, b0, col0, row0, tl.b);
-            if constexpr (kTwo) tma_store_3d(&td2, stg + kStaging, col0, row0, tl.b);
+          fence_proxy_async_smem();
+          named_bar_sync(1, 128);
+          if (threadIdx.x == 0 && !direct) {
+            if (row0 < p.M && col0 < p.N) {
+              tma_store_3d(&td, b0, col0, row0, tl.b);
+              if constexpr (EPI == kEpiUpdate) tma_store_3d(&td2, b1, col0, row0, tl.b);
+              if constexpr (!kX)
+                if (mirror) store_mirror(&tl_low, b1, row0, col0, tl.b, p);
+            }
+            bulk_commit_group();
           }
-          bulk_commit_group();
         }
       }
+      if (!ok) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(mapa(smem_u32(&accempty[buf]), 0));
@@ -534,14 +586,14 @@ static int go(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& t
               const CUtensorMap& tlow, const CUtensorMap& td, const CUtensorMap& td2, const WideParams& p, int kernel_id,
               cudaStream_t st) {
   auto* fn = wide_kernel<B_MN, EPI>;
-  const int rc = ensure_smem_attr((const void*)fn, kSmem, kernel_id);
+  const int rc = ensure_smem_attr((const void*)fn, smem_of(EPI), kernel_id);
   if (rc) return rc;
   const int64_t tiles = (int64_t)p.tiles_per_batch * p.batch;
   const int pairs = (int)std::min<int64_t>(tiles, 74);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * pairs);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmem;
+  cfg.dynamicSmemBytes = smem_of(EPI);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -571,7 +623,7 @@ constexpr int kNarrowSmem = kNarrowBar + 256 + 1024;
 template <bool B_MN, int EPI>
 __global__ void __launch_bounds__(kThreads, 2)
 narrow_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
-              const __grid_constant__ CUtensorMap td, const __grid_constant__ CUtensorMap td2,
+              const __grid_constant__ CUtensorMap tmir, const __grid_constant__ CUtensorMap td, const __grid_constant__ CUtensorMap td2,
               const __grid_constant__ WideParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -671,17 +723,17 @@ narrow_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
       const bool direct = EPI == kEpiLast && p.out_t != nullptr;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t out[16], lo[16];
-        ns_values<EPI>(p, back[h], ca, cb, taddr + 32 * h, out, lo);
+        uint32_t acc[32], out[16], lo[16];
+        tmem_ld32(taddr + 32 * h, acc);
+        tmem_wait_ld();
+        ns_values<EPI>(p, back[h], ca, cb, acc, out, lo);
         if (direct) {
           if (live)
             store_columns(p.out_t + (int64_t)b * p.out_t_batch + row, p.out_t_ld, col0 + 32 * h, p.N,
                           out);
           continue;
         }
-        if (mirror && live)
-          store_columns(reinterpret_cast<uint16_t*>(p.sym_out) + (int64_t)b * p.sym_batch + row,
-                        p.sym_ld, col0 + 32 * h, p.N, out);
+        if (mirror) stage_mirror(smem + kStaging, r, h, out);
         stage_half(smem, r, h, out);
         if constexpr (EPI == kEpiUpdate) stage_half(smem + kStaging, r, h, lo);
       }
@@ -692,6 +744,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
           if (row0 < p.M && col0 < p.N) {
             tma_store_3d(&td, smem, col0, row0, b);
             if constexpr (EPI == kEpiUpdate) tma_store_3d(&td2, smem + kStaging, col0, row0, b);
+            if (mirror) store_mirror(&tmir, smem + kStaging, row0, col0, b, p);
           }
           bulk_commit_group();
           bulk_wait_group_read0();
@@ -712,8 +765,8 @@ narrow_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
 }
 
 template <bool B_MN, int EPI>
-static int narrow_go(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& td,
-                     const CUtensorMap& td2, const WideParams& p, int kernel_id, cudaStream_t st) {
+static int narrow_go(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tmir,
+                     const CUtensorMap& td, const CUtensorMap& td2, const WideParams& p, int kernel_id, cudaStream_t st) {
   auto* fn = narrow_kernel<B_MN, EPI>;
   const int rc = ensure_smem_attr((const void*)fn, kNarrowSmem, kernel_id);
   if (rc) return rc;
@@ -727,7 +780,7 @@ static int narrow_go(const CUtensorMap& ta, const CUtensorMap& tb, const CUtenso
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = p.early ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, ta, tb, td, td2, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, ta, tb, tmir, td, td2, p);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return record_cuda_error(e);
@@ -789,6 +842,9 @@ int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t 
   tlow = ta;
   if (!rc && p.low != nullptr)
     rc = make_tmap_3d(&tlow, Mat3{p.low, 1, p.M, p.low_ld, 0, p.low_stride, 1}, 64, 128);
+  // the orthogonalisation's: X read back, and the mirrored store's 64 x 64 boxes
+  if (!rc && o.e.p != nullptr && p.low == nullptr) rc = encode(&te, o.e, 128);
+  if (!rc && p.symmetric) rc = encode(&tlow, o.d, 64);
   td = ta;
   if (!rc && o.d.p != nullptr) rc = encode(&td, o.d, 128);
   td2 = td;
@@ -798,7 +854,7 @@ int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t 
   if (epi == EPI && o.b_mn == MN) return wide::go<MN, EPI>(ta, tb, te, tlow, td, td2, p, ID, st);
 #define FA_NARROW(EPI, MN, ID)                    \
   if (narrow && epi == EPI && o.b_mn == MN)       \
-    return wide::narrow_go<MN, EPI>(ta, tb, td, td2, p, ID, st);
+    return wide::narrow_go<MN, EPI>(ta, tb, tlow, td, td2, p, ID, st);
   FA_NARROW(kEpiGram, false, kKernelNarrow)
   FA_NARROW(kEpiPoly, false, kKernelNarrow + 1)
   FA_NARROW(kEpiUpdate, true, kKernelNarrow + 2)

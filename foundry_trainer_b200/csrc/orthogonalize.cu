@@ -634,9 +634,6 @@ static int wide_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, i
       p.early = 2;
       p.symmetric = 1;
       p.alpha = 1.f / 1024.f;
-      p.sym_out = q;
-      p.sym_batch = qb;
-      p.sym_ld = ldq;
       if ((rc = launch_gemm_wide(op, p, kEpiGram, st, &maps))) return rc;
     }
     {  // (b Q + c Q^2) 64
@@ -653,9 +650,6 @@ static int wide_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, i
       p.in_hi = q;
       p.in_batch = qb;
       p.in_ld = ldq;
-      p.sym_out = pq;
-      p.sym_batch = qb;
-      p.sym_ld = ldq;
       if ((rc = launch_gemm_wide(op, p, kEpiPoly, st, &maps))) return rc;
     }
     const bool last = s + 1 == steps;
@@ -674,9 +668,10 @@ static int wide_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, i
     p.in_lo = lo;
     p.in_batch = xb;
     p.in_ld = ldx;
+    op.e = x_mat(h);
+    op.d2 = x_mat(lo);
     if (!last) {
       op.d = x_mat(hi[(s + 1) & 1]);
-      op.d2 = x_mat(lo);
     } else {
       p.alpha = 1.f / 256.f;
       if (tall) {
