@@ -794,15 +794,17 @@ static bool can_vector(int es, int dim, const Mat* m, int nm, const Par& par) {
 }
 
 // Rows of a ring kernel's turn, threads and ring depth for a row of nv
-// vectors: 256 threads while two vectors each suffice, R V = 4 vectors of
-// every tensor in registers a turn.
+// vectors: R V = 4 vectors of every tensor in registers a turn. The forward
+// takes two vectors a thread as soon as two warps remain (its two block-wide
+// sums a turn cost the same for either: 16384 x 2048 bf16 30 -> 25 us), the
+// backward, which has one, from 256 threads on (40 us at one, 41 at two).
 struct RingPlan {
   int V, R, threads, stages, smem, per_sm;
 };
 
 static RingPlan ring_plan(int nv, int tensors) {
   RingPlan p{};
-  p.V = nv <= 256 ? 1 : (nv <= 1024 ? 2 : 4);
+  p.V = nv <= (tensors == 1 ? 64 : 256) ? 1 : (nv <= 1024 ? 2 : 4);
   p.R = 4 / p.V;
   p.threads = ((nv + p.V - 1) / p.V + 31) / 32 * 32;
   const int stage = tensors * p.R * nv * 16;
