@@ -438,7 +438,7 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
     if constexpr (OUT == kSkinnyCols) {
       // out[j, i], a column a token
       const float bias = p.bias != nullptr ? __bfloat162float(p.bias[i]) : 0.f;
-      const bool mixed = adapters && plan.cnt > 1;
+      const bool mixed = adapters && p.ids != nullptr && plan.cnt > 0;
 #pragma unroll 2
       for (int j = j0; j < min(j1, cols); j += 4) {
         float acc[4];

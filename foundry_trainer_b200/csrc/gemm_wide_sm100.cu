@@ -455,8 +455,8 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
       ok = mbar_wait_w(&accfull[buf], (it >> 1) & 1);
       if (named_bar_any(1, 128, !ok)) { ok = false; break; }
       tc_fence_after();
-      // a block of several adapters: its rows must not see each other's
-      const bool mixed = EPI == kEpiLinear && p.raw_x != nullptr && slots_of(p, tl.m) > 1;
+      // a block with adapters of requests: a row must not see those of others
+      const bool mixed = EPI == kEpiLinear && p.raw_x != nullptr && slots_of(p, tl.m) > 0;
       const bool mirror = p.symmetric && tl.n < tl.m;
 #pragma unroll 1
       for (int c = 0; c < kBN / 64; ++c) {

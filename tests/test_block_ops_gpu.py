@@ -268,3 +268,9 @@ def test_lora_rows_do_not_touch_other_adapters():
                                        1.0, None)
         sup.within(got[even], want, tol, f"{N} rows beside a broken adapter")
         assert torch.isnan(got[~even]).all()
+        # rows without an adapter beside a broken one
+        ids[::2] = -1
+        got = ops.lora_linear_many(x, w, a2, b2, ids, scales)
+        want, tol, _, _ = sup.lora_ref(x[even].double(), w.double(), a[0].double() * 0,
+                                       b[0].double() * 0, 1.0, None)
+        sup.within(got[even], want, tol, f"{N} rows without an adapter")
