@@ -52,7 +52,9 @@ def gradient(seed, *shape, rank=4, noise=0.1, dtype=BF):
 SHAPES = [(1, 1), (1, 8, 8), (3, 16, 4096), (2, 4096, 16), (5, 12, 1000), (2, 1001, 7), (1, 33, 65),
           (2, 64, 2048), (2, 2056, 64), (1, 64, 64), (1, 5, 3), (4, 48, 3001), (1, 65, 65),
           (2, 72, 200), (1, 200, 72), (1, 256, 512), (2, 300, 1000), (1, 1000, 300), (1, 777, 777),
-          (1, 1024, 2048), (1, 1500, 520)]
+          (1, 1024, 2048), (1, 1500, 520),
+          # the SM-pair form of all three products, upright and tall, ragged
+          (1, 4096, 4104), (1, 4500, 4100), (3, 2305, 2500)]
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
