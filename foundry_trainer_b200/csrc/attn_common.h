@@ -32,11 +32,11 @@ enum KernelId {
   kKernelF32Bwd = 3,   // + 0..1: dK/dV and dQ
   kKernelWide = 5,     // + 0..5: the wide product by operand layout and epilogue
   kKernelSkinny = 11,  // + 0..4 by operand layout and output
-  kKernelThin = 16,    // + 0..11: the thin orthogonalisation by type, side and rank
-  kKernelNorm = 28,    // + 0..11: the ring layer norm by direction, type and width
-  kKernelSkinnyBig = 40,  // + 0..4: the same with one block an SM
-  kKernelNarrow = 45,  // + 0..3: the narrow product by epilogue
-  kKernelCount = 49
+  kKernelSkinnyBig = 16,  // + 0..4: the same with one block an SM
+  kKernelNarrow = 21,  // + 0..3: the narrow product by epilogue
+  kKernelNorm = 25,    // + 0..11: the ring layer norm by direction, type and width
+  kKernelThin = 37,    // + 0..15: the thin orthogonalisation by type, side and rank
+  kKernelCount = 53
 };
 
 // FA_OK when the last CUDA runtime call / launch on this thread succeeded;

@@ -85,7 +85,7 @@ struct Thin {
   static constexpr int kN = R / 8;
   static constexpr int kTiles = kN * (kN + 1) / 2;
   // Gram sums: warps that split the positions, and per set of 8 x 8 tiles
-  static constexpr int kSplit = R == 64 ? 4 : 16;
+  static constexpr int kSplit = R >= 48 ? 4 : 16;
   static constexpr int kPart = kSplit * kTiles * 64;
   static constexpr int kRest = 5 * kMat > kPart ? 5 * kMat : kPart;
   static constexpr int kSmem = (kMat + kTiles * 64 + kRest) * 8;
@@ -124,7 +124,7 @@ struct Turn {
 
 // One cluster per matrix (blockIdx.x / parts). TALL: the long side is the rows.
 template <typename T, int R, bool TALL>
-__global__ void __launch_bounds__(kThinThreads, R == 64 ? 1 : 2)
+__global__ void __launch_bounds__(kThinThreads, R >= 48 ? 1 : 2)
 thin_kernel(const T* g, int64_t g_batch, int64_t g_row, __nv_bfloat16* o, int64_t o_batch,
             int64_t o_row, int r, int len, int parts, int steps, int vec, int ovec, double ca,
             double cb, double cc, double eps) {
@@ -145,16 +145,20 @@ thin_kernel(const T* g, int64_t g_batch, int64_t g_row, __nv_bfloat16* o, int64_
   // ---- Gram matrix of the share
   {
     constexpr int EB = Turn<T, TALL>::EB, kTurn = 4 * EB;
-    // tiles of a warp: all, or at R = 64 a quarter: rows 0-3 or 4-7 of the
-    // tile triangle (10 tiles), or rows 0-3 with columns 4-5 or 6-7 (8)
-    constexpr int NF = R == 64 ? 4 : C::kN;
+    // tiles of a warp: all, or from R = 48 on a quarter of the triangle: its
+    // first or second half of rows against themselves (10 tiles at R = 64), or
+    // the first half's rows with two of the other columns (8)
+    constexpr bool kRoles = R >= 48;
+    constexpr int NF = kRoles ? C::kN / 2 : C::kN;
     constexpr int ND = NF * (NF + 1) / 2;
-    const int role = R == 64 ? warp & 3 : 0, set = R == 64 ? warp >> 2 : warp;
-    const int base = role == 1 ? 4 : 0;
+    constexpr int NR = kRoles ? NF : 0;  // rows of the rectangles
+    const int role = kRoles ? warp & 3 : 0, set = kRoles ? warp >> 2 : warp;
+    const int base = role == 1 ? NF : 0;
+    const int cols = role == 2 ? NF : NF + 2;  // (R = 48: the second has one column)
     double acc[ND][2];
 #pragma unroll
     for (int i = 0; i < ND; ++i) acc[i][0] = acc[i][1] = 0.0;
-    if (R < 64 || role < 2) {
+    if (!kRoles || role < 2) {
       for (int l = l0 + set * kTurn; l < l1; l += C::kSplit * kTurn) {
         Turn<T, TALL> f[NF];
 #pragma unroll
@@ -172,24 +176,21 @@ thin_kernel(const T* g, int64_t g_batch, int64_t g_row, __nv_bfloat16* o, int64_
             for (int j = i; j < NF; ++j) dmma(acc[k++], x[i], x[j]);
         }
       }
-    } else {
-      const int cols = role == 2 ? 4 : 6;
+    } else if constexpr (kRoles) {
       for (int l = l0 + set * kTurn; l < l1; l += C::kSplit * kTurn) {
-        Turn<T, TALL> f[4], h[2];
+        Turn<T, TALL> f[NR], h[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i].load(gm, g_row, r, i * 8 + gg, l, l1, vec, qq);
+        for (int i = 0; i < NR; ++i) f[i].load(gm, g_row, r, i * 8 + gg, l, l1, vec, qq);
 #pragma unroll
         for (int i = 0; i < 2; ++i) h[i].load(gm, g_row, r, (cols + i) * 8 + gg, l, l1, vec, qq);
 #pragma unroll
         for (int u = 0; u < EB; ++u) {
           const double y0 = h[0].at(u), y1 = h[1].at(u);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < NR; ++i) {
             const double x = f[i].at(u);
-            if constexpr (ND >= 8) {
-              dmma(acc[2 * i], x, y0);
-              dmma(acc[2 * i + 1], x, y1);
-            }
+            dmma(acc[2 * i], x, y0);
+            dmma(acc[2 * i + 1], x, y1);
           }
         }
       }
@@ -203,17 +204,18 @@ thin_kernel(const T* g, int64_t g_batch, int64_t g_row, __nv_bfloat16* o, int64_
       w[0] = d[0];
       w[1] = d[1];
     };
-    if (R < 64 || role < 2) {
+    if (!kRoles || role < 2) {
       int k = 0;
 #pragma unroll
       for (int i = 0; i < NF; ++i)
 #pragma unroll
         for (int j = i; j < NF; ++j) put(base + i, base + j, acc[k++]);
-    } else if constexpr (ND >= 8) {
+    } else if constexpr (kRoles) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < NR; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) put(i, (role == 2 ? 4 : 6) + j, acc[2 * i + j]);
+        for (int j = 0; j < 2; ++j)
+          if (cols + j < C::kN) put(i, cols + j, acc[2 * i + j]);
     }
   }
   __syncthreads();
@@ -575,7 +577,9 @@ static int thin_pick(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob,
     return thin_go<T, 16, TALL>(g, gb, gr, o, ob, orow, batch, r, len, steps, c, eps, kid, st);
   if (r <= 32)
     return thin_go<T, 32, TALL>(g, gb, gr, o, ob, orow, batch, r, len, steps, c, eps, kid + 1, st);
-  return thin_go<T, 64, TALL>(g, gb, gr, o, ob, orow, batch, r, len, steps, c, eps, kid + 2, st);
+  if (r <= 48)
+    return thin_go<T, 48, TALL>(g, gb, gr, o, ob, orow, batch, r, len, steps, c, eps, kid + 2, st);
+  return thin_go<T, 64, TALL>(g, gb, gr, o, ob, orow, batch, r, len, steps, c, eps, kid + 3, st);
 }
 
 template <typename T>
@@ -704,7 +708,7 @@ int launch_orthogonalize(int dtype, int batch, int rows, int cols, const void* g
   if (m > ns::kThinMost)
     return bf ? ns::wide_go<__nv_bfloat16>(g, gb, gr, o, ob, orow, batch, rows, cols, steps, c, eps, ws, st)
               : ns::wide_go<float>(g, gb, gr, o, ob, orow, batch, rows, cols, steps, c, eps, ws, st);
-  const int kid = kKernelThin + (bf ? 0 : 6) + (tall ? 3 : 0);
+  const int kid = kKernelThin + (bf ? 0 : 8) + (tall ? 4 : 0);
 #define FA_THIN(T, TALL) \
   ns::thin_pick<T, TALL>(g, gb, gr, o, ob, orow, batch, m, n, steps, c, eps, kid, st)
   if (bf) return tall ? FA_THIN(__nv_bfloat16, true) : FA_THIN(__nv_bfloat16, false);
