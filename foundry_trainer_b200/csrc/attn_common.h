@@ -36,7 +36,8 @@ enum KernelId {
   kKernelNarrow = 21,  // + 0..3: the narrow product by epilogue
   kKernelNorm = 25,    // + 0..11: the ring layer norm by direction, type and width
   kKernelThin = 37,    // + 0..15: the thin orthogonalisation by type, side and rank
-  kKernelCount = 53
+  kKernelNormLong = 53,   // + 0..9: the layer norm's backward of long rows by type and width
+  kKernelCount = 63
 };
 
 // FA_OK when the last CUDA runtime call / launch on this thread succeeded;

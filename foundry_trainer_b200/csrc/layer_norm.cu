@@ -54,11 +54,17 @@ __device__ __forceinline__ float to_f<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// E consecutive elements at p: one 16-byte access when E > 1, one element else
+// E consecutive elements at p: one access (16 bytes, or 2 elements, or 1)
 template <typename T, int E>
 __device__ __forceinline__ void load_e(const T* p, float* e) {
   if constexpr (E == 1) {
     e[0] = to_f<T>(*p);
+  } else if constexpr (E == 2 && sizeof(T) == 4) {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    e[0] = v.x; e[1] = v.y;
+  } else if constexpr (E == 2) {
+    const uint32_t v = *reinterpret_cast<const uint32_t*>(p);
+    e[0] = bf16_lo(v); e[1] = bf16_hi(v);
   } else if constexpr (sizeof(T) == 4) {
     const float4 v = *reinterpret_cast<const float4*>(p);
     e[0] = v.x; e[1] = v.y; e[2] = v.z; e[3] = v.w;
@@ -69,11 +75,33 @@ __device__ __forceinline__ void load_e(const T* p, float* e) {
   }
 }
 
+// The same from column c of a row, zeros past its end. One-element accesses load
+// some element in any case: with a branch for each the many loads of a long row
+// went out one by one (2000 x 12001 bf16: forward 130 -> 77 us, backward 220 ->
+// 97; with pairs the branch is the faster: 6 x 646 x 5426 fp32 42 and 61 us
+// against 46 and 79).
+template <typename T, int E>
+__device__ __forceinline__ void load_in(const T* row, int c, int dim, float* e) {
+  if constexpr (E == 1) {
+    load_e<T, E>(row + (c < dim ? c : 0), e);
+    e[0] = c < dim ? e[0] : 0.f;
+  } else if (c < dim) {
+    load_e<T, E>(row + c, e);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) e[i] = 0.f;
+  }
+}
+
 template <typename T, int E>
 __device__ __forceinline__ void store_e(T* p, const float* e) {
   if constexpr (E == 1) {
     if constexpr (sizeof(T) == 4) *p = e[0];
     else *p = __float2bfloat16_rn(e[0]);
+  } else if constexpr (E == 2 && sizeof(T) == 4) {
+    *reinterpret_cast<float2*>(p) = make_float2(e[0], e[1]);
+  } else if constexpr (E == 2) {
+    *reinterpret_cast<uint32_t*>(p) = pack_bf16(e[0], e[1]);
   } else if constexpr (sizeof(T) == 4) {
     *reinterpret_cast<float4*>(p) = make_float4(e[0], e[1], e[2], e[3]);
   } else {
@@ -96,12 +124,12 @@ __device__ __forceinline__ void load_par(const void* base, int64_t at, int bf16,
       const uint2 v = *reinterpret_cast<const uint2*>(p);
       e[0] = bf16_lo(v.x); e[1] = bf16_hi(v.x); e[2] = bf16_lo(v.y); e[3] = bf16_hi(v.y);
     } else {
-      e[0] = __bfloat162float(*p);
+      load_e<__nv_bfloat16, E>(p, e);
     }
   } else {
     const float* p = reinterpret_cast<const float*>(base) + at;
-    if constexpr (E == 1) {
-      e[0] = *p;
+    if constexpr (E <= 2) {
+      load_e<float, E>(p, e);
     } else {
 #pragma unroll
       for (int i = 0; i < E; i += 4) load_e<float, 4>(p + i, e + i);
@@ -117,11 +145,13 @@ __device__ __forceinline__ void load_pars(const void* base, int64_t at, int bf16
   if (base != nullptr && bf16) {
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      if (c + v * step < dim) load_par<E>(base, at + c + v * step, 1, none, e[v]);
+      if (E == 1 || c + v * step < dim)
+        load_par<E>(base, at + (c + v * step < dim ? c + v * step : 0), 1, none, e[v]);
   } else if (base != nullptr) {
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      if (c + v * step < dim) load_par<E>(base, at + c + v * step, 0, none, e[v]);
+      if (E == 1 || c + v * step < dim)
+        load_par<E>(base, at + (c + v * step < dim ? c + v * step : 0), 0, none, e[v]);
   } else {
 #pragma unroll
     for (int v = 0; v < V; ++v)
@@ -167,16 +197,18 @@ fwd_kernel(Mat x, Mat y, Par par, int64_t n_rows, int rows, int dim, float eps, 
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int c = (t + v * team) * E;
-    if (c < dim) {
-      load_e<T, E>(xr + c, e[v]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < E; ++i) e[v][i] = 0.f;
-    }
+    load_in<T, E>(xr, c, dim, e[v]);
   }
-  float w[V][E], b[V][E];
-  load_pars<E, V>(par.w, g * par.stride, par.bf16, 1.f - par.off, t * E, team * E, dim, w);
-  load_pars<E, V>(par.b, g * par.stride, par.bf16, 0.f, t * E, team * E, dim, b);
+  // the parameters are under way with the row; at 32 values a thread they would
+  // spill, and come half by half after the statistics
+  constexpr int kTurns = !WARP && V * E >= 32 ? 2 : 1, VT = V / kTurns;
+  float w[VT][E], b[VT][E];
+  auto parameters = [&](int first) {
+    const int c = (t + first * team) * E;
+    load_pars<E, VT>(par.w, g * par.stride, par.bf16, 1.f - par.off, c, team * E, dim, w);
+    load_pars<E, VT>(par.b, g * par.stride, par.bf16, 0.f, c, team * E, dim, b);
+  };
+  if constexpr (kTurns == 1) parameters(0);
   float s = 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v)
@@ -201,13 +233,18 @@ fwd_kernel(Mat x, Mat y, Par par, int64_t n_rows, int rows, int dim, float eps, 
   }
   T* yr = reinterpret_cast<T*>(y.p) + g * y.sg + r * y.sr;
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int c = (t + v * team) * E;
-    if (c < dim) {
-      float o[E];
+  for (int k = 0; k < kTurns; ++k) {
+    if constexpr (kTurns > 1) parameters(k * VT);
 #pragma unroll
-      for (int i = 0; i < E; ++i) o[i] = fmaf(e[v][i] * rstd, par.off + w[v][i], b[v][i]);
-      store_e<T, E>(yr + c, o);
+    for (int v = 0; v < VT; ++v) {
+      const int c = (t + (k * VT + v) * team) * E;
+      if (c < dim) {
+        float o[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          o[i] = fmaf(e[k * VT + v][i] * rstd, par.off + w[v][i], b[v][i]);
+        store_e<T, E>(yr + c, o);
+      }
     }
   }
 }
@@ -236,23 +273,16 @@ bwd_kernel(Mat x, Mat dy, Mat dx, Par par, const float* stats, int64_t n_rows, i
   const int me = WARP ? (int)(threadIdx.x >> 5) : 0;
   const int g = blockIdx.x / chunks, chunk = blockIdx.x - g * chunks;
   const int r0 = chunk * per, r1 = min(rows, r0 + per);
-  // off + w stays in registers, except at 32 columns a thread (dim > 8192),
-  // where it is read again for every row
-  constexpr bool kKeepW = V * E < 32;
-  float w[kKeepW ? V : 1][E], aw[V][E], ab[V][E];
+  float w[V][E], aw[V][E], ab[V][E];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int c = (t + v * team) * E;
 #pragma unroll
-    for (int i = 0; i < E; ++i) aw[v][i] = ab[v][i] = 0.f;
-    if constexpr (kKeepW) {
+    for (int i = 0; i < E; ++i) aw[v][i] = ab[v][i] = w[v][i] = 0.f;
+    if (c < dim) {
+      load_par<E>(par.w, (int64_t)g * par.stride + c, par.bf16, 1.f - par.off, w[v]);
 #pragma unroll
-      for (int i = 0; i < E; ++i) w[v][i] = 0.f;
-      if (c < dim) {
-        load_par<E>(par.w, (int64_t)g * par.stride + c, par.bf16, 1.f - par.off, w[v]);
-#pragma unroll
-        for (int i = 0; i < E; ++i) w[v][i] += par.off;
-      }
+      for (int i = 0; i < E; ++i) w[v][i] += par.off;
     }
   }
   const T* xg = reinterpret_cast<const T*>(x.p) + (int64_t)g * x.sg;
@@ -287,25 +317,13 @@ bwd_kernel(Mat x, Mat dy, Mat dx, Par par, const float* stats, int64_t n_rows, i
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const bool in = live && (t + v * team) * E < dim;
-        float* wv = w[kKeepW ? v : 0];
-        if constexpr (!kKeepW) {
-          if (in) {
-            load_par<E>(par.w, (int64_t)g * par.stride + (t + v * team) * E, par.bf16,
-                        1.f - par.off, wv);
-#pragma unroll
-            for (int i = 0; i < E; ++i) wv[i] += par.off;
-          } else {
-#pragma unroll
-            for (int i = 0; i < E; ++i) wv[i] = 0.f;
-          }
-        }
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           h[k][v][i] = in ? (h[k][v][i] - mean) * rs[k] : 0.f;
           const float dv = d[k][v][i];
           ab[v][i] += dv;
           aw[v][i] = fmaf(dv, h[k][v][i], aw[v][i]);
-          const float tt = dv * wv[i];
+          const float tt = dv * w[v][i];
           d[k][v][i] = tt;
           s1 += tt;
           s2 = fmaf(tt, h[k][v][i], s2);
@@ -380,6 +398,97 @@ bwd_kernel(Mat x, Mat dy, Mat dx, Par par, const float* stats, int64_t n_rows, i
           dst[dim + c + i] = ab[v][i];
         }
       }
+    }
+  }
+}
+
+// The same for rows of 16 to 32 values a thread: off + w and the columns' sums
+// are in shared memory, (3, dim) fp32 that each thread reads and writes at its
+// own columns only; registers hold the row alone. (All of it in registers left
+// one block an SM and the weight's loads in the row's way: 6 x 646 x 5426 fp32
+// 190 -> 61 us, its bytes 39.)
+template <typename T, int E, int V>
+__global__ void __launch_bounds__(512)
+bwd_long_kernel(Mat x, Mat dy, Mat dx, Par par, const float* stats, int64_t n_rows, int rows,
+                int dim, int per, int chunks, float* part) {
+  extern __shared__ __align__(16) float lsm[];
+  __shared__ float red[2][32][2];
+  float *sw = lsm, *saw = lsm + dim, *sab = lsm + 2 * dim;
+  const int t = threadIdx.x, team = blockDim.x;
+  const int g = blockIdx.x / chunks, chunk = blockIdx.x - g * chunks;
+  const int r0 = chunk * per, r1 = min(rows, r0 + per);
+  const int wid = t >> 5, nw = team >> 5, lane = t & 31;
+#pragma unroll 4
+  for (int c = t * E; c < dim; c += team * E) {
+    float w[E], zero[E] = {};
+    load_par<E>(par.w, (int64_t)g * par.stride + c, par.bf16, 1.f - par.off, w);
+#pragma unroll
+    for (int i = 0; i < E; ++i) w[i] += par.off;
+    store_e<float, E>(sw + c, w);
+    store_e<float, E>(saw + c, zero);
+    store_e<float, E>(sab + c, zero);
+  }
+  const float inv = 1.f / (float)dim;
+  int flip = 0;
+  for (int r = r0; r < r1; ++r) {
+    const T* xr = reinterpret_cast<const T*>(x.p) + (int64_t)g * x.sg + (int64_t)r * x.sr;
+    const T* dyr = reinterpret_cast<const T*>(dy.p) + (int64_t)g * dy.sg + (int64_t)r * dy.sr;
+    T* dxr = reinterpret_cast<T*>(dx.p) + (int64_t)g * dx.sg + (int64_t)r * dx.sr;
+    const int64_t row = (int64_t)g * rows + r;
+    float h[V][E], d[V][E];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int c = (t + v * team) * E;
+      load_in<T, E>(xr, c, dim, h[v]);
+      load_in<T, E>(dyr, c, dim, d[v]);
+    }
+    const float mean = stats[row], rs = stats[n_rows + row];
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int c = (t + v * team) * E;
+      if (c < dim) {
+        float w[E], aw[E], ab[E];
+        load_e<float, E>(sw + c, w);
+        load_e<float, E>(saw + c, aw);
+        load_e<float, E>(sab + c, ab);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          h[v][i] = (h[v][i] - mean) * rs;
+          ab[i] += d[v][i];
+          aw[i] = fmaf(d[v][i], h[v][i], aw[i]);
+          d[v][i] *= w[i];
+          s[0] += d[v][i];
+          s[1] = fmaf(d[v][i], h[v][i], s[1]);
+        }
+        store_e<float, E>(saw + c, aw);
+        store_e<float, E>(sab + c, ab);
+      }
+    }
+    warp_sums<2>(s);
+    if (lane == 0) red[flip][wid][0] = s[0], red[flip][wid][1] = s[1];
+    __syncthreads();
+    s[0] = s[1] = 0.f;
+    for (int i = 0; i < nw; ++i) s[0] += red[flip][i][0], s[1] += red[flip][i][1];
+    flip ^= 1;  // double-buffered, so one barrier a row suffices
+    const float c1 = s[0] * inv, c2 = s[1] * inv;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int c = (t + v * team) * E;
+      if (c < dim) {
+        float o[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] = rs * (d[v][i] - c1 - h[v][i] * c2);
+        store_e<T, E>(dxr + c, o);
+      }
+    }
+  }
+  float* dst = part + (int64_t)blockIdx.x * 2 * dim;
+  for (int c = t * E; c < dim; c += team * E) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      dst[c + i] = saw[c + i];
+      dst[dim + c + i] = sab[c + i];
     }
   }
 }
@@ -773,24 +882,24 @@ join_kernel(const float* part, int parts, int dim, float* dw, float* db) {
 }
 
 constexpr int kSms = 148;
+constexpr int kMaxDim = 16384;
 
-static bool vec16(const void* p, int64_t a, int64_t b, int es) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (a * es) % 16 == 0 && (b * es) % 16 == 0;
-}
-
-// 16-byte accesses everywhere, or one element at a time
-static bool can_vector(int es, int dim, const Mat* m, int nm, const Par& par) {
-  const int e = 16 / es;
-  if (dim % e != 0) return false;
-  for (int i = 0; i < nm; ++i)
-    if (!vec16(m[i].p, m[i].sg, m[i].sr, es)) return false;
+// Elements per access: 16 bytes' worth, 2, or 1, whichever every row start, the
+// width and the parameters allow.
+static int access_width(int es, int dim, const Mat* m, int nm, const Par& par) {
   const int ps = par.bf16 ? 2 : 4;
-  const int need = std::min(16, e * ps);  // load_par's widest access
-  for (const void* p : {par.w, par.b})
-    if (p != nullptr &&
-        (reinterpret_cast<uintptr_t>(p) % need != 0 || (par.stride * ps) % need != 0))
-      return false;
-  return true;
+  for (int e : {16 / es, 2}) {
+    bool ok = dim % e == 0;
+    for (int i = 0; i < nm; ++i)
+      ok = ok && reinterpret_cast<uintptr_t>(m[i].p) % (e * es) == 0 && m[i].sg % e == 0 &&
+           m[i].sr % e == 0;
+    const int need = std::min(16, e * ps);  // load_par's widest access
+    for (const void* p : {par.w, par.b})
+      ok = ok && (p == nullptr || (reinterpret_cast<uintptr_t>(p) % need == 0 &&
+                                   (par.stride * ps) % need == 0));
+    if (ok) return e;
+  }
+  return 1;
 }
 
 // Rows of a ring kernel's turn, threads and ring depth for a row of nv
@@ -858,7 +967,7 @@ static int fwd_pick(const Mat& x, const Mat& y, const Par& par, int groups, int 
                     float eps, float* stats, cudaStream_t st) {
   const int nv = (dim + E - 1) / E;
   const int64_t n = (int64_t)groups * rows;
-  if constexpr (E > 1) {
+  if constexpr (E > 2) {
     // a few rows a block at least, or the ring's set-up is all there is
     if (use_ring(nv) && n >= 8 * kSms) {
       const RingPlan p = ring_plan(nv, 1);
@@ -869,36 +978,47 @@ static int fwd_pick(const Mat& x, const Mat& y, const Par& par, int groups, int 
       return fwd_ring_go<T, E, 4>(x, y, par, groups, rows, dim, eps, stats, p, kid + 2, st);
     }
   }
-  // a warp per row while a lane's share stays at 32 values or below and the
-  // rows are many; few rows take a block each
-  constexpr int kMost = 32 / E;
+  // a warp per row while the rows are many and a lane's share is at most 32
+  // values (with pairs 8: 4000 x 514 bf16 6.9 us as blocks, 9.9 as warps of 16
+  // pairs; single elements stay with warps: 1000 x 1001 fp32 4.0 against 4.8);
+  // else a block per row, of up to 512 threads and 32 values each
   const int need = (nv + 31) / 32;
-  if (need <= 1 || (need <= kMost && n >= 2 * kSms)) {
+  constexpr int kLane = E == 2 ? 4 : 32 / E;
+  if (need <= 1 || (need <= kLane && n >= 2 * kSms)) {
     const int th = n >= 8 * kSms ? 256 : (n >= 2 * kSms ? 128 : 32);
     if (need <= 1) return fwd_go<T, E, 1, true>(x, y, par, n, rows, dim, eps, stats, th, st);
-    if constexpr (kMost >= 8)
-      if (need <= kMost / 4)
-        return fwd_go<T, E, kMost / 4, true>(x, y, par, n, rows, dim, eps, stats, th, st);
-    return fwd_go<T, E, kMost, true>(x, y, par, n, rows, dim, eps, stats, th, st);
+    if constexpr (kLane >= 8)
+      if (need <= kLane / 4)
+        return fwd_go<T, E, kLane / 4, true>(x, y, par, n, rows, dim, eps, stats, th, st);
+    return fwd_go<T, E, kLane, true>(x, y, par, n, rows, dim, eps, stats, th, st);
   }
   auto th = [&](int v) { return ((nv + v - 1) / v + 31) / 32 * 32; };
-  if (nv <= 512) return fwd_go<T, E, 1, false>(x, y, par, n, rows, dim, eps, stats, th(1), st);
-  return fwd_go<T, E, kMost, false>(x, y, par, n, rows, dim, eps, stats, th(kMost), st);
+  if constexpr (E > 2) {
+    if (nv <= 512) return fwd_go<T, E, 1, false>(x, y, par, n, rows, dim, eps, stats, th(1), st);
+    return fwd_go<T, E, 32 / E, false>(x, y, par, n, rows, dim, eps, stats, th(32 / E), st);
+  } else {
+    if (nv <= 4 * 512) return fwd_go<T, E, 4, false>(x, y, par, n, rows, dim, eps, stats, th(4), st);
+    if (nv <= 16 / E * 512)
+      return fwd_go<T, E, 16 / E, false>(x, y, par, n, rows, dim, eps, stats, th(16 / E), st);
+    return fwd_go<T, E, 32 / E, false>(x, y, par, n, rows, dim, eps, stats, th(32 / E), st);
+  }
 }
 
 struct BwdPlan {
   Split s;
-  bool ring;
+  bool ring, lng;
 };
 
 // The backward's blocks, each of which leaves one partial sum of dw and db:
-// with the ring as many as are resident, else four an SM.
+// with the ring, or sums in shared memory (beyond 8 values a thread of 512), as
+// many as are resident, else four an SM.
 static BwdPlan bwd_plan(int es, bool vec, int groups, int rows, int dim) {
   const int nv = dim / (16 / es);
   BwdPlan p{};
   p.ring = vec && use_ring(nv);
-  p.s = p.ring ? split_of(groups, rows, ring_plan(nv, 2).per_sm * kSms, 4)
-               : split_of(groups, rows, 4 * kSms, 4);
+  p.lng = !p.ring && dim > 8 * 512;
+  const int slots = p.ring ? ring_plan(nv, 2).per_sm : p.lng ? (dim > 16 * 512 ? 1 : 2) : 4;
+  p.s = split_of(groups, rows, slots * kSms, p.lng ? 1 : 4);
   return p;
 }
 
@@ -908,6 +1028,19 @@ static int bwd_go(const Mat& x, const Mat& dy, const Mat& dx, const Par& par, co
                   cudaStream_t st) {
   const int smem = WARP ? threads / 32 * 2 * dim * 4 : 0;
   bwd_kernel<T, E, V, R, WARP><<<(unsigned)((int64_t)groups * s.chunks), threads, smem, st>>>(
+      x, dy, dx, par, stats, (int64_t)groups * rows, rows, dim, s.per, s.chunks, part);
+  return launch_status();
+}
+
+template <typename T, int E, int V>
+static int bwd_long_go(const Mat& x, const Mat& dy, const Mat& dx, const Par& par,
+                       const float* stats, int groups, int rows, int dim, const Split& s, int kid,
+                       float* part, cudaStream_t st) {
+  auto* fn = bwd_long_kernel<T, E, V>;
+  const int rc = ensure_smem_attr((const void*)fn, 3 * kMaxDim * 4, kid);
+  if (rc) return rc;
+  const int nv = (dim + E - 1) / E, threads = ((nv + V - 1) / V + 31) / 32 * 32;
+  fn<<<(unsigned)((int64_t)groups * s.chunks), threads, 3 * dim * 4, st>>>(
       x, dy, dx, par, stats, (int64_t)groups * rows, rows, dim, s.per, s.chunks, part);
   return launch_status();
 }
@@ -930,7 +1063,7 @@ static int bwd_pick(const Mat& x, const Mat& dy, const Mat& dx, const Par& par,
                     float* part, cudaStream_t st) {
   const int nv = (dim + E - 1) / E;
   const Split& s = pl.s;
-  if constexpr (E > 1) {
+  if constexpr (E > 2) {
     if (pl.ring) {
       const RingPlan p = ring_plan(nv, 2);
       const int kid = kKernelNorm + 6 + (sizeof(T) == 2 ? 0 : 3);
@@ -942,15 +1075,23 @@ static int bwd_pick(const Mat& x, const Mat& dy, const Mat& dx, const Par& par,
   if (nv <= 32)  // a warp holds the row (dim <= 256): 8 teams, 16 KB of shared memory at most
     return bwd_go<T, E, 1, 4, true>(x, dy, dx, par, stats, groups, rows, dim, s, 256, part, st);
   auto th = [&](int v) { return ((nv + v - 1) / v + 31) / 32 * 32; };
-  if constexpr (E == 1) {
-    if (nv <= 4 * 512)
-      return bwd_go<T, E, 4, 2, false>(x, dy, dx, par, stats, groups, rows, dim, s, th(4), part, st);
-    return bwd_go<T, E, 32, 1, false>(x, dy, dx, par, stats, groups, rows, dim, s, th(32), part, st);
-  } else {  // 33 to 63 vectors, or fp32 rows of more than 32 KB
+  constexpr int kLong = kKernelNormLong + (sizeof(T) == 2 ? 0 : 5);
+  if constexpr (E > 2) {
+    // 33 to 63 vectors, or fp32 rows of more than 32 KB
     if constexpr (E == 4)
-      if (nv > 2048)
-        return bwd_go<T, E, 8, 1, false>(x, dy, dx, par, stats, groups, rows, dim, s, th(8), part, st);
+      if (pl.lng)
+        return bwd_long_go<T, E, 8>(x, dy, dx, par, stats, groups, rows, dim, s, kLong + 4, part, st);
     return bwd_go<T, E, 1, 4, false>(x, dy, dx, par, stats, groups, rows, dim, s, th(1), part, st);
+  } else {
+    constexpr int kid = kLong + 2 * (E - 1);
+    if (!pl.lng) {
+      if (nv <= 4 / E * 512)
+        return bwd_go<T, E, 4 / E, 2, false>(x, dy, dx, par, stats, groups, rows, dim, s, th(4 / E), part, st);
+      return bwd_go<T, E, 8 / E, 1, false>(x, dy, dx, par, stats, groups, rows, dim, s, th(8 / E), part, st);
+    }
+    if (nv <= 16 / E * 512)
+      return bwd_long_go<T, E, 16 / E>(x, dy, dx, par, stats, groups, rows, dim, s, kid, part, st);
+    return bwd_long_go<T, E, 32 / E>(x, dy, dx, par, stats, groups, rows, dim, s, kid + 1, part, st);
   }
 }
 
@@ -966,14 +1107,15 @@ int launch_layer_norm_fwd(int dtype, int groups, int rows, int dim, const fa_ten
   if (n == 0) return FA_OK;
   const ln::Mat m[2] = {ln_mat(x), ln_mat(y)};
   const ln::Par par{w, b, par_stride, par_dtype == FA_DTYPE_BF16, unit_offset ? 1.f : 0.f};
-  if (dtype == FA_DTYPE_BF16) {
-    return ln::can_vector(2, dim, m, 2, par)
-               ? ln::fwd_pick<__nv_bfloat16, 8>(m[0], m[1], par, groups, rows, dim, eps, stats, st)
-               : ln::fwd_pick<__nv_bfloat16, 1>(m[0], m[1], par, groups, rows, dim, eps, stats, st);
-  }
-  return ln::can_vector(4, dim, m, 2, par)
-             ? ln::fwd_pick<float, 4>(m[0], m[1], par, groups, rows, dim, eps, stats, st)
-             : ln::fwd_pick<float, 1>(m[0], m[1], par, groups, rows, dim, eps, stats, st);
+  const int es = dtype == FA_DTYPE_BF16 ? 2 : 4;
+  const int e = ln::access_width(es, dim, m, 2, par);
+#define FA_LN(T, E) ln::fwd_pick<T, E>(m[0], m[1], par, groups, rows, dim, eps, stats, st)
+  if (es == 2)
+    return e == 8   ? FA_LN(__nv_bfloat16, 8)
+           : e == 2 ? FA_LN(__nv_bfloat16, 2)
+                    : FA_LN(__nv_bfloat16, 1);
+  return e == 4 ? FA_LN(float, 4) : e == 2 ? FA_LN(float, 2) : FA_LN(float, 1);
+#undef FA_LN
 }
 
 size_t layer_norm_bwd_workspace(int groups, int rows, int dim) {
@@ -994,16 +1136,19 @@ int launch_layer_norm_bwd(int dtype, int groups, int rows, int dim, const fa_ten
   const int es = dtype == FA_DTYPE_BF16 ? 2 : 4;
   const ln::Mat m[3] = {ln_mat(x), ln_mat(dy), ln_mat(dx)};
   const ln::Par par{w, nullptr, par_stride, par_dtype == FA_DTYPE_BF16, unit_offset ? 1.f : 0.f};
-  const bool vec = ln::can_vector(es, dim, m, 3, par);
-  const ln::BwdPlan pl = ln::bwd_plan(es, vec, groups, rows, dim);
+  const int e = ln::access_width(es, dim, m, 3, par);
+  const ln::BwdPlan pl = ln::bwd_plan(es, e == 16 / es, groups, rows, dim);
   if (groups > 0) {
     int rc;
+#define FA_LN(T, E) \
+  ln::bwd_pick<T, E>(m[0], m[1], m[2], par, stats, groups, rows, dim, pl, part, st)
     if (es == 2)
-      rc = vec ? ln::bwd_pick<__nv_bfloat16, 8>(m[0], m[1], m[2], par, stats, groups, rows, dim, pl, part, st)
-               : ln::bwd_pick<__nv_bfloat16, 1>(m[0], m[1], m[2], par, stats, groups, rows, dim, pl, part, st);
+      rc = e == 8   ? FA_LN(__nv_bfloat16, 8)
+           : e == 2 ? FA_LN(__nv_bfloat16, 2)
+                    : FA_LN(__nv_bfloat16, 1);
     else
-      rc = vec ? ln::bwd_pick<float, 4>(m[0], m[1], m[2], par, stats, groups, rows, dim, pl, part, st)
-               : ln::bwd_pick<float, 1>(m[0], m[1], m[2], par, stats, groups, rows, dim, pl, part, st);
+      rc = e == 4 ? FA_LN(float, 4) : e == 2 ? FA_LN(float, 2) : FA_LN(float, 1);
+#undef FA_LN
     if (rc != FA_OK) return rc;
   }
   if (dw == nullptr && db == nullptr) return FA_OK;
@@ -1018,10 +1163,11 @@ int launch_layer_norm_bwd(int dtype, int groups, int rows, int dim, const fa_ten
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = groups > 0 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, ln::join_kernel, (const float*)part, parts, dim, dw, db);
-  if (e != cudaSuccess) {
+  const cudaError_t err =
+      cudaLaunchKernelEx(&cfg, ln::join_kernel, (const float*)part, parts, dim, dw, db);
+  if (err != cudaSuccess) {
     cudaGetLastError();
-    return record_cuda_error(e);
+    return record_cuda_error(err);
   }
   return launch_status();
 }

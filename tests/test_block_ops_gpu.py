@@ -59,6 +59,14 @@ NORM_CASES = [
     (1, 1201, 8200, BF, True, True),
     (1, 5, 16384, F32, False, False),
     (1, 1200, 300, F32, True, True),
+    # even widths that no 16-byte access divides, in each of their forms
+    (2, 600, 26, BF, False, False),
+    (1, 700, 250, F32, True, True),
+    (1, 1300, 514, BF, False, False),
+    (7, 5, 5798, BF, False, True),
+    (2, 9, 4098, F32, True, False),
+    (2, 20, 8190, BF, True, True),
+    (1, 7, 16382, F32, False, False),
 ]
 
 
