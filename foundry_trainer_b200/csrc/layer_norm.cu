@@ -183,7 +183,7 @@ __device__ __forceinline__ float team_sum(float v, float* red) {
 // One row per warp (WARP) or per block; thread t of the row's `team` threads
 // owns vectors t, t + team, ... (V of them, E elements each).
 template <typename T, int E, int V, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 512)
+__global__ void __launch_bounds__(WARP ? 256 : 512, WARP && E == 1 && V == 32 ? 3 : 0)
 fwd_kernel(Mat x, Mat y, Par par, int64_t n_rows, int rows, int dim, float eps, float* stats) {
   __shared__ float red[32];
   const int team = WARP ? 32 : blockDim.x;
@@ -200,8 +200,9 @@ fwd_kernel(Mat x, Mat y, Par par, int64_t n_rows, int rows, int dim, float eps, 
     load_in<T, E>(xr, c, dim, e[v]);
   }
   // the parameters are under way with the row; at 32 values a thread they would
-  // spill, and come half by half after the statistics
-  constexpr int kTurns = !WARP && V * E >= 32 ? 2 : 1, VT = V / kTurns;
+  // spill or leave half the warps (3001 x 1001 bf16 10.8 -> 8.3 us), and come
+  // in turns after the statistics
+  constexpr int kTurns = V * E < 32 ? 1 : !WARP ? 2 : E == 1 ? 4 : 1, VT = V / kTurns;
   float w[VT][E], b[VT][E];
   auto parameters = [&](int first) {
     const int c = (t + first * team) * E;
@@ -980,7 +981,7 @@ static int fwd_pick(const Mat& x, const Mat& y, const Par& par, int groups, int 
   }
   // a warp per row while the rows are many and a lane's share is at most 32
   // values (with pairs 8: 4000 x 514 bf16 6.9 us as blocks, 9.9 as warps of 16
-  // pairs; single elements stay with warps: 1000 x 1001 fp32 4.0 against 4.8);
+  // pairs; single elements stay with warps: 1000 x 1001 fp32 4.4 against 4.8);
   // else a block per row, of up to 512 threads and 32 values each
   const int need = (nv + 31) / 32;
   constexpr int kLane = E == 2 ? 4 : 32 / E;
@@ -990,6 +991,8 @@ static int fwd_pick(const Mat& x, const Mat& y, const Par& par, int groups, int 
     if constexpr (kLane >= 8)
       if (need <= kLane / 4)
         return fwd_go<T, E, kLane / 4, true>(x, y, par, n, rows, dim, eps, stats, th, st);
+    if constexpr (E == 1)
+      if (need <= 16) return fwd_go<T, E, 16, true>(x, y, par, n, rows, dim, eps, stats, th, st);
     return fwd_go<T, E, kLane, true>(x, y, par, n, rows, dim, eps, stats, th, st);
   }
   auto th = [&](int v) { return ((nv + v - 1) / v + 31) / 32 * 32; };

@@ -392,7 +392,7 @@ thin_kernel(const T* g, int64_t g_batch, int64_t g_row, __nv_bfloat16* o, int64_
 
 // ------------------------------------------------------------ the wide form
 
-constexpr int kNormBlocks = 256;  // partial sums of squares per matrix
+constexpr int kNormBlocks = 592;  // partial sums of squares per matrix: four an SM
 
 // part[mat][block] = sum of squares over every kNormBlocks-th row, in fp64 (the
 // squares of fp32 values may leave fp32's range). `vec`: 16-byte loads.
@@ -438,7 +438,8 @@ norm_kernel(const T* g, int64_t g_batch, int64_t g_row, int m, int n, int vec, d
 // |G| + eps = nu 2^e, 1 <= nu < 2, from the partial sums (256 threads)
 __device__ __forceinline__ double norm_of(const double* part, double eps, int* e) {
   __shared__ double red[8];
-  double s = part[threadIdx.x];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < kNormBlocks; i += 256) s += part[i];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (lane_id() == 0) red[warp_id()] = s;
