@@ -180,4 +180,33 @@ __device__ __forceinline__ void pdl_wait_previous() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// Whether `n` bf16 values from p (16-byte aligned) on hold a NaN or an infinity.
+__device__ __forceinline__ bool any_non_finite(const __nv_bfloat16* p, int n) {
+  uint32_t bad = 0;
+  auto word = [&](uint32_t w) {  // a half whose exponent is all ones
+    bad |= (uint32_t)((w & 0x7f80u) == 0x7f80u) | (uint32_t)((w & 0x7f800000u) == 0x7f800000u);
+  };
+  int k = 0;
+  for (; k + 8 <= n; k += 8) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + k));
+    word(v.x), word(v.y), word(v.z), word(v.w);
+  }
+  for (; k < n; ++k) word((uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p) + k));
+  return bad != 0;
+}
+
+// A block's adapters whose factors' row holds a NaN or an infinity: how many of
+// the `cnt` in `list`, as kNoneBad, the slot of the only one, or kSeveralBad. Such a
+// factor is what may have reached the rows of other adapters (as zero times
+// it); where there is none, a non-finite sum is a row's own.
+enum : int { kNoneBad = -1, kSeveralBad = -2 };
+static __device__ __noinline__ int bad_factors(const __nv_bfloat16* f, int64_t f_adapter, int rank,
+                                        const int* list, int cnt) {
+  int bad = kNoneBad;
+  for (int q = 0; q < cnt; ++q)
+    if (any_non_finite(f + (int64_t)list[q] * f_adapter, rank))
+      bad = bad == kNoneBad ? q : kSeveralBad;
+  return bad;
+}
+
 }  // namespace fa

@@ -126,8 +126,8 @@ __device__ __forceinline__ void plan_tokens(TokenPlan& pl, const int* ids, int c
 }
 
 // One output value from its own token's operands alone, for values that a
-// block of several adapters left non-finite (zero times a NaN or infinity of
-// another token's adapter).
+// block with adapters left non-finite where another token's adapter holds a NaN
+// or an infinity (zero times it).
 __device__ __noinline__ float one_value(const SkinnyParams& p, int j, int i) {
   const __nv_bfloat16* x = p.raw_x + (int64_t)j * p.raw_ldx;
   const __nv_bfloat16* w = p.raw_w + (int64_t)i * p.raw_ldw;
@@ -439,6 +439,8 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
       // out[j, i], a column a token
       const float bias = p.bias != nullptr ? __bfloat162float(p.bias[i]) : 0.f;
       const bool mixed = adapters && p.ids != nullptr && plan.cnt > 0;
+      constexpr int kUnknown = -3;
+      int bad = kUnknown;  // of this output row's factors
 #pragma unroll 2
       for (int j = j0; j < min(j1, cols); j += 4) {
         float acc[4];
@@ -446,7 +448,11 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if (j + k >= cols) break;
-          if (mixed && !isfinite(acc[k])) acc[k] = one_value(p, j_base + j + k, i);
+          if (mixed && !isfinite(acc[k])) {
+            if (bad == kUnknown)
+              bad = bad_factors(p.raw_f + (int64_t)i * p.raw_ldf, p.raw_fe, p.rank, plan.list, plan.cnt);
+            if (bad != kNoneBad && bad != plan.slot[j + k]) acc[k] = one_value(p, j_base + j + k, i);
+          }
           p.out[(int64_t)(j_base + j + k) * p.out_ld + i] = __float2bfloat16_rn(acc[k] + bias);
         }
       }

@@ -192,8 +192,8 @@ __device__ __forceinline__ int slots_of(const WideParams& p, int m) {
 }
 
 // One output value from its own row's operands alone. Only for values that a
-// block of several adapters left non-finite: there a row's zeros in another
-// adapter's K block met a NaN or infinity of that adapter (0 x inf = NaN).
+// block with adapters left non-finite: there a row's zeros in another adapter's
+// K block met a NaN or infinity of that adapter (0 x inf = NaN).
 __device__ __noinline__ float one_value(const WideParams& p, int row, int col, int m) {
   const __nv_bfloat16* x = p.raw_x + (int64_t)row * p.raw_ldx;
   const __nv_bfloat16* w = p.raw_w + (int64_t)col * p.raw_ldw;
@@ -471,14 +471,28 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
           float* v = reinterpret_cast<float*>(acc);
           tmem_wait_ld();
           if (mixed) {
-            // zero times a non-finite entry of another row's adapter
+            // zero times a non-finite entry of another row's adapter: only where
+            // the column's factors hold one (a row that is NaN itself is left)
             float z = 0.f;
 #pragma unroll
             for (int i = 0; i < 64; ++i) z = fmaf(v[i], 0.f, z);
-            if (z != 0.f && live) {
+            const bool odd = z != 0.f && live;
+            if (__any_sync(0xffffffffu, odd)) {
+              int bad[2];  // of columns lane and lane + 32
 #pragma unroll
-              for (int i = 0; i < 64; ++i)
-                if (!isfinite(v[i]) && col0 + i < p.N) v[i] = one_value(p, row, col0 + i, tl.m);
+              for (int h = 0; h < 2; ++h) {
+                const int col = col0 + lane + 32 * h;
+                bad[h] = col < p.N ? bad_factors(p.raw_f + (int64_t)col * p.raw_ldf, p.raw_fe, p.rank,
+                                                 p.list_ids + (int64_t)tl.m * 256, slots_of(p, tl.m))
+                                   : (int)kNoneBad;
+              }
+              const int own = live ? p.slot[row] : -1;
+#pragma unroll
+              for (int i = 0; i < 64; ++i) {
+                const int b = __shfl_sync(0xffffffffu, bad[i >> 5], i & 31);
+                if (odd && !isfinite(v[i]) && b != kNoneBad && b != own)
+                  v[i] = one_value(p, row, col0 + i, tl.m);
+              }
             }
           }
           if (p.bias != nullptr) {

@@ -282,3 +282,38 @@ def test_lora_rows_do_not_touch_other_adapters():
         want, tol, _, _ = sup.lora_ref(x[even].double(), w.double(), a[0].double() * 0,
                                        b[0].double() * 0, 1.0, None)
         sup.within(got[even], want, tol, f"{N} rows without an adapter")
+
+
+@pytest.mark.parametrize("N", [1, 48, 200, 600])
+def test_lora_rows_do_not_meet_broken_factors(N):
+    # a request whose b is broken in some columns or everywhere, rows without
+    # an adapter, and a row that is NaN itself
+    from foundry_trainer_b200 import ops
+    g = _gen(12)
+    x, w, a, b, _ = _lora_inputs(g, N, 256, 512, 12, False, 3)
+    scales = torch.ones(3, device="cuda")
+    pattern = torch.tensor([0, -1, 1, 0, 2], device="cuda")
+    for broken, kinds in (((1,), (0, -1, 2)), ((1, 2), (0, -1))):
+        for cols in (slice(None), slice(70, 71)):
+            b2 = b.clone()
+            for e in broken:
+                b2[e, cols] = float("inf")
+                b2[e, cols, 0] = float("nan")
+            ids = pattern[torch.arange(N, device="cuda") % 5].to(torch.int32)
+            x2 = x.clone()
+            if N > 10:
+                x2[10] = float("nan")
+            got = ops.lora_linear_many(x2, w, a, b2, ids, scales)
+            for e in kinds:
+                rows = ids == e
+                if N > 10:
+                    assert torch.isnan(got[10]).all()
+                    rows[10] = False
+                gain = 1.0 if e >= 0 else 0.0
+                want, tol, _, _ = sup.lora_ref(x[rows].double(), w.double(), a[max(e, 0)].double(),
+                                               b[max(e, 0)].double() * gain, 1.0, None)
+                sup.within(got[rows], want, tol, f"{N} rows, adapter {e} beside {broken}")
+            for e in broken:
+                assert torch.isnan(got[ids == e][:, cols]).all()
+    from foundry_trainer_b200 import _lib
+    assert _lib.load().fa_device_status() == 0
