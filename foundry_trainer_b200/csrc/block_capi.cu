@@ -155,6 +155,7 @@ int fa_lora_linear_fwd(int dtype, int rows, int in_dim, int out_dim, int rank,
     SkinnyParams s;
     s.rows = rows;
     s.cols = s.n = s.low_ld = ld;
+    s.rank = rank;
     s.K = in_dim;
     s.out = lw;
     s.out_ld = 2 * ld;
@@ -238,6 +239,7 @@ int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
     SkinnyParams s;
     s.rows = rows;
     s.cols = s.n = s.low_ld = ld;
+    s.rank = rank;
     s.K = out_dim;
     s.out = u;
     s.out_ld = 2 * ld;
@@ -358,6 +360,7 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
     SkinnyParams s;
     s.rows = rows;
     s.cols = s.n = s.low_ld = ld;
+    s.rank = rank;
     s.K = in_dim;
     s.E = n_adapters;
     s.out = low;

@@ -142,6 +142,11 @@ __device__ __noinline__ float one_value(const SkinnyParams& p, int j, int i) {
   return acc;
 }
 
+// What rounding v to `rounded` dropped; nothing where that is an infinity
+__device__ __forceinline__ float remainder(float v, float rounded) {
+  return isfinite(rounded) ? v - rounded : 0.f;
+}
+
 template <bool BIG_MN, bool SMALL_MN, int OUT>
 __global__ void __launch_bounds__(kThreads, 2)
 skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ CUtensorMap tsmall,
@@ -471,15 +476,20 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
         for (int j = lo; j < hi; j += 4) {  // (all bounds are multiples of 4)
           float acc[4];
           sum4(j, acc);
-          __nv_bfloat16* o = p.out + (int64_t)i * p.out_ld + j - sl * p.low_ld;
+          const int jj = j - sl * p.low_ld;
+          __nv_bfloat16* o = p.out + (int64_t)i * p.out_ld + jj;
+          // behind the rank zeros, whatever the row holds (a zero factor times
+          // an infinity is none)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) acc[k] *= sc;
+          for (int k = 0; k < 4; ++k) acc[k] = jj + k < p.rank ? acc[k] * sc : 0.f;
           const uint2 v = make_uint2(pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3]));
           *reinterpret_cast<uint2*>(o) = v;
-          if (p.lo_at != 0)
+          if (p.lo_at != 0) {
+            const float d[4] = {remainder(acc[0], bf16_lo(v.x)), remainder(acc[1], bf16_hi(v.x)),
+                                remainder(acc[2], bf16_lo(v.y)), remainder(acc[3], bf16_hi(v.y))};
             *reinterpret_cast<uint2*>(o + p.lo_at) =
-                make_uint2(pack_bf16(acc[0] - bf16_lo(v.x), acc[1] - bf16_hi(v.x)),
-                           pack_bf16(acc[2] - bf16_lo(v.y), acc[3] - bf16_hi(v.y)));
+                make_uint2(pack_bf16(d[0], d[1]), pack_bf16(d[2], d[3]));
+          }
         }
       } else if (p.slot != nullptr && p.slot[i] < 0 && s0 == 0 && part == 0) {
         // a row without an adapter: zeros (a block whose other rows share one
@@ -544,7 +554,7 @@ low_rows_kernel(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int
     const __nv_bfloat16 hi = __float2bfloat16_rn(acc);
     low[row * low_stride + j] = hi;
     if (lo_at != 0)
-      low[row * low_stride + lo_at + j] = __float2bfloat16_rn(acc - __bfloat162float(hi));
+      low[row * low_stride + lo_at + j] = __float2bfloat16_rn(remainder(acc, __bfloat162float(hi)));
   }
 }
 

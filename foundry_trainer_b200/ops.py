@@ -269,8 +269,9 @@ def lora_linear_bwd(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch.
                     need_dx: bool = True, need_factors: bool = True, stream=None):
     """Gradients of lora_linear with w frozen: (dx, da, db) in bf16, each None
     when not needed. `low` is what the forward returned for the same x, a and
-    scale. Identical bits across repeats. (The bias's gradient, where it
-    trains, is dy summed over its rows.)"""
+    scale. Identical bits across repeats. A gradient that an infinity reaches is
+    not finite, infinity or NaN. (The bias's gradient, where it trains, is dy
+    summed over its rows.)"""
     return _lib.binding().lora_linear_bwd(x, w, a, b, dy, low, scale, need_dx, need_factors, stream)
 
 

@@ -317,3 +317,32 @@ def test_lora_rows_do_not_meet_broken_factors(N):
                 assert torch.isnan(got[ids == e][:, cols]).all()
     from foundry_trainer_b200 import _lib
     assert _lib.load().fa_device_status() == 0
+
+
+@pytest.mark.parametrize("N", [40, 300])
+def test_lora_linear_with_an_infinity(N):
+    # one infinite input: its row of y follows the formula, db gets infinities of
+    # its row's signs, not NaN. Its column of da is not finite; infinities there
+    # may be NaN, as u = hi + lo is multiplied in two parts: inf hi + inf lo is
+    # NaN where the remainder has the other sign.
+    from foundry_trainer_b200 import ops
+    g = _gen(13)
+    x, w, a, b, _ = _lora_inputs(g, N, 128, 264, 12, False)
+    dy = torch.randn(N, 264, generator=g, device="cuda").to(BF)
+    x[7, 5] = float("inf")
+    b[:20] = (w[:20, 5].sign()[:, None] * a[:, 5].sign()) * b[:20].abs()  # of the base's sign
+    y, low = ops.lora_linear(x, w, a, b, scale=0.5)
+    dx, da, db = ops.lora_linear_bwd(x, w, a, b, dy, low, scale=0.5)
+    assert torch.equal(low[7, :12].float(), a[:, 5].float().sign() * float("inf"))
+    assert not low[:, 12:16].any() and torch.isfinite(low[7, 16:]).all()
+    assert torch.equal(db.float(), dy[7].float().sign()[:, None] * a[:, 5].float().sign()
+                       * float("inf"))
+    assert not torch.isfinite(da[:, 5]).any()
+    assert torch.isfinite(da[:, :5]).all() and torch.isfinite(da[:, 6:]).all()
+    assert torch.isfinite(dx).all()
+    rest = torch.arange(N, device="cuda") != 7
+    assert torch.isfinite(y[rest]).all() and not torch.isfinite(y[7]).any()
+    # where base and adapter agree in sign for every rank, y is that infinity
+    same = ((a[:, 5].sign() * b.sign()) == w[:, 5].sign()[:, None]).all(1)
+    assert same.sum() >= 20
+    assert torch.equal(y[7, same].float(), w[same, 5].float().sign() * float("inf"))
