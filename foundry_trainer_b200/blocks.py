@@ -152,9 +152,9 @@ class _LayerNormMod(torch.autograd.Function):
 
 
 def _aligned(x: torch.Tensor) -> torch.Tensor:
-    """x (rows, n) with contiguous rows that start on 16 bytes (a copy only
-    where they do not)."""
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
+    """x (rows, n) with contiguous rows of their own that start on 16 bytes (a
+    copy only where they do not)."""
+    if x.stride(-1) != 1 and x.shape[-1] > 1 or x.shape[0] > 1 and x.stride(0) < x.shape[-1]:
         x = x.contiguous()
     if x.shape[0] > 1 and x.stride(0) % 8 or x.data_ptr() % 16:
         n = x.shape[-1]

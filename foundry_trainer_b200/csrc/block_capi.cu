@@ -37,12 +37,14 @@ static int check_rows(const fa_tensor_t* t, int es) {
   return FA_OK;
 }
 
-static int check_matrix(const fa_matrix_t* m) {
+// (rows, cols) with rows that start on 16 bytes and do not overlap (a TMA
+// descriptor's strides span their dimension)
+static int check_matrix(const fa_matrix_t* m, int64_t rows, int64_t cols) {
   if (m == nullptr || m->data == nullptr) return FA_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(m->data) % 16 != 0 || m->stride_row % 8 != 0 ||
       m->stride_batch % 8 != 0 || m->stride_row < 0 || m->stride_batch < 0)
     return FA_ERR_ALIGNMENT;
-  return FA_OK;
+  return rows > 1 && m->stride_row < cols ? FA_ERR_ALIGNMENT : FA_OK;
 }
 
 constexpr int kMaxRank = 256;
@@ -138,7 +140,11 @@ int fa_lora_linear_fwd(int dtype, int rows, int in_dim, int out_dim, int rank,
                        const fa_matrix_t* y, void* low, void* stream) {
   FA_TRY(check_lora(dtype, rows, in_dim, out_dim, rank, scale));
   if (rows == 0) return FA_OK;
-  for (const fa_matrix_t* m : {x, w, a, b, y}) FA_TRY(check_matrix(m));
+  FA_TRY(check_matrix(x, rows, in_dim));
+  FA_TRY(check_matrix(w, out_dim, in_dim));
+  FA_TRY(check_matrix(a, rank, in_dim));
+  FA_TRY(check_matrix(b, out_dim, rank));
+  FA_TRY(check_matrix(y, rows, out_dim));
   if (low == nullptr) return FA_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(low) % 16 != 0 || reinterpret_cast<uintptr_t>(bias) % 2 != 0)
     return FA_ERR_ALIGNMENT;
@@ -220,11 +226,15 @@ int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
     }
     return FA_OK;
   }
-  for (const fa_matrix_t* m : {b, dy}) FA_TRY(check_matrix(m));
-  if (dx != nullptr)
-    for (const fa_matrix_t* m : {w, a, dx}) FA_TRY(check_matrix(m));
+  FA_TRY(check_matrix(b, out_dim, rank));
+  FA_TRY(check_matrix(dy, rows, out_dim));
+  if (dx != nullptr) {
+    FA_TRY(check_matrix(w, out_dim, in_dim));
+    FA_TRY(check_matrix(a, rank, in_dim));
+    FA_TRY(check_matrix(dx, rows, in_dim));
+  }
   if (da != nullptr) {
-    FA_TRY(check_matrix(x));
+    FA_TRY(check_matrix(x, rows, in_dim));
     if (low == nullptr) return FA_ERR_INVALID_ARG;
     if (reinterpret_cast<uintptr_t>(low) % 16 != 0) return FA_ERR_ALIGNMENT;
   }
@@ -330,7 +340,11 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
   FA_TRY(check_lora(dtype, rows, in_dim, out_dim, rank, 1.f));
   if (n_adapters <= 0) return FA_ERR_INVALID_ARG;
   if (rows == 0) return FA_OK;
-  for (const fa_matrix_t* m : {x, w, a, b, y}) FA_TRY(check_matrix(m));
+  FA_TRY(check_matrix(x, rows, in_dim));
+  FA_TRY(check_matrix(w, out_dim, in_dim));
+  FA_TRY(check_matrix(a, rank, in_dim));
+  FA_TRY(check_matrix(b, out_dim, rank));
+  FA_TRY(check_matrix(y, rows, out_dim));
   if (ids == nullptr || scales == nullptr) return FA_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(ids) % 4 != 0 || reinterpret_cast<uintptr_t>(scales) % 4 != 0 ||
       reinterpret_cast<uintptr_t>(bias) % 2 != 0)
@@ -338,6 +352,8 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
   const size_t need = fa_lora_linear_many_workspace_bytes(rows, rank);
   if (workspace == nullptr || workspace_bytes < need) return FA_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return FA_ERR_ALIGNMENT;
+  if (n_adapters > 1 && (a->stride_batch < in_dim || b->stride_batch < rank))
+    return FA_ERR_ALIGNMENT;
   FA_TRY(check_sm100());
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int ld = low_dim(rank);

@@ -149,6 +149,35 @@ def test_c_abi_lora_validates_without_a_gpu():
     assert lib.fa_pad_rows(0, 4, None, 4, None, 8, None) == _lib.FA_OK
 
 
+def test_c_abi_lora_refuses_rows_that_overlap():
+    # expanded operands: a row or an adapter stride of zero, or below the width
+    lib = _lib.load()
+    ALI = _lib.FA_ERR_ALIGNMENT
+    M = lambda sr, sb=0: _lib.fa_matrix_t(4096, sb, sr)
+    for at in range(5):
+        for bad in (0, 56):
+            ms = [M(64) for _ in range(5)]
+            ms[at] = M(min(bad, 8) if at == 3 else bad)
+            rc = lib.fa_lora_linear_fwd(1, 4, 64, 64, 16, *[C.byref(m) for m in ms[:4]], 1.0, None,
+                                        C.byref(ms[4]), 4096, None)
+            assert rc == ALI, (at, bad)
+            rc = lib.fa_lora_linear_bwd(1, 4, 64, 64, 16, *[C.byref(m) for m in ms[:4]], 1.0, 4096,
+                                        C.byref(ms[4]), C.byref(M(64)), 4096, 4096, 4096, 1 << 20, None)
+            assert rc == ALI, (at, bad)
+    for sa, sb in ((0, 1024), (1024, 0)):
+        rc = lib.fa_lora_linear_many(1, 4, 64, 64, 16, 3, C.byref(M(64)), C.byref(M(64)),
+                                     C.byref(M(64, sa)), C.byref(M(16, sb)), 4096, 4096, None,
+                                     C.byref(M(64)), 4096, 1 << 20, None)
+        assert rc == ALI
+
+
+def test_aligned_rows_of_expanded_tensors():
+    x = torch.randn(1, 24).to(BF).expand(5, 24)
+    y = blocks._aligned(x)
+    assert y.stride() == (24, 1) and torch.equal(x, y)
+    assert blocks._aligned(y) is y
+
+
 def test_c_abi_orthogonalize_validates_without_a_gpu():
     lib = _lib.load()
 
