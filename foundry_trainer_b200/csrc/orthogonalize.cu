@@ -261,7 +261,7 @@ thin_kernel(const T* g, int64_t g_batch, int64_t g_row, __nv_bfloat16* o, int64_
   double tr = 0.0;
 #pragma unroll 8
   for (int i = 0; i < R; ++i) tr += A[i * LD + i];
-  const double inv = 1.0 / (sqrt(tr) + eps);
+  double inv = 1.0 / (sqrt(tr) + eps);
   __syncthreads();
   for (int i = tid; i < R * R; i += kThinThreads) A[(i / R) * LD + i % R] *= inv * inv;
   __syncthreads();
@@ -329,8 +329,14 @@ thin_kernel(const T* g, int64_t g_batch, int64_t g_row, __nv_bfloat16* o, int64_
     __syncthreads();
   }
   // P / |G| in fp32 (its largest entries are a few hundred times the
-  // result's: 24 bits leave the bf16 result its own rounding), in A's place
+  // result's: 24 bits leave the bf16 result its own rounding), in A's place.
+  // Where |G| is so small or large that fp32 would lose the quotient, a power
+  // of two goes to G's entries instead.
   float* pf = reinterpret_cast<float*>(A);
+  int up = isfinite(inv) && inv > 0.0 ? ilogb(inv) : 0;
+  up = up > 60 || up < -60 ? max(-126, min(126, up)) : 0;
+  const float gain = (float)scalbn(1.0, up);
+  inv = scalbn(inv, -up);
   for (int i = tid; i < R * R; i += kThinThreads) pf[i] = (float)(P[(i / R) * LD + i % R] * inv);
   __syncthreads();
 
@@ -341,6 +347,7 @@ thin_kernel(const T* g, int64_t g_batch, int64_t g_row, __nv_bfloat16* o, int64_
 #pragma unroll
     for (int i = 0; i < R / 2; ++i) sum[i] = 0;
     auto add = [&](int j, float x) {
+      x *= gain;
       const uint64_t xx = f2_pack(x, x);
       const ulonglong2* pr = reinterpret_cast<const ulonglong2*>(pf + j * R);
 #pragma unroll
@@ -464,7 +471,8 @@ split_kernel(const T* g, int64_t g_batch, int64_t g_row, int m, int n, const dou
   const int mat = blockIdx.z;
   int e;
   const double nu = norm_of(part + (int64_t)mat * kNormBlocks, eps, &e);
-  const float scale = (float)scalbn(1.0, 8 - e);
+  // 2^(8 - e) in two factors: it may lie outside fp32's range
+  const float scale = (float)scalbn(1.0, (8 - e) / 2), scale2 = (float)scalbn(1.0, 8 - e - (8 - e) / 2);
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < steps) {
     const int s = threadIdx.x;
     const double v = s == 0 ? nu : 1.0;
@@ -483,7 +491,7 @@ split_kernel(const T* g, int64_t g_batch, int64_t g_row, int m, int n, const dou
     const int r = (threadIdx.x >> 6) + 4 * k;
     float v = 0.f;
     if (i0 + r < m && j0 + c < n) v = ld_f<T>(gm + (int64_t)(i0 + r) * g_row + j0 + c);
-    tile[r][c] = v * scale;
+    tile[r][c] = v * scale * scale2;
   }
   __syncthreads();
   // two columns a thread

@@ -125,3 +125,16 @@ def test_orthogonalize_keeps_weak_directions_of_a_thin_factor():
         want = (u[:, i] @ ref @ v[:, i]).item()
         have = (u[:, i] @ got @ v[:, i]).item()
         assert abs(want - have) <= bound((16, 2048)) * max(abs(want), 0.05), (i, want, have)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("m,n", [(16, 512), (500, 20), (60, 256), (160, 256), (256, 160)])
+def test_orthogonalize_at_the_ends_of_the_range(m, n, dtype):
+    # norms near the smallest and largest values of the type, without an eps
+    from foundry_trainer_b200 import ops
+    g = gradient(3, m, n, dtype=dtype)
+    for scale in (2.0 ** -122, 2.0 ** -70, 2.0 ** 70, 2.0 ** 126):
+        x = (g.float() * scale).to(dtype)
+        assert x.isfinite().all() and x.any()
+        o = ops.orthogonalize(x, eps=0.0)
+        assert rel(o, plain(x, eps=0.0)) <= bound((m, n)), scale
