@@ -234,6 +234,8 @@ class FusedKernels:
         per sample: (B, dim) or (B, 1, dim)."""
         if scale.dim() == 3 and scale.shape[1] == 1:
             shift, scale = shift[:, 0], scale[:, 0]
+        if x.stride(-1) != 1 and x.shape[-1] > 1:
+            x = x.contiguous()
         if scale.dim() == 1 and x.dim() != 2:
             y = _LayerNormMod.apply(x.reshape(-1, x.shape[-1]), shift, scale, eps)
             return y.view(x.shape)

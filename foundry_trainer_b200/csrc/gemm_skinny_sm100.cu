@@ -715,6 +715,7 @@ static float wide_time(int64_t out, int64_t K, int rows) {
 // contraction over clusters (256 rows, 16384 -> 4096: 42 us against 82); many
 // fill them at half the staged bytes (512 rows, 4096 -> 16384: 97 against 52).
 bool linear_as_columns(int64_t out, int64_t K, int rows) {
+  if (rows > kMaxColumns * 65535) return false;  // a block of tokens a grid row
   return rows <= 64 || cols_time(out, K, rows) < wide_time(out, K, rows);
 }
 

@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -119,6 +120,12 @@ struct Place {
   void* ptr() const { return stream.stream(); }
 };
 
+// a tensor to write to: every element its own
+void writable(const Tensor& t) {
+  if (at::has_internal_overlap(t) == at::MemOverlap::Yes)
+    refuse("out has elements that share memory (an expanded tensor)");
+}
+
 Tensor scratch(size_t bytes, const Tensor& like) {
   return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
@@ -222,7 +229,10 @@ PyObject* layer_norm(PyObject* const* a) {
   const NormShape s = norm_shape(x);
   const int dt = dtype_code(x);
   NormParams p = norm_params(x, w, b);
-  if (out.defined()) like_x(x, out, "out");
+  if (out.defined()) {
+    like_x(x, out, "out");
+    writable(out);
+  }
   need_cuda(x);
   same_device(x, w, "weight");
   same_device(x, b, "bias");
@@ -280,9 +290,12 @@ Tensor rows_of(const Tensor& t, const char* name) {
   if (t.dim() == 2) return t;
   if (t.dim() < 2) refuse(std::string(name) + ": expected (..., features), got " + shape_of(t));
   const int64_t k = t.size(-1);
-  if (t.numel() == 0) return t.reshape({t.numel() == 0 && k > 0 ? 0 : 0, k});
-  // one stride has to run through all leading dimensions
   int64_t want = -1, rows = 1;
+  if (t.numel() == 0) {
+    for (int64_t d = 0; d < t.dim() - 1; ++d) rows *= t.size(d);
+    return at::empty({rows, k}, t.options());
+  }
+  // one stride has to run through all leading dimensions
   for (int64_t d = t.dim() - 2; d >= 0; --d) {
     if (t.size(d) == 1) continue;
     if (want >= 0 && t.stride(d) != want)
@@ -490,6 +503,11 @@ PyObject* orthogonalize(PyObject* const* a_) {
               eps = (float)number(a_[5]);
   if (g.dim() < 2) refuse("expected (..., m, n), got " + shape_of(g));
   const int dt = dtype_code(g);
+  if (out.defined()) {
+    if (out.sizes() != g.sizes() || out.scalar_type() != at::kBFloat16)
+      refuse("out must be bf16 with g's shape");
+    writable(out);
+  }
   need_cuda(g);
   same_device(g, out, "out");
   const Tensor g3 = matrices_of(g, "g");
@@ -497,8 +515,6 @@ PyObject* orthogonalize(PyObject* const* a_) {
   const Place at(g, a_[7]);
   Tensor o, o3;
   if (out.defined()) {
-    if (out.sizes() != g.sizes() || out.scalar_type() != at::kBFloat16)
-      refuse("out must be bf16 with g's shape");
     o = out;
     o3 = matrices_of(out, "out");
   } else {

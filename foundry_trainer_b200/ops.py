@@ -239,7 +239,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     unit_offset the gain is 1 + weight (the modulation of layer_norm_mod,
     lib.rs:60-71). weight and bias: (D,), or (groups, D) for one pair per
     group; None: no gain or no bias. Any strides with a contiguous last
-    dimension, D <= 16384. Returns (y, stats), stats the fp32
+    dimension, D <= 16384; `out` may be x. Returns (y, stats), stats the fp32
     (2, groups * rows) means and reciprocal deviations layer_norm_bwd reads."""
     return _lib.binding().layer_norm(x, weight, bias, unit_offset, eps, out, stream)
 

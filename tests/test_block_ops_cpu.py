@@ -231,3 +231,10 @@ def test_fused_linear_refuses_a_trained_weight_and_stacked_gradients():
         k.linear(w, "l", z(3, 5, 16), 1.0)
     with torch.no_grad(), pytest.raises(ValueError, match="one adapter id"):
         blocks.FusedKernels().linear(w, "l", z(2, 5, 16), 1.0)
+
+
+def test_out_must_not_share_elements():
+    with pytest.raises(ValueError, match="share memory"):
+        ops.layer_norm(z(4, 8), out=z(1, 8).expand(4, 8))
+    with pytest.raises(ValueError, match="share memory"):
+        ops.orthogonalize(z(3, 4, 8), out=z(1, 4, 8).expand(3, 4, 8))

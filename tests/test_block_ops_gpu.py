@@ -346,3 +346,28 @@ def test_lora_linear_with_an_infinity(N):
     same = ((a[:, 5].sign() * b.sign()) == w[:, 5].sign()[:, None]).all(1)
     assert same.sum() >= 20
     assert torch.equal(y[7, same].float(), w[same, 5].float().sign() * float("inf"))
+
+
+def test_lora_linear_without_rows():
+    from foundry_trainer_b200 import ops
+    g = _gen(14)
+    x, w, a, b, _ = _lora_inputs(g, 4, 64, 48, 16, False)
+    for shape in ((0, 64), (3, 0, 64), (0, 5, 64)):
+        e = x.new_empty(shape)
+        y, low = ops.lora_linear(e, w, a, b)
+        assert y.shape == (*shape[:-1], 48)
+        dx, da, db = ops.lora_linear_bwd(e, w, a, b, y, low)
+        assert dx.shape == shape and not da.any() and not db.any()
+        ids = torch.zeros(0, device="cuda", dtype=torch.int32)
+        y = ops.lora_linear_many(e, w, a[None], b[None], ids, torch.ones(1, device="cuda"))
+        assert y.shape == (*shape[:-1], 48)
+
+
+def test_layer_norm_in_place():
+    from foundry_trainer_b200 import ops
+    g = _gen(15)
+    for shape in ((5, 7), (3, 2048), (4000, 1024), (2, 3000, 514)):
+        x = torch.randn(*shape, generator=g, device="cuda").to(BF)
+        y, stats = ops.layer_norm(x)
+        z, again = ops.layer_norm(x, out=x)
+        assert z is x and torch.equal(x, y) and torch.equal(stats, again)
