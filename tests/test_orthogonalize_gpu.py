@@ -54,7 +54,9 @@ SHAPES = [(1, 1), (1, 8, 8), (3, 16, 4096), (2, 4096, 16), (5, 12, 1000), (2, 10
           (2, 72, 200), (1, 200, 72), (1, 256, 512), (2, 300, 1000), (1, 1000, 300), (1, 777, 777),
           (1, 1024, 2048), (1, 1500, 520),
           # the SM-pair form of all three products, upright and tall, ragged
-          (1, 4096, 4104), (1, 4500, 4100), (3, 2305, 2500)]
+          (1, 4096, 4104), (1, 4500, 4100), (3, 2305, 2500),
+          # tall rows of 8 bytes, and of no such number
+          (3, 1000, 12), (2, 700, 36), (2, 300, 61)]
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
