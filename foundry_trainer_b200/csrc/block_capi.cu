@@ -263,19 +263,18 @@ int fa_lora_linear_bwd(int dtype, int rows, int in_dim, int out_dim, int rank,
     s.cols = rank;
     s.n = ld;
     s.K = rows;
-    s.has_lo = 1;
     s.rows = in_dim;  // da = (x^T U)^T
     s.out = reinterpret_cast<__nv_bfloat16*>(da);
     s.out_ld = 1;
     s.out_j = in_dim;
-    FA_TRY(launch_gemm_skinny(mat(x, 1, rows, in_dim), true, dense(u, rows, ld, 2 * ld), true, s,
-                              kSkinnyGrad, true, st, dense(u + ld, rows, ld, 2 * ld)));
-    s.rows = out_dim;  // db = dy^T low
-    s.out = reinterpret_cast<__nv_bfloat16*>(db);
-    s.out_ld = rank;
-    s.out_j = 1;
-    FA_TRY(launch_gemm_skinny(mat(dy, 1, rows, out_dim), true, dense(low, rows, ld, 2 * ld), true, s,
-                              kSkinnyGrad, true, st, dense(bfp(low) + ld, rows, ld, 2 * ld)));
+    s.rows2 = out_dim;  // db = dy^T low
+    s.out2 = reinterpret_cast<__nv_bfloat16*>(db);
+    s.out_ld2 = rank;
+    s.out_j2 = 1;
+    const Mat3 big[2] = {mat(x, 1, rows, in_dim), mat(dy, 1, rows, out_dim)};
+    const Mat3 small[2] = {dense(u, rows, ld, 2 * ld), dense(low, rows, ld, 2 * ld)};
+    const Mat3 rest[2] = {dense(u + ld, rows, ld, 2 * ld), dense(bfp(low) + ld, rows, ld, 2 * ld)};
+    FA_TRY(launch_skinny_grads(big, small, rest, s, st));
   }
   if (dx == nullptr) return FA_OK;
   if (linear_as_columns(in_dim, out_dim, rows)) {

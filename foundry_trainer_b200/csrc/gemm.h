@@ -76,7 +76,7 @@ constexpr int kMaxColumns = 256;
 enum SkinnyOut {
   kSkinnyCols = 0,  // out[j, i] bf16 + bias[i] + the adapters' term of row j
   kSkinnyLow = 1,   // out[i, j] bf16, scaled: a row's own adapter's columns
-  kSkinnyGrad = 2   // out[j out_j + i out_ld] bf16
+  kSkinnyGrad = 2   // out[j out_j + i out_ld] bf16, Small with its remainders
 };
 
 struct SkinnyParams {
@@ -92,10 +92,12 @@ struct SkinnyParams {
   int low_ld = 0, rank = 0, E = 1;
   int64_t low_stride = 0;
   // kSkinnyLow: where each row's remainders (what rounding to bf16 dropped, as
-  // bf16) go behind its values; 0: nowhere. kSkinnyGrad: Small's remainders
-  // are `fac`, multiplied too.
+  // bf16) go behind its values; 0: nowhere
   int lo_at = 0;
-  int has_lo = 0;
+  // kSkinnyGrad: the second product
+  int rows2 = 0;
+  __nv_bfloat16* out2 = nullptr;
+  int64_t out_ld2 = 0, out_j2 = 0;
   const int* ids = nullptr;
   // plain views of Small, Big and the adapters, for tokens of several
   const __nv_bfloat16* raw_x = nullptr;
@@ -117,6 +119,10 @@ struct SkinnyParams {
 int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool small_mn,
                        SkinnyParams p, int out, bool early, cudaStream_t st,
                        const Mat3& fac = Mat3{});
+// Both factors' gradients in one launch (kSkinnyGrad): Big (K, rows) and Small
+// with its remainders (K, n), each stored with its short side contiguous.
+int launch_skinny_grads(const Mat3* big, const Mat3* small, const Mat3* small_lo, SkinnyParams p,
+                        cudaStream_t st);
 // whether a linear of `rows` tokens runs as kSkinnyCols rather than wide
 bool linear_as_columns(int64_t out, int64_t K, int rows);
 int launch_low_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int64_t a_e,

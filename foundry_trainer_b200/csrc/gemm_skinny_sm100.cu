@@ -147,11 +147,18 @@ __device__ __forceinline__ float remainder(float v, float rounded) {
   return isfinite(rounded) ? v - rounded : 0.f;
 }
 
+// Descriptors of Big, Small and `fac`; of the gradients' two products (da and db
+// in one launch, as grid rows: each alone leaves SMs idle and costs a launch).
+template <int OUT>
+struct Maps {
+  static constexpr int kProducts = OUT == kSkinnyGrad ? 2 : 1;
+  CUtensorMap big[kProducts], small[kProducts], fac[kProducts];
+};
+
 template <bool BIG_MN, bool SMALL_MN, int OUT>
 __global__ void __launch_bounds__(kThreads, 2)
-skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ CUtensorMap tsmall,
-              const __grid_constant__ CUtensorMap tfac, const __grid_constant__ SkinnyParams p, int split, int stage_bytes, int stages,
-              int bar_off, int exchange, int tmem_cols) {
+skinny_kernel(const __grid_constant__ Maps<OUT> maps, const __grid_constant__ SkinnyParams p,
+              int split, int stage_bytes, int stages, int bar_off, int exchange, int tmem_cols) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -167,6 +174,10 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
   const int warp = warp_id(), lane = lane_id();
   const int tile = blockIdx.x / split, part = blockIdx.x - tile * split;
   const int i0 = tile * 128;
+  const int which = OUT == kSkinnyGrad ? blockIdx.y : 0;
+  const CUtensorMap *tbig = &maps.big[which], *tsmall = &maps.small[which], *tfac = &maps.fac[which];
+  const int rows = which ? p.rows2 : p.rows;
+  if (OUT == kSkinnyGrad && i0 >= rows) return;  // the same for the whole cluster
 
   // columns of this pass: adapters [s0, s0 + ns) of the tile's list, or all;
   // of a linear the tokens j_base .. j_base + cols
@@ -193,8 +204,8 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
     mbar_init(planned, 1);
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tbig);
-    tma_prefetch_desc(&tsmall);
+    tma_prefetch_desc(tbig);
+    tma_prefetch_desc(tsmall);
   }
   if (warp == 5) {
     tmem_alloc(slot, tmem_cols);
@@ -218,7 +229,7 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
     if (lane == 0) {
       if constexpr (OUT != kSkinnyCols) pdl_wait_previous();
       const int small_blocks = (n + 63) >> 6;
-      const bool two = OUT == kSkinnyGrad && p.has_lo;
+      constexpr bool two = OUT == kSkinnyGrad;
       const uint32_t bytes = kBig + (SMALL_MN ? (two ? 2 : 1) * small_blocks * 8192
                                               : (OUT == kSkinnyCols ? p.n * 128 : n * 128));
       int s = 0;
@@ -230,24 +241,24 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
         mbar_arrive_expect_tx(&full[s], bytes);
         if constexpr (OUT == kSkinnyCols) mbar_arrive(&full[s]);  // else: the builders' arrival
         if constexpr (BIG_MN) {
-          tma_load_3d(sa, &tbig, &full[s], i0, kb * 64, 0);
-          tma_load_3d(sa + 8192, &tbig, &full[s], i0 + 64, kb * 64, 0);
+          tma_load_3d(sa, tbig, &full[s], i0, kb * 64, 0);
+          tma_load_3d(sa + 8192, tbig, &full[s], i0 + 64, kb * 64, 0);
         } else {
-          tma_load_3d(sa, &tbig, &full[s], kb * 64, i0, 0);
+          tma_load_3d(sa, tbig, &full[s], kb * 64, i0, 0);
         }
         if constexpr (SMALL_MN) {
           for (int j = 0; j < small_blocks; ++j)
-            tma_load_3d(sb + j * 8192, &tsmall, &full[s], j * 64, kb * 64, 0);
+            tma_load_3d(sb + j * 8192, tsmall, &full[s], j * 64, kb * 64, 0);
           if (two)
             for (int j = 0; j < small_blocks; ++j)
-              tma_load_3d(sb + (small_blocks + j) * 8192, &tfac, &full[s], j * 64, kb * 64, 0);
+              tma_load_3d(sb + (small_blocks + j) * 8192, tfac, &full[s], j * 64, kb * 64, 0);
         } else if constexpr (OUT == kSkinnyLow) {
           for (int q = 0; q < ns; ++q) {
             const int e = p.list_ids != nullptr ? p.list_ids[(int64_t)(i0 >> 8) * 256 + s0 + q] : 0;
-            tma_load_3d(sb + q * p.low_ld * 128, &tsmall, &full[s], kb * 64, 0, e);
+            tma_load_3d(sb + q * p.low_ld * 128, tsmall, &full[s], kb * 64, 0, e);
           }
         } else {
-          tma_load_3d(sb, &tsmall, &full[s], kb * 64, j_base, 0);
+          tma_load_3d(sb, tsmall, &full[s], kb * 64, j_base, 0);
         }
         if (++s == stages) { s = 0; ph ^= 1; }
       }
@@ -259,10 +270,10 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
           mbar_arrive(&grant[s]);
           mbar_arrive_expect_tx(&full[s], kBig);
           if constexpr (BIG_MN) {
-            tma_load_3d(sa, &tfac, &full[s], i0, j * 64, e);
-            tma_load_3d(sa + 8192, &tfac, &full[s], i0 + 64, j * 64, e);
+            tma_load_3d(sa, tfac, &full[s], i0, j * 64, e);
+            tma_load_3d(sa + 8192, tfac, &full[s], i0 + 64, j * 64, e);
           } else {
-            tma_load_3d(sa, &tfac, &full[s], j * 64, i0, e);
+            tma_load_3d(sa, tfac, &full[s], j * 64, i0, e);
           }
           if (++s == stages) { s = 0; ph ^= 1; }
         }
@@ -286,7 +297,7 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
       for (int kk = 0; kk < 4; ++kk)
         umma_ss_w(tmem, a + (BIG_MN ? 128 : 2) * kk, b + (SMALL_MN ? 128 : 2) * kk, idesc,
                   kb > kb0 || kk > 0);
-      if (OUT == kSkinnyGrad && p.has_lo) {
+      if (OUT == kSkinnyGrad) {
         const uint64_t b2 = b + (uint32_t)(((n + 63) >> 6) * (8192 >> 4));
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
@@ -439,7 +450,7 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
     }
     acc[0] = a.x; acc[1] = a.y; acc[2] = a.z; acc[3] = a.w;
   };
-  if (warp < 4 && good && i < p.rows) {
+  if (warp < 4 && good && i < rows) {
     if constexpr (OUT == kSkinnyCols) {
       // out[j, i], a column a token
       const float bias = p.bias != nullptr ? __bfloat162float(p.bias[i]) : 0.f;
@@ -497,13 +508,14 @@ skinny_kernel(const __grid_constant__ CUtensorMap tbig, const __grid_constant__ 
         for (int j = 0; j < p.low_ld; ++j) p.out[(int64_t)i * p.out_ld + j] = __float2bfloat16_rn(0.f);
       }
     } else {
+      __nv_bfloat16* out = which ? p.out2 : p.out;
+      const int64_t ld = which ? p.out_ld2 : p.out_ld, lj = which ? p.out_j2 : p.out_j;
       for (int j = j0; j < min(j1, p.cols); j += 4) {
         float acc[4];
         sum4(j, acc);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (j + k < p.cols)
-            p.out[(int64_t)(j + k) * p.out_j + (int64_t)i * p.out_ld] = __float2bfloat16_rn(acc[k]);
+          if (j + k < p.cols) out[(int64_t)(j + k) * lj + (int64_t)i * ld] = __float2bfloat16_rn(acc[k]);
       }
     }
   }
@@ -596,14 +608,16 @@ plan_kernel(const int* ids, int rows, int E, int* cnt, int* list, int* slot) {
 }
 
 template <bool BIG_MN, bool SMALL_MN, int OUT>
-static int go(const CUtensorMap& tbig, const CUtensorMap& tsmall, const CUtensorMap& tfac,
-              const SkinnyParams& p, int passes, int kernel_id, bool early, cudaStream_t st) {
+static int go(const Maps<OUT>& maps, const SkinnyParams& p, int passes, int kernel_id, bool early,
+              cudaStream_t st) {
   auto* fn = skinny_kernel<BIG_MN, SMALL_MN, OUT>;
-  const Layout l = layout_of(p.n, SMALL_MN, OUT == kSkinnyGrad && p.has_lo);
+  const Layout l = layout_of(p.n, SMALL_MN, OUT == kSkinnyGrad);
   // the largest layout's request, once per kernel
   const int rc = ensure_smem_attr((const void*)fn, kOneSmem, kernel_id);
   if (rc) return rc;
-  const int tiles = (p.rows + 127) / 128, kbs = (p.K + 63) / 64;
+  const int tiles = (std::max(p.rows, p.rows2) + 127) / 128, kbs = (p.K + 63) / 64;
+  const int64_t work = OUT == kSkinnyGrad ? (p.rows + 127) / 128 + (p.rows2 + 127) / 128
+                                          : (int64_t)tiles * passes;
   // contraction split: the one whose rounds of resident clusters times blocks
   // per CTA (and about two blocks' time for the exchange) is smallest. A wave
   // that spills over costs a whole round: with 72 clusters of 4 where 66 fit,
@@ -617,7 +631,7 @@ static int go(const CUtensorMap& tbig, const CUtensorMap& tsmall, const CUtensor
                                      kernel_id + (two ? 0 : kKernelSkinnyBig - kKernelSkinny), &fit);
     if (rf) return rf;
     if (fit <= 0) continue;
-    const int64_t rounds = ((int64_t)tiles * passes + fit - 1) / fit;
+    const int64_t rounds = (work + fit - 1) / fit;
     const int64_t cost = rounds * ((kbs + c - 1) / c + 2);
     if (cost < best) best = cost, split = c;
   }
@@ -635,7 +649,7 @@ static int go(const CUtensorMap& tbig, const CUtensorMap& tsmall, const CUtensor
   cfg.attrs = at;
   cfg.numAttrs = early ? 2 : 1;
   const int bar_off = l.smem - kBarBytes - 1024;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, tbig, tsmall, tfac, p, split, l.stage, l.stages,
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, maps, p, split, l.stage, l.stages,
                                            bar_off, l.exchange, l.cols);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -646,10 +660,22 @@ static int go(const CUtensorMap& tbig, const CUtensorMap& tsmall, const CUtensor
 
 }  // namespace skinny
 
+template <bool BIG_MN, bool SMALL_MN, int OUT>
+static int launch(const Mat3& big, const Mat3& small, const Mat3& fac, const SkinnyParams& p,
+                  int passes, int kernel_id, bool early, cudaStream_t st) {
+  skinny::Maps<OUT> m;
+  int rc = make_tmap_3d(&m.big[0], big, 64, BIG_MN ? 64 : 128);
+  const int box = OUT == kSkinnyLow ? p.low_ld : p.n;
+  if (!rc) rc = make_tmap_3d(&m.small[0], small, 64, SMALL_MN ? 64 : box);
+  m.fac[0] = m.big[0];
+  if (!rc && OUT == kSkinnyCols && p.low != nullptr)
+    rc = make_tmap_3d(&m.fac[0], fac, 64, BIG_MN ? 64 : 128);
+  return rc ? rc : skinny::go<BIG_MN, SMALL_MN, OUT>(m, p, passes, kernel_id, early, st);
+}
+
 int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool small_mn,
                        SkinnyParams p, int out, bool early, cudaStream_t st, const Mat3& fac) {
   if (p.rows == 0) return FA_OK;
-  CUtensorMap tb, ts, tf;
   int passes = 1;
   if (out == kSkinnyCols) {  // even blocks of up to 256 tokens
     passes = (p.cols + kMaxColumns - 1) / kMaxColumns;
@@ -663,26 +689,27 @@ int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool sma
     p.n = p.slots_per_pass * p.low_ld;
     passes = (most + p.slots_per_pass - 1) / p.slots_per_pass;
   }
-  int rc = big_mn ? make_tmap_3d(&tb, big, 64, 64) : make_tmap_3d(&tb, big, 64, 128);
-  const int box = out == kSkinnyLow ? p.low_ld : p.n;
-  if (!rc) rc = small_mn ? make_tmap_3d(&ts, small, 64, 64) : make_tmap_3d(&ts, small, 64, box);
-  tf = tb;
-  if (!rc && out == kSkinnyGrad && p.has_lo) rc = make_tmap_3d(&tf, fac, 64, 64);
-  if (!rc && out == kSkinnyCols && p.low != nullptr)
-    rc = big_mn ? make_tmap_3d(&tf, fac, 64, 64) : make_tmap_3d(&tf, fac, 64, 128);
-  if (rc) return rc;
-  using namespace skinny;
   if (out == kSkinnyCols && !big_mn && !small_mn)
-    return go<false, false, kSkinnyCols>(tb, ts, tf, p, passes, kKernelSkinny, early, st);
+    return launch<false, false, kSkinnyCols>(big, small, fac, p, passes, kKernelSkinny, early, st);
   if (out == kSkinnyCols && big_mn && !small_mn)
-    return go<true, false, kSkinnyCols>(tb, ts, tf, p, passes, kKernelSkinny + 1, early, st);
+    return launch<true, false, kSkinnyCols>(big, small, fac, p, passes, kKernelSkinny + 1, early, st);
   if (out == kSkinnyLow && !big_mn && !small_mn)
-    return go<false, false, kSkinnyLow>(tb, ts, tf, p, passes, kKernelSkinny + 2, early, st);
+    return launch<false, false, kSkinnyLow>(big, small, fac, p, passes, kKernelSkinny + 2, early, st);
   if (out == kSkinnyLow && !big_mn && small_mn)
-    return go<false, true, kSkinnyLow>(tb, ts, tf, p, passes, kKernelSkinny + 3, early, st);
-  if (out == kSkinnyGrad && big_mn && small_mn)
-    return go<true, true, kSkinnyGrad>(tb, ts, tf, p, passes, kKernelSkinny + 4, early, st);
+    return launch<false, true, kSkinnyLow>(big, small, fac, p, passes, kKernelSkinny + 3, early, st);
   return FA_ERR_UNSUPPORTED;
+}
+
+int launch_skinny_grads(const Mat3* big, const Mat3* small, const Mat3* small_lo, SkinnyParams p,
+                        cudaStream_t st) {
+  skinny::Maps<kSkinnyGrad> m;
+  for (int i = 0; i < 2; ++i) {
+    int rc = make_tmap_3d(&m.big[i], big[i], 64, 64);
+    if (!rc) rc = make_tmap_3d(&m.small[i], small[i], 64, 64);
+    if (!rc) rc = make_tmap_3d(&m.fac[i], small_lo[i], 64, 64);
+    if (rc) return rc;
+  }
+  return skinny::go<true, true, kSkinnyGrad>(m, p, 2, kKernelSkinny + 4, true, st);
 }
 
 // Estimated microseconds of a linear as token columns: rounds of resident CTAs
