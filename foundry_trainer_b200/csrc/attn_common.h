@@ -32,12 +32,13 @@ enum KernelId {
   kKernelF32Bwd = 3,   // + 0..1: dK/dV and dQ
   kKernelWide = 5,     // + 0..5: the wide product by operand layout and epilogue
   kKernelSkinny = 11,  // + 0..4 by operand layout and output
-  kKernelSkinnyBig = 16,  // + 0..4: the same with one block an SM
-  kKernelNarrow = 21,  // + 0..3: the narrow product by epilogue
-  kKernelNorm = 25,    // + 0..11: the ring layer norm by direction, type and width
-  kKernelThin = 37,    // + 0..15: the thin orthogonalisation by type, side and rank
-  kKernelNormLong = 53,   // + 0..9: the layer norm's backward of long rows by type and width
-  kKernelCount = 63
+  kKernelSkinnyPack = 16,  // + 0..3: with packed adapters
+  kKernelSkinnyBig = 20,  // + 0..8: both with one block an SM
+  kKernelNarrow = 29,  // + 0..3: the narrow product by epilogue
+  kKernelNorm = 33,    // + 0..11: the ring layer norm by direction, type and width
+  kKernelThin = 45,    // + 0..15: the thin orthogonalisation by type, side and rank
+  kKernelNormLong = 61,   // + 0..9: the layer norm's backward of long rows by type and width
+  kKernelCount = 71
 };
 
 // FA_OK when the last CUDA runtime call / launch on this thread succeeded;

@@ -17,7 +17,8 @@ struct Mat3 {
   int bf16 = 1;  // else fp16
 };
 
-// 3-D TMA descriptor over `m`, box (inner, rows, 1), SWIZZLE_128B, zero fill.
+// 3-D TMA descriptor over `m`, box (inner, rows, 1), swizzled over the box's
+// inner width (32, 64 or 128 bytes), zero fill.
 int make_tmap_3d(CUtensorMap* map, const Mat3& m, int box_inner, int box_rows);
 
 enum WideEpi {

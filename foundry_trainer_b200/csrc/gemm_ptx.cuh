@@ -180,6 +180,18 @@ __device__ __forceinline__ void pdl_wait_previous() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// K-major operand tiles of rows of 32 or 64 bytes (16 or 32 K), swizzled over
+// their own width: descriptor (layout 6 or 4, eight rows apart) and the offset
+// of 16-byte chunk c of row r.
+__device__ __forceinline__ uint64_t kmajor_narrow_desc(uint32_t base, uint32_t row_bytes) {
+  return (uint64_t)((base >> 4) & 0x3FFFu) | (1ull << 16) |
+         ((uint64_t)((row_bytes * 8) >> 4) << 32) | (1ull << 46) |
+         ((row_bytes == 32 ? 6ull : 4ull) << 61);
+}
+__device__ __forceinline__ uint32_t narrow_offset(uint32_t r, uint32_t c, uint32_t row_bytes) {
+  return r * row_bytes + ((row_bytes == 32 ? c ^ ((r >> 2) & 1u) : c ^ ((r >> 1) & 3u)) << 4);
+}
+
 // Whether `n` bf16 values from p (16-byte aligned) on hold a NaN or an infinity.
 __device__ __forceinline__ bool any_non_finite(const __nv_bfloat16* p, int n) {
   uint32_t bad = 0;

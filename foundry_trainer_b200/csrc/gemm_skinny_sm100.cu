@@ -155,8 +155,10 @@ struct Maps {
   CUtensorMap big[kProducts], small[kProducts], fac[kProducts];
 };
 
-template <bool BIG_MN, bool SMALL_MN, int OUT>
-__global__ void __launch_bounds__(kThreads, 2)
+// (Bounds of 256 threads: registers are given to four warps at a time, so that
+// two blocks of six warps fit an SM as two of eight would, up to 128 a thread.)
+template <bool BIG_MN, bool SMALL_MN, int OUT, int PACK, int HOLD>
+__global__ void __launch_bounds__(256, 2)
 skinny_kernel(const __grid_constant__ Maps<OUT> maps, const __grid_constant__ SkinnyParams p,
               int split, int stage_bytes, int stages, int bar_off, int exchange, int tmem_cols) {
   extern __shared__ uint8_t smem_raw[];
@@ -223,6 +225,10 @@ skinny_kernel(const __grid_constant__ Maps<OUT> maps, const __grid_constant__ Sk
   // K blocks that hold (adapter, 64 ranks)
   const bool adapters = OUT == kSkinnyCols && p.low != nullptr;
   const int kbe = (p.rank + 63) >> 6;
+  // With requests' adapters of at most 32 ranks a block holds two or four of
+  // them, each with tiles of its own width (64 x 4096 x 16384 with 48 adapters
+  // of rank 16: 47 us, 53 as blocks of one)
+  constexpr int pack = PACK;
 
   pdl_launch_next();
   if (warp == 4) {
@@ -263,17 +269,25 @@ skinny_kernel(const __grid_constant__ Maps<OUT> maps, const __grid_constant__ Sk
         if (++s == stages) { s = 0; ph ^= 1; }
       }
       if (ok && adapters && (ok = mbar_wait(planned, 0))) {
-        for (int x = part; x < plan.cnt * kbe; x += split) {
+        const int blocks = pack > 1 ? (plan.cnt + pack - 1) / pack : plan.cnt * kbe;
+        for (int x = part; x < blocks; x += split) {
           if (!(ok = mbar_wait(&empty[s], ph ^ 1))) break;
           uint8_t* sa = smem + s * stage_bytes;
-          const int e = plan.list[x / kbe], j = x % kbe;
           mbar_arrive(&grant[s]);
-          mbar_arrive_expect_tx(&full[s], kBig);
-          if constexpr (BIG_MN) {
-            tma_load_3d(sa, tfac, &full[s], i0, j * 64, e);
-            tma_load_3d(sa + 8192, tfac, &full[s], i0 + 64, j * 64, e);
+          if constexpr (pack > 1) {
+            const int some = min(pack, plan.cnt - x * pack), each = kBig / pack;
+            mbar_arrive_expect_tx(&full[s], some * each);
+            for (int u = 0; u < some; ++u)
+              tma_load_3d(sa + u * each, tfac, &full[s], 0, i0, plan.list[x * pack + u]);
           } else {
-            tma_load_3d(sa, tfac, &full[s], j * 64, i0, e);
+            const int e = plan.list[x / kbe], j = x % kbe;
+            mbar_arrive_expect_tx(&full[s], kBig);
+            if constexpr (BIG_MN) {
+              tma_load_3d(sa, tfac, &full[s], i0, j * 64, e);
+              tma_load_3d(sa + 8192, tfac, &full[s], i0 + 64, j * 64, e);
+            } else {
+              tma_load_3d(sa, tfac, &full[s], j * 64, i0, e);
+            }
           }
           if (++s == stages) { s = 0; ph ^= 1; }
         }
@@ -308,15 +322,26 @@ skinny_kernel(const __grid_constant__ Maps<OUT> maps, const __grid_constant__ Sk
       if (++s == stages) { s = 0; ph ^= 1; }
     }
     if (ok && adapters && (ok = mbar_wait_w(planned, 0))) {
-      const int blocks = plan.cnt * kbe;
+      const int blocks = pack > 1 ? (plan.cnt + pack - 1) / pack : plan.cnt * kbe;
       for (int x = part; x < blocks; x += split) {
         if (!(ok = mbar_wait_w(&full[s], ph))) break;
         tc_fence_after();
-        const uint64_t a = a0 + (uint32_t)(s * (stage_bytes >> 4));
-        const uint64_t b = b0 + (uint32_t)(s * (stage_bytes >> 4));
-        const int steps = min(4, (p.rank - (x % kbe) * 64 + 15) >> 4);
-        for (int kk = 0; kk < steps; ++kk)
-          umma_ss_w(tmem, a + (BIG_MN ? 128 : 2) * kk, b + 2 * kk, idesc, 1);
+        if constexpr (pack > 1) {
+          const int some = min(pack, plan.cnt - x * pack), steps = (p.rank + 15) >> 4;
+          uint64_t a = kmajor_narrow_desc(base + s * stage_bytes, 128 / pack);
+          uint64_t b = kmajor_narrow_desc(base + s * stage_bytes + kBig, 128 / pack);
+          for (int u = 0; u < some; ++u) {
+            for (int kk = 0; kk < steps; ++kk) umma_ss_w(tmem, a + 2 * kk, b + 2 * kk, idesc, 1);
+            a += (uint32_t)(kBig / pack >> 4);
+            b += (uint32_t)(n * 128 / pack >> 4);
+          }
+        } else {
+          const uint64_t a = a0 + (uint32_t)(s * (stage_bytes >> 4));
+          const uint64_t b = b0 + (uint32_t)(s * (stage_bytes >> 4));
+          const int steps = min(4, (p.rank - (x % kbe) * 64 + 15) >> 4);
+          for (int kk = 0; kk < steps; ++kk)
+            umma_ss_w(tmem, a + (BIG_MN ? 128 : 2) * kk, b + 2 * kk, idesc, 1);
+        }
         umma_commit_w(&empty[s]);
         if (++s == stages) { s = 0; ph ^= 1; }
       }
@@ -335,14 +360,14 @@ skinny_kernel(const __grid_constant__ Maps<OUT> maps, const __grid_constant__ Sk
       // producer, which has waited for every earlier use of it, grants it: a
       // parity wait on `empty` from here would skip phases and could return
       // for an earlier one.
-      const int blocks = plan.cnt * kbe;
+      const int blocks = pack > 1 ? (plan.cnt + pack - 1) / pack : plan.cnt * kbe;
       int s = (kb1 - kb0) % stages;
       uint32_t turns = 0;  // bit s: parity of the slot's next grant
       // A lane's 16-byte pieces of the operand are the same in every block
-      // while one block holds the rank: up to 16 are kept in registers (with
+      // while one block holds the rank: up to HOLD are kept in registers (with
       // their place, and the adapter's slot above it) and a block is stores
       // alone.
-      constexpr int kHold = 16;
+      constexpr int kHold = HOLD;
       const int chunks0 = min(8, p.low_ld >> 3);
       const bool held = kbe == 1 && n * chunks0 <= kHold * 32;
       uint4 hold[kHold];
@@ -354,9 +379,10 @@ skinny_kernel(const __grid_constant__ Maps<OUT> maps, const __grid_constant__ Sk
           at[k] = -1;
           hold[k] = make_uint4(0, 0, 0, 0);
           if (i < n * chunks0) {
-            at[k] = (int)sw128_offset(j, c) | 511 << 16;
+            const int place = (int)(pack > 1 ? narrow_offset(j, c, 128 / pack) : sw128_offset(j, c));
+            at[k] = place | 511 << 16;
             if (j < cols && plan.slot[j] >= 0) {
-              at[k] = (int)sw128_offset(j, c) | plan.slot[j] << 16;
+              at[k] = place | plan.slot[j] << 16;
               hold[k] = *reinterpret_cast<const uint4*>(low + (int64_t)j * p.low_stride + c * 8);
             }
           }
@@ -366,14 +392,28 @@ skinny_kernel(const __grid_constant__ Maps<OUT> maps, const __grid_constant__ Sk
         if ((s & 3) != warp) continue;
         if (!(ok = mbar_wait_w(&grant[s], (turns >> s) & 1))) break;
         turns ^= 1u << s;
-        const int q = x / kbe;
+        const int q = pack > 1 ? x * pack : x / kbe;
+        const int some = pack > 1 ? min(pack, plan.cnt - q) : 1;
         uint8_t* sb = smem + s * stage_bytes + kBig;
         if (held) {
+          for (int u = 0; u < some; ++u) {
 #pragma unroll
-          for (int k = 0; k < kHold; ++k)
-            if (at[k] >= 0)
-              *reinterpret_cast<uint4*>(sb + (at[k] & 0xffff)) =
-                  (at[k] >> 16) == q ? hold[k] : make_uint4(0, 0, 0, 0);
+            for (int k = 0; k < kHold; ++k)
+              if (at[k] >= 0)
+                *reinterpret_cast<uint4*>(sb + u * (n * 128 / pack) + (at[k] & 0xffff)) =
+                    (at[k] >> 16) == q + u ? hold[k] : make_uint4(0, 0, 0, 0);
+          }
+        } else if constexpr (pack > 1) {
+          for (int u = 0; u < some; ++u) {
+#pragma unroll 8
+            for (int i = lane; i < n * chunks0; i += 32) {
+              const int j = i / chunks0, c = i - j * chunks0;
+              uint4 v = make_uint4(0, 0, 0, 0);
+              if (j < cols && plan.slot[j] == q + u)
+                v = *reinterpret_cast<const uint4*>(low + (int64_t)j * p.low_stride + c * 8);
+              *reinterpret_cast<uint4*>(sb + u * (n * 128 / pack) + narrow_offset(j, c, 128 / pack)) = v;
+            }
+          }
         } else {
           const int k0 = (x - q * kbe) * 64, chunks = min(8, (p.low_ld - k0) >> 3);
 #pragma unroll 8
@@ -607,32 +647,42 @@ plan_kernel(const int* ids, int rows, int E, int* cnt, int* list, int* slot) {
   if (t == 0) cnt[blockIdx.x] = total;
 }
 
-template <bool BIG_MN, bool SMALL_MN, int OUT>
+template <bool BIG_MN, bool SMALL_MN, int OUT, int PACK = 1, int HOLD = 16>
 static int go(const Maps<OUT>& maps, const SkinnyParams& p, int passes, int kernel_id, bool early,
               cudaStream_t st) {
-  auto* fn = skinny_kernel<BIG_MN, SMALL_MN, OUT>;
+  auto* fn = skinny_kernel<BIG_MN, SMALL_MN, OUT, PACK, HOLD>;
   const Layout l = layout_of(p.n, SMALL_MN, OUT == kSkinnyGrad);
   // the largest layout's request, once per kernel
   const int rc = ensure_smem_attr((const void*)fn, kOneSmem, kernel_id);
   if (rc) return rc;
-  const int tiles = (std::max(p.rows, p.rows2) + 127) / 128, kbs = (p.K + 63) / 64;
+  const int tiles = (std::max(p.rows, p.rows2) + 127) / 128;
   const int64_t work = OUT == kSkinnyGrad ? (p.rows + 127) / 128 + (p.rows2 + 127) / 128
                                           : (int64_t)tiles * passes;
+  // K blocks, the requests' adapters' among them (as many as there may be)
+  int kbs = (p.K + 63) / 64, most = kbs;
+  if (OUT == kSkinnyCols && p.ids != nullptr)
+    most += (std::min(p.E, p.n) + PACK - 1) / PACK * ((p.rank + 63) / 64);
   // contraction split: the one whose rounds of resident clusters times blocks
-  // per CTA (and about two blocks' time for the exchange) is smallest. A wave
-  // that spills over costs a whole round: with 72 clusters of 4 where 66 fit,
-  // 302 MB took 74 us.
+  // per CTA (1.6 times as long where two CTAs share an SM), and some blocks' time
+  // for start and exchange, is smallest. A wave that spills
+  // over costs a whole round: with 72 clusters of 4 where 66 fit, 302 MB took 74
+  // us; 64 x 4096 x 16384 with 48 adapters takes 46 us unsplit on 128 SMs, 38
+  // as two per tile; one token at 4096 x 4096 9.5 us split by 4, 9.9 by 8.
+  // (The occupancy calculator takes a kernel with tensor memory to fill it, one
+  // block an SM; two of at most 128 columns do run together.)
   const bool two = l.smem <= kTwoSmem;
   int split = 1;
-  int64_t best = INT64_MAX;
+  float best = 1e30f;
   for (int c = 1; c <= 8 && c <= kbs; ++c) {
     int fit = 0;
     const int rf = clusters_that_fit((const void*)fn, kThreads, two ? kTwoSmem : kOneSmem, c,
                                      kernel_id + (two ? 0 : kKernelSkinnyBig - kKernelSkinny), &fit);
     if (rf) return rf;
     if (fit <= 0) continue;
+    if (two) fit *= 2;
     const int64_t rounds = (work + fit - 1) / fit;
-    const int64_t cost = rounds * ((kbs + c - 1) / c + 2);
+    const float shared = std::min<int64_t>(work, fit) * c > 148 && two ? 1.6f : 1.f;
+    const float cost = rounds * ((most + c - 1) / c * shared + 2.f + 0.8f * c);
     if (cost < best) best = cost, split = c;
   }
   cudaLaunchConfig_t cfg{};
@@ -660,7 +710,7 @@ static int go(const Maps<OUT>& maps, const SkinnyParams& p, int passes, int kern
 
 }  // namespace skinny
 
-template <bool BIG_MN, bool SMALL_MN, int OUT>
+template <bool BIG_MN, bool SMALL_MN, int OUT, int PACK = 1, int HOLD = 16>
 static int launch(const Mat3& big, const Mat3& small, const Mat3& fac, const SkinnyParams& p,
                   int passes, int kernel_id, bool early, cudaStream_t st) {
   skinny::Maps<OUT> m;
@@ -669,8 +719,8 @@ static int launch(const Mat3& big, const Mat3& small, const Mat3& fac, const Ski
   if (!rc) rc = make_tmap_3d(&m.small[0], small, 64, SMALL_MN ? 64 : box);
   m.fac[0] = m.big[0];
   if (!rc && OUT == kSkinnyCols && p.low != nullptr)
-    rc = make_tmap_3d(&m.fac[0], fac, 64, BIG_MN ? 64 : 128);
-  return rc ? rc : skinny::go<BIG_MN, SMALL_MN, OUT>(m, p, passes, kernel_id, early, st);
+    rc = make_tmap_3d(&m.fac[0], fac, 64 / PACK, BIG_MN ? 64 : 128);
+  return rc ? rc : skinny::go<BIG_MN, SMALL_MN, OUT, PACK, HOLD>(m, p, passes, kernel_id, early, st);
 }
 
 int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool small_mn,
@@ -689,6 +739,20 @@ int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool sma
     p.n = p.slots_per_pass * p.low_ld;
     passes = (most + p.slots_per_pass - 1) / p.slots_per_pass;
   }
+  // requests' adapters of at most 32 ranks: packed; the builders' registers by
+  // what they hold (64 x 4096 x 4096, rank 12: 16.2 us with 8, 17.2 with 16)
+#define FA_PACK(PACK, HOLD, ID)                                                               \
+  return launch<false, false, kSkinnyCols, PACK, HOLD>(big, small, fac, p, passes,            \
+                                                       kKernelSkinnyPack + ID, early, st)
+  if (out == kSkinnyCols && !big_mn && !small_mn && p.ids != nullptr && p.low_ld == 16) {
+    if (p.n <= 128) FA_PACK(4, 8, 0);
+    FA_PACK(4, 16, 1);
+  }
+  if (out == kSkinnyCols && !big_mn && !small_mn && p.ids != nullptr && p.low_ld == 32) {
+    if (p.n <= 64) FA_PACK(2, 8, 2);
+    FA_PACK(2, 16, 3);
+  }
+#undef FA_PACK
   if (out == kSkinnyCols && !big_mn && !small_mn)
     return launch<false, false, kSkinnyCols>(big, small, fac, p, passes, kKernelSkinny, early, st);
   if (out == kSkinnyCols && big_mn && !small_mn)
