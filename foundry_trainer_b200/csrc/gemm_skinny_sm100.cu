@@ -663,11 +663,12 @@ static int go(const Maps<OUT>& maps, const SkinnyParams& p, int passes, int kern
   if (OUT == kSkinnyCols && p.ids != nullptr)
     most += (std::min(p.E, p.n) + PACK - 1) / PACK * ((p.rank + 63) / 64);
   // contraction split: the one whose rounds of resident clusters times blocks
-  // per CTA (1.6 times as long where two CTAs share an SM), and some blocks' time
-  // for start and exchange, is smallest. A wave that spills
-  // over costs a whole round: with 72 clusters of 4 where 66 fit, 302 MB took 74
-  // us; 64 x 4096 x 16384 with 48 adapters takes 46 us unsplit on 128 SMs, 38
-  // as two per tile; one token at 4096 x 4096 9.5 us split by 4, 9.9 by 8.
+  // per CTA, longer ones where two CTAs share an SM, and some blocks' time for
+  // start and exchange, is smallest (factors fitted to some 20 shapes). A wave
+  // that spills over costs a whole round: with 72 clusters of 4 where 66 fit, 302
+  // MB took 74 us; 64 x 4096 x 16384 with 48 adapters takes 46 us unsplit on 128
+  // SMs, 38 as two per tile; the gradients at 4608 x 2560 x 2560 11 us split by
+  // 6 over shared SMs, 15 by 3.
   // (The occupancy calculator takes a kernel with tensor memory to fill it, one
   // block an SM; two of at most 128 columns do run together.)
   const bool two = l.smem <= kTwoSmem;
@@ -681,8 +682,9 @@ static int go(const Maps<OUT>& maps, const SkinnyParams& p, int passes, int kern
     if (fit <= 0) continue;
     if (two) fit *= 2;
     const int64_t rounds = (work + fit - 1) / fit;
-    const float shared = std::min<int64_t>(work, fit) * c > 148 && two ? 1.6f : 1.f;
-    const float cost = rounds * ((most + c - 1) / c * shared + 2.f + 0.8f * c);
+    const bool sharing = two && std::min<int64_t>(work, fit) * c > 148;
+    const float block = !sharing ? 1.f : OUT == kSkinnyCols ? 1.25f : 1.6f;
+    const float cost = rounds * ((most + c - 1) / c * block + 2.f + (OUT == kSkinnyCols ? 1.f : 0.5f) * c);
     if (cost < best) best = cost, split = c;
   }
   cudaLaunchConfig_t cfg{};
