@@ -13,7 +13,10 @@
 // and 32 KB are read per SM for 512 cycles of tensor work, within the 128
 // bytes a cycle of shared memory that a single-CTA 128 x 256 tile exceeds. A
 // 256 x 128 tile was measured to take as long as the 256 x 256 one, so there
-// is no narrower form.
+// is no narrower form. At 9216 x 4096 x 16384 with an adapter of rank 32: 793
+// us forward, 803 us for dx, 1.56 PFLOP/s with the tensor cores 91 to 93
+// percent busy and the clock at 1.4 GHz under the power cap (the library
+// product's sustained rate there is 1.40).
 // The pair is persistent over tiles; the accumulator is double-buffered in
 // tensor memory (2 kBN columns), so a tile's epilogue runs under the next
 // tile's products.

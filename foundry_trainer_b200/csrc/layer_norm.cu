@@ -23,7 +23,13 @@
 // the block barrier of the rows' sums also tells that thread that the slot is
 // free. Loads straight into registers were latency-bound: at 4608 x 2048 bf16
 // forward 18.5 us, backward 24 us. The direct form serves every other width,
-// stride and alignment, and the forward's smallest calls.
+// stride and alignment (16-byte accesses, pairs or single elements), and the
+// forward's smallest calls; its backward of long rows keeps the column sums in
+// shared memory.
+//
+// At 36864 x 4096 bf16: forward 101 us, 5.96 TB/s of the copy's 6.55; backward
+// 153 us, 5.92 TB/s. At 4608 x 2048: 10.8 and 14.4 us (5.8 and 8.6 at the
+// copy's rate), one wave's ramp and tail. One row of 2048: 2.5 us.
 #include <cuda_bf16.h>
 
 #include <algorithm>

@@ -31,6 +31,11 @@
 // steps contract. Against 64 bits: 2.3e-3 of the result's norm on Gaussian
 // noise, 1.7e-3 on a few strong directions over noise; the final rounding to
 // bf16 alone is 1.7e-3.
+//
+// Measured: 16 x (16 x 4096) bf16 13 us, 8 x (64 x 4096) 78 us (fp64 tensor
+// instructions, about half their rate); 4096 x 8192 fp32 2.1 to 2.2 ms under
+// the power cap, its products 102 (Gram), 60 (Q^2) and 190 us (update); 1024 x
+// 1024 148 us, 512 x 512 89 us, 16 products of 5 to 9 us in a chain.
 #include <cuda_bf16.h>
 
 #include <algorithm>
