@@ -433,9 +433,9 @@ def run_block(args, rank, world, local):
         "e2e": e2e,
         # per step: q, k prologues + v concat + fwd; dO concat + delta + bwd +
         # dQ finish + q, k prologue backwards; fused: 4 norms and the backward
-        # of two; 8 adapter linears of 2 forward, 3 backward and the input
+        # of two; 8 adapter linears of 2 forward, 2 backward and the input
         # gradient of two
-        "gpu_launches": (10 + (48 if args.fused_block else 0)) * K,
+        "gpu_launches": (10 + (40 if args.fused_block else 0)) * K,
         "clocks": clocks,
     }
     print(json.dumps(line), flush=True)
