@@ -34,11 +34,11 @@ enum KernelId {
   kKernelSkinny = 11,  // + 0..4 by operand layout and output
   kKernelSkinnyPack = 16,  // + 0..3: with packed adapters
   kKernelSkinnyBig = 20,  // + 0..8: both with one block an SM
-  kKernelNarrow = 29,  // + 0..3: the narrow product by epilogue
-  kKernelNorm = 33,    // + 0..11: the ring layer norm by direction, type and width
-  kKernelThin = 45,    // + 0..15: the thin orthogonalisation by type, side and rank
-  kKernelNormLong = 61,   // + 0..9: the layer norm's backward of long rows by type and width
-  kKernelCount = 71
+  kKernelNarrow = 29,  // + 0..4: the narrow product by epilogue, then split
+  kKernelNorm = 34,    // + 0..11: the ring layer norm by direction, type and width
+  kKernelThin = 46,    // + 0..15: the thin orthogonalisation by type, side and rank
+  kKernelNormLong = 62,   // + 0..9: the layer norm's backward of long rows by type and width
+  kKernelCount = 72
 };
 
 // FA_OK when the last CUDA runtime call / launch on this thread succeeded;

@@ -40,6 +40,7 @@ struct WideParams {
   int M = 0, N = 0, K = 0, batch = 1;
   int fmt = 1;  // 0 fp16, 1 bf16 operands
   int tiles_m = 0, tiles_n = 0, tiles_per_batch = 0, symmetric = 0;
+  int split = 1;  // kEpiGram in narrow tiles: CTAs (a cluster) that share a tile's contraction
   // adapters: low (M, low_ld) bf16 of rows low_stride apart, low_ld = the rank
   // rounded up to 16;
   // per 256-row block the adapters in use and their count, per row its slot

@@ -635,10 +635,14 @@ constexpr int kNarrowBN = 64;
 constexpr int kNarrowStage = kStageA + kNarrowBN * 128;
 constexpr int kNarrowStages = 4;
 constexpr int kNarrowBar = kNarrowStages * kNarrowStage;
+constexpr int kNarrowSums = 128 * kNarrowBN * 4;
+constexpr int kNarrowSplit = 4;  // most CTAs a tile
+static_assert((kNarrowSplit - 1) * kNarrowSums <= kNarrowBar, "the sums lie over the ring");
 constexpr int kNarrowSmem = kNarrowBar + 256 + 1024;
 
-template <bool B_MN, int EPI>
-__global__ void __launch_bounds__(kThreads, 2)
+// (bounds of 256 threads: registers are given to four warps at a time)
+template <bool B_MN, int EPI, bool SPLIT>
+__global__ void __launch_bounds__(256, 2)
 narrow_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
               const __grid_constant__ CUtensorMap tmir, const __grid_constant__ CUtensorMap td, const __grid_constant__ CUtensorMap td2,
               const __grid_constant__ WideParams p) {
@@ -674,8 +678,11 @@ narrow_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
   pdl_launch_next();
   pdl_wait_previous();
 
-  const int b = blockIdx.x / p.tiles_per_batch;
-  const int i = blockIdx.x - b * p.tiles_per_batch;
+  // a tile's contraction may be shared by the CTAs of a cluster (p.split)
+  const int split = SPLIT ? p.split : 1;
+  const int tile = blockIdx.x / split, part = blockIdx.x - tile * split;
+  const int b = tile / p.tiles_per_batch;
+  const int i = tile - b * p.tiles_per_batch;
   int tm, tn;
   if (p.symmetric) {
     triangle(i, 2, tm, tn);  // 128-row block m: column tiles 0 .. 2 m + 1
@@ -685,12 +692,13 @@ narrow_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
   }
   const int row0 = tm * 128, col0 = tn * kNarrowBN;
   const int kbs = (p.K + 63) >> 6;
+  const int kb0 = (int)((int64_t)kbs * part / split), kb1 = (int)((int64_t)kbs * (part + 1) / split);
   bool ok = true;
   if (warp == 4) {
     if (lane == 0) {
       int s = 0;
       uint32_t ph = 0;
-      for (int kb = 0; kb < kbs; ++kb) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         if (!(ok = mbar_wait(&empty[s], ph ^ 1))) break;
         uint8_t* sa = smem + s * kNarrowStage;
         mbar_arrive_expect_tx(&full[s], kNarrowStage);
@@ -701,6 +709,8 @@ narrow_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
       }
       if (!ok) *abort_flag = 1;
     }
+    __syncwarp();
+    if (SPLIT) cluster_sync(), cluster_sync();  // (with the epilogue's)
   } else if (warp == 5) {
     const uint32_t idesc = idesc_f16(p.fmt, 128, kNarrowBN, false, B_MN);
     const uint32_t base = smem_u32(smem);
@@ -708,19 +718,21 @@ narrow_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
     const uint64_t b0 = B_MN ? mnmajor_desc(base + kStageA, 0, 8192) : kmajor_desc(base + kStageA, 0, 0);
     int s = 0;
     uint32_t ph = 0;
-    for (int kb = 0; kb < kbs; ++kb) {
+    for (int kb = kb0; kb < kb1; ++kb) {
       if (!(ok = mbar_wait_w(&full[s], ph))) break;
       tc_fence_after();
       const uint64_t a = a0 + (uint32_t)(s * (kNarrowStage >> 4));
       const uint64_t bb = b0 + (uint32_t)(s * (kNarrowStage >> 4));
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
-        umma_ss_w(tmem, a + 2 * kk, bb + (B_MN ? 128 : 2) * kk, idesc, kb > 0 || kk > 0);
+        umma_ss_w(tmem, a + 2 * kk, bb + (B_MN ? 128 : 2) * kk, idesc, kb > kb0 || kk > 0);
       umma_commit_w(&empty[s]);
-      if (kb == kbs - 1) umma_commit_w(done);
+      if (kb == kb1 - 1) umma_commit_w(done);
       if (++s == kNarrowStages) { s = 0; ph ^= 1; }
     }
     if (!ok) *abort_flag = 1;
+    __syncwarp();
+    if (SPLIT) cluster_sync(), cluster_sync();
   } else {
     const int r = threadIdx.x, row = row0 + r;
     const bool live = row < p.M;
@@ -733,16 +745,58 @@ narrow_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
     back[0].load(p, b, row, live, col0);
     back[1].load(p, b, row, live, col0 + 32);
     ok = mbar_wait_w(done, 0);
-    if (!named_bar_any(1, 128, !ok)) {
-      tc_fence_after();
-      const uint32_t taddr = tmem + ((uint32_t)(warp * 32) << 16);
+    const bool bad = named_bar_any(1, 128, !ok);
+    tc_fence_after();
+    const uint32_t taddr = tmem + ((uint32_t)(warp * 32) << 16);
+    if constexpr (SPLIT) {
+      // the other CTAs' sums go to the first one's ring, which is idle when all
+      // have waited for their products: (split - 1, 64 / 4, 128, 4) fp32
+      cluster_sync();
+      if (part > 0 && !bad) {
+        const uint32_t dst = mapa(smem_u32(smem) + (uint32_t)((part - 1) * kNarrowSums + r * 16), 0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t acc[32];
+          tmem_ld32(taddr + 32 * h, acc);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; c += 4)
+            st_cluster_v4(dst + (uint32_t)((32 * h + c) * 512), acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+        }
+      }
+      cluster_sync();
+    }
+    if (!bad && part == 0) {
       const bool mirror = p.symmetric && tn < 2 * tm;
       const bool direct = EPI == kEpiLast && p.out_t != nullptr;
+      uint32_t first[SPLIT ? 32 : 1];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t acc[32], out[16], lo[16];
         tmem_ld32(taddr + 32 * h, acc);
         tmem_wait_ld();
+        if constexpr (SPLIT) {  // in CTA order
+          float* v = reinterpret_cast<float*>(acc);
+          for (int q = 0; q < split - 1; ++q) {
+            const float4* s = reinterpret_cast<const float4*>(smem + q * kNarrowSums) + r;
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              const float4 w = s[(32 * h + c) * 32];
+              v[c] += w.x; v[c + 1] += w.y; v[c + 2] += w.z; v[c + 3] += w.w;
+            }
+          }
+          // the staged tiles lie over the sums
+          if (h == 0) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) first[c] = acc[c];
+            continue;
+          }
+          named_bar_sync(1, 128);
+          uint32_t o0[16];
+          ns_values<EPI>(p, back[0], ca, cb, first, o0, lo);
+          if (mirror) stage_mirror(smem + kStaging, r, 0, o0);
+          stage_half(smem, r, 0, o0);
+        }
         ns_values<EPI>(p, back[h], ca, cb, acc, out, lo);
         if (direct) {
           if (live)
@@ -767,7 +821,7 @@ narrow_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
           bulk_wait_group_read0();
         }
       }
-    } else {
+    } else if (bad) {
       *abort_flag = 1;
     }
   }
@@ -781,22 +835,25 @@ narrow_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CU
   }
 }
 
-template <bool B_MN, int EPI>
+template <bool B_MN, int EPI, bool SPLIT = false>
 static int narrow_go(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tmir,
                      const CUtensorMap& td, const CUtensorMap& td2, const WideParams& p, int kernel_id, cudaStream_t st) {
-  auto* fn = narrow_kernel<B_MN, EPI>;
+  auto* fn = narrow_kernel<B_MN, EPI, SPLIT>;
   const int rc = ensure_smem_attr((const void*)fn, kNarrowSmem, kernel_id);
   if (rc) return rc;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((int64_t)p.tiles_per_batch * p.batch));
+  cfg.gridDim = dim3((unsigned)((int64_t)p.tiles_per_batch * p.batch * p.split));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kNarrowSmem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[0].val.programmaticStreamSerializationAllowed = p.early != 0;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = p.split;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = p.early ? 1 : 0;
+  cfg.numAttrs = SPLIT ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, ta, tb, tmir, td, td2, p);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -807,14 +864,21 @@ static int narrow_go(const CUtensorMap& ta, const CUtensorMap& tb, const CUtenso
 
 // Which form is sooner done: rounds of 296 resident tiles of 128 x 64, 0.4 us a
 // K block while an SM holds two (0.2 us one), or of 74 pairs' tiles of 256 x
-// 256, 0.29 us a K block.
-static bool use_narrow(const WideParams& p) {
+// 256, 0.29 us a K block. A Gram product of few tiles and a long contraction
+// splits it over up to four CTAs a tile, for some 2 us (2 x
+// 272 x 2792: 195 -> 145 us a call, 100 x 8192 207 -> 123).
+static bool use_narrow(WideParams& p, int epi) {
   const int64_t m1 = (p.M + 127) / 128, n1 = (p.N + 63) / 64;
   const int64_t m2 = (p.M + 255) / 256, n2 = (p.N + 255) / 256;
   const int64_t t1 = (p.symmetric ? m1 * (m1 + 1) : m1 * n1) * p.batch;
   const int64_t t2 = (p.symmetric ? m2 * (m2 + 1) / 2 : m2 * n2) * p.batch;
   const int64_t kbs = (p.K + 63) / 64;
-  const float narrow = 4.f + (t1 <= 148 ? 0.2f * kbs : (t1 + 295) / 296 * kbs * 0.4f);
+  float narrow = 4.f + (t1 <= 148 ? 0.2f * kbs : (t1 + 295) / 296 * kbs * 0.4f);
+  p.split = 1;
+  for (int c = 2; epi == kEpiGram && c <= kNarrowSplit && t1 * c <= 148 && c <= kbs; ++c) {
+    const float time = 6.f + 0.2f * ((kbs + c - 1) / c);
+    if (time < narrow) narrow = time, p.split = c;
+  }
   const float pairs = 9.f + (t2 + 73) / 74 * kbs * 0.29f;
   return narrow < pairs;
 }
@@ -838,7 +902,7 @@ int TmapMemo::get(CUtensorMap* map, const Mat3& m, int rows) {
 
 int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t st,
                      TmapMemo* maps) {
-  const bool narrow = epi != kEpiLinear && wide::use_narrow(p);
+  const bool narrow = epi != kEpiLinear && wide::use_narrow(p, epi);
   const int tile_n = narrow ? wide::kNarrowBN : wide::kBN, tile_m = narrow ? 128 : 256;
   p.tiles_m = (p.M + tile_m - 1) / tile_m;
   p.tiles_n = (p.N + tile_n - 1) / tile_n;
@@ -872,6 +936,8 @@ int launch_gemm_wide(const WideOperands& o, WideParams p, int epi, cudaStream_t 
 #define FA_NARROW(EPI, MN, ID)                    \
   if (narrow && epi == EPI && o.b_mn == MN)       \
     return wide::narrow_go<MN, EPI>(ta, tb, tlow, td, td2, p, ID, st);
+  if (narrow && epi == kEpiGram && p.split > 1)
+    return wide::narrow_go<false, kEpiGram, true>(ta, tb, tlow, td, td2, p, kKernelNarrow + 4, st);
   FA_NARROW(kEpiGram, false, kKernelNarrow)
   FA_NARROW(kEpiPoly, false, kKernelNarrow + 1)
   FA_NARROW(kEpiUpdate, true, kKernelNarrow + 2)
