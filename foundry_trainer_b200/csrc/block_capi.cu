@@ -365,7 +365,8 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
   int* list = reinterpret_cast<int*>(ws);
   ws += align256(blocks * 256 * 4);
   int* slot = reinterpret_cast<int*>(ws);
-  const bool dots = rows <= kDotRowsMany, columns = linear_as_columns(out_dim, in_dim, rows);
+  const bool dots = rows <= kDotRowsMany;
+  const bool columns = linear_as_columns(out_dim, in_dim, rows, n_adapters, rank);
   if (!dots || !columns) FA_TRY(launch_adapter_plan(ids, rows, n_adapters, cnt, list, slot, st));
   if (dots) {
     FA_TRY(launch_low_rows(bfp(x->data), x->stride_row, bfp(a->data), a->stride_batch,

@@ -126,7 +126,7 @@ int launch_gemm_skinny(const Mat3& big, bool big_mn, const Mat3& small, bool sma
 int launch_skinny_grads(const Mat3* big, const Mat3* small, const Mat3* small_lo, SkinnyParams p,
                         cudaStream_t st);
 // whether a linear of `rows` tokens runs as kSkinnyCols rather than wide
-bool linear_as_columns(int64_t out, int64_t K, int rows);
+bool linear_as_columns(int64_t out, int64_t K, int rows, int adapters = 0, int rank = 0);
 int launch_low_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int64_t a_e,
                     int64_t a_r, const int* ids, int E, const float* scales, float scale, int rows,
                     int K, int rank, int low_ld, __nv_bfloat16* low, int64_t low_stride, int lo_at,

@@ -176,6 +176,7 @@ skinny_kernel(const __grid_constant__ Maps<OUT> maps, const __grid_constant__ Sk
   uint64_t* grant = planned + 1;
   uint32_t* slot = reinterpret_cast<uint32_t*>(grant + kMaxStages);
   __shared__ TokenPlan plan;
+  __shared__ uint8_t tokens_s[OUT == kSkinnyCols ? 4 : 1][kMaxTokens];  // of an adapter, per warp
   volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
   const int warp = warp_id(), lane = lane_id();
   const int tile = blockIdx.x / split, part = blockIdx.x - tile * split;
@@ -407,26 +408,37 @@ skinny_kernel(const __grid_constant__ Maps<OUT> maps, const __grid_constant__ Sk
                 *reinterpret_cast<uint4*>(sb + u * (n * 128 / pack) + (at[k] & 0xffff)) =
                     (at[k] >> 16) == q + u ? hold[k] : make_uint4(0, 0, 0, 0);
           }
-        } else if constexpr (pack > 1) {
-          for (int u = 0; u < some; ++u) {
-#pragma unroll 8
-            for (int i = lane; i < n * chunks0; i += 32) {
-              const int j = i / chunks0, c = i - j * chunks0;
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (j < cols && plan.slot[j] == q + u)
-                v = *reinterpret_cast<const uint4*>(low + (int64_t)j * p.low_stride + c * 8);
-              *reinterpret_cast<uint4*>(sb + u * (n * 128 / pack) + narrow_offset(j, c, 128 / pack)) = v;
-            }
-          }
         } else {
-          const int k0 = (x - q * kbe) * 64, chunks = min(8, (p.low_ld - k0) >> 3);
+          // zeros, then only the tokens that use the adapter, their places by
+          // ballots (256 tokens of 200 adapters of rank 32, 4096 x 4096: 95 us
+          // when every block looked at every token, 63 now)
+          const int k0 = pack > 1 ? 0 : (x - q * kbe) * 64;
+          const int chunks = pack > 1 ? 8 / pack : min(8, (p.low_ld - k0) >> 3);
+          uint8_t* mine = tokens_s[warp];
+          for (int u = 0; u < some; ++u) {
+            uint8_t* to = sb + u * (n * 128 / pack);
+            int cnt = 0;
+            for (int g = 0; g < n; g += 32) {
+              const bool use = g + lane < cols && plan.slot[g + lane] == q + u;
+              const uint32_t m = __ballot_sync(0xffffffffu, use);
+              if (use) mine[cnt + __popc(m & ((1u << lane) - 1u))] = (uint8_t)(g + lane);
+              cnt += __popc(m);
+            }
+#pragma unroll 4
+            for (int i = lane; i < n * 8 / pack; i += 32)
+              *reinterpret_cast<uint4*>(to + i * 16) = make_uint4(0, 0, 0, 0);
+            __syncwarp();
+            const int lg = chunks <= 2 ? 1 : chunks <= 4 ? 2 : 3;  // lanes a row, 16 bytes each
+            const int c = lane & ((1 << lg) - 1);
 #pragma unroll 8
-          for (int i = lane; i < n * chunks; i += 32) {
-            const int j = i / chunks, c = i - j * chunks;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (j < cols && plan.slot[j] == q)
-              v = *reinterpret_cast<const uint4*>(low + (int64_t)j * p.low_stride + k0 + c * 8);
-            *reinterpret_cast<uint4*>(sb + sw128_offset(j, c)) = v;
+            for (int i = lane >> lg; i < cnt; i += 32 >> lg) {
+              const int j = mine[i];
+              if (c < chunks)
+                *reinterpret_cast<uint4*>(
+                    to + (pack > 1 ? narrow_offset(j, c, 128 / pack) : sw128_offset(j, c))) =
+                    *reinterpret_cast<const uint4*>(low + (int64_t)j * p.low_stride + k0 + c * 8);
+            }
+            __syncwarp();
           }
         }
         fence_proxy_async_smem();
@@ -811,9 +823,19 @@ static float wide_time(int64_t out, int64_t K, int rows) {
 // Few 256 x 256 tiles leave SM pairs idle, where token columns split the
 // contraction over clusters (256 rows, 16384 -> 4096: 42 us against 82); many
 // fill them at half the staged bytes (512 rows, 4096 -> 16384: 97 against 52).
-bool linear_as_columns(int64_t out, int64_t K, int rows) {
+// Up to 256 rows of requests may use as many adapters as there are, each a K
+// block that one warp of a pair builds (1 us, 2.5 beyond rank 32) and that
+// columns split over a cluster's CTAs and their four warps (128 rows of 14
+// adapters of rank 64 at 408 x 920: 50 us as pairs, 25 as columns).
+bool linear_as_columns(int64_t out, int64_t K, int rows, int adapters, int rank) {
   if (rows > kMaxColumns * 65535) return false;  // a block of tokens a grid row
-  return rows <= 64 || cols_time(out, K, rows) < wide_time(out, K, rows);
+  float wide = wide_time(out, K, rows), cols = cols_time(out, K, rows);
+  if (rows <= kMaxColumns) {
+    const int blocks = std::min(adapters, rows) * ((rank + 63) / 64);
+    wide += blocks * (rank <= 32 ? 1.f : 2.5f);
+    cols += blocks * 0.3f;
+  }
+  return rows <= 64 || cols < wide;
 }
 
 int launch_low_rows(const __nv_bfloat16* x, int64_t ldx, const __nv_bfloat16* a, int64_t a_e,
