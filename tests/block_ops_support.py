@@ -1,5 +1,5 @@
 """Plain 64-bit forms of the block operators and the error bounds the tests
-hold the kernels to (checker side only).
+hold the kernels to (used by the tests only).
 
 Every bound is a sum of roundings: half a step of the stored type per
 rounding (u = finfo.eps / 2, relative to the value rounded), and for a sum of
