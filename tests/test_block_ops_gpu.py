@@ -223,6 +223,14 @@ MANY_CASES = [
     (40, 8192, 128, 64, 40, "random"),
     (64, 4096, 6144, 16, 48, "random"),
     (200, 2048, 3000, 96, 200, "random"),
+    # operands built from an adapter's own rows only: pairs and columns, ranks
+    # of one and of two K blocks, packed adapters beyond what a warp keeps
+    (700, 408, 920, 64, 14, "random"),
+    (301, 256, 520, 80, 5, "random"),
+    (226, 408, 920, 64, 14, "random"),
+    (256, 1024, 512, 32, 100, "random"),
+    (250, 512, 384, 12, 37, "random"),
+    (129, 264, 256, 16, 3, "runs"),
 ]
 
 

@@ -56,7 +56,9 @@ SHAPES = [(1, 1), (1, 8, 8), (3, 16, 4096), (2, 4096, 16), (5, 12, 1000), (2, 10
           # the SM-pair form of all three products, upright and tall, ragged
           (1, 4096, 4104), (1, 4500, 4100), (3, 2305, 2500),
           # tall rows of 8 bytes, and of no such number
-          (3, 1000, 12), (2, 700, 36), (2, 300, 61)]
+          (3, 1000, 12), (2, 700, 36), (2, 300, 61),
+          # few tiles and a long contraction
+          (1, 100, 8200), (2, 3001, 130)]
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
