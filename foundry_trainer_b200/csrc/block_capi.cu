@@ -49,6 +49,10 @@ static int check_matrix(const fa_matrix_t* m, int64_t rows, int64_t cols) {
 
 constexpr int kMaxRank = 256;
 constexpr int kMaxSteps = 64;
+// Rows that another request's broken factor reached are multiplied again under the
+// next tile's bounded wait (2e9 cycles): 430 cycles a tile and column of x with
+// all SMs at it, a quarter of the wait at this width.
+constexpr int kMaxInMany = 1 << 20;
 
 static int check_lora(int dtype, int rows, int in_dim, int out_dim, int rank, float scale) {
   if (dtype != FA_DTYPE_BF16) return FA_ERR_UNSUPPORTED;
@@ -338,6 +342,7 @@ int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, 
                         size_t workspace_bytes, void* stream) {
   FA_TRY(check_lora(dtype, rows, in_dim, out_dim, rank, 1.f));
   if (n_adapters <= 0) return FA_ERR_INVALID_ARG;
+  if (in_dim > kMaxInMany) return FA_ERR_TOO_LARGE;
   if (rows == 0) return FA_OK;
   FA_TRY(check_matrix(x, rows, in_dim));
   FA_TRY(check_matrix(w, out_dim, in_dim));

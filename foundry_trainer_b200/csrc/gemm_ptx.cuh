@@ -221,4 +221,95 @@ static __device__ __noinline__ int bad_factors(const __nv_bfloat16* f, int64_t f
   return bad;
 }
 
+// D (16 x 8) += A (16 x 16) B (16 x 8), bf16 with fp32 sums: lane (g, q) = (lane / 4,
+// lane % 4) holds the k pairs q and q + 4 of A's rows g and g + 8 and of B's
+// column g, and D's columns 2 q, 2 q + 1 in those rows.
+__device__ __forceinline__ void mma_bf16(float* d, uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// k .. k + 8 of a row of K values (16-byte aligned), zeros past its end
+__device__ __forceinline__ uint4 row_piece(const __nv_bfloat16* row, int64_t k, int K) {
+  if (k + 8 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (k + i < K)
+      w[i >> 1] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(row + k + i)) << (16 * (i & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// out[c] = sum over k < K of A[lane, k] B[c, k], c < 32, from memory: the base
+// product of 32 rows and 32 columns again, without any adapter. `a_rows` and
+// `b_rows` rows exist (rows past them repeat the last one; their results mean
+// nothing). For the whole warp. Only for values that another request's broken
+// factor reached (0 x inf = NaN). With one of three adapters NaN throughout, 600
+// rows x 4096 x 1024 take 0.21 ms (44 us with sound ones; a scalar sum a value, each
+// lane at a row of its own: 8.4 ms), 6000 x 4096 x 4096 5.3 ms (0.19; bound by L2).
+// The order of the terms does not matter as long as A and B agree: lane q
+// takes the eight values from 8 q on of every 32, as two products of 16.
+static __device__ __noinline__ void base_products(const __nv_bfloat16* a, int64_t lda, int a_rows,
+                                                  const __nv_bfloat16* b, int64_t ldb, int b_rows,
+                                                  int K, float* out) {
+  const int lane = lane_id(), g = lane >> 2, q = lane & 3;
+  const __nv_bfloat16 *ar[4], *br[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    ar[i] = a + (int64_t)min(8 * i + g, a_rows - 1) * lda;
+    br[i] = b + (int64_t)min(8 * i + g, b_rows - 1) * ldb;
+  }
+  float d[2][4][4] = {};
+#pragma unroll 1
+  for (int64_t k = 8 * q; k < (int64_t)(K + 31) / 32 * 32; k += 32) {
+    uint4 u[4], w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i] = row_piece(ar[i], k, K), w[i] = row_piece(br[i], k, K);
+    __syncwarp();
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const uint4 &lo = u[2 * m], &hi = u[2 * m + 1];
+        mma_bf16(d[m][n], lo.x, hi.x, lo.y, hi.y, w[n].x, w[n].y);
+        mma_bf16(d[m][n], lo.z, hi.z, lo.w, hi.w, w[n].z, w[n].w);
+      }
+  }
+  // row `lane`'s values are with lanes 4 (lane % 8) .. + 3, as rows lane / 16, lane / 8 % 2
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    const int from = 4 * (lane & 7) + ((c & 7) >> 1);
+    float v = 0.f;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const float o = __shfl_sync(0xffffffffu, d[h >> 1][c >> 3][2 * (h & 1) + (c & 1)], from);
+      if (h == lane >> 3) v = o;
+    }
+    out[c] = v;
+  }
+}
+
+// sum over k < rank of low[k] f[k] (both 16-byte aligned): a row's own adapter
+static __device__ __noinline__ float own_term(const __nv_bfloat16* low, const __nv_bfloat16* f,
+                                              int rank) {
+  float acc = 0.f;
+  int k = 0;
+  for (; k + 8 <= rank; k += 8) {
+    const uint4 u = *reinterpret_cast<const uint4*>(low + k);
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(f + k));
+    const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      acc = fmaf(bf16_lo(uw[i]), bf16_lo(vw[i]), acc);
+      acc = fmaf(bf16_hi(uw[i]), bf16_hi(vw[i]), acc);
+    }
+  }
+  for (; k < rank; ++k) acc = fmaf(__bfloat162float(low[k]), __bfloat162float(f[k]), acc);
+  return acc;
+}
+
 }  // namespace fa

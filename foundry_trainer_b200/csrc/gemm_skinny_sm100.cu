@@ -129,21 +129,58 @@ __device__ __forceinline__ void plan_tokens(TokenPlan& pl, const int* ids, int c
   named_bar_sync(1, 128);
 }
 
-// One output value from its own token's operands alone, for values that a
-// block with adapters left non-finite where another token's adapter holds a NaN
-// or an infinity (zero times it).
-__device__ __noinline__ float one_value(const SkinnyParams& p, int j, int i) {
-  const __nv_bfloat16* x = p.raw_x + (int64_t)j * p.raw_ldx;
-  const __nv_bfloat16* w = p.raw_w + (int64_t)i * p.raw_ldw;
-  float acc = 0.f;
-  for (int k = 0; k < p.K; ++k) acc = fmaf(__bfloat162float(x[k]), __bfloat162float(w[k]), acc);
-  const int e = p.ids[j];
-  if (e >= 0 && e < p.E) {
-    const __nv_bfloat16* f = p.raw_f + (int64_t)e * p.raw_fe + (int64_t)i * p.raw_ldf;
-    const __nv_bfloat16* l = p.low + (int64_t)j * p.low_stride;
-    for (int k = 0; k < p.rank; ++k) acc = fmaf(__bfloat162float(l[k]), __bfloat162float(f[k]), acc);
+// The four columns from j on of tile row r, summed in CTA order: recv (split, own
+// / 4, 128, 4), columns j0 on.
+__device__ __forceinline__ void sum_columns(const float* recv, int split, int own, int j, int r,
+                                            float* acc) {
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int q = 0; q < split; ++q) {
+    const float4 v = *reinterpret_cast<const float4*>(recv + (q * own + j) * 128 + r * 4);
+    a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
   }
-  return acc;
+  acc[0] = a.x; acc[1] = a.y; acc[2] = a.z; acc[3] = a.w;
+}
+
+// A warp's 32 rows and the tokens [j0, j1) of its CTA, of which some value is not
+// finite: those that another token's broken factor reached (zero times a NaN or
+// an infinity) are stored again, from their own operands alone, 32 tokens at a
+// time. Apart from the kernel's own code, which it costs no registers.
+__device__ __noinline__ void repair_tokens(const SkinnyParams& p, const TokenPlan& plan,
+                                           const float* recv, int split, int own, int j0, int j1,
+                                           int j_base, int i0) {
+  const int first = i0 + 32 * warp_id(), i = first + lane_id();
+  const bool in = i < p.rows;
+  const int bad = in ? bad_factors(p.raw_f + (int64_t)i * p.raw_ldf, p.raw_fe, p.rank, plan.list,
+                                   plan.cnt)
+                     : (int)kNoneBad;
+  if (!__any_sync(0xffffffffu, bad != kNoneBad)) return;
+  const float bias = in && p.bias != nullptr ? __bfloat162float(p.bias[i]) : 0.f;
+  for (int jb = j0; jb < j1; jb += 32) {
+    const int n = min(32, j1 - jb);
+    uint32_t want = 0;
+    for (int k = 0; k < n; k += 4) {
+      float acc[4];
+      sum_columns(recv, split, own, jb + k - j0, threadIdx.x, acc);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (bad != kNoneBad && k + u < n && !isfinite(acc[u]) && bad != plan.slot[jb + k + u])
+          want |= 1u << (k + u);
+    }
+    if (!__any_sync(0xffffffffu, want != 0)) continue;
+    float base[32];
+    base_products(p.raw_w + (int64_t)first * p.raw_ldw, p.raw_ldw, min(32, p.rows - first),
+                  p.raw_x + (int64_t)(j_base + jb) * p.raw_ldx, p.raw_ldx, n, p.K, base);
+    for (int k = 0; k < n; ++k) {
+      if (!(want >> k & 1)) continue;
+      const int64_t j = j_base + jb + k;
+      const int s = plan.slot[jb + k];
+      float v = base[k];
+      if (s >= 0)
+        v += own_term(p.low + j * p.low_stride,
+                      p.raw_f + (int64_t)plan.list[s] * p.raw_fe + (int64_t)i * p.raw_ldf, p.rank);
+      p.out[j * p.out_ld + i] = __float2bfloat16_rn(v + bias);
+    }
+  }
 }
 
 // What rounding v to `rounded` dropped; nothing where that is an infinity
@@ -497,22 +534,12 @@ skinny_kernel(const __grid_constant__ Maps<OUT> maps, const __grid_constant__ Sk
     tmem_dealloc(tmem, tmem_cols);
   }
   const int i = i0 + r;
-  // the four columns from j on, summed in CTA order
-  auto sum4 = [&](int j, float* acc) {
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int q = 0; q < split; ++q) {
-      const float4 v = *reinterpret_cast<const float4*>(recv + (q * own + j - j0) * 128 + r * 4);
-      a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
-    }
-    acc[0] = a.x; acc[1] = a.y; acc[2] = a.z; acc[3] = a.w;
-  };
-  if (warp < 4 && good && i < rows) {
-    if constexpr (OUT == kSkinnyCols) {
-      // out[j, i], a column a token
+  auto sum4 = [&](int j, float* acc) { sum_columns(recv, split, own, j - j0, r, acc); };
+  if constexpr (OUT == kSkinnyCols) {
+    // out[j, i], a column a token
+    bool odd = false;  // a value of this row is not finite
+    if (warp < 4 && good && i < rows) {
       const float bias = p.bias != nullptr ? __bfloat162float(p.bias[i]) : 0.f;
-      const bool mixed = adapters && p.ids != nullptr && plan.cnt > 0;
-      constexpr int kUnknown = -3;
-      int bad = kUnknown;  // of this output row's factors
 #pragma unroll 2
       for (int j = j0; j < min(j1, cols); j += 4) {
         float acc[4];
@@ -520,15 +547,16 @@ skinny_kernel(const __grid_constant__ Maps<OUT> maps, const __grid_constant__ Sk
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if (j + k >= cols) break;
-          if (mixed && !isfinite(acc[k])) {
-            if (bad == kUnknown)
-              bad = bad_factors(p.raw_f + (int64_t)i * p.raw_ldf, p.raw_fe, p.rank, plan.list, plan.cnt);
-            if (bad != kNoneBad && bad != plan.slot[j + k]) acc[k] = one_value(p, j_base + j + k, i);
-          }
+          odd = odd || !isfinite(acc[k]);
           p.out[(int64_t)(j_base + j + k) * p.out_ld + i] = __float2bfloat16_rn(acc[k] + bias);
         }
       }
-    } else if constexpr (OUT == kSkinnyLow) {
+    }
+    if (adapters && p.ids != nullptr && plan.cnt > 0 && warp < 4 && __any_sync(0xffffffffu, odd))
+      repair_tokens(p, plan, recv, split, own, j0, min(j1, cols), j_base, i0);
+  }
+  if (warp < 4 && good && i < rows) {
+    if constexpr (OUT == kSkinnyLow) {
       // out[i, j]: the columns of the row's own adapter, scaled, in bf16, the
       // operand type of the products that follow: one rounding of a term that
       // is added to the output's fp32 sum. The factors' gradients have no
@@ -563,7 +591,7 @@ skinny_kernel(const __grid_constant__ Maps<OUT> maps, const __grid_constant__ Sk
         // adapter is multiplied whole)
         for (int j = 0; j < p.low_ld; ++j) p.out[(int64_t)i * p.out_ld + j] = __float2bfloat16_rn(0.f);
       }
-    } else {
+    } else if constexpr (OUT == kSkinnyGrad) {
       __nv_bfloat16* out = which ? p.out2 : p.out;
       const int64_t ld = which ? p.out_ld2 : p.out_ld, lj = which ? p.out_j2 : p.out_j;
       for (int j = j0; j < min(j1, p.cols); j += 4) {

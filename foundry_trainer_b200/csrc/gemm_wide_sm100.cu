@@ -194,22 +194,23 @@ __device__ __forceinline__ int slots_of(const WideParams& p, int m) {
   return p.list_cnt != nullptr ? p.list_cnt[m] : 1;
 }
 
-// One output value from its own row's operands alone. Only for values that a
-// block with adapters left non-finite: there a row's zeros in another adapter's
-// K block met a NaN or infinity of that adapter (0 x inf = NaN).
-__device__ __noinline__ float one_value(const WideParams& p, int row, int col, int m) {
-  const __nv_bfloat16* x = p.raw_x + (int64_t)row * p.raw_ldx;
-  const __nv_bfloat16* w = p.raw_w + (int64_t)col * p.raw_ldw;
-  float acc = 0.f;
-  for (int k = 0; k < p.K; ++k) acc = fmaf(__bfloat162float(x[k]), __bfloat162float(w[k]), acc);
-  const int s = p.slot[row];
-  if (s >= 0) {
-    const __nv_bfloat16* f = p.raw_f + (int64_t)p.list_ids[(int64_t)m * 256 + s] * p.raw_fe +
-                             (int64_t)col * p.raw_ldf;
-    const __nv_bfloat16* l = p.low + (int64_t)row * p.low_stride;
-    for (int k = 0; k < p.rank; ++k) acc = fmaf(__bfloat162float(l[k]), __bfloat162float(f[k]), acc);
-  }
-  return acc;
+// 32 columns from col0 on of this lane's row (32 rows from row0 on a warp) from
+// the rows' own operands alone, where `want` has the column's bit. Only for values
+// that a block with adapters left non-finite: there a row's zeros in another
+// adapter's K block met a NaN or infinity of that adapter (0 x inf = NaN).
+__device__ __noinline__ void own_values(const WideParams& p, int row0, int col0, int m,
+                                        uint32_t want, float* v) {
+  float base[32];
+  base_products(p.raw_x + (int64_t)row0 * p.raw_ldx, p.raw_ldx, min(32, p.M - row0),
+                p.raw_w + (int64_t)col0 * p.raw_ldw, p.raw_ldw, min(32, p.N - col0), p.K, base);
+  const int row = row0 + lane_id();
+  const int s = want != 0 ? p.slot[row] : -1;
+  const __nv_bfloat16* l = p.low + (int64_t)row * p.low_stride;
+  const __nv_bfloat16* f =
+      s >= 0 ? p.raw_f + (int64_t)p.list_ids[(int64_t)m * 256 + s] * p.raw_fe : nullptr;
+  for (int c = 0; c < 32; ++c)
+    if (want >> c & 1)
+      v[c] = base[c] + (s >= 0 ? own_term(l, f + (int64_t)(col0 + c) * p.raw_ldf, p.rank) : 0.f);
 }
 
 template <bool B_MN, int EPI>
@@ -513,10 +514,20 @@ wide_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUte
               }
               const int own = live ? p.slot[row] : -1;
 #pragma unroll
-              for (int i = 0; i < 64; ++i) {
-                const int b = __shfl_sync(0xffffffffu, bad[i >> 5], i & 31);
-                if (odd && !isfinite(v[i]) && b != kNoneBad && b != own)
-                  v[i] = one_value(p, row, col0 + i, tl.m);
+              for (int h = 0; h < 2; ++h) {
+                uint32_t want = 0;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                  const int b = __shfl_sync(0xffffffffu, bad[h], i);
+                  if (odd && !isfinite(v[32 * h + i]) && b != kNoneBad && b != own) want |= 1u << i;
+                }
+                if (__any_sync(0xffffffffu, want != 0)) {
+                  float mine[32];
+                  own_values(p, row0 + 32 * warp, col0 + 32 * h, tl.m, want, mine);
+#pragma unroll
+                  for (int i = 0; i < 32; ++i)
+                    if (want >> i & 1) v[32 * h + i] = mine[i];
+                }
               }
             }
           }

@@ -404,7 +404,9 @@ int fa_pad_rows(int64_t rows, int cols, const void* src, int64_t src_stride, voi
  * a (n_adapters, rank, in_dim), b (n_adapters, out_dim, rank), `ids` (rows)
  * int32 on the device: row i uses adapter ids[i] with scales[ids[i]] (fp32,
  * n_adapters); an id outside [0, n_adapters) means the shared projection
- * alone. The ids may be in any order; runs of equal ids are cheaper.
+ * alone. The ids may be in any order; runs of equal ids are cheaper. NaN and
+ * infinities of an adapter stay in its own rows (those of its neighbours cost
+ * time). in_dim <= 2^20.
  */
 int fa_lora_linear_many(int dtype, int rows, int in_dim, int out_dim, int rank, int n_adapters,
                         const fa_matrix_t* x, const fa_matrix_t* w, const fa_matrix_t* a,

@@ -238,3 +238,16 @@ def test_out_must_not_share_elements():
         ops.layer_norm(z(4, 8), out=z(1, 8).expand(4, 8))
     with pytest.raises(ValueError, match="share memory"):
         ops.orthogonalize(z(3, 4, 8), out=z(1, 4, 8).expand(3, 4, 8))
+
+
+def test_c_abi_lora_many_bounds_its_contraction():
+    # (what a broken neighbour costs grows with it, under a bounded wait)
+    lib = _lib.load()
+
+    def many(K):
+        m = _lib.fa_matrix_t(4096, 1 << 30, 1 << 24)
+        return lib.fa_lora_linear_many(1, 4, K, 64, 16, 2, C.byref(m), C.byref(m), C.byref(m),
+                                       C.byref(m), 4096, 4096, None, C.byref(m), None, 0, None)
+
+    assert many((1 << 20) + 1) == _lib.FA_ERR_TOO_LARGE
+    assert many(1 << 20) == _lib.FA_ERR_WORKSPACE  # the next check
