@@ -1,0 +1,57 @@
+"""The wide form's error as an rms over the result, which X kept as two fp16
+parts gives and one part does not.
+
+The result's rounding to bf16: an error uniform over a step of 2^-7 of a value's
+power of two, so at most 2^-7 / sqrt(12) = 2.26e-3 of the value as an rms (1.7e-3
+over many mantissas). Before it five steps, each with three operands rounded to
+fp16: 2^-10 / sqrt(12) = 2.8e-4 each at most, independent, within the matrix's own
+directions, where the following steps carry an error with a gain of 1.9 on
+average: sqrt(15) 2.8e-4 1.9 = 2.1e-3. Together sqrt(2.26^2 + 2.1^2) e-3 = 3.1e-3.
+A rounding of X itself is noise in all directions, of which the steps amplify
+those where the matrix has no strength up to 485-fold; the same iteration with
+the low part dropped, rounded on the CPU as the kernels round, is off by 5.4e-3
+to 1.3e-2 on these inputs (1.7e-3 to 1.9e-3 with it)."""
+import pytest
+import torch
+
+from tests.test_orthogonalize_gpu import gradient, plain, rel
+
+pytestmark = pytest.mark.gpu
+
+BOUND = 3.1e-3
+
+
+def falling(seed, batch, m, n):
+    """Matrices whose singular values fall from 1 to 1e-4."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = min(m, n)
+    q = lambda k: torch.linalg.qr(torch.randn(batch, k, r, generator=g, device="cuda",
+                                              dtype=torch.float64))[0]
+    s = torch.logspace(0, -4, r, device="cuda", dtype=torch.float64)
+    return ((q(m) * s) @ q(n).mT).float()
+
+
+# narrow tiles (upright, tall, a long contraction split, ragged), and matrices
+# that fill the SM pairs in all three products
+@pytest.mark.parametrize("batch,m,n", [(1, 128, 2048), (1, 2048, 128), (2, 72, 200), (1, 1000, 204),
+                                       (1, 768, 1024), (1, 100, 8200), (2, 1536, 4096),
+                                       (2, 4096, 1536)])
+def test_weak_directions_of_a_matrix(batch, m, n):
+    from foundry_trainer_b200 import ops
+    x = falling(m + n, batch, m, n)
+    ref = plain(x)
+    got = ops.orthogonalize(x)
+    torch.cuda.synchronize()
+    assert ops.device_status() == 0
+    for o, r in zip(got, ref):
+        assert rel(o, r) <= BOUND, rel(o, r)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("batch,m,n", [(2, 72, 200), (1, 300, 1000), (1, 1000, 300), (1, 1024, 2048),
+                                       (2, 1536, 4096)])
+def test_rms_error_of_gradients(batch, m, n, dtype):
+    from foundry_trainer_b200 import ops
+    for k, kw in enumerate((dict(rank=4, noise=0.1), dict(rank=1, noise=1.0))):
+        g = gradient(k, batch, m, n, dtype=dtype, **kw)
+        assert rel(ops.orthogonalize(g), plain(g)) <= BOUND, (k, rel(ops.orthogonalize(g), plain(g)))
