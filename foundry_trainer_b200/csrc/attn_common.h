@@ -187,6 +187,7 @@ int launch_layer_norm_bwd(int dtype, int groups, int rows, int dim, const fa_ten
 // Newton-Schulz orthogonalisation (orthogonalize.cu): g (batch, rows, cols)
 // in `dtype`, o bf16; strides in elements; c = (a, b, c)
 size_t orthogonalize_workspace(int batch, int rows, int cols, int steps);
+bool orthogonalize_in_range(int rows, int cols, int steps, const float* c);
 int launch_orthogonalize(int dtype, int batch, int rows, int cols, const void* g, int64_t gb,
                          int64_t gr, void* o, int64_t ob, int64_t orow, int steps, const float* c,
                          float eps, void* ws, cudaStream_t st);

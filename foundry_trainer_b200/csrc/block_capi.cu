@@ -462,6 +462,8 @@ int fa_orthogonalize(int dtype, int batch, int rows, int cols, const void* g, in
   if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c) || !(eps >= 0.f) ||
       !std::isfinite(eps))
     return FA_ERR_INVALID_ARG;
+  const float coef[3] = {a, b, c};
+  if (!orthogonalize_in_range(rows, cols, steps, coef)) return FA_ERR_UNSUPPORTED;
   if (batch == 0) return FA_OK;
   if (g == nullptr || o == nullptr) return FA_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(g) % (dtype == FA_DTYPE_BF16 ? 2 : 4) != 0 ||
@@ -471,7 +473,6 @@ int fa_orthogonalize(int dtype, int batch, int rows, int cols, const void* g, in
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return FA_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return FA_ERR_ALIGNMENT;
   FA_TRY(check_sm100());
-  const float coef[3] = {a, b, c};
   return launch_orthogonalize(dtype, batch, rows, cols, g, g_stride_batch, g_stride_row, o,
                               o_stride_batch, o_stride_row, steps, coef, eps, workspace,
                               reinterpret_cast<cudaStream_t>(stream));

@@ -28,9 +28,10 @@
 // G has no strength. X is therefore kept as the sum of two fp16 matrices, hi
 // and lo (22 bits); the products read hi, and the epilogue adds a (hi + lo)
 // in fp32. Errors of the products stay within G's own directions, where the
-// steps contract. Against 64 bits: 2.3e-3 of the result's norm on Gaussian
-// noise, 1.7e-3 on a few strong directions over noise; the final rounding to
-// bf16 alone is 1.7e-3.
+// steps contract. Against 64 bits: 2.4e-3 of the result's norm on Gaussian
+// noise, 1.7e-3 to 1.9e-3 on a few strong directions over noise; the final
+// rounding to bf16 alone is 1.7e-3. Coefficients whose steps would take singular
+// values out of fp16's range are refused (in_range).
 //
 // Measured: 16 x (16 x 4096) bf16 13 us, 8 x (64 x 4096) 78 us (fp64 tensor
 // instructions, about half their rate); 4096 x 8192 fp32 2.1 to 2.2 ms under
@@ -730,7 +731,45 @@ static int wide_go(const void* g, int64_t gb, int64_t gr, void* o, int64_t ob, i
 
 constexpr int kThinMost = 64;
 
+// Whether the wide form's fp16 operands hold every step's: singular values start
+// in [0, 1]; s, their bound, becomes the largest |p| on [0, s] with each step, p(x) =
+// a x + b x^3 + c x^5, which lies at s or where p' = 0 (a quadratic in x^2). No entry of
+// X, Q or b Q + c Q^2 exceeds its largest singular value; stored are 256 X, 64 Q and
+// 64 (b Q + c Q^2), and fp16 ends at 65504 (64000 leaves room for the roundings
+// of the steps before).
+static bool in_range(int steps, const float* coef) {
+  const double a = coef[0], b = coef[1], c = coef[2], most = 64000.0;
+  double s = 1.0;
+  for (int k = 0; k < steps; ++k) {
+    const double u = s * s;
+    double poly = std::abs(u * (b + c * u));  // the largest |b v + c v^2|, v <= u
+    if (c != 0.0) {
+      const double v = -b / (2.0 * c);
+      if (v > 0.0 && v < u) poly = std::max(poly, std::abs(v * (b + c * v)));
+    }
+    if (!(256.0 * s <= most && 64.0 * u <= most && 64.0 * poly <= most)) return false;
+    auto p = [&](double v) { return std::sqrt(v) * std::abs(a + v * (b + c * v)); };  // at x^2 = v
+    double top = p(u);
+    auto look = [&](double v) {
+      if (v > 0.0 && v < u) top = std::max(top, p(v));
+    };
+    const double disc = 9.0 * b * b - 20.0 * a * c;
+    if (c != 0.0 && disc >= 0.0) {
+      look((-3.0 * b + std::sqrt(disc)) / (10.0 * c));
+      look((-3.0 * b - std::sqrt(disc)) / (10.0 * c));
+    } else if (c == 0.0 && b != 0.0) {
+      look(-a / (3.0 * b));
+    }
+    s = top;
+  }
+  return true;
+}
+
 }  // namespace ns
+
+bool orthogonalize_in_range(int rows, int cols, int steps, const float* coef) {
+  return std::min(rows, cols) <= ns::kThinMost || ns::in_range(steps, coef);
+}
 
 size_t orthogonalize_workspace(int batch, int rows, int cols, int steps) {
   const int m = std::min(rows, cols), n = std::max(rows, cols);

@@ -295,7 +295,9 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5,
     f32: X = g / (|g|_F + eps), then `steps` times X = a X + (b Q + c Q^2) X
     with Q = X X^T (of the transpose when m > n). Returns bf16, (..., m, n):
     a step's direction, whose singular values the iteration itself leaves
-    spread by some 20 percent. Identical bits across repeats."""
+    spread by some 20 percent. Coefficients that take singular values far above
+    one (the header has the limits; NS_COEFFS stay at 1.2) are refused where
+    both sides exceed 64. Identical bits across repeats."""
     a, b, c = coeffs
     return _lib.binding().orthogonalize(g, steps, a, b, c, eps, out, stream)
 

@@ -420,9 +420,11 @@ size_t fa_lora_linear_many_workspace_bytes(int rows, int rank);
  * (rows, cols) matrices G in `dtype` (f32 or bf16; columns contiguous),
  *   X = G / (|G|_F + eps);  steps times: X = a X + (b Q + c Q^2) X, Q = X X^T
  * (on the transposed matrix when rows > cols), written to o as bf16 (columns
- * contiguous, 16-byte aligned, strides multiples of 8). Singular values have
- * to stay below about 100 for the given a, b, c (fp16 operands); 1 <= steps
- * <= 64. Identical bits across repeats. workspace:
+ * contiguous, 16-byte aligned, strides multiples of 8); 1 <= steps <= 64. With a
+ * short side above 64 the operands are fp16: 64 s^2 and 64 |b s^2 + c s^4| have to
+ * stay below 64000 for every singular value s that enters a step, from [0, 1] on
+ * (s < 4.8 for b = -4.775, c = 2.0315; their steps stay below 1.3); other
+ * coefficients are answered with FA_ERR_UNSUPPORTED. Identical bits across repeats. workspace:
  * fa_orthogonalize_workspace_bytes() (0 while the short side is at most 64),
  * 16-byte aligned. No counterpart in the reference, whose optimiser is AdamW.
  */

@@ -251,3 +251,25 @@ def test_c_abi_lora_many_bounds_its_contraction():
 
     assert many((1 << 20) + 1) == _lib.FA_ERR_TOO_LARGE
     assert many(1 << 20) == _lib.FA_ERR_WORKSPACE  # the next check
+
+
+def test_c_abi_orthogonalize_refuses_coefficients_beyond_fp16():
+    lib = _lib.load()
+
+    def go(m, steps, a, b, c):
+        return lib.fa_orthogonalize(0, 1, m, 320, 4096, m * 320, 320, 4096, m * 320, 320, steps, a,
+                                    b, c, 1e-7, None, 0, None)
+
+    UNS, WS = _lib.FA_ERR_UNSUPPORTED, _lib.FA_ERR_WORKSPACE  # (the next check)
+    default = (3.4445, -4.7750, 2.0315)
+    for steps in (1, 5, 64):
+        assert go(65, steps, *default) == WS
+    # p(1) = 4.7, then 64 (b 4.7^2 + c 4.7^4) = 56700; the last step's result is bf16
+    assert go(65, 2, 7.4435, *default[1:]) == WS and go(65, 3, 7.4435, *default[1:]) == UNS
+    assert go(65, 2, 7.6435, *default[1:]) == UNS  # 4.9: 67600
+    assert go(65, 2, 31.0, 0.0, 0.0) == WS and go(65, 2, 32.0, 0.0, 0.0) == UNS  # Q alone
+    assert go(65, 1, 1.0, 1001.0, 0.0) == UNS and go(65, 1, 1.0, 0.0, -1001.0) == UNS
+    assert go(65, 1, 0.0, 4004.0, -4004.0) == UNS  # its largest inside: 4004 / 4 at s^2 = 1/2
+    assert go(65, 1, 0.0, 3990.0, -3990.0) == WS
+    # short sides up to 64 are fp64 throughout
+    assert go(64, 3, 32.0, 0.0, 0.0) not in (UNS, WS)

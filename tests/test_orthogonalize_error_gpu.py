@@ -55,3 +55,35 @@ def test_rms_error_of_gradients(batch, m, n, dtype):
     for k, kw in enumerate((dict(rank=4, noise=0.1), dict(rank=1, noise=1.0))):
         g = gradient(k, batch, m, n, dtype=dtype, **kw)
         assert rel(ops.orthogonalize(g), plain(g)) <= BOUND, (k, rel(ops.orthogonalize(g), plain(g)))
+
+
+@pytest.mark.parametrize("m,n", [(96, 320), (320, 96), (40, 512)])
+def test_coefficients_near_the_range_of_fp16(m, n):
+    # One step takes a singular value of 1 to 4.7, where 64 (b Q + c Q^2) is 56700
+    # of fp16's 65504, all of it in one entry. Its relative error: the first step's
+    # roundings of Q, b Q + c Q^2 and X, 2^-11 each of terms of 2.7 (the sum) and 6.8
+    # (|b| + |c|) to 4.7: 1.6e-3, times s p'(s) / p(s) = 5.2 at 4.7; the second's, four
+    # of 2^-11; the result's, 2^-8: 1.5e-2 if all align.
+    from foundry_trainer_b200 import _lib, ops
+    co = (7.4435, -4.7750, 2.0315)
+    g = torch.zeros(2, m, n, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    v = torch.randn(max(m, n), generator=gen, device="cuda")
+    u = torch.randn(min(m, n), generator=gen, device="cuda")
+    one, spread = (v[None], u[:, None] * v) if m <= n else (v[:, None], v[:, None] * u)
+    if m <= n:
+        g[0, 7:8] = one
+    else:
+        g[0, :, 7:8] = one
+    g[1] = spread
+    ref = plain(g, 2, co)
+    got = ops.orthogonalize(g, steps=2, coeffs=co)
+    assert torch.isfinite(got).all()
+    for o, r in zip(got, ref):
+        assert rel(o, r) <= 1.5e-2, rel(o, r)
+    if min(m, n) > 64:
+        with pytest.raises(_lib.FaError):
+            ops.orthogonalize(g, steps=3, coeffs=co)
+    else:
+        ref = plain(g, 3, co)
+        assert rel(ops.orthogonalize(g, steps=3, coeffs=co), ref) <= 5 * 1.5e-2
