@@ -216,7 +216,8 @@ class FusedKernels:
         weight, bias = _get(w, f"weights/{name}.weight"), w.get(f"weights/{name}.bias")
         if a.dim() == 2:
             return _LoraLinear.apply(x, weight, a, b, bias, lora_scale)
-        if torch.is_grad_enabled() and any(t.requires_grad for t in (x, weight, a, b)):
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (x, weight, a, b, bias)
+                                           if t is not None):
             raise ValueError(f"{name}: stacked adapters serve without gradients (torch.no_grad)")
         if self.adapters is None or self.adapters.shape != x.shape[:1]:
             raise ValueError(f"{name}: stacked adapters need one adapter id per sample, "

@@ -273,3 +273,12 @@ def test_c_abi_orthogonalize_refuses_coefficients_beyond_fp16():
     assert go(65, 1, 0.0, 3990.0, -3990.0) == WS
     # short sides up to 64 are fp64 throughout
     assert go(64, 3, 32.0, 0.0, 0.0) not in (UNS, WS)
+
+
+def test_fused_linear_refuses_a_trained_bias_beside_stacked_factors():
+    # (its gradient would be missing without a word)
+    w = {"weights/l.weight": z(8, 16), "weights/l.lora_a": z(3, 4, 16),
+         "weights/l.lora_b": z(3, 8, 4), "weights/l.bias": z(8).requires_grad_(True)}
+    k = blocks.FusedKernels(torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(ValueError, match="without gradients"):
+        k.linear(w, "l", z(2, 5, 16), 1.0)
