@@ -168,9 +168,6 @@ class _LoraLinear(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, a, b, bias, scale):
-        if ctx.needs_input_grad[1]:
-            raise ValueError("the fused linear trains the LoRA factors (and its bias); "
-                             "its weight must not require a gradient")
         x2 = _aligned(x.reshape(-1, x.shape[-1]))
         y, low = ops.lora_linear(x2, weight, a, b, scale=scale, bias=bias)
         ctx.save_for_backward(x2, weight, a, b, low)
@@ -215,6 +212,9 @@ class FusedKernels:
             return linear(w, name, x, lora_scale)
         weight, bias = _get(w, f"weights/{name}.weight"), w.get(f"weights/{name}.bias")
         if a.dim() == 2:
+            if torch.is_grad_enabled() and weight.requires_grad:
+                raise ValueError("the fused linear trains the LoRA factors (and its bias); "
+                                 "its weight must not require a gradient")
             return _LoraLinear.apply(x, weight, a, b, bias, lora_scale)
         if torch.is_grad_enabled() and any(t.requires_grad for t in (x, weight, a, b, bias)
                                            if t is not None):

@@ -282,3 +282,13 @@ def test_fused_linear_refuses_a_trained_bias_beside_stacked_factors():
     k = blocks.FusedKernels(torch.zeros(2, dtype=torch.int32))
     with pytest.raises(ValueError, match="without gradients"):
         k.linear(w, "l", z(2, 5, 16), 1.0)
+
+
+def test_fused_linear_takes_a_trainable_weight_without_gradients():
+    # sampling with a model whose weights are parameters: on to the kernel, which
+    # here misses its GPU
+    w = {"weights/l.weight": z(8, 16).requires_grad_(True), "weights/l.lora_a": z(4, 16),
+         "weights/l.lora_b": z(8, 4)}
+    for graph_free in (torch.no_grad(), torch.inference_mode()):
+        with graph_free, pytest.raises(ValueError, match="CUDA device"):
+            blocks.FusedKernels().linear(w, "l", z(2, 16), 1.0)

@@ -326,3 +326,16 @@ def test_a_batch_of_requests_with_an_adapter_each():
             for a, b in ((oi[i:i + 1], si), (ot[i:i + 1], st)):
                 assert bs.rel_l2(a, b) <= 1e-2, (i, e, bs.rel_l2(a, b))
     assert E == stacked[tr.keys[0]].shape[0]
+
+
+def test_fused_linear_of_a_trainable_weight_without_gradients():
+    g = _gen(12)
+    w = {"weights/l.weight": _rn(g, 256, 128), "weights/l.lora_a": _rn(g, 16, 128),
+         "weights/l.lora_b": _rn(g, 256, 16)}
+    x = _rn(g, 2, 70, 128)
+    want = blocks.FusedKernels().linear(w, "l", x, 0.5)
+    w = {k: t.clone().requires_grad_(True) for k, t in w.items()}
+    for graph_free in (torch.no_grad(), torch.inference_mode()):
+        with graph_free:
+            y = blocks.FusedKernels().linear(w, "l", x, 0.5)
+        assert torch.equal(y, want) and not y.requires_grad
