@@ -372,13 +372,20 @@ void check_lora(const Tensor& x2, const Tensor& w, const Tensor& a, const Tensor
 int64_t low_dim(int64_t rank) { return (rank + 15) / 16 * 32; }
 
 // b with rows that start on 16 bytes: itself, or a copy (a rank that is no
-// multiple of 8)
+// multiple of 8, a slice)
 Tensor aligned_b(const Tensor& b, const Place& at) {
   if (b.stride(-1) != 1 && b.size(-1) > 1) refuse("b: the last dimension must be contiguous");
-  const bool ok = (b.size(-2) == 1 || b.stride(-2) % 8 == 0) &&
+  const bool ok = reinterpret_cast<uintptr_t>(b.data_ptr()) % 16 == 0 &&
+                  (b.size(-2) == 1 || b.stride(-2) % 8 == 0) &&
                   (b.dim() == 2 || b.size(0) == 1 || b.stride(0) % 8 == 0);
   if (ok || b.numel() == 0) return b;
   const int64_t r = b.size(-1), ld = (r + 7) / 8 * 8;
+  // adapters that are no one strided set of rows (a slice of each)
+  if (b.dim() == 3 && b.size(0) > 1 && b.size(1) > 1 && b.stride(0) != b.size(1) * b.stride(1)) {
+    Tensor t = at::empty({b.size(0), b.size(1), ld}, b.options()).narrow(2, 0, r);
+    t.copy_(b.detach());
+    return t;
+  }
   Tensor rows = rows_of(b, "b");
   Tensor t = at::empty({rows.size(0), ld}, b.options());
   checked(fa_pad_rows((int64_t)rows.size(0), (int)r, rows.data_ptr(), rows.stride(0), t.data_ptr(),

@@ -379,3 +379,30 @@ def test_layer_norm_in_place():
         y, stats = ops.layer_norm(x)
         z, again = ops.layer_norm(x, out=x)
         assert z is x and torch.equal(x, y) and torch.equal(stats, again)
+
+
+def test_lora_linear_takes_any_rows_of_b():
+    # slices whose rows start anywhere, of one matrix and of stacked ones
+    from foundry_trainer_b200 import ops
+    g = _gen(16)
+    E, N, K, M, r = 3, 90, 128, 200, 16
+    x, w, a, _, bias = _lora_inputs(g, N, K, M, r, True, E)
+    ids = (torch.arange(N, device="cuda") % (E + 1) - 1).to(torch.int32)
+    scales = torch.rand(E, generator=g, device="cuda") + 0.5
+    dy = _rn(g, N, M)
+    big = _rn(g, E, M + 5, 40, std=0.5)
+    # a row stride of 16 bytes or not, a first element on 16 bytes or not
+    for rows, cols in ((slice(0, M), slice(3, 3 + r)), (slice(1, M + 1), slice(8, 8 + r)),
+                       (slice(5, M + 5), slice(0, 12)), (slice(0, M), slice(1, 1 + r))):
+        for whole in (big, _rn(g, E, M + 5, 37, std=0.5), big[:, :M + 3].contiguous()[:, :M + 5]):
+            b = whole[:, :M][:, :, cols] if rows.stop > whole.shape[1] else whole[:, rows, cols]
+            aa = a[:, :b.shape[2]]
+            got = ops.lora_linear_many(x, w, aa, b, ids, scales, bias=bias)
+            want = ops.lora_linear_many(x, w, aa, b.contiguous(), ids, scales, bias=bias)
+            assert torch.equal(got, want)
+            y, low = ops.lora_linear(x, w, aa[1], b[1], bias=bias)
+            y2, low2 = ops.lora_linear(x, w, aa[1], b[1].contiguous(), bias=bias)
+            assert torch.equal(y, y2) and torch.equal(low, low2)
+            for p, q in zip(ops.lora_linear_bwd(x, w, aa[1], b[1], dy, low),
+                            ops.lora_linear_bwd(x, w, aa[1], b[1].contiguous(), dy, low)):
+                assert torch.equal(p, q)
