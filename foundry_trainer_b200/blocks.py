@@ -535,6 +535,11 @@ class AdamW:
             p.copy_((p.float() - (m / bc1) / denom * self.lr).to(p.dtype))
 
 
+# Elements that Muon orthogonalises in one call: 1 GB of fp32 updates and some 2 GB
+# of workspace, by far more than fill the GPU.
+_MUON_ELEMENTS = 1 << 28
+
+
 @dataclass
 class Muon:
     """Momentum with orthogonalised updates (ops.orthogonalize) for matrix
@@ -542,8 +547,8 @@ class Muon:
       m <- momentum m + (1 - momentum) g,  u = m, or with nesterov
       momentum m + (1 - momentum) g;  p <- (1 - lr weight_decay) p
       - lr sqrt(max(1, rows / cols)) orthogonalize(u).
-    fp32 momentum; matrices of one shape are orthogonalised in one call. The
-    reference has no counterpart."""
+    fp32 momentum; matrices of one shape are orthogonalised in one call, up to
+    _MUON_ELEMENTS of them at a time. The reference has no counterpart."""
     lr: float = 0.02
     momentum: float = 0.95
     nesterov: bool = True
@@ -564,7 +569,11 @@ class Muon:
         same: Dict[tuple, List[int]] = {}
         for i, p in enumerate(params):
             same.setdefault((tuple(p.shape), p.device), []).append(i)
+        some = []  # (shape, indices) of one call each
         for (shape, _), at in same.items():
+            most = max(1, _MUON_ELEMENTS // max(1, shape[0] * shape[1]))
+            some += [(shape, at[k:k + most]) for k in range(0, len(at), most)]
+        for shape, at in some:
             u = torch.stack([grads[i].float() for i in at])
             for row, i in zip(u, at):
                 state[i].lerp_(row, 1.0 - self.momentum)

@@ -292,3 +292,30 @@ def test_fused_linear_takes_a_trainable_weight_without_gradients():
     for graph_free in (torch.no_grad(), torch.inference_mode()):
         with graph_free, pytest.raises(ValueError, match="CUDA device"):
             blocks.FusedKernels().linear(w, "l", z(2, 16), 1.0)
+
+
+def test_muon_bounds_what_it_orthogonalises_at_once(monkeypatch):
+    # (32 matrices of 4096 x 14336 in one call took 7.5 GB of updates and 13 GB of
+    # workspace)
+    sizes = []
+
+    def fake(u, **kw):
+        sizes.append(u.numel())
+        return (u * 0.5).to(BF)
+
+    monkeypatch.setattr(ops, "orthogonalize", fake)
+    shapes = [(8, 16)] * 7 + [(16, 8)] * 2 + [(64, 64)]
+    g = torch.Generator().manual_seed(1)
+    first = [torch.randn(*s, generator=g) for s in shapes]
+    grads = [torch.randn(*s, generator=g) for s in shapes]
+    results = []
+    for most in (None, 300):  # two of the small ones, one large one
+        if most:
+            monkeypatch.setattr(blocks, "_MUON_ELEMENTS", most)
+        p, opt = [t.clone() for t in first], blocks.Muon(weight_decay=0.1)
+        state = opt.init(p)
+        sizes.clear()
+        opt.step(p, grads, state, 1)
+        results.append(p + state)
+    assert sorted(sizes) == [128, 256, 256, 256, 256, 4096]
+    assert all(torch.equal(a, b) for a, b in zip(*results))
