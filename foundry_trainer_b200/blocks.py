@@ -196,7 +196,10 @@ class FusedKernels:
     arithmetic as `layer_norm_mod` and `linear` with fewer roundings (y = x W^T
     + b + s (x A^T) B^T is rounded once, the low-rank term before it once).
     bf16 linears, bf16 or f32 norms; linears without LoRA factors stay
-    torch's. On the GPU only.
+    torch's. On the GPU only. Narrower than torch's, and raising beyond it: LoRA
+    linears in bf16 alone, of an input width that is a multiple of 8 and a rank
+    of at most 256; shift and scale of one dtype. Their weight is frozen: it may
+    require a gradient only where none is recorded.
 
     `adapters`: serving a batch of requests that each have their own LoRA.
     Factors stacked over the E adapters ((E, rank, in), (E, out, rank)) apply

@@ -31,7 +31,7 @@ constexpr int kThreads = 192;
 constexpr int kBig = 16384;  // 128 x 64 elements
 constexpr int kMaxStages = 8;
 constexpr int kBarBytes = 256;
-constexpr int kTwoSmem = 109 * 1024;  // two CTAs an SM, beside their static 2.6 KB
+constexpr int kTwoSmem = 109 * 1024;  // two CTAs an SM, beside their static 3.6 KB
 constexpr int kOneSmem = 220 * 1024;
 constexpr int kMaxTokens = kMaxColumns;
 

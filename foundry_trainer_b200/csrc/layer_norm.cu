@@ -975,7 +975,9 @@ static int fwd_pick(const Mat& x, const Mat& y, const Par& par, int groups, int 
   const int nv = (dim + E - 1) / E;
   const int64_t n = (int64_t)groups * rows;
   if constexpr (E > 2) {
-    // a few rows a block at least, or the ring's set-up is all there is
+    // a few rows a block, or the ring's set-up is all there is. (It goes by the
+    // rows of all groups: many groups of one or two rows take the ring too,
+    // whose blocks then turn once.)
     if (use_ring(nv) && n >= 8 * kSms) {
       const RingPlan p = ring_plan(nv, 1);
       const int kid = kKernelNorm + (sizeof(T) == 2 ? 0 : 3);

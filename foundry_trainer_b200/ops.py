@@ -281,11 +281,13 @@ def lora_linear_many(x: torch.Tensor, w: torch.Tensor, a: torch.Tensor, b: torch
     """lora_linear for rows of many requests at once: a (E, rank, in),
     b (E, out, rank), scales (E,) fp32, ids (rows,) int32 on the device; row i
     uses adapter ids[i], and an id outside [0, E) means w alone. From one
-    token to packed prompts; ids in any order. Returns y."""
+    token to packed prompts; ids in any order; `in` at most 2^20. NaN and
+    infinities of an adapter stay in its own rows. Returns y."""
     return _lib.binding().lora_linear_many(x, w, a, b, ids, scales, bias, stream)
 
 
-NS_COEFFS = (3.4445, -4.7750, 2.0315)  # five steps take [0.005, 1] to about [0.7, 1.2]
+# as published for the Muon optimiser; five steps take [0.005, 1] to about [0.7, 1.2]
+NS_COEFFS = (3.4445, -4.7750, 2.0315)
 
 
 def orthogonalize(g: torch.Tensor, *, steps: int = 5,
