@@ -339,3 +339,45 @@ def test_fused_linear_of_a_trainable_weight_without_gradients():
         with graph_free:
             y = blocks.FusedKernels().linear(w, "l", x, 0.5)
         assert torch.equal(y, want) and not y.requires_grad
+
+
+def test_calls_at_once_on_three_streams():
+    # each call repeats its bits, whatever runs beside it: clusters, tensor memory,
+    # early starts and workspaces of calls on other streams
+    from foundry_trainer_b200 import ops
+    g = _gen(14)
+    x, w = _rn(g, 900, 1024), _rn(g, 1544, 1024, std=0.03)
+    a, b = _rn(g, 5, 12, 1024, std=0.03), _rn(g, 5, 1544, 12)
+    dy = _rn(g, 900, 1544)
+    ids = torch.randint(-1, 5, (900,), generator=g, device="cuda", dtype=torch.int32)
+    scales = torch.ones(5, device="cuda")
+    square, thin = _rn(g, 2, 300, 700), _rn(g, 6, 2000, 24)
+    norm_w = _rn(g, 1024, std=0.2)
+
+    def train():
+        y, low = ops.lora_linear(x, w, a[0], b[0])
+        return (y, *ops.lora_linear_bwd(x, w, a[0], b[0], dy, low))
+
+    def serve():
+        return tuple(ops.lora_linear_many(x[:n], w, a, b, ids[:n], scales) for n in (1, 60, 200, 900))
+
+    def rest():
+        y, stats = ops.layer_norm(x, norm_w, None)
+        return (ops.orthogonalize(square), *ops.layer_norm_bwd(x, norm_w, x, stats),
+                ops.orthogonalize(thin), y)
+
+    calls = [train, serve, rest]
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for turn in range(3):
+        got = [[] for _ in calls]
+        for _ in range(8):
+            for k, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[k].append(calls[(k + turn) % 3]())
+        torch.cuda.synchronize()
+        assert ops.device_status() == 0
+        for k in range(3):
+            for one in got[k]:
+                assert all(torch.equal(p, q) for p, q in zip(one, want[(k + turn) % 3]))
