@@ -424,9 +424,10 @@ size_t fa_lora_linear_many_workspace_bytes(int rows, int rank);
  * short side above 64 the operands are fp16: 64 s^2 and 64 |b s^2 + c s^4| have to
  * stay below 64000 for every singular value s that enters a step, from [0, 1] on
  * (s < 4.8 for b = -4.775, c = 2.0315; their steps stay below 1.3); other
- * coefficients are answered with FA_ERR_UNSUPPORTED. Identical bits across repeats. workspace:
- * fa_orthogonalize_workspace_bytes() (0 while the short side is at most 64),
- * 16-byte aligned. No counterpart in the reference, whose optimiser is AdamW.
+ * coefficients are answered with FA_ERR_UNSUPPORTED. Identical bits across
+ * repeats. workspace: fa_orthogonalize_workspace_bytes() (0 while the short side
+ * is at most 64), 16-byte aligned. No counterpart in the reference, whose
+ * optimiser is AdamW.
  */
 int fa_orthogonalize(int dtype, int batch, int rows, int cols, const void* g,
                      int64_t g_stride_batch, int64_t g_stride_row, void* o,
