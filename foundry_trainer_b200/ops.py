@@ -299,7 +299,7 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5,
     a step's direction, whose singular values the iteration itself leaves
     spread by some 20 percent. Coefficients that take singular values far above
     one (the header has the limits; NS_COEFFS stay at 1.2) are refused where
-    both sides exceed 64. Identical bits across repeats."""
+    both sides exceed 64. `out` may be a bf16 g. Identical bits across repeats."""
     a, b, c = coeffs
     return _lib.binding().orthogonalize(g, steps, a, b, c, eps, out, stream)
 

@@ -88,3 +88,14 @@ def test_coefficients_near_the_range_of_fp16(m, n):
     else:
         ref = plain(g, 3, co)
         assert rel(ops.orthogonalize(g, steps=3, coeffs=co), ref) <= 5 * 1.5e-2
+
+
+@pytest.mark.parametrize("shape", [(5, 16, 4096), (3, 1000, 24), (2, 61, 304), (2, 400, 56), (1, 96, 320),
+                                   (2, 320, 96), (1, 1536, 2048)])
+def test_out_may_be_the_input(shape):
+    # nothing reads an element of the input after its place has been written
+    from foundry_trainer_b200 import ops
+    g = gradient(4, *shape)
+    want = ops.orthogonalize(g)
+    got = ops.orthogonalize(g, out=g)
+    assert got is g and torch.equal(g, want)
